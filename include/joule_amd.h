@@ -44,6 +44,9 @@ extern "C" {
 
 #define JM_DTYPE_F32 0
 #define JM_DTYPE_BF16 1
+/* KV caches only (jm_store_set_kv_dtype): 4-bit rows in groups of 64 or 32 */
+#define JM_DTYPE_Q4 2
+#define JM_DTYPE_Q4_G32 3
 
 /* Byte-identical to the reference's KernelCfg (decode_kernel.c:269-286), so
  * a host that already fills one (decoder3.py:95-119) passes it unchanged.
@@ -202,7 +205,8 @@ int jm_store_copy_workspace(const jm_store* s, int field, void* dst, uint64_t by
 /* One sequence's cache of one layer, the reference's KVCache
  * (decode_kernel.c:328-331): k and v [maxT][n_kv][hd] in device memory,
  * bfloat16 by default; float32, the reference's own type, after
- * jm_store_set_kv_dtype(store, JM_DTYPE_F32). */
+ * jm_store_set_kv_dtype(store, JM_DTYPE_F32); 4-bit planes after
+ * jm_store_set_kv_dtype(store, JM_DTYPE_Q4 or JM_DTYPE_Q4_G32). */
 typedef struct jm_kv_cache {
     void* k;
     void* v;
@@ -343,7 +347,9 @@ int jm_store_set_max_layers(jm_store* s, int n);
  * JM_DTYPE_BF16 (the default: half the bytes per attention read) or
  * JM_DTYPE_F32, the reference's KVCache (decode_kernel.c:328-331), whose
  * appended rows then keep float32 values and whose attention runs in
- * float32 arithmetic throughout. */
+ * float32 arithmetic throughout; or JM_DTYPE_Q4 / JM_DTYPE_Q4_G32, 4-bit rows
+ * (jm_kv_cache then holds planes of jm_kv_q4_bytes(cfg->maxT, cfg->n_kv, 64 or
+ * 32) bytes). */
 int jm_store_set_kv_dtype(jm_store* s, int dtype);
 
 /* A dense model's FFN (layer_ffn_batch with E == 0, decode_kernel.c:
@@ -460,6 +466,104 @@ int jm_get_q4_gemm_min_tokens(void);
  * multiples of 128).  Reads no device memory.  No counterpart in the
  * reference. */
 int jm_gemm_plan(int rows0, int rows1, int rows2, int K, int B, int* slices);
+
+/* ---- the 4-bit KV cache ----
+ *
+ * No counterpart in the reference, whose KVCache is float32
+ * (decode_kernel.c:328-331).  A cache row of a head (128 values of k or of v)
+ * is held in the expert store's Q4 format (q4_store.py:40-67): groups of 64 or
+ * 32 values, each with the scale fp16(fp32(absmax / 7)), the codes
+ * clip(round_half_even(x / scale), -8, 7) + 8: 68 or 72 bytes instead of
+ * bf16's 256.  A group that holds a NaN or an infinity, or a magnitude above
+ * 7 * 65504, reads back as NaN.
+ *
+ * A plane (the k or the v rows of one sequence and layer) is
+ * jm_kv_q4_bytes(maxT, n_kv, group) bytes: rows are kept head by head, the codes
+ * in the order in which the matrix cores take them, so a plane is read and
+ * written only by these calls and by the decoder (jm_store_set_kv_dtype with
+ * JM_DTYPE_Q4 or JM_DTYPE_Q4_G32, planes of cfg->maxT and cfg->n_kv).  Its
+ * contents before a row is written do not matter. */
+
+/* The caches of n_seq sequences in one layer: sequence s's planes at
+ * k + s * seq_stride and v + s * seq_stride (16-byte aligned, seq_stride a
+ * multiple of 16). */
+typedef struct jm_kv_q4 {
+    void* k;
+    void* v;
+    uint64_t seq_stride;
+    int n_seq;
+    int maxT;
+    int n_kv;
+    int group;
+} jm_kv_q4;
+
+/* Bytes of one plane; a negative code for maxT or n_kv <= 0 or a group other
+ * than 64 and 32. */
+int64_t jm_kv_q4_bytes(int maxT, int n_kv, int group);
+
+/* The N tokens of a call: sequence s has the tokens cu[s] .. cu[s + 1] - 1 at
+ * cache rows start[s], start[s] + 1, ...  start int32 [n_seq] and cu int32
+ * [n_seq + 1] (ascending) are in DEVICE memory; with cu NULL every sequence has
+ * one token, in order (N = n_seq).  Tokens from cu[n_seq] on, and tokens whose
+ * row lies outside [0, maxT), are skipped: nothing is written for them, here or
+ * in the outputs below, which keep what they held.
+ *
+ * Tensors are [N][heads][128] in dtype JM_DTYPE_F32 or JM_DTYPE_BF16; the
+ * strides (in elements, multiples of 4) are those of tokens and heads, the last
+ * dimension is contiguous; pointers are aligned to 4 elements.  Outputs are
+ * contiguous.  The calls run on the current device. */
+
+/* k and v of the tokens into their cache rows. */
+int jm_kv_q4_write(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* k, int64_t k_token,
+                   int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int dtype, void* stream);
+
+/* The values that the tokens' cache rows hold, exact in float32 and rounded to
+ * nearest even in bf16. */
+int jm_kv_q4_read(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, void* k, void* v, int dtype,
+                  void* stream);
+
+/* out [N][n_heads][128] = softmax(scale q . K) V over the rows 0 .. the token's
+ * own, which are in the cache already (jm_kv_q4_write); n_heads / n_kv is 1, 2, 4
+ * or 8.  A token whose row is below 0 sees none: its output is 0 (the one
+ * exception to the above).  Scores, weights and sums are float32.  out may be q
+ * where q is contiguous.  Workspace: as jm_q4_gemm_f32's. */
+int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
+                  int64_t q_head, int n_heads, float scale, int dtype, void* out, void* stream);
+
+/* ---- sampling ----
+ *
+ * Beside jm_decode_layers_batch_argmax; no counterpart in the native reference.
+ * out_tok[b] (int32, device) = a token of row b of logits [B][V] (dtype
+ * JM_DTYPE_F32 or JM_DTYPE_BF16, rows ld elements apart), drawn with the row's
+ * random number u[b] in [0, 1) (float32, device):
+ *   - the weight of a token is w = round(2^40 exp((l - max l) / temperature)), in
+ *     64-bit arithmetic, a whole number, so that no order of summation changes a
+ *     token;
+ *   - the tokens are ordered by logit, ties by the lower index first, and a prefix
+ *     of that order is kept: the first top_k (0 or less: all), of these those
+ *     before which less than top_p of the top_k's weight lies (1 or more: all),
+ *     of these those of w >= min_p 2^40 (0: all); the first always;
+ *   - the token is the first whose running sum passes floor(u * the kept sum).
+ * A temperature of 0 or less takes the first of the order (the argmax).  A NaN
+ * logit is treated as -infinity; -infinity has weight 0; where the largest
+ * logit is +infinity, those equal to it have the weight 2^40 and the others 0.  A
+ * row with no logit above -infinity gives token -1 (and probability 0).  u
+ * outside [0, 1) counts as the nearest in it, NaN as 0.
+ * out_p (optional, float32 [B]) receives the token's weight over the kept sum.
+ * V is at most 2^20.  Workspace: as jm_q4_gemm_f32's. */
+typedef struct jm_sampling {
+    float temperature;
+    int top_k;
+    float top_p;
+    float min_p;
+    const float* temperature_b;     /* device [B], one a row, or NULL: the scalar above */
+    const int32_t* top_k_b;
+    const float* top_p_b;
+    const float* min_p_b;
+} jm_sampling;
+
+int jm_sample(const void* logits, int dtype, int64_t ld, int B, int V, const jm_sampling* how, const float* u,
+              int32_t* out_tok, float* out_p, void* stream);
 
 #ifdef __cplusplus
 }

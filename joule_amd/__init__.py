@@ -8,6 +8,9 @@ reference's on-disk Q4 layout.
 
 Modules
   q4_store  the Q4 format (quantise / dequantise, store writer, index)
+  decoder   the decode step around the block, KV caches
+  kv_q4     4-bit KV caches: write, read, attention
+  sampling  the next token under temperature, top-k, top-p and min-p
   moe       HbmExpertStore: the store in HBM and layer_ffn_batch
   backend   KernelBackend plugin API with HipBackend (q4_gemv / q4_gemm)
   synth     seeded synthetic workloads

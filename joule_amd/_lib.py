@@ -15,6 +15,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libjoule_amd.so"
 
 JM_DTYPE_F32 = 0
 JM_DTYPE_BF16 = 1
+JM_DTYPE_Q4 = 2             # KV caches: 4-bit rows in groups of 64
+JM_DTYPE_Q4_G32 = 3         # ... of 32
 
 # Every function declared in include/joule_amd.h, with its argument types.
 _c = ctypes
@@ -61,6 +63,11 @@ SIGNATURES = {
     "jm_set_q4_gemm_min_tokens": ([_i], _i),
     "jm_get_q4_gemm_min_tokens": ([], _i),
     "jm_gemm_plan": ([_i] * 5 + [_vp], _i),
+    "jm_kv_q4_bytes": ([_i] * 3, _i64),
+    "jm_kv_q4_write": ([_vp] * 3 + [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _vp], _i),
+    "jm_kv_q4_read": ([_vp] * 3 + [_i, _vp, _vp, _i, _vp], _i),
+    "jm_kv_q4_attn": ([_vp] * 3 + [_i, _vp, _i64, _i64, _i, _c.c_float, _i, _vp, _vp], _i),
+    "jm_sample": ([_vp, _i, _i64, _i, _i] + [_vp] * 5, _i),
 }
 
 
@@ -78,6 +85,17 @@ class ExpertJob(ctypes.Structure):
     _fields_ = [("pk_g", _vp), ("sc_g", _vp), ("pk_u", _vp), ("sc_u", _vp), ("pk_d", _vp), ("sc_d", _vp),
                 ("m_gg", _i), ("d_in", _i), ("m_d", _i), ("d_m", _i), ("group", _i),
                 ("x", _vp), ("scratch", _vp), ("prob", _c.c_float)]
+
+
+class KvQ4(ctypes.Structure):
+    """jm_kv_q4: the 4-bit caches of n_seq sequences in one layer."""
+    _fields_ = [("k", _vp), ("v", _vp), ("seq_stride", _u64), ("n_seq", _i), ("maxT", _i), ("n_kv", _i), ("group", _i)]
+
+
+class Sampling(ctypes.Structure):
+    """jm_sampling: the settings of jm_sample, one for all rows or one a row."""
+    _fields_ = [("temperature", _c.c_float), ("top_k", _i), ("top_p", _c.c_float), ("min_p", _c.c_float),
+                ("temperature_b", _vp), ("top_k_b", _vp), ("top_p_b", _vp), ("min_p_b", _vp)]
 
 
 STAGES = ("route", "gateup", "down")

@@ -16,7 +16,7 @@ registry (src/jouleai/arch/registry.py:56-94 ``get_spec``):
   gate/up/down projections as the FFN weights (decoder3.py:251-280);
 * ``HipNativeDecoder`` keeps per-sequence KV caches across calls and offers
   ``decode_batch`` / ``decode_batch_argmax`` as NativeDecoder does
-  (decoder3.py:580-629).
+  (decoder3.py:580-629), and ``decode_batch_sample``.
 """
 
 from __future__ import annotations
@@ -30,6 +30,7 @@ import torch
 
 from .decoder import DecoderShape, DecoderWeights, HipDecoder, KVCacheSet
 from .dense import DenseFfnStore, dense_ffn_shape
+from .kv_q4 import Q4KVCacheSet
 from .moe import HbmExpertStore, MoEShape
 from .q4_store import BIN_NAME, INDEX_NAME, convert_experts_q4
 
@@ -186,10 +187,13 @@ class HipNativeDecoder:
     is the reference's "seq{b}"."""
 
     def __init__(self, model_dir: str | Path, max_tokens: int = 4096, converted_dir: str | Path | None = None,
-                 max_batch: int = 8, device: str | torch.device = "cuda"):
+                 max_batch: int = 8, device: str | torch.device = "cuda", kv_group: int = 0):
+        """kv_group 64 or 32: 4-bit caches in groups of that many values
+        (Q4KVCacheSet) instead of bf16 ones."""
         self.dec = load_decoder(model_dir, max_tokens, converted_dir, device=device)
         self.shape = self.dec.shape
-        self.kv = KVCacheSet(self.shape, max_batch, device=device)
+        self.kv = (Q4KVCacheSet(self.shape, max_batch, group=kv_group, device=device) if kv_group
+                   else KVCacheSet(self.shape, max_batch, device=device))
         self._seq_pos: dict[str, int] = {}
 
     def reset(self) -> None:
@@ -217,6 +221,18 @@ class HipNativeDecoder:
             self._seq_pos[f"seq{b}"] = p + 1
         lg = logits.cpu().numpy()
         return [int(lg[b].argmax()) for b in range(B)]
+
+    def decode_batch_sample(self, tokens: list[int], positions: list[int], u, temperature=1.0, top_k=0, top_p=1.0,
+                            min_p=0.0) -> list[int]:
+        """The next token per sequence, drawn with the random numbers u (one a
+        sequence, in [0, 1)); settings as sampling.sample takes them."""
+        dev = self.kv.data.device
+        out, _ = self.dec.decode_layers_batch_sample(
+            self._embed(tokens), positions, self.kv, torch.as_tensor(np.asarray(u, dtype=np.float32), device=dev),
+            temperature, top_k, top_p, min_p)
+        for b, p in enumerate(positions):
+            self._seq_pos[f"seq{b}"] = p + 1
+        return [int(v) for v in out.cpu().tolist()]
 
     def prefill(self, tokens: list[int]) -> np.ndarray:
         """NativeDecoder.prefill (decoder3.py:490-509): one prompt into seq0's

@@ -39,15 +39,10 @@ int hip_fail(hipError_t e, const char* what) {
 
 namespace {
 
-// Workspace of the plugin products (jm_q4_gemm_f32 / jm_q4_gemv_f32): one
-// buffer per (device, stream), the policy of jm_plugin_ws.h (reuse, grow
-// with the old buffer retired, or a stream-ordered allocation under
-// capture, freed after the call).
-struct PluginWs {
-    void* p = nullptr;
-    bool async = false;
-};
-
+// Workspace of the calls without a store (the plugin products, the 4-bit
+// cache's attention, sampling): one buffer per (device, stream), the policy of
+// jm_plugin_ws.h (reuse, grow with the old buffer retired, or a stream-ordered
+// allocation under capture, freed after the call).
 struct PluginBuf {
     int dev;
     hipStream_t st;
@@ -58,6 +53,10 @@ struct PluginBuf {
 std::mutex g_pws_mu;
 std::vector<PluginBuf> g_pws;
 std::vector<void*> g_pws_retired;           // replaced buffers, kept until the process ends
+
+}  // namespace
+
+namespace jm {
 
 int plugin_ws(hipStream_t st, size_t bytes, PluginWs* out) {
     int dev = 0;
@@ -92,6 +91,10 @@ int plugin_ws(hipStream_t st, size_t bytes, PluginWs* out) {
     out->p = p;
     return 0;
 }
+
+}  // namespace jm
+
+namespace {
 
 // token count from which jm_q4_gemm_f32 takes the matrix cores
 std::atomic<int> g_q4_gemm_min_t{JM_Q4_GEMM_MIN_T};
@@ -797,8 +800,8 @@ int jm_q4_gemm_f32(float* out, const float* X, int T, const uint8_t* packed, con
     const size_t dig_bytes = align256((size_t)T * ng * JM_NDIG * (group / 8) * 4);
     const size_t sc_bytes = align256((size_t)T * ng * 4);
     const size_t need = mfma ? jm::q4_gemm_mfma_ws(T, m, d, group) : dig_bytes + sc_bytes;
-    PluginWs ws;
-    if (int rc = plugin_ws(st, need, &ws)) return rc;
+    jm::PluginWs ws;
+    if (int rc = jm::plugin_ws(st, need, &ws)) return rc;
     hipError_t e;
     if (mfma) {
         e = jm::launch_q4_gemm_mfma(packed, scales, X, T, m, d, group, ws.p, out, st);
@@ -899,8 +902,8 @@ int jm_expert_job(const jm_expert_job_t* j, void* stream) {
     const size_t dx = align256((size_t)(d / G) * JM_NDIG * (G / 8) * 4), sx = align256((size_t)(d / G) * 4);
     const size_t gu = align256((size_t)2 * m * 4);
     const size_t da = align256((size_t)(m / G) * JM_NDIG * (G / 8) * 4), sa = align256((size_t)(m / G) * 4);
-    PluginWs ws;
-    if (int rc = plugin_ws(st, dx + sx + gu + da + sa, &ws)) return rc;
+    jm::PluginWs ws;
+    if (int rc = jm::plugin_ws(st, dx + sx + gu + da + sa, &ws)) return rc;
     char* p = (char*)ws.p;
     uint32_t* dig_x = (uint32_t*)p;
     float* sc_x = (float*)(p + dx);

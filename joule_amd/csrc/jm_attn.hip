@@ -28,6 +28,7 @@
 // every query head of that KV head.
 #include "jm_device.h"
 #include "jm_kernels.h"
+#include "jm_q4kv.h"
 
 namespace jm {
 
@@ -848,6 +849,36 @@ k_kv_append(AttnArgs a) {
     else kv_store(k, a, b, kh, pos, threadIdx.x, (gptr<uint16_t>)kvp[0], (gptr<uint16_t>)kvp[1], nullptr);
 }
 
+// The same for 4-bit caches, always ahead of the attention (jm_kvq4.hip): wave 0
+// of block (KV head, token) encodes the token's k and v rows into its planes,
+// the other waves finish the KV head's query heads, two per wave, into q
+// [token][head][128].
+template <int NG>
+__global__ void __launch_bounds__(320)
+k_kv_append_q4(AttnArgs a, Q4KvArgs c, float* __restrict__ q) {
+    constexpr int HD = 128;
+    const int kh = blockIdx.x, b = blockIdx.y;
+    const int pos = a.pos[b], j = threadIdx.x & 31;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (w > 0) {
+        const int qpk = a.H / a.KH, i = (threadIdx.x >> 5) - 2;
+        const int head = kh * qpk + (i < qpk ? i : 0), row = head * HD + 4 * j;
+        Fin4 f;
+        fin4_load(f, a, b, row, a.bq, row, qk_weight(a, true, head), true, pos, j);
+        float v[4];
+        fin4_value(v, f, a, b, row, a.qn ? a.qk_norm : 0, true, j);
+        if (i < qpk) *(float4*)(q + ((size_t)b * a.H + head) * HD + 4 * j) = make_float4(v[0], v[1], v[2], v[3]);
+        return;
+    }
+    const int lane = threadIdx.x;
+    KvFin k;
+    kv_load(k, a, b, kh, pos, lane);
+    float v[4];
+    fin4_value(v, k.f, a, b, k.row, k.isk && a.kn ? a.qk_norm : 0, k.isk, j);
+    const Q4Head<NG> h(q4_plane(c, b, k.isk ? 0 : 1), kh, c.KH, c.R);
+    q4_store_row<NG>(v, k.isk, pos, j, h);
+}
+
 // The 4 waves' partial outputs of a split block (wave w's at red + w *
 // wstride, [QPK][128]) merged with the split's max (the flash-decoding
 // merge within the block) into part_o / part_ml:
@@ -1616,6 +1647,18 @@ hipError_t launch_attn(const AttnArgs& a, int qpk, float* att, hipStream_t st) {
     }
     const bool tile = !a.append && a.shared && !a.kv_f32 && attn_tile_takes(a.B, a.KH, qpk);
     if (qpk != 1 && qpk != 2 && qpk != 4 && qpk != 8) return hipErrorInvalidValue;
+    if (a.kv_group) {
+        // the query heads go to att, where the attention replaces them by its output
+        Q4KvArgs c{};
+        c.n_seq = c.N = a.B; c.maxT = a.maxT; c.KH = a.KH; c.group = a.kv_group; c.R = q4_plane_rows(a.maxT);
+        c.tab = a.kv; c.pos = a.pos; c.L = a.L; c.layer = a.layer;
+        const dim3 ga((unsigned)a.KH, (unsigned)a.B), gb(64 * (1 + (qpk + 1) / 2));
+        if (a.kv_group == 64) hipLaunchKernelGGL(k_kv_append_q4<2>, ga, gb, 0, st, a, c, att);
+        else hipLaunchKernelGGL(k_kv_append_q4<4>, ga, gb, 0, st, a, c, att);
+        hipError_t e0 = hipGetLastError();
+        if (e0 != hipSuccess) return e0;
+        return launch_q4_attn(c, att, false, (long long)a.H * 128, 128, a.H, a.rsdiv, att, st);
+    }
     if (!a.append) {
         // (the partial outputs' buffer, unused by k_attn_tile, holds the query heads for it)
         AttnArgs ap = a;

@@ -210,7 +210,7 @@ int enqueue_step(jm_store* s, const jm_kernel_cfg* c, const jm_kernel_w* W, cons
         at.qkss = s->qkss;
         at.eps = c->eps; at.rsdiv = 1.0f / sdiv;
         at.cos = W->cos; at.sin = W->sin;
-        at.pos = pos_dev; at.kv = s->tab; at.kv_f32 = s->kv_f32; at.L = L; at.layer = l;
+        at.pos = pos_dev; at.kv = s->tab; at.kv_f32 = s->kv_f32; at.kv_group = s->kv_group; at.maxT = c->maxT; at.L = L; at.layer = l;
         at.S = S; at.part_o = s->part_o; at.part_ml = s->part_ml;
         at.append = append ? 1 : 0;
         at.shared = shared ? 1 : 0;
@@ -424,6 +424,7 @@ int decode_impl(jm_store* s, const jm_kernel_cfg* c, const jm_kernel_w* W, const
         key.append = append ? 1 : 0;
         key.shared = shared ? 1 : 0;
         key.kv_f32 = s->kv_f32;
+        key.kv_group = s->kv_group;
         if (!s->gexec || memcmp(&key, &s->gkey, sizeof key) != 0) {
             if (s->gexec) {
                 JM_HIP(hipStreamSynchronize(st), "hipStreamSynchronize before recapture");
@@ -601,9 +602,10 @@ int jm_store_set_dense_ffn(jm_store* s, const uint16_t* w1, const uint16_t* w2, 
 
 int jm_store_set_kv_dtype(jm_store* s, int dtype) {
     if (!s) return fail(JM_ERR_ARG, "store is NULL");
-    if (dtype != JM_DTYPE_BF16 && dtype != JM_DTYPE_F32)
-        return fail(JM_ERR_ARG, "dtype must be JM_DTYPE_BF16 or JM_DTYPE_F32 (got %d)", dtype);
+    if (dtype != JM_DTYPE_BF16 && dtype != JM_DTYPE_F32 && dtype != JM_DTYPE_Q4 && dtype != JM_DTYPE_Q4_G32)
+        return fail(JM_ERR_ARG, "dtype must be JM_DTYPE_BF16, JM_DTYPE_F32, JM_DTYPE_Q4 or JM_DTYPE_Q4_G32 (got %d)", dtype);
     s->kv_f32 = dtype == JM_DTYPE_F32 ? 1 : 0;
+    s->kv_group = dtype == JM_DTYPE_Q4 ? 64 : dtype == JM_DTYPE_Q4_G32 ? 32 : 0;
     return 0;
 }
 

@@ -255,6 +255,8 @@ struct AttnArgs {
     const int* pos;           // [B] position each token writes (T = pos + 1)
     const unsigned long long* kv;   // [B*L][2] k, v caches [maxT][KH][128], bf16 or (kv_f32) float32
     int kv_f32;               // 1: the caches hold float32 (the reference's KVCache), 0: bf16
+    int kv_group;             // 4-bit caches: their group, 64 or 32; 0: as kv_f32 says
+    int maxT;                 // rows of a cache (4-bit planes are laid out by it)
     int L, layer;
     int append;               // 1: every token has its own cache; the attention appends its k and v
                               // rows itself.  0: k_kv_append appends every row first
@@ -332,6 +334,55 @@ hipError_t launch_sum_slices(const float* resid, const float* part, int ns, int 
                              hipStream_t st);
 hipError_t launch_rms_rows(const float* x, const uint16_t* w, int B, int d, float eps, float* out,
                            hipStream_t st);
+
+// ---- the 4-bit KV cache (jm_kvq4.hip; jm_q4kv.h has the planes' layout)
+
+// rows of a plane: maxT rounded up to 64, so that no tile of rows leaves it
+constexpr int q4_plane_rows(int maxT) { return (maxT + 63) / 64 * 64; }
+struct Q4KvArgs {
+    void* k;                  // planes of sequence 0; sequence s at + s * seq_stride bytes
+    void* v;
+    unsigned long long seq_stride;
+    int n_seq, maxT, KH, group;
+    int R;                    // rows a plane holds, q4_plane_rows(maxT)
+    const int* start;         // [n_seq] cache row of each sequence's first token of the call
+    const int* cu;            // [n_seq + 1] its first token's index (cu[n_seq]: the end), or NULL: token t is
+                              // sequence t's only one
+    int N;                    // tokens of the call
+    // the decoder's form instead (pos non-NULL): token t at row pos[t] of the
+    // planes tab[(t * L + layer) * 2], + 1
+    const unsigned long long* tab;
+    const int* pos;
+    int L, layer;
+};
+// k, v [N][KH][128] (bf16 or float32; strides of token and head: k, v in turn) into the cache
+hipError_t launch_q4_write(const Q4KvArgs& c, const void* k, const void* v, bool bf, const long long (&strides)[4],
+                           hipStream_t st);
+// the same rows back, k, v [N][KH][128]
+hipError_t launch_q4_read(const Q4KvArgs& c, void* k, void* v, bool bf, hipStream_t st);
+// out [N][H][128] = attention of q [N][H][128] over rows 0 .. the token's own
+hipError_t launch_q4_attn(const Q4KvArgs& c, const void* q, bool bf, long long qts, long long qhs, int H, float scale,
+                          void* out, hipStream_t st);
+
+// ---- sampling (jm_sample.hip)
+#define JM_SAMPLE_MAX_V (1 << 20)
+struct SampleArgs {
+    const void* logits;       // [B][V], rows ld elements apart
+    int bf;                   // bf16 (else float32)
+    long long ld;
+    int B, V;
+    float temperature;        // the settings of every row, or one a row [B]
+    int top_k;
+    float top_p, min_p;
+    const float* temperature_b;
+    const int* top_k_b;
+    const float* top_p_b;
+    const float* min_p_b;
+    const float* u;           // [B]
+    int* out_tok;             // [B]
+    float* out_p;             // [B] or NULL
+};
+hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
 
 hipError_t launch_dequant(const uint8_t* packed, const uint16_t* scales, long long numel, int group,
                           float* out, hipStream_t st);

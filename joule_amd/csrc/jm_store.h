@@ -63,6 +63,7 @@ struct DecKey {
     int lm_V;
     int nl;                     // layers the step runs (jm_store_set_max_layers)
     int kv_f32;                 // element type of the caches (jm_store_set_kv_dtype)
+    int kv_group;
     int dense_min;
     int ndig;
     int append;                 // the attention appends the k and v rows itself (no cache shared by two tokens)
@@ -116,6 +117,7 @@ struct jm_store {
     float* ddn;
     const uint16_t* dw[3];      // a dense store's FFN weights for jm_layer_ffn_batch (jm_store_set_dense_ffn)
     int kv_f32;                 // the caches the decoder reads and writes hold float32 (else bf16)
+    int kv_group;               // ... 4-bit rows in groups of 64 or 32 (0: as kv_f32 says)
     unsigned long long* tab;    // [B*L][2] KV pointers, then [B] positions (device)
     unsigned long long* tab_host;   // pinned staging of tab
     size_t tab_cap;             // bytes of tab / tab_host
@@ -138,6 +140,15 @@ namespace jm {
 // Record a message for jm_last_error() (per calling thread) and return code.
 int fail(int code, const char* fmt, ...);
 int hip_fail(hipError_t e, const char* what);
+
+// Workspace of `bytes` for one call's kernels on st, on the current device
+// (jm_plugin_ws.h has the policy); async: free it with hipFreeAsync(p, st)
+// once they are enqueued.
+struct PluginWs {
+    void* p = nullptr;
+    bool async = false;
+};
+int plugin_ws(hipStream_t st, size_t bytes, PluginWs* out);
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }

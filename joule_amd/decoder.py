@@ -9,7 +9,8 @@ Host-side mirror of the reference's native decoder surface
 * ``rope_tables`` builds the cos/sin tables as ``NativeDecoder._rope_tables``
   does (rotate-half layout, ``emb = cat(freqs, freqs)``);
 * ``KVCacheSet`` holds the bf16 caches of B sequences x L layers and the
-  ``KVCache[B*L]`` array (entry b*L + l) the call takes;
+  ``KVCache[B*L]`` array (entry b*L + l) the call takes (``Q4KVCacheSet`` in
+  kv_q4.py: 4-bit ones, taken wherever a KVCacheSet is);
 * ``HipDecoder.decode_layers_batch(x, positions, kv)`` runs every layer
   (attention, then the store's MoE block) and returns the final-normed hidden
   state [B, d].  The lm_head is applied by the caller.
@@ -19,6 +20,7 @@ The arithmetic is in libjoule_amd.so; PyTorch holds device memory.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -286,7 +288,14 @@ class HipDecoder:
 
     def _kv_dtype(self, kv: KVCacheSet) -> None:
         """The store reads and appends caches of kv's element type."""
-        dt = _lib.JM_DTYPE_F32 if kv.data.dtype == torch.float32 else _lib.JM_DTYPE_BF16
+        if kv.data.dtype == torch.uint8:
+            # 4-bit planes are laid out by the row count and the KV heads
+            if kv.shape.maxT != self.shape.maxT or kv.shape.n_kv != self.shape.n_kv or \
+                    kv.shape.n_layers != self.shape.n_layers:
+                raise ValueError("the 4-bit caches were made for another shape")
+            dt = _lib.JM_DTYPE_Q4 if kv.group == 64 else _lib.JM_DTYPE_Q4_G32
+        else:
+            dt = _lib.JM_DTYPE_F32 if kv.data.dtype == torch.float32 else _lib.JM_DTYPE_BF16
         if getattr(self, "_kvdt", None) != dt:
             _lib.check(_lib.lib().jm_store_set_kv_dtype(self.store._h, dt), "jm_store_set_kv_dtype")
             self._kvdt = dt
@@ -349,6 +358,18 @@ class HipDecoder:
             pos.ctypes.data_as(ctypes.c_void_p), _lib.ptr(x), B, _lib.ptr(out_tok), None,
             _lib.stream_handle(stream)), "jm_decode_layers_batch_argmax")
         return out_tok
+
+    def decode_layers_batch_sample(self, x: torch.Tensor, positions, kv: KVCacheSet, u: torch.Tensor,
+                                   temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                                   out_tok: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The step of decode_layers_batch, then (tokens int32 [B],
+        probabilities [B]) drawn from its logits with the random numbers u [B]
+        (sampling.sample, which says what the settings mean)."""
+        from .sampling import sample
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            logits = torch.empty((x.shape[0], self.shape.V), dtype=torch.float32, device=x.device)
+            self.decode_layers_batch(x, positions, kv, logits=logits)
+            return sample(logits, u, temperature, top_k, top_p, min_p, out_tok=out_tok)
 
     def embed(self, tokens: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """out [B, d] float32 = bf16 embedding rows of tokens [B] (int32, CUDA),
