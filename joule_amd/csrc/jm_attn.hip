@@ -1657,7 +1657,10 @@ hipError_t launch_attn(const AttnArgs& a, int qpk, float* att, hipStream_t st) {
         else hipLaunchKernelGGL(k_kv_append_q4<4>, ga, gb, 0, st, a, c, att);
         hipError_t e0 = hipGetLastError();
         if (e0 != hipSuccess) return e0;
-        return launch_q4_attn(c, att, false, (long long)a.H * 128, 128, a.H, a.rsdiv, att, st);
+        // (the partial outputs' buffers hold a.S ranges, one per 128 rows of the longest prefix)
+        Q4AttnPlan p = q4_attn_plan(c, a.H);
+        p.S = p.S < a.S ? p.S : a.S;
+        return launch_q4_attn(c, p, att, false, (long long)a.H * 128, 128, a.H, a.rsdiv, att, a.part_o, a.part_ml, st);
     }
     if (!a.append) {
         // (the partial outputs' buffer, unused by k_attn_tile, holds the query heads for it)

@@ -95,8 +95,17 @@ int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
     if (a.N == 0) return 0;
     if (int rc = q4_tensor("q", q, dtype, q_token, q_head)) return rc;
     if (int rc = q4_tensor("out", out, dtype, 0, 0)) return rc;
-    JM_HIP(jm::launch_q4_attn(a, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, (hipStream_t)stream),
-           "4-bit attention launch");
+    hipStream_t st = (hipStream_t)stream;
+    const jm::Q4AttnPlan p = jm::q4_attn_plan(a, n_heads);
+    jm::PluginWs ws;
+    if (p.o_floats)
+        if (int rc = jm::plugin_ws(st, (p.o_floats + p.ml_floats) * 4, &ws)) return rc;
+    float* part = (float*)ws.p;
+    const hipError_t e = jm::launch_q4_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part,
+                                            part + p.o_floats, st);
+    const hipError_t f = ws.async ? hipFreeAsync(ws.p, st) : hipSuccess;
+    if (e != hipSuccess) return jm::hip_fail(e, "4-bit attention launch");
+    if (f != hipSuccess) return jm::hip_fail(f, "hipFreeAsync");
     return 0;
 }
 
