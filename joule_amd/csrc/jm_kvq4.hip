@@ -84,13 +84,11 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 // waves and k_q4_merge the ranges.  No cache byte goes through LDS: rows come in
 // the order in which the matrix cores take them (jm_q4kv.h).
 //
-// Operands.  A code is a 16-bit float as it stands: the bits 0 .. 15 are the
-// subnormals 0 .. 15 x 2^-24, the bits 16 x the same (up to 240) 16 times
-// those, and products with subnormals are exact in the matrix cores' float32
-// sums.  One AND gives two codes, from nibbles 0 and 4 of a dword (or 1 and 5,
-// 16 times too large, which the other operand or the end takes back).  The 8
-// that the format subtracts is taken off per group: K's as the accumulator's
-// start, -8 sum(q); V's from one more product, with a constant operand.
+// Operands.  One AND-OR gives two codes as fp16, 1024 + q from nibbles 0 and 4
+// of a dword, or 1024 + 16 q from 1 and 5, and one packed subtraction q - 8, or 16
+// times that (which the other operand or the end takes back), exactly.  (The
+// codes' bits as subnormals, without either, came out of the matrix cores right
+// to only 2^-14 of a sum: 7e-5 of the output instead of 5e-7.)
 //
 //   scores   v_mfma_f32_16x16x32_f16, 16 cache rows as A, the 8 query rows as B
 //            in columns n < 8, q brought to [1, 2) by a power of two and rounded
@@ -115,6 +113,16 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(f16x8, make_uint4(a, b, c, d));
+}
+
+// The codes less 8 of nibbles 0 and 4 of w, and 16 times those of nibbles 1 and 5.
+__device__ __forceinline__ uint32_t q4_even(uint32_t w) {
+    const f16x2 h = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
+    return __builtin_bit_cast(uint32_t, h);
+}
+__device__ __forceinline__ uint32_t q4_odd(uint32_t w) {
+    const f16x2 h = __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(uint32_t, h);
 }
 
 __device__ __forceinline__ float pow2f(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -247,7 +255,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     // the query columns: dimensions 32 st + 8 g + e, pairs (e, e + 4)
     const bool lo_col = !BF && n >= 8;
     f16x8 qb[4];
-    float qinit[NG], lf;
+    float lf;
     {
         float x[4][8];
         float top = 0.0f;
@@ -271,9 +279,8 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
         // the power of two below the column's largest value
         const uint32_t ex = min(max(__float_as_uint(top) >> 23, 2u), 252u);
         const float f = __uint_as_float((254u - ex) << 23);
-        // 2^24 of the codes, the halves' factor, q's power of two and the scale
-        lf = __fmul_rn(__fmul_rn(__uint_as_float(ex << 23), a.scale2), lo_col ? 16777216.0f / Q4_LO : 16777216.0f);
-        float sum[NG] = {};
+        // q's power of two, the scale and the halves' factor
+        lf = __fmul_rn(__fmul_rn(__uint_as_float(ex << 23), a.scale2), lo_col ? 1.0f / Q4_LO : 1.0f);
 #pragma unroll
         for (int st = 0; st < 4; st++) {
             uint32_t b[4];
@@ -282,25 +289,16 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
                 uint32_t hi, lo;
                 split_f16x2(__fmul_rn(x[st][e], f), __fmul_rn(x[st][e + 4], f), hi, lo);
                 const f16x2 h = __builtin_bit_cast(f16x2, lo_col ? lo : hi);
-                sum[st / GS] += (float)h[0] + (float)h[1];
                 // codes of nibbles 1, 3, 5 and 7 come 16 times too large
                 b[e] = __builtin_bit_cast(uint32_t, e & 1 ? h * (_Float16)0.0625f : h);
             }
             qb[st] = as_f16x8(b[0], b[1], b[2], b[3]);
         }
-#pragma unroll
-        for (int e = 0; e < NG; e++) {
-            sum[e] += swz_xor16_f(sum[e]);
-            sum[e] += __shfl_xor(sum[e], 32, JM_WAVE);
-            qinit[e] = sum[e] * (-8.0f / 16777216.0f);
-        }
     }
 
-    f32x4 O[8], osum[NG];
+    f32x4 O[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) O[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < NG; e++) osum[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float ref = -INFINITY, l = 0.0f;
 
     for (; t < t_end; t += 4) {
@@ -312,12 +310,12 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             f32x4 S = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < NG; e++) {
-                f32x4 acc = f32x4{qinit[e], qinit[e], qinit[e], qinit[e]};
+                f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int st = e * GS; st < (e + 1) * GS; st++) {
                     const uint32_t d = cur.k[rt][st], d8 = d >> 8;
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        as_f16x8(d & 0x000F000Fu, d & 0x00F000F0u, d8 & 0x000F000Fu, d8 & 0x00F000F0u), qb[st], acc, 0, 0, 0);
+                        as_f16x8(q4_even(d), q4_odd(d), q4_even(d8), q4_odd(d8)), qb[st], acc, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[i] = __builtin_fmaf(q4_scale(cur.ks, rt, i, e), acc[i], S[i]);
@@ -360,8 +358,6 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             l *= f;
 #pragma unroll
             for (int j = 0; j < 8; j++) O[j] *= f;
-#pragma unroll
-            for (int e = 0; e < NG; e++) osum[e] *= f;
             ref = nref;
         }
         const float r0 = ref == -INFINITY ? 0.0f : ref;     // (a column that has seen nothing yet)
@@ -403,17 +399,13 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             for (int b8 = 0; b8 < 2; b8++) {
                 const int j = 4 * h + 2 * b8, e = 16 * j / (HD / NG);
                 O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    as_f16x8(v[0] & 0x000F000Fu, v[1] & 0x000F000Fu, v[2] & 0x000F000Fu, v[3] & 0x000F000Fu), pb[e], O[j], 0, 0, 0);
+                    as_f16x8(q4_even(v[0]), q4_even(v[1]), q4_even(v[2]), q4_even(v[3])), pb[e], O[j], 0, 0, 0);
                 O[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    as_f16x8(v[0] & 0x00F000F0u, v[1] & 0x00F000F0u, v[2] & 0x00F000F0u, v[3] & 0x00F000F0u), pb[e], O[j + 1], 0, 0, 0);
+                    as_f16x8(q4_odd(v[0]), q4_odd(v[1]), q4_odd(v[2]), q4_odd(v[3])), pb[e], O[j + 1], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[i] >>= 8;
             }
         }
-#pragma unroll
-        for (int e = 0; e < NG; e++)
-            osum[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u),
-                                                             pb[e], osum[e], 0, 0, 0);
         cur = nxt;
     }
 
@@ -425,9 +417,8 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
         float o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float v = (j & 1 ? O[j][i] * 0.0625f : O[j][i]) - osum[16 * j / (HD / NG)][i];
+            const float v = O[j][i] * (j & 1 ? 0.0625f : 1.0f);
             o[i] = BF ? v : __builtin_fmaf(dpp_f<DPP_ROR8>(v), 1.0f / Q4_LO, v);
-            o[i] *= 16777216.0f;
         }
         if (n < 8) *(float4*)&ow[w][n][16 * j + 4 * g] = make_float4(o[0], o[1], o[2], o[3]);
     }
