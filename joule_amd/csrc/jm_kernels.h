@@ -389,7 +389,8 @@ struct SampleArgs {
     int* out_tok;             // [B]
     float* out_p;             // [B] or NULL
 };
-hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
+size_t sample_ws_bytes(int B, int V);
+hipError_t launch_sample(const SampleArgs& a, void* ws, hipStream_t st);
 
 hipError_t launch_dequant(const uint8_t* packed, const uint16_t* scales, long long numel, int group,
                           float* out, hipStream_t st);

@@ -5,13 +5,78 @@
 // index ascending), so that the kept set is the shortest of three prefixes and
 // all that is ever needed is "the weight of the first n tokens" and "the token
 // at which the running weight passes x".  With whole-number weights
-// w = round(2^40 exp((l - max) / T)) both are exact in any order of summation.
+// w = round(2^40 exp((l - max) / T)) both are exact in any order of summation,
+// so no sort of the vocabulary is needed, only histograms:
+//
+//   k_sample_max     each row's maximum, by chunks
+//   k_sample_hist    counts and weights of SM_BINS equal steps of (max - l) / T,
+//                    by chunks; the row's last chunk adds them up and marks the
+//                    few bins in which a border (of top-k, top-p, min-p or the
+//                    draw itself) can lie
+//   k_sample_pick    the tokens of the marked bins, listed; the row's last chunk
+//                    sorts the list, finds the borders in it one after the other
+//                    and the token
+//
+// A row whose marked bins hold more than SM_CAP tokens (many equal logits, a
+// very high temperature) is selected by its keys instead, in the last kernel.
+//
+// Bound: the logits are read three times, the first time from memory, and 20
+// float64 operations a token in the histogram; a row takes three launches and
+// two hand-overs between its chunks however short it is.
+#include <algorithm>
+
 #include "jm_device.h"
 #include "jm_kernels.h"
 
 namespace jm {
 
 constexpr unsigned long long SM_ONE = 1ull << 40;      // the largest logit's weight
+constexpr int SM_T = 1024;                             // threads a block
+constexpr int SM_BINS = 1024;
+constexpr int SM_CAP = 4096;                           // tokens a row's list holds
+// past this (max - l) / T a weight is 0: 41 ln 2, and a bin more for rounding
+constexpr float SM_SPAN = 28.45f;
+
+// What the histogram's last chunk leaves for the row.
+struct SmPlan {
+    uint32_t mark[SM_BINS / 32];
+    unsigned long long m1;      // the weight that top-k keeps, where no bin splits it
+    int kbin;                   // 1: it lies in a marked bin
+    int mbin;                   // min-p: the first of the marked bins around its border
+    unsigned long long m3_before;   // the weight before that bin
+    int n;                      // tokens in the marked bins; -1: a row with nothing to draw
+};
+
+// A row's part of the workspace.
+struct SmRow {
+    unsigned* ticket;           // [2] chunks done of the two kernels that hand over; [2]: the list's length
+    float* cmax;                // [SP]
+    SmPlan* plan;
+    unsigned long long* umass;  // [SM_BINS] weight of the unmarked bins before a bin
+    unsigned* ucnt;             // [SM_BINS]
+    unsigned long long* hmass;  // [SP][SM_BINS]
+    unsigned* hcnt;
+    ulonglong2* list;           // [SM_CAP] key, weight
+};
+
+__host__ __device__ __forceinline__ size_t sm_row_bytes(int SP) {
+    return 16 + ((size_t)SP * 4 + 15) / 16 * 16 + (sizeof(SmPlan) + 15) / 16 * 16 + (size_t)SM_BINS * 12 * (1 + SP) +
+           (size_t)SM_CAP * 16;
+}
+
+__device__ __forceinline__ SmRow sm_row(char* ws, int b, int SP) {
+    SmRow r;
+    char* p = ws + (size_t)b * sm_row_bytes(SP);
+    r.ticket = (unsigned*)p; p += 16;
+    r.cmax = (float*)p; p += ((size_t)SP * 4 + 15) / 16 * 16;
+    r.plan = (SmPlan*)p; p += (sizeof(SmPlan) + 15) / 16 * 16;
+    r.list = (ulonglong2*)p; p += (size_t)SM_CAP * 16;
+    r.umass = (unsigned long long*)p; p += (size_t)SM_BINS * 8;
+    r.hmass = (unsigned long long*)p; p += (size_t)SM_BINS * 8 * SP;
+    r.ucnt = (unsigned*)p; p += (size_t)SM_BINS * 4;
+    r.hcnt = (unsigned*)p;
+    return r;
+}
 
 // The order of the logits as unsigned integers (larger first): NaN below
 // everything, -0 as +0.
@@ -21,131 +86,543 @@ __device__ __forceinline__ uint32_t sm_key(float l) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ unsigned long long sm_weight(float l, float mx, double inv_t) {
-    if (l == mx) return SM_ONE;
-    if (!(l > -INFINITY)) return 0;
-    return (unsigned long long)rint(exp(((double)l - (double)mx) * inv_t) * (double)SM_ONE);
+__device__ __forceinline__ float sm_unkey(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+__device__ __forceinline__ unsigned long long sm_key64(float l, int i) {
+    return ((unsigned long long)sm_key(l) << 32) | (uint32_t)~i;
+}
+
+// round(2^40 2^t) for t <= 0: 2^f by its series on |f| <= 1/2 (the first term
+// left out is below 2^-52), rounded to a whole number by adding 2^52.
+__device__ __forceinline__ unsigned long long sm_exp2(double t) {
+    const double k = rint(t), f = t - k;
+    double p = 2.5678435993488196e-11;
+    p = __builtin_fma(f, p, 4.4455382718708101e-10);
+    p = __builtin_fma(f, p, 7.0549116208011209e-09);
+    p = __builtin_fma(f, p, 1.0178086009239696e-07);
+    p = __builtin_fma(f, p, 1.3215486790144305e-06);
+    p = __builtin_fma(f, p, 1.5252733804059838e-05);
+    p = __builtin_fma(f, p, 0.00015403530393381606);
+    p = __builtin_fma(f, p, 0.0013333558146428441);
+    p = __builtin_fma(f, p, 0.0096181291076284769);
+    p = __builtin_fma(f, p, 0.055504108664821576);
+    p = __builtin_fma(f, p, 0.24022650695910069);
+    p = __builtin_fma(f, p, 0.69314718055994529);
+    p = __builtin_fma(f, p, 1.0);
+    p = ldexp(p, (int)k + 40) + 4503599627370496.0;
+    return (unsigned long long)__double_as_longlong(p) & ((1ull << 52) - 1);
+}
+
+// A row's settings.
+struct SmHow {
+    float mx;                   // the largest logit
+    double c;                   // log2(e) / T
+    float cb;                   // bins a logit
+    int k;                      // 0: all
+    float p, mp, u;
+};
+
+__device__ __forceinline__ void sm_how(SmHow& h, const SampleArgs& a, int b) {
+    float T = a.temperature_b ? a.temperature_b[b] : a.temperature;
+    h.k = a.top_k_b ? a.top_k_b[b] : a.top_k;
+    h.p = a.top_p_b ? a.top_p_b[b] : a.top_p;
+    h.mp = a.min_p_b ? a.min_p_b[b] : a.min_p;
+    h.u = a.u[b];
+    if (!(T > 0.0f)) { T = 1.0f; h.k = 1; }
+    h.c = 1.4426950408889634 / (double)T;
+    h.cb = fminf((float)(SM_BINS / (double)SM_SPAN / (double)T), 3.0e38f);
+}
+
+__device__ __forceinline__ unsigned long long sm_weight(const SmHow& h, float l) {
+    if (l == h.mx) return SM_ONE;
+    const double t = ((double)l - (double)h.mx) * h.c;
+    return t >= -41.5 ? sm_exp2(t) : 0ull;             // (NaN: 0)
+}
+
+// The bin of a logit: monotone in l, each step being so.
+__device__ __forceinline__ int sm_bin(const SmHow& h, float l) {
+    if (l == h.mx) return 0;
+    return (int)fminf(__fmul_rn(__fsub_rn(h.mx, l), h.cb), (float)(SM_BINS - 1));
 }
 
 __device__ __forceinline__ float sm_logit(const SampleArgs& a, size_t row, int i) {
     return a.bf ? bf16_bits_to_f32(((const uint16_t*)a.logits)[row + i]) : ((const float*)a.logits)[row + i];
 }
 
-// One block per row.  A selection walks down the 64-bit keys (logit order, then
-// the index from the top) 8 bits at a time: a histogram of the elements that
-// share the prefix found so far, then the digit at which the running sum
-// passes the target.
-__global__ void __launch_bounds__(1024)
-k_sample_row(SampleArgs a) {
-    __shared__ unsigned long long hist[256], sh[20];
-    __shared__ float smax[16];
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const size_t row = (size_t)b * a.ld;
-    float T = a.temperature_b ? a.temperature_b[b] : a.temperature;
-    int k = a.top_k_b ? a.top_k_b[b] : a.top_k;
-    const float p = a.top_p_b ? a.top_p_b[b] : a.top_p, mp = a.min_p_b ? a.min_p_b[b] : a.min_p;
-    if (!(T > 0.0f)) { T = 1.0f; k = 1; }
-    const double inv_t = 1.0 / (double)T;
+__device__ __forceinline__ float sm_row_max(const SmRow& r, int SP) {
     float mx = -INFINITY;
-    for (int i = tid; i < a.V; i += 1024) mx = fmaxf(mx, sm_logit(a, row, i));
-    mx = seg_max<64>(mx);
-    if ((tid & 63) == 0) smax[tid >> 6] = mx;
+    for (int i = threadIdx.x & 63; i < SP; i += 64) mx = fmaxf(mx, r.cmax[i]);
+    return seg_max<64>(mx);
+}
+
+// Whether this block is the last of the row's to come here; what the others
+// wrote before is then visible to all of its threads.
+__device__ __forceinline__ bool sm_last(unsigned* ticket, int SP, unsigned* flag) {
+    __threadfence();
     __syncthreads();
-    for (int i = 0; i < 16; i++) mx = fmaxf(mx, smax[i]);
-    if (mx == -INFINITY) {
-        if (tid == 0) {
+    if (threadIdx.x == 0) *flag = atomicAdd(ticket, 1u) == (unsigned)SP - 1;
+    __syncthreads();
+    const bool last = *flag;
+    if (last) __threadfence();
+    return last;
+}
+
+__global__ void __launch_bounds__(SM_T)
+k_sample_max(SampleArgs a, char* ws, int SP, int chunk) {
+    __shared__ float red[SM_T / 64];
+    const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x;
+    const size_t row = (size_t)b * a.ld;
+    const int i1 = min((s + 1) * chunk, a.V);
+    float mx = -INFINITY;
+    for (int i0 = s * chunk + tid; i0 < i1; i0 += 8 * SM_T) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, v[e]);
+    }
+    mx = seg_max<64>(mx);
+    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    __syncthreads();
+    const SmRow r = sm_row(ws, b, SP);
+    if (tid == 0) {
+        for (int i = 1; i < SM_T / 64; i++) mx = fmaxf(mx, red[i]);
+        r.cmax[s] = mx;
+    }
+    if (s == 0 && tid < 3) r.ticket[tid] = 0;
+}
+
+// The first bin whose running weight in incl[] satisfies pass (monotone), by
+// the whole block: out receives it (SM_BINS - 1 if there is none).
+template <typename F>
+__device__ __forceinline__ int sm_find(F pass, int* out) {
+    __syncthreads();
+    if (threadIdx.x == 0) *out = SM_BINS - 1;
+    __syncthreads();
+    if ((int)threadIdx.x < SM_BINS && pass((int)threadIdx.x) && (threadIdx.x == 0 || !pass((int)threadIdx.x - 1)))
+        *out = threadIdx.x;
+    __syncthreads();
+    return *out;
+}
+static_assert(SM_BINS == SM_T, "a bin a thread");
+
+__global__ void __launch_bounds__(SM_T)
+k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
+    __shared__ unsigned long long mass[SM_BINS], incl[SM_BINS], wtot[16];
+    __shared__ unsigned cnt[SM_BINS], cincl[SM_BINS], ctot[16], flag, mark[SM_BINS / 32];
+    __shared__ int found;
+    const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x, lane = tid & 63;
+    const size_t row = (size_t)b * a.ld;
+    const int i1 = min((s + 1) * chunk, a.V);
+    const SmRow r = sm_row(ws, b, SP);
+    SmHow h;
+    sm_how(h, a, b);
+    h.mx = sm_row_max(r, SP);
+    mass[tid] = 0;
+    cnt[tid] = 0;
+    __syncthreads();
+    if (h.mx > -INFINITY)
+        for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const unsigned long long w = i0 + e * SM_T < i1 ? sm_weight(h, v[e]) : 0ull;
+                const int bin = sm_bin(h, v[e]);
+                const unsigned long long live = __ballot(w != 0);
+                if (!live) continue;
+                // lanes that share one bin (equal logits) add up first
+                const int first = __builtin_amdgcn_readlane(bin, __ffsll((long long)live) - 1);
+                if (!__ballot(w != 0 && bin != first)) {
+                    unsigned long long t = w;
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, JM_WAVE);
+                    if (lane == 0) {
+                        atomicAdd(&mass[first], t);
+                        atomicAdd(&cnt[first], (unsigned)__popcll(live));
+                    }
+                } else if (w) {
+                    atomicAdd(&mass[bin], w);
+                    atomicAdd(&cnt[bin], 1u);
+                }
+            }
+        }
+    __syncthreads();
+    if (SP > 1) {
+        r.hmass[(size_t)s * SM_BINS + tid] = mass[tid];
+        r.hcnt[(size_t)s * SM_BINS + tid] = cnt[tid];
+        if (!sm_last(r.ticket, SP, &flag)) return;
+        unsigned long long m = 0;
+        unsigned n = 0;
+        for (int i = 0; i < SP; i++) {
+            m += r.hmass[(size_t)i * SM_BINS + tid];
+            n += r.hcnt[(size_t)i * SM_BINS + tid];
+        }
+        mass[tid] = m;
+        cnt[tid] = n;
+    }
+    if (h.mx == -INFINITY) {
+        if (tid == 0) r.plan->n = -1;
+        return;
+    }
+    // running sums over the bins
+    auto scan = [&](unsigned long long m, unsigned n, unsigned long long& mi, unsigned& ni) {
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned long long mo = __shfl_up(m, o, JM_WAVE);
+            const unsigned no = __shfl_up(n, o, JM_WAVE);
+            if (lane >= o) { m += mo; n += no; }
+        }
+        __syncthreads();
+        if (lane == 63) { wtot[tid >> 6] = m; ctot[tid >> 6] = n; }
+        __syncthreads();
+        for (int i = 0; i < (tid >> 6); i++) { m += wtot[i]; n += ctot[i]; }
+        mi = m;
+        ni = n;
+    };
+    const unsigned long long my_m = mass[tid];
+    const unsigned my_n = cnt[tid];
+    unsigned long long mi;
+    unsigned ni;
+    scan(my_m, my_n, mi, ni);
+    incl[tid] = mi;
+    cincl[tid] = ni;
+    if (tid < SM_BINS / 32) mark[tid] = 0;
+    __syncthreads();
+    auto before = [&](int i) { return i > 0 ? incl[i - 1] : 0ull; };
+    const unsigned long long total = incl[SM_BINS - 1];
+    auto set = [&](int lo, int hi) {
+        if (tid >= lo && tid <= hi) atomicOr(&mark[tid >> 5], 1u << (tid & 31));
+    };
+    // top-k
+    unsigned long long m1lo = total, m1hi = total;
+    int kbin = 0;
+    if (h.k > 0 && (unsigned)h.k < cincl[SM_BINS - 1]) {
+        const unsigned k = (unsigned)h.k;
+        const int i = sm_find([&](int j) { return cincl[j] >= k; }, &found);
+        m1hi = m1lo = incl[i];
+        if (cincl[i] > k) {
+            m1lo = before(i);
+            kbin = 1;
+            set(i, i);
+        }
+    }
+    unsigned long long lo = m1lo, hi = m1hi;
+    if (h.p < 1.0f) {
+        const double xl = (double)h.p * (double)m1lo, xh = (double)h.p * (double)m1hi;
+        const int il = sm_find([&](int j) { return (double)incl[j] >= xl; }, &found);
+        const int ih = sm_find([&](int j) { return (double)incl[j] >= xh; }, &found);
+        set(il, ih);
+        lo = min(lo, before(il));
+        hi = min(hi, incl[ih]);
+    }
+    int mbin = 0;
+    if (h.mp > 0.0f) {
+        // the bin where weights pass the border (rounded ones: half a unit
+        // below it), and its neighbours, which rounding here may mean
+        const double wmin = fmin(ceil((double)h.mp * (double)SM_ONE), (double)SM_ONE);
+        const float z = -__logf((float)((wmin - 0.5) / (double)SM_ONE)) * (SM_BINS / SM_SPAN);
+        const int i = (int)fminf(fmaxf(z, 0.0f), (float)(SM_BINS - 1));
+        mbin = max(i - 1, 0);
+        const int mh = min(i + 1, SM_BINS - 1);
+        set(mbin, mh);
+        lo = min(lo, before(mbin));
+        hi = min(hi, incl[mh]);
+    }
+    lo = max(lo, SM_ONE);
+    hi = max(hi, SM_ONE);
+    const float u = h.u > 0.0f ? h.u : 0.0f;
+    const unsigned long long tl = u < 1.0f ? min((unsigned long long)((double)u * (double)lo), lo - 1) : lo - 1;
+    const unsigned long long th = u < 1.0f ? min((unsigned long long)((double)u * (double)hi), hi - 1) : hi - 1;
+    const int sl = sm_find([&](int j) { return incl[j] > tl; }, &found);
+    const int sh = sm_find([&](int j) { return incl[j] > th; }, &found);
+    set(sl, sh);
+    __syncthreads();
+    const bool marked = mark[tid >> 5] >> (tid & 31) & 1;
+    scan(marked ? 0ull : my_m, marked ? 0u : my_n, mi, ni);
+    r.umass[tid] = mi;
+    r.ucnt[tid] = ni;
+    if (tid < SM_BINS / 32) r.plan->mark[tid] = mark[tid];
+    if (tid == SM_BINS - 1) {
+        r.plan->m1 = m1hi;
+        r.plan->kbin = kbin;
+        r.plan->mbin = mbin;
+        r.plan->m3_before = before(mbin);
+        r.plan->n = (int)(cincl[SM_BINS - 1] - ni);
+    }
+}
+
+// The borders and the token of a row from its tokens in descending order
+// (weight, and running weight and count with it), one or more a thread: each(f)
+// calls f(key, weight, running weight, running count) for every one.
+template <typename E>
+__device__ __forceinline__ void sm_finish(const SampleArgs& a, int b, const SmHow& h, const SmPlan& plan, E each,
+                                          unsigned long long* sh) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) {
+        sh[0] = plan.m1;
+        sh[1] = ~0ull;
+        sh[2] = 0;
+    }
+    __syncthreads();
+    if (plan.kbin) {
+        each([&](unsigned long long, unsigned long long, unsigned long long run, unsigned n) {
+            if (n == (unsigned)h.k) sh[0] = run;
+        });
+        __syncthreads();
+    }
+    const unsigned long long m1 = sh[0];
+    const double x = (double)h.p * (double)m1;
+    const double wmin = ceil((double)h.mp * (double)SM_ONE);
+    if (h.p < 1.0f || h.mp > 0.0f) {
+        each([&](unsigned long long key, unsigned long long w, unsigned long long run, unsigned) {
+            if (h.p < 1.0f && (double)run >= x) atomicMin(&sh[1], run);
+            if (h.mp > 0.0f && (double)w >= wmin && sm_bin(h, sm_unkey((uint32_t)(key >> 32))) >= plan.mbin) atomicAdd(&sh[2], w);
+        });
+        __syncthreads();
+    }
+    unsigned long long M = m1;
+    if (h.p < 1.0f) M = min(M, sh[1]);
+    if (h.mp > 0.0f) M = min(M, wmin > (double)SM_ONE ? SM_ONE : plan.m3_before + sh[2]);
+    M = max(M, SM_ONE);
+    const float u = h.u > 0.0f ? h.u : 0.0f;
+    const unsigned long long t = u < 1.0f ? min((unsigned long long)((double)u * (double)M), M - 1) : M - 1;
+    each([&](unsigned long long key, unsigned long long w, unsigned long long run, unsigned) {
+        if (run > t && run - w <= t) {
+            a.out_tok[b] = (int)~(uint32_t)key;
+            if (a.out_p) a.out_p[b] = (float)((double)w / (double)M);
+        }
+    });
+}
+
+// The row selected by its keys, 11 bits at a time from the top: a histogram of
+// the tokens that share the prefix found so far, then the digit at which the
+// running sum (of weights, or of tokens) passes the target.  Six passes over the
+// row a border, in one block: for rows whose list would be too long.
+__device__ __forceinline__ void sm_by_keys(const SampleArgs& a, int b, const SmHow& h, const SmPlan& plan,
+                                           unsigned long long* hist, unsigned long long* sh) {
+    constexpr int BITS = 11, ND = 1 << BITS;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const size_t row = (size_t)b * a.ld;
+    auto each = [&](auto f) {
+        for (int i0 = tid; i0 < a.V; i0 += 4 * SM_T) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, a.V - 1));
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (i0 + e * SM_T < a.V) f(i0 + e * SM_T, v[e]);
+        }
+    };
+    // the key found; sh[0]: the sum before it
+    auto select = [&](bool counting, unsigned long long target) {
+        unsigned long long prefix = 0, before = 0;
+        for (int top = 64; top > 0;) {
+            const int bits = min(top, BITS), low = top - bits;
+            __syncthreads();
+            for (int i = tid; i < ND; i += SM_T) hist[i] = 0;
+            __syncthreads();
+            each([&](int i, float l) {
+                const unsigned long long key = sm_key64(l, i);
+                if (top < 64 && (key >> top) != (prefix >> top)) return;
+                const unsigned long long w = sm_weight(h, l);
+                if (w) atomicAdd(&hist[(key >> low) & (ND - 1)], counting ? 1ull : w);
+            });
+            __syncthreads();
+            // from the largest digit down: wave 0, 32 digits a lane
+            if (tid < 64) {
+                unsigned long long own = 0;
+                for (int i = 0; i < ND / 64; i++) own += hist[ND - 1 - (lane * (ND / 64) + i)];
+                unsigned long long upto = own;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const unsigned long long t = __shfl_up(upto, o, JM_WAVE);
+                    if (lane >= o) upto += t;
+                }
+                unsigned long long run = before + upto - own;
+                if (run + own > target && run <= target)
+                    for (int i = 0; i < ND / 64; i++) {
+                        const int d = ND - 1 - (lane * (ND / 64) + i);
+                        if (run + hist[d] > target) {
+                            sh[0] = run;
+                            sh[1] = (unsigned long long)d;
+                            break;
+                        }
+                        run += hist[d];
+                    }
+            }
+            __syncthreads();
+            before = sh[0];
+            prefix |= sh[1] << low;
+            top = low;
+        }
+        return prefix;
+    };
+    auto weight_of = [&](unsigned long long key) { return sm_weight(h, sm_unkey((uint32_t)(key >> 32))); };
+    // a count's border: the weight up to and with that token
+    auto sum_if = [&](auto take) {
+        __syncthreads();
+        if (tid == 0) sh[2] = 0;
+        __syncthreads();
+        unsigned long long t = 0;
+        each([&](int i, float l) {
+            const unsigned long long w = sm_weight(h, l);
+            if (take(sm_key64(l, i), w)) t += w;
+        });
+        atomicAdd(&sh[2], t);
+        __syncthreads();
+        return sh[2];
+    };
+    unsigned long long M = plan.m1;
+    if (plan.kbin) {
+        const unsigned long long key = select(true, (unsigned long long)h.k - 1);
+        M = sum_if([&](unsigned long long k, unsigned long long) { return k >= key; });
+    }
+    if (h.p < 1.0f) {
+        const double x = ceil((double)h.p * (double)M);
+        const unsigned long long key = select(false, x > 1.0 ? (unsigned long long)x - 1 : 0ull);
+        M = min(M, sh[0] + weight_of(key));
+    }
+    if (h.mp > 0.0f) {
+        const double x = ceil((double)h.mp * (double)SM_ONE);
+        M = min(M, x > (double)SM_ONE ? SM_ONE : sum_if([&](unsigned long long, unsigned long long w) { return (double)w >= x; }));
+    }
+    M = max(M, SM_ONE);
+    const float u = h.u > 0.0f ? h.u : 0.0f;
+    const unsigned long long t = u < 1.0f ? min((unsigned long long)((double)u * (double)M), M - 1) : M - 1;
+    const unsigned long long key = select(false, t);
+    if (tid == 0) {
+        a.out_tok[b] = (int)~(uint32_t)key;
+        if (a.out_p) a.out_p[b] = (float)((double)weight_of(key) / (double)M);
+    }
+}
+
+__global__ void __launch_bounds__(SM_T)
+k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
+    __shared__ unsigned long long key[SM_CAP], wt[SM_CAP], sh[4], wtot[16];
+    __shared__ unsigned flag, mark[SM_BINS / 32];
+    const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x, lane = tid & 63;
+    const size_t row = (size_t)b * a.ld;
+    const int i1 = min((s + 1) * chunk, a.V);
+    const SmRow r = sm_row(ws, b, SP);
+    SmHow h;
+    sm_how(h, a, b);
+    h.mx = sm_row_max(r, SP);
+    const int n = r.plan->n;
+    if (n < 0) {
+        if (s == 0 && tid == 0) {
             a.out_tok[b] = -1;
             if (a.out_p) a.out_p[b] = 0.0f;
         }
         return;
     }
-    // the running weight (or, counting, the number of elements) passes
-    // `target`: the key of that element and the weight up to and with it
-    auto select = [&](bool counting, unsigned long long target, unsigned long long& key) {
-        unsigned long long prefix = 0, before = 0, wsum = 0;
-        for (int level = 0; level < 8; level++) {
-            const int sh8 = 56 - 8 * level;
-            __syncthreads();
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < a.V; i += 1024) {
-                const float l = sm_logit(a, row, i);
-                const unsigned long long w = sm_weight(l, mx, inv_t);
-                if (!w) continue;
-                const unsigned long long kk = ((unsigned long long)sm_key(l) << 32) | (uint32_t)~i;
-                if (level && (kk >> (sh8 + 8)) != (prefix >> (sh8 + 8))) continue;
-                atomicAdd(&hist[(kk >> sh8) & 255], counting ? 1ull : w);
+    if (n <= SM_CAP) {
+        if (tid < SM_BINS / 32) mark[tid] = r.plan->mark[tid];
+        __syncthreads();
+        for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int bin = sm_bin(h, v[e]);
+                bool in = i0 + e * SM_T < i1 && (mark[bin >> 5] >> (bin & 31) & 1);
+                if (!__any(in)) continue;
+                const unsigned long long w = in ? sm_weight(h, v[e]) : 0ull;
+                in = w != 0;
+                const unsigned long long who = __ballot(in);
+                if (!who) continue;
+                unsigned at = 0;
+                if (lane == 0) at = atomicAdd(&r.ticket[2], (unsigned)__popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
+                if (in && at < SM_CAP) r.list[at] = make_ulonglong2(sm_key64(v[e], i0 + e * SM_T), w);
             }
-            __syncthreads();
-            if (tid == 0) {
-                unsigned long long run = before;
-                int d = 255;
-                for (; d > 0; d--) {
-                    if (run + hist[d] > target) break;
-                    run += hist[d];
-                }
-                sh[0] = run;
-                sh[1] = d;
-            }
-            __syncthreads();
-            before = sh[0];
-            prefix |= sh[1] << sh8;
         }
-        key = prefix;
-        (void)wsum;
-        return before;
-    };
-    auto sum_from = [&](unsigned long long key, unsigned long long wmin) {
-        unsigned long long s = 0;
-        for (int i = tid; i < a.V; i += 1024) {
-            const float l = sm_logit(a, row, i);
-            const unsigned long long w = sm_weight(l, mx, inv_t);
-            const unsigned long long kk = ((unsigned long long)sm_key(l) << 32) | (uint32_t)~i;
-            if (kk >= key && w >= wmin) s += w;
-        }
-        __syncthreads();
-        if (tid == 0) sh[2] = 0;
-        __syncthreads();
-        atomicAdd(&sh[2], s);
-        __syncthreads();
-        const unsigned long long r = sh[2];
-        return r;
-    };
-    unsigned long long key = 0, M;
-    if (k > 0 && k < a.V) {
-        select(true, (unsigned long long)k - 1, key);
-        M = sum_from(key, 0);
+    }
+    if (SP > 1) {
+        if (!sm_last(r.ticket + 1, SP, &flag)) return;
     } else {
-        M = sum_from(0, 0);
+        __threadfence();
+        __syncthreads();
     }
-    if (p < 1.0f) {
-        const double x = (double)p * (double)M;
-        unsigned long long kp;
-        // the first element whose running weight reaches x
-        const unsigned long long c = x > 0.0 ? (unsigned long long)ceil(x) : 0ull;
-        select(false, c ? c - 1 : 0ull, kp);
-        M = min(M, sum_from(kp, 0));
+    const SmPlan& plan = *r.plan;
+    if (n > SM_CAP) {
+        sm_by_keys(a, b, h, plan, key, sh);
+        return;
     }
-    if (mp > 0.0f) {
-        const double x = ceil((double)mp * (double)SM_ONE);
-        M = min(M, x > (double)SM_ONE ? SM_ONE : sum_from(0, (unsigned long long)x));
-        M = max(M, SM_ONE);
+    // the list in descending order of its keys (a bitonic network)
+    int n2 = 2;
+    while (n2 < n) n2 <<= 1;
+    for (int i = tid; i < n2; i += SM_T) {
+        const ulonglong2 x = i < n ? r.list[i] : make_ulonglong2(0ull, 0ull);
+        key[i] = x.x;
+        wt[i] = x.y;
     }
-    float u = a.u[b];
-    u = u > 0.0f ? u : 0.0f;
-    unsigned long long t = u < 1.0f ? (unsigned long long)floor((double)u * (double)M) : M - 1;
-    t = min(t, M - 1);
-    select(false, t, key);
-    if (tid == 0) {
-        const int i = (int)~(uint32_t)key;
-        a.out_tok[b] = i;
-        if (a.out_p) a.out_p[b] = (float)((double)sm_weight(sm_logit(a, row, i), mx, inv_t) / (double)M);
+    for (int k = 2; k <= n2; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            for (int i = tid; i < n2 / 2; i += SM_T) {
+                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                const unsigned long long x = key[lo], y = key[hi];
+                if ((x < y) == ((lo & k) == 0)) {
+                    key[lo] = y;
+                    key[hi] = x;
+                    const unsigned long long t = wt[lo];
+                    wt[lo] = wt[hi];
+                    wt[hi] = t;
+                }
+            }
+        }
+    __syncthreads();
+    // running sums: 4 consecutive entries a thread
+    constexpr int E = SM_CAP / SM_T;
+    unsigned long long run[E], t = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (E * tid + e < n) t += wt[E * tid + e];
+        run[e] = t;
     }
+    unsigned long long upto = t;
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long x = __shfl_up(upto, o, JM_WAVE);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 63) wtot[tid >> 6] = upto;
+    __syncthreads();
+    for (int i = 0; i < (tid >> 6); i++) upto += wtot[i];
+    unsigned cnt[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * tid + e;
+        cnt[e] = 0;
+        if (i >= n) continue;
+        const int bin = sm_bin(h, sm_unkey((uint32_t)(key[i] >> 32)));
+        run[e] += upto - t + r.umass[bin];
+        cnt[e] = i + 1 + r.ucnt[bin];
+    }
+    sm_finish(a, b, h, plan, [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (E * tid + e < n) f(key[E * tid + e], wt[E * tid + e], run[e], cnt[e]);
+    }, sh);
 }
 
-hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
+// Chunks of a row: two blocks a CU over all rows, at least 8 tokens a thread.
+static int sm_chunks(int B, int V) {
+    return std::max(1, std::min(512 / B, (V + 8 * SM_T - 1) / (8 * SM_T)));
+}
+
+size_t sample_ws_bytes(int B, int V) { return (size_t)B * sm_row_bytes(sm_chunks(B, V)); }
+
+hipError_t launch_sample(const SampleArgs& a, void* ws, hipStream_t st) {
     if (a.B == 0) return hipSuccess;
-    hipLaunchKernelGGL(k_sample_row, dim3((unsigned)a.B), dim3(1024), 0, st, a);
+    const int SP = sm_chunks(a.B, a.V), chunk = (a.V + SP - 1) / SP;
+    const dim3 grid((unsigned)a.B * SP);
+    hipLaunchKernelGGL(k_sample_max, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
+    hipLaunchKernelGGL(k_sample_hist, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
+    hipLaunchKernelGGL(k_sample_pick, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
     return hipGetLastError();
 }
 

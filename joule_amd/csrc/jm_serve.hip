@@ -129,7 +129,13 @@ int jm_sample(const void* logits, int dtype, int64_t ld, int B, int V, const jm_
     a.temperature = how->temperature; a.top_k = how->top_k; a.top_p = how->top_p; a.min_p = how->min_p;
     a.temperature_b = how->temperature_b; a.top_k_b = how->top_k_b; a.top_p_b = how->top_p_b; a.min_p_b = how->min_p_b;
     a.u = u; a.out_tok = out_tok; a.out_p = out_p;
-    JM_HIP(jm::launch_sample(a, (hipStream_t)stream), "sampling launch");
+    hipStream_t st = (hipStream_t)stream;
+    jm::PluginWs ws;
+    if (int rc = jm::plugin_ws(st, jm::sample_ws_bytes(B, V), &ws)) return rc;
+    const hipError_t e = jm::launch_sample(a, ws.p, st);
+    const hipError_t f = ws.async ? hipFreeAsync(ws.p, st) : hipSuccess;
+    if (e != hipSuccess) return jm::hip_fail(e, "sampling launch");
+    if (f != hipSuccess) return jm::hip_fail(f, "hipFreeAsync");
     return 0;
 }
 

@@ -136,7 +136,8 @@ def test_one_logit_far_above_and_many_far_below():
     x = np.full((6, V), -26.0, np.float32) + np.random.default_rng(1).random((6, V)).astype(np.float32)
     x[:, 123] = [0.0, 1.0, 2.0, 3.0, 10.0, 100.0]
     for u in (0.5, 0.99999994):
-        for how in (dict(), dict(top_k=100), dict(top_p=0.9999999), dict(temperature=3.0, top_p=0.99)):
+        for how in (dict(), dict(top_k=100), dict(top_p=0.9999999), dict(temperature=3.0, top_p=0.99), dict(min_p=1.2e-12),
+                    dict(min_p=3e-12), dict(min_p=1e-30), dict(min_p=4e-11, temperature=1.1)):
             _check(x, [u] * 6, **how)
 
 
