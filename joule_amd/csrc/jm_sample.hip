@@ -8,8 +8,9 @@
 // w = round(2^40 exp((l - max) / T)) both are exact in any order of summation,
 // so no sort of the vocabulary is needed, only histograms:
 //
-//   k_sample_max     each row's maximum, by chunks
-//   k_sample_hist    counts and weights of SM_BINS equal steps of (max - l) / T,
+//   k_sample_max     each row's maximum and minimum, by chunks
+//   k_sample_hist    weights (and, for top-k, counts) of SM_BINS equal steps of l
+//                    from the maximum to the minimum, or to where weights end,
 //                    by chunks; the row's last chunk adds them up and marks the
 //                    few bins in which a border (of top-k, top-p, min-p or the
 //                    draw itself) can lie
@@ -44,13 +45,13 @@ struct SmPlan {
     int kbin;                   // 1: it lies in a marked bin
     int mbin;                   // min-p: the first of the marked bins around its border
     unsigned long long m3_before;   // the weight before that bin
-    int n;                      // tokens in the marked bins; -1: a row with nothing to draw
+    int none;                   // a row with nothing to draw
 };
 
 // A row's part of the workspace.
 struct SmRow {
     unsigned* ticket;           // [2] chunks done of the two kernels that hand over; [2]: the list's length
-    float* cmax;                // [SP]
+    float2* cmm;                // [SP] largest and smallest logit of the chunk
     SmPlan* plan;
     unsigned long long* umass;  // [SM_BINS] weight of the unmarked bins before a bin
     unsigned* ucnt;             // [SM_BINS]
@@ -60,7 +61,7 @@ struct SmRow {
 };
 
 __host__ __device__ __forceinline__ size_t sm_row_bytes(int SP) {
-    return 16 + ((size_t)SP * 4 + 15) / 16 * 16 + (sizeof(SmPlan) + 15) / 16 * 16 + (size_t)SM_BINS * 12 * (1 + SP) +
+    return 16 + ((size_t)SP * 8 + 15) / 16 * 16 + (sizeof(SmPlan) + 15) / 16 * 16 + (size_t)SM_BINS * 12 * (1 + SP) +
            (size_t)SM_CAP * 16;
 }
 
@@ -68,7 +69,7 @@ __device__ __forceinline__ SmRow sm_row(char* ws, int b, int SP) {
     SmRow r;
     char* p = ws + (size_t)b * sm_row_bytes(SP);
     r.ticket = (unsigned*)p; p += 16;
-    r.cmax = (float*)p; p += ((size_t)SP * 4 + 15) / 16 * 16;
+    r.cmm = (float2*)p; p += ((size_t)SP * 8 + 15) / 16 * 16;
     r.plan = (SmPlan*)p; p += (sizeof(SmPlan) + 15) / 16 * 16;
     r.list = (ulonglong2*)p; p += (size_t)SM_CAP * 16;
     r.umass = (unsigned long long*)p; p += (size_t)SM_BINS * 8;
@@ -119,12 +120,13 @@ __device__ __forceinline__ unsigned long long sm_exp2(double t) {
 struct SmHow {
     float mx;                   // the largest logit
     double c;                   // log2(e) / T
-    float cb;                   // bins a logit
+    float cb;                   // bins a unit of l
+    float zb;                   // bins a unit of (max - l) / T
     int k;                      // 0: all
     float p, mp, u;
 };
 
-__device__ __forceinline__ void sm_how(SmHow& h, const SampleArgs& a, int b) {
+__device__ __forceinline__ void sm_how(SmHow& h, const SampleArgs& a, int b, const SmRow& r, int SP) {
     float T = a.temperature_b ? a.temperature_b[b] : a.temperature;
     h.k = a.top_k_b ? a.top_k_b[b] : a.top_k;
     h.p = a.top_p_b ? a.top_p_b[b] : a.top_p;
@@ -132,7 +134,17 @@ __device__ __forceinline__ void sm_how(SmHow& h, const SampleArgs& a, int b) {
     h.u = a.u[b];
     if (!(T > 0.0f)) { T = 1.0f; h.k = 1; }
     h.c = 1.4426950408889634 / (double)T;
-    h.cb = fminf((float)(SM_BINS / (double)SM_SPAN / (double)T), 3.0e38f);
+    float mx = -INFINITY, mn = INFINITY;
+    for (int i = threadIdx.x & 63; i < SP; i += 64) {
+        const float2 v = r.cmm[i];
+        mx = fmaxf(mx, v.x);
+        mn = fminf(mn, v.y);
+    }
+    h.mx = seg_max<64>(mx);
+    // (0 / 0 where all are alike: no span)
+    const float span = fminf(__fsub_rn(h.mx, -seg_max<64>(-mn)), __fmul_rn(SM_SPAN, T));
+    h.cb = fminf(__fdiv_rn((float)SM_BINS, span), 3.0e38f);
+    h.zb = __fmul_rn(T, h.cb);
 }
 
 __device__ __forceinline__ unsigned long long sm_weight(const SmHow& h, float l) {
@@ -151,45 +163,53 @@ __device__ __forceinline__ float sm_logit(const SampleArgs& a, size_t row, int i
     return a.bf ? bf16_bits_to_f32(((const uint16_t*)a.logits)[row + i]) : ((const float*)a.logits)[row + i];
 }
 
-__device__ __forceinline__ float sm_row_max(const SmRow& r, int SP) {
-    float mx = -INFINITY;
-    for (int i = threadIdx.x & 63; i < SP; i += 64) mx = fmaxf(mx, r.cmax[i]);
-    return seg_max<64>(mx);
-}
-
 // Whether this block is the last of the row's to come here; what the others
 // wrote before is then visible to all of its threads.
 __device__ __forceinline__ bool sm_last(unsigned* ticket, int SP, unsigned* flag) {
-    __threadfence();
+    // (one thread's fences serve the block: the barriers order the others'
+    // accesses with it)
     __syncthreads();
-    if (threadIdx.x == 0) *flag = atomicAdd(ticket, 1u) == (unsigned)SP - 1;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        const bool last = atomicAdd(ticket, 1u) == (unsigned)SP - 1;
+        if (last) __threadfence();
+        *flag = last;
+    }
     __syncthreads();
-    const bool last = *flag;
-    if (last) __threadfence();
-    return last;
+    return *flag;
 }
 
 __global__ void __launch_bounds__(SM_T)
 k_sample_max(SampleArgs a, char* ws, int SP, int chunk) {
-    __shared__ float red[SM_T / 64];
+    __shared__ float red[2][SM_T / 64];
     const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x;
     const size_t row = (size_t)b * a.ld;
     const int i1 = min((s + 1) * chunk, a.V);
-    float mx = -INFINITY;
+    float mx = -INFINITY, mn = INFINITY;
     for (int i0 = s * chunk + tid; i0 < i1; i0 += 8 * SM_T) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
 #pragma unroll
-        for (int e = 0; e < 8; e++) mx = fmaxf(mx, v[e]);
+        for (int e = 0; e < 8; e++) {
+            mx = fmaxf(mx, v[e]);
+            mn = fminf(mn, v[e] > -INFINITY ? v[e] : INFINITY);
+        }
     }
     mx = seg_max<64>(mx);
-    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    mn = -seg_max<64>(-mn);
+    if ((tid & 63) == 0) {
+        red[0][tid >> 6] = mx;
+        red[1][tid >> 6] = mn;
+    }
     __syncthreads();
     const SmRow r = sm_row(ws, b, SP);
     if (tid == 0) {
-        for (int i = 1; i < SM_T / 64; i++) mx = fmaxf(mx, red[i]);
-        r.cmax[s] = mx;
+        for (int i = 1; i < SM_T / 64; i++) {
+            mx = fmaxf(mx, red[0][i]);
+            mn = fminf(mn, red[1][i]);
+        }
+        r.cmm[s] = make_float2(mx, mn);
     }
     if (s == 0 && tid < 3) r.ticket[tid] = 0;
 }
@@ -218,8 +238,8 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     const int i1 = min((s + 1) * chunk, a.V);
     const SmRow r = sm_row(ws, b, SP);
     SmHow h;
-    sm_how(h, a, b);
-    h.mx = sm_row_max(r, SP);
+    sm_how(h, a, b, r, SP);
+    const bool counts = h.k > 0 && h.k < a.V;               // (block-uniform)
     mass[tid] = 0;
     cnt[tid] = 0;
     __syncthreads();
@@ -242,30 +262,43 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
                     for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, JM_WAVE);
                     if (lane == 0) {
                         atomicAdd(&mass[first], t);
-                        atomicAdd(&cnt[first], (unsigned)__popcll(live));
+                        if (counts) atomicAdd(&cnt[first], (unsigned)__popcll(live));
                     }
                 } else if (w) {
                     atomicAdd(&mass[bin], w);
-                    atomicAdd(&cnt[bin], 1u);
+                    if (counts) atomicAdd(&cnt[bin], 1u);
                 }
             }
         }
     __syncthreads();
     if (SP > 1) {
         r.hmass[(size_t)s * SM_BINS + tid] = mass[tid];
-        r.hcnt[(size_t)s * SM_BINS + tid] = cnt[tid];
+        if (counts) r.hcnt[(size_t)s * SM_BINS + tid] = cnt[tid];
         if (!sm_last(r.ticket, SP, &flag)) return;
         unsigned long long m = 0;
         unsigned n = 0;
-        for (int i = 0; i < SP; i++) {
-            m += r.hmass[(size_t)i * SM_BINS + tid];
-            n += r.hcnt[(size_t)i * SM_BINS + tid];
+        // (the other chunks' lines come from memory: 8 requests at a time)
+        for (int i0 = 0; i0 < SP; i0 += 8) {
+            unsigned long long mv[8];
+            unsigned nv[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const size_t at = (size_t)min(i0 + i, SP - 1) * SM_BINS + tid;
+                mv[i] = r.hmass[at];
+                nv[i] = counts ? r.hcnt[at] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i0 + i < SP) {
+                    m += mv[i];
+                    n += nv[i];
+                }
         }
         mass[tid] = m;
         cnt[tid] = n;
     }
     if (h.mx == -INFINITY) {
-        if (tid == 0) r.plan->n = -1;
+        if (tid == 0) r.plan->none = 1;
         return;
     }
     // running sums over the bins
@@ -299,7 +332,7 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     // top-k
     unsigned long long m1lo = total, m1hi = total;
     int kbin = 0;
-    if (h.k > 0 && (unsigned)h.k < cincl[SM_BINS - 1]) {
+    if (counts && (unsigned)h.k < cincl[SM_BINS - 1]) {
         const unsigned k = (unsigned)h.k;
         const int i = sm_find([&](int j) { return cincl[j] >= k; }, &found);
         m1hi = m1lo = incl[i];
@@ -323,7 +356,7 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
         // the bin where weights pass the border (rounded ones: half a unit
         // below it), and its neighbours, which rounding here may mean
         const double wmin = fmin(ceil((double)h.mp * (double)SM_ONE), (double)SM_ONE);
-        const float z = -__logf((float)((wmin - 0.5) / (double)SM_ONE)) * (SM_BINS / SM_SPAN);
+        const float z = -__logf((float)((wmin - 0.5) / (double)SM_ONE)) * h.zb;
         const int i = (int)fminf(fmaxf(z, 0.0f), (float)(SM_BINS - 1));
         mbin = max(i - 1, 0);
         const int mh = min(i + 1, SM_BINS - 1);
@@ -350,7 +383,7 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
         r.plan->kbin = kbin;
         r.plan->mbin = mbin;
         r.plan->m3_before = before(mbin);
-        r.plan->n = (int)(cincl[SM_BINS - 1] - ni);
+        r.plan->none = 0;
     }
 }
 
@@ -508,37 +541,33 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
     const int i1 = min((s + 1) * chunk, a.V);
     const SmRow r = sm_row(ws, b, SP);
     SmHow h;
-    sm_how(h, a, b);
-    h.mx = sm_row_max(r, SP);
-    const int n = r.plan->n;
-    if (n < 0) {
+    sm_how(h, a, b, r, SP);
+    if (r.plan->none) {
         if (s == 0 && tid == 0) {
             a.out_tok[b] = -1;
             if (a.out_p) a.out_p[b] = 0.0f;
         }
         return;
     }
-    if (n <= SM_CAP) {
-        if (tid < SM_BINS / 32) mark[tid] = r.plan->mark[tid];
-        __syncthreads();
-        for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
-            float v[8];
+    if (tid < SM_BINS / 32) mark[tid] = r.plan->mark[tid];
+    __syncthreads();
+    for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
+        float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
+        for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int bin = sm_bin(h, v[e]);
-                bool in = i0 + e * SM_T < i1 && (mark[bin >> 5] >> (bin & 31) & 1);
-                if (!__any(in)) continue;
-                const unsigned long long w = in ? sm_weight(h, v[e]) : 0ull;
-                in = w != 0;
-                const unsigned long long who = __ballot(in);
-                if (!who) continue;
-                unsigned at = 0;
-                if (lane == 0) at = atomicAdd(&r.ticket[2], (unsigned)__popcll(who));
-                at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
-                if (in && at < SM_CAP) r.list[at] = make_ulonglong2(sm_key64(v[e], i0 + e * SM_T), w);
-            }
+        for (int e = 0; e < 8; e++) {
+            const int bin = sm_bin(h, v[e]);
+            bool in = i0 + e * SM_T < i1 && (mark[bin >> 5] >> (bin & 31) & 1);
+            if (!__any(in)) continue;
+            const unsigned long long w = in ? sm_weight(h, v[e]) : 0ull;
+            in = w != 0;
+            const unsigned long long who = __ballot(in);
+            if (!who) continue;
+            unsigned at = 0;
+            if (lane == 0) at = atomicAdd(&r.ticket[2], (unsigned)__popcll(who));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
+            if (in && at < SM_CAP) r.list[at] = make_ulonglong2(sm_key64(v[e], i0 + e * SM_T), w);
         }
     }
     if (SP > 1) {
@@ -548,6 +577,7 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
         __syncthreads();
     }
     const SmPlan& plan = *r.plan;
+    const int n = (int)r.ticket[2];         // tokens met, listed or not
     if (n > SM_CAP) {
         sm_by_keys(a, b, h, plan, key, sh);
         return;
@@ -609,9 +639,9 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
     }, sh);
 }
 
-// Chunks of a row: two blocks a CU over all rows, at least 8 tokens a thread.
+// Chunks of a row: two blocks a CU over all rows, at least 16 tokens a thread.
 static int sm_chunks(int B, int V) {
-    return std::max(1, std::min(512 / B, (V + 8 * SM_T - 1) / (8 * SM_T)));
+    return std::max(1, std::min(512 / B, (V + 16 * SM_T - 1) / (16 * SM_T)));
 }
 
 size_t sample_ws_bytes(int B, int V) { return (size_t)B * sm_row_bytes(sm_chunks(B, V)); }
