@@ -41,8 +41,7 @@ constexpr float SM_SPAN = 28.45f;
 // What the histogram's last chunk leaves for the row.
 struct SmPlan {
     uint32_t mark[SM_BINS / 32];
-    unsigned long long m1;      // the weight that top-k keeps, where no bin splits it
-    int kbin;                   // 1: it lies in a marked bin
+    unsigned long long m1;      // the weight that top-k keeps, where it is known (0: the list tells)
     int mbin;                   // min-p: the first of the marked bins around its border
     unsigned long long m3_before;   // the weight before that bin
     int none;                   // a row with nothing to draw
@@ -153,6 +152,12 @@ __device__ __forceinline__ unsigned long long sm_weight(const SmHow& h, float l)
     return t >= -41.5 ? sm_exp2(t) : 0ull;             // (NaN: 0)
 }
 
+// The running weight that the drawn token is the first to pass, of a kept sum M.
+__device__ __forceinline__ unsigned long long sm_target(float u, unsigned long long M) {
+    if (!(u < 1.0f) && u == u) return M - 1;
+    return min((unsigned long long)((double)(u > 0.0f ? u : 0.0f) * (double)M), M - 1);
+}
+
 // The bin of a logit: monotone in l, each step being so.
 __device__ __forceinline__ int sm_bin(const SmHow& h, float l) {
     if (l == h.mx) return 0;
@@ -163,19 +168,26 @@ __device__ __forceinline__ float sm_logit(const SampleArgs& a, size_t row, int i
     return a.bf ? bf16_bits_to_f32(((const uint16_t*)a.logits)[row + i]) : ((const float*)a.logits)[row + i];
 }
 
+// What the chunks of a row hand to its last one in the same launch is written
+// through the XCD's L2 and read past it (device scope), so that no cache has to
+// be written back or emptied: with fences that do, 512 blocks took 12 us more.
+template <typename T>
+__device__ __forceinline__ void sm_put(T* p, T v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T sm_get(T* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Whether this block is the last of the row's to come here; what the others
-// wrote before is then visible to all of its threads.
+// put before is then there for sm_get.
 __device__ __forceinline__ bool sm_last(unsigned* ticket, int SP, unsigned* flag) {
-    // (one thread's fences serve the block: the barriers order the others'
-    // accesses with it)
+    __asm__ volatile("s_waitcnt vmcnt(0)" : : : "memory");     // this wave's stores are through
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        const bool last = atomicAdd(ticket, 1u) == (unsigned)SP - 1;
-        if (last) __threadfence();
-        *flag = last;
-    }
+    if (threadIdx.x == 0) *flag = atomicAdd(ticket, 1u) == (unsigned)SP - 1;
     __syncthreads();
+    __asm__ volatile("" : : : "memory");
     return *flag;
 }
 
@@ -214,32 +226,60 @@ k_sample_max(SampleArgs a, char* ws, int SP, int chunk) {
     if (s == 0 && tid < 3) r.ticket[tid] = 0;
 }
 
-// The first bin whose running weight in incl[] satisfies pass (monotone), by
-// the whole block: out receives it (SM_BINS - 1 if there is none).
+// Running sum over the lanes (DPP: within rows of 16, then row ends onto the
+// rows behind), 64 bits.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long sm_dpp_add(unsigned long long v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + (((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ unsigned long long sm_wave_scan(unsigned long long v) {
+    v = sm_dpp_add<0x111, 0xF>(v);          // row_shr 1, 2, 4, 8
+    v = sm_dpp_add<0x112, 0xF>(v);
+    v = sm_dpp_add<0x114, 0xF>(v);
+    v = sm_dpp_add<0x118, 0xF>(v);
+    v = sm_dpp_add<0x142, 0xA>(v);          // lane 15 onto row 1, 47 onto row 3
+    v = sm_dpp_add<0x143, 0xC>(v);          // lane 31 onto rows 2 and 3
+    return v;
+}
+// ... over the block's threads; tot: 16 words of LDS that nothing else uses
+__device__ __forceinline__ unsigned long long sm_block_scan(unsigned long long v, unsigned long long* tot) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    v = sm_wave_scan(v);
+    __syncthreads();
+    if (lane == 63) tot[w] = v;
+    __syncthreads();
+    const unsigned long long t = sm_wave_scan(lane < SM_T / 64 ? tot[lane] : 0ull);
+    const int from = __builtin_amdgcn_readfirstlane(w) - 1;
+    if (from < 0) return v;
+    return v + (((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(t >> 32), from) << 32) |
+                (unsigned)__builtin_amdgcn_readlane((int)(unsigned)t, from));
+}
+
+// Thread i tells the first bin at which pass (monotone) holds, through *out,
+// which starts as SM_BINS - 1; read it after a barrier.
 template <typename F>
-__device__ __forceinline__ int sm_find(F pass, int* out) {
-    __syncthreads();
-    if (threadIdx.x == 0) *out = SM_BINS - 1;
-    __syncthreads();
-    if ((int)threadIdx.x < SM_BINS && pass((int)threadIdx.x) && (threadIdx.x == 0 || !pass((int)threadIdx.x - 1)))
-        *out = threadIdx.x;
-    __syncthreads();
-    return *out;
+__device__ __forceinline__ void sm_find(F pass, int* out) {
+    const int i = (int)threadIdx.x;
+    if (pass(i) && (i == 0 || !pass(i - 1))) *out = i;
 }
 static_assert(SM_BINS == SM_T, "a bin a thread");
 
-__global__ void __launch_bounds__(SM_T)
+__global__ void __launch_bounds__(SM_T, 8)
 k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     __shared__ unsigned long long mass[SM_BINS], incl[SM_BINS], wtot[16];
-    __shared__ unsigned cnt[SM_BINS], cincl[SM_BINS], ctot[16], flag, mark[SM_BINS / 32];
-    __shared__ int found;
+    __shared__ unsigned cnt[SM_BINS], cincl[SM_BINS], flag, mark[SM_BINS / 32];
+    __shared__ int found[5];
     const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x, lane = tid & 63;
     const size_t row = (size_t)b * a.ld;
     const int i1 = min((s + 1) * chunk, a.V);
     const SmRow r = sm_row(ws, b, SP);
     SmHow h;
     sm_how(h, a, b, r, SP);
-    const bool counts = h.k > 0 && h.k < a.V;               // (block-uniform)
+    // (block-uniform) top-k matters; few enough that all it keeps fits the
+    // list, where weights are formed: then only counts are needed here
+    const bool counts = h.k > 0 && h.k < a.V, few = counts && h.k <= SM_CAP / 4;
     mass[tid] = 0;
     cnt[tid] = 0;
     __syncthreads();
@@ -249,46 +289,47 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const unsigned long long w = i0 + e * SM_T < i1 ? sm_weight(h, v[e]) : 0ull;
-                const int bin = sm_bin(h, v[e]);
-                const unsigned long long live = __ballot(w != 0);
-                if (!live) continue;
-                // lanes that share one bin (equal logits) add up first
-                const int first = __builtin_amdgcn_readlane(bin, __ffsll((long long)live) - 1);
-                if (!__ballot(w != 0 && bin != first)) {
-                    unsigned long long t = w;
+            for (int e = 0; e < 8; e++) v[e] = i0 + e * SM_T < i1 ? v[e] : -INFINITY;
+            if (few) {
 #pragma unroll
-                    for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, JM_WAVE);
-                    if (lane == 0) {
-                        atomicAdd(&mass[first], t);
-                        if (counts) atomicAdd(&cnt[first], (unsigned)__popcll(live));
-                    }
-                } else if (w) {
-                    atomicAdd(&mass[bin], w);
-                    if (counts) atomicAdd(&cnt[bin], 1u);
+                for (int e = 0; e < 8; e++) {
+                    // (the last bin, where everything far below piles up, is
+                    // what is taken if the others do not reach k)
+                    const int bin = sm_bin(h, v[e]);
+                    if (bin < SM_BINS - 1) atomicAdd(&cnt[bin], 1u);
                 }
+                continue;
+            }
+            unsigned long long w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = sm_weight(h, v[e]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (!w[e]) continue;
+                const int bin = sm_bin(h, v[e]);
+                atomicAdd(&mass[bin], w[e]);
+                if (counts) atomicAdd(&cnt[bin], 1u);
             }
         }
     __syncthreads();
     if (SP > 1) {
-        r.hmass[(size_t)s * SM_BINS + tid] = mass[tid];
-        if (counts) r.hcnt[(size_t)s * SM_BINS + tid] = cnt[tid];
+        if (!few) sm_put(&r.hmass[(size_t)s * SM_BINS + tid], mass[tid]);
+        if (counts) sm_put(&r.hcnt[(size_t)s * SM_BINS + tid], cnt[tid]);
         if (!sm_last(r.ticket, SP, &flag)) return;
         unsigned long long m = 0;
         unsigned n = 0;
-        // (the other chunks' lines come from memory: 8 requests at a time)
-        for (int i0 = 0; i0 < SP; i0 += 8) {
-            unsigned long long mv[8];
-            unsigned nv[8];
+        // (the other chunks' lines come from memory: 16 requests at a time)
+        for (int i0 = 0; i0 < SP; i0 += 16) {
+            unsigned long long mv[16];
+            unsigned nv[16];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 16; i++) {
                 const size_t at = (size_t)min(i0 + i, SP - 1) * SM_BINS + tid;
-                mv[i] = r.hmass[at];
-                nv[i] = counts ? r.hcnt[at] : 0;
+                mv[i] = few ? 0ull : sm_get(&r.hmass[at]);
+                nv[i] = counts ? sm_get(&r.hcnt[at]) : 0;
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 16; i++)
                 if (i0 + i < SP) {
                     m += mv[i];
                     n += nv[i];
@@ -301,28 +342,33 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
         if (tid == 0) r.plan->none = 1;
         return;
     }
-    // running sums over the bins
-    auto scan = [&](unsigned long long m, unsigned n, unsigned long long& mi, unsigned& ni) {
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned long long mo = __shfl_up(m, o, JM_WAVE);
-            const unsigned no = __shfl_up(n, o, JM_WAVE);
-            if (lane >= o) { m += mo; n += no; }
-        }
-        __syncthreads();
-        if (lane == 63) { wtot[tid >> 6] = m; ctot[tid >> 6] = n; }
-        __syncthreads();
-        for (int i = 0; i < (tid >> 6); i++) { m += wtot[i]; n += ctot[i]; }
-        mi = m;
-        ni = n;
-    };
     const unsigned long long my_m = mass[tid];
     const unsigned my_n = cnt[tid];
-    unsigned long long mi;
-    unsigned ni;
-    scan(my_m, my_n, mi, ni);
-    incl[tid] = mi;
-    cincl[tid] = ni;
     if (tid < SM_BINS / 32) mark[tid] = 0;
+    if (tid < 5) found[tid] = SM_BINS - 1;
+    if (few) {
+        // every token up to top-k's border goes on the list
+        cincl[tid] = (unsigned)sm_block_scan(my_n, wtot);
+        __syncthreads();
+        sm_find([&](int j) { return cincl[j] >= (unsigned)h.k; }, &found[0]);
+        __syncthreads();
+        const int last = found[0];
+        r.umass[tid] = 0;
+        r.ucnt[tid] = 0;
+        if (tid < SM_BINS / 32) {
+            const int n = last + 1 - 32 * tid;
+            r.plan->mark[tid] = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1;
+        }
+        if (tid == 0) {
+            r.plan->m1 = 0;
+            r.plan->mbin = 0;
+            r.plan->m3_before = 0;
+            r.plan->none = 0;
+        }
+        return;
+    }
+    incl[tid] = sm_block_scan(my_m, wtot);
+    if (counts) cincl[tid] = (unsigned)sm_block_scan(my_n, wtot);
     __syncthreads();
     auto before = [&](int i) { return i > 0 ? incl[i - 1] : 0ull; };
     const unsigned long long total = incl[SM_BINS - 1];
@@ -331,22 +377,24 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     };
     // top-k
     unsigned long long m1lo = total, m1hi = total;
-    int kbin = 0;
     if (counts && (unsigned)h.k < cincl[SM_BINS - 1]) {
         const unsigned k = (unsigned)h.k;
-        const int i = sm_find([&](int j) { return cincl[j] >= k; }, &found);
+        sm_find([&](int j) { return cincl[j] >= k; }, &found[0]);
+        __syncthreads();
+        const int i = found[0];
         m1hi = m1lo = incl[i];
         if (cincl[i] > k) {
             m1lo = before(i);
-            kbin = 1;
             set(i, i);
         }
     }
     unsigned long long lo = m1lo, hi = m1hi;
     if (h.p < 1.0f) {
         const double xl = (double)h.p * (double)m1lo, xh = (double)h.p * (double)m1hi;
-        const int il = sm_find([&](int j) { return (double)incl[j] >= xl; }, &found);
-        const int ih = sm_find([&](int j) { return (double)incl[j] >= xh; }, &found);
+        sm_find([&](int j) { return (double)incl[j] >= xl; }, &found[1]);
+        sm_find([&](int j) { return (double)incl[j] >= xh; }, &found[2]);
+        __syncthreads();
+        const int il = found[1], ih = found[2];
         set(il, ih);
         lo = min(lo, before(il));
         hi = min(hi, incl[ih]);
@@ -364,66 +412,62 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
         lo = min(lo, before(mbin));
         hi = min(hi, incl[mh]);
     }
-    lo = max(lo, SM_ONE);
-    hi = max(hi, SM_ONE);
-    const float u = h.u > 0.0f ? h.u : 0.0f;
-    const unsigned long long tl = u < 1.0f ? min((unsigned long long)((double)u * (double)lo), lo - 1) : lo - 1;
-    const unsigned long long th = u < 1.0f ? min((unsigned long long)((double)u * (double)hi), hi - 1) : hi - 1;
-    const int sl = sm_find([&](int j) { return incl[j] > tl; }, &found);
-    const int sh = sm_find([&](int j) { return incl[j] > th; }, &found);
-    set(sl, sh);
+    const unsigned long long tl = sm_target(h.u, max(lo, SM_ONE)), th = sm_target(h.u, max(hi, SM_ONE));
+    sm_find([&](int j) { return incl[j] > tl; }, &found[3]);
+    sm_find([&](int j) { return incl[j] > th; }, &found[4]);
+    __syncthreads();
+    set(found[3], found[4]);
     __syncthreads();
     const bool marked = mark[tid >> 5] >> (tid & 31) & 1;
-    scan(marked ? 0ull : my_m, marked ? 0u : my_n, mi, ni);
-    r.umass[tid] = mi;
-    r.ucnt[tid] = ni;
+    r.umass[tid] = sm_block_scan(marked ? 0ull : my_m, wtot);
+    if (counts) r.ucnt[tid] = (unsigned)sm_block_scan(marked ? 0u : my_n, wtot);
     if (tid < SM_BINS / 32) r.plan->mark[tid] = mark[tid];
-    if (tid == SM_BINS - 1) {
-        r.plan->m1 = m1hi;
-        r.plan->kbin = kbin;
+    if (tid == 0) {
+        r.plan->m1 = m1lo == m1hi ? m1hi : 0;
         r.plan->mbin = mbin;
         r.plan->m3_before = before(mbin);
         r.plan->none = 0;
     }
 }
 
-// The borders and the token of a row from its tokens in descending order
-// (weight, and running weight and count with it), one or more a thread: each(f)
-// calls f(key, weight, running weight, running count) for every one.
+// The borders and the token of a row from its list in descending order: each(f)
+// calls f(key, weight, running weight, running count) for every entry of this
+// thread; one entry at most answers to each question.
 template <typename E>
-__device__ __forceinline__ void sm_finish(const SampleArgs& a, int b, const SmHow& h, const SmPlan& plan, E each,
-                                          unsigned long long* sh) {
+__device__ __forceinline__ void sm_finish(const SampleArgs& a, int b, const SmHow& h, const SmPlan& plan, int n, E each,
+                                          unsigned long long* sh, unsigned long long* tot) {
     const int tid = threadIdx.x;
-    __syncthreads();
-    if (tid == 0) {
-        sh[0] = plan.m1;
-        sh[1] = ~0ull;
-        sh[2] = 0;
-    }
-    __syncthreads();
-    if (plan.kbin) {
-        each([&](unsigned long long, unsigned long long, unsigned long long run, unsigned n) {
-            if (n == (unsigned)h.k) sh[0] = run;
+    unsigned long long M = plan.m1;
+    if (!M) {
+        // (fewer than k on the list: those are all there are)
+        each([&](int i, unsigned long long, unsigned long long, unsigned long long run, unsigned c) {
+            if (c == (unsigned)h.k || (i == n - 1 && c < (unsigned)h.k)) sh[0] = run;
         });
         __syncthreads();
+        M = sh[0];
     }
-    const unsigned long long m1 = sh[0];
-    const double x = (double)h.p * (double)m1;
-    const double wmin = ceil((double)h.mp * (double)SM_ONE);
-    if (h.p < 1.0f || h.mp > 0.0f) {
-        each([&](unsigned long long key, unsigned long long w, unsigned long long run, unsigned) {
-            if (h.p < 1.0f && (double)run >= x) atomicMin(&sh[1], run);
-            if (h.mp > 0.0f && (double)w >= wmin && sm_bin(h, sm_unkey((uint32_t)(key >> 32))) >= plan.mbin) atomicAdd(&sh[2], w);
+    if (h.p < 1.0f) {
+        const double x = fmax((double)h.p * (double)M, 0.5);
+        each([&](int, unsigned long long, unsigned long long w, unsigned long long run, unsigned) {
+            if ((double)run >= x && (double)(run - w) < x) sh[1] = run;
         });
         __syncthreads();
+        M = min(M, sh[1]);
     }
-    unsigned long long M = m1;
-    if (h.p < 1.0f) M = min(M, sh[1]);
-    if (h.mp > 0.0f) M = min(M, wmin > (double)SM_ONE ? SM_ONE : plan.m3_before + sh[2]);
+    if (h.mp > 0.0f) {
+        const double wmin = ceil((double)h.mp * (double)SM_ONE);
+        unsigned long long t = 0;
+        each([&](int, unsigned long long key, unsigned long long w, unsigned long long, unsigned) {
+            if ((double)w >= wmin && sm_bin(h, sm_unkey((uint32_t)(key >> 32))) >= plan.mbin) t += w;
+        });
+        t = sm_block_scan(t, tot);
+        if (tid == SM_T - 1) sh[2] = t;
+        __syncthreads();
+        M = min(M, wmin > (double)SM_ONE ? SM_ONE : plan.m3_before + sh[2]);
+    }
     M = max(M, SM_ONE);
-    const float u = h.u > 0.0f ? h.u : 0.0f;
-    const unsigned long long t = u < 1.0f ? min((unsigned long long)((double)u * (double)M), M - 1) : M - 1;
-    each([&](unsigned long long key, unsigned long long w, unsigned long long run, unsigned) {
+    const unsigned long long t = sm_target(h.u, M);
+    each([&](int, unsigned long long key, unsigned long long w, unsigned long long run, unsigned) {
         if (run > t && run - w <= t) {
             a.out_tok[b] = (int)~(uint32_t)key;
             if (a.out_p) a.out_p[b] = (float)((double)w / (double)M);
@@ -436,7 +480,7 @@ __device__ __forceinline__ void sm_finish(const SampleArgs& a, int b, const SmHo
 // running sum (of weights, or of tokens) passes the target.  Six passes over the
 // row a border, in one block: for rows whose list would be too long.
 __device__ __forceinline__ void sm_by_keys(const SampleArgs& a, int b, const SmHow& h, const SmPlan& plan,
-                                           unsigned long long* hist, unsigned long long* sh) {
+                                           unsigned long long* hist, unsigned long long* sh, unsigned long long* tot) {
     constexpr int BITS = 11, ND = 1 << BITS;
     const int tid = threadIdx.x, lane = tid & 63;
     const size_t row = (size_t)b * a.ld;
@@ -496,20 +540,18 @@ __device__ __forceinline__ void sm_by_keys(const SampleArgs& a, int b, const SmH
     auto weight_of = [&](unsigned long long key) { return sm_weight(h, sm_unkey((uint32_t)(key >> 32))); };
     // a count's border: the weight up to and with that token
     auto sum_if = [&](auto take) {
-        __syncthreads();
-        if (tid == 0) sh[2] = 0;
-        __syncthreads();
         unsigned long long t = 0;
         each([&](int i, float l) {
             const unsigned long long w = sm_weight(h, l);
             if (take(sm_key64(l, i), w)) t += w;
         });
-        atomicAdd(&sh[2], t);
+        t = sm_block_scan(t, tot);
+        if (tid == SM_T - 1) sh[2] = t;
         __syncthreads();
         return sh[2];
     };
     unsigned long long M = plan.m1;
-    if (plan.kbin) {
+    if (!M) {
         const unsigned long long key = select(true, (unsigned long long)h.k - 1);
         M = sum_if([&](unsigned long long k, unsigned long long) { return k >= key; });
     }
@@ -523,8 +565,7 @@ __device__ __forceinline__ void sm_by_keys(const SampleArgs& a, int b, const SmH
         M = min(M, x > (double)SM_ONE ? SM_ONE : sum_if([&](unsigned long long, unsigned long long w) { return (double)w >= x; }));
     }
     M = max(M, SM_ONE);
-    const float u = h.u > 0.0f ? h.u : 0.0f;
-    const unsigned long long t = u < 1.0f ? min((unsigned long long)((double)u * (double)M), M - 1) : M - 1;
+    const unsigned long long t = sm_target(h.u, M);
     const unsigned long long key = select(false, t);
     if (tid == 0) {
         a.out_tok[b] = (int)~(uint32_t)key;
@@ -532,10 +573,10 @@ __device__ __forceinline__ void sm_by_keys(const SampleArgs& a, int b, const SmH
     }
 }
 
-__global__ void __launch_bounds__(SM_T)
+__global__ void __launch_bounds__(SM_T, 8)
 k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
     __shared__ unsigned long long key[SM_CAP], wt[SM_CAP], sh[4], wtot[16];
-    __shared__ unsigned flag, mark[SM_BINS / 32];
+    __shared__ unsigned flag, have, mark[SM_BINS / 32], bucket[2 * SM_T + 1], mbefore[SM_BINS / 32 + 1];
     const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x, lane = tid & 63;
     const size_t row = (size_t)b * a.ld;
     const int i1 = min((s + 1) * chunk, a.V);
@@ -550,6 +591,7 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
         return;
     }
     if (tid < SM_BINS / 32) mark[tid] = r.plan->mark[tid];
+    if (tid == 0) have = 0;
     __syncthreads();
     for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
         float v[8];
@@ -565,63 +607,95 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
             const unsigned long long who = __ballot(in);
             if (!who) continue;
             unsigned at = 0;
-            if (lane == 0) at = atomicAdd(&r.ticket[2], (unsigned)__popcll(who));
+            if (lane == 0) at = atomicAdd(&have, (unsigned)__popcll(who));
             at = __builtin_amdgcn_readfirstlane(at) + __popcll(who & ((1ull << lane) - 1));
-            if (in && at < SM_CAP) r.list[at] = make_ulonglong2(sm_key64(v[e], i0 + e * SM_T), w);
+            if (in && at < SM_CAP) {
+                key[at] = sm_key64(v[e], i0 + e * SM_T);
+                wt[at] = w;
+            }
         }
     }
-    if (SP > 1) {
-        if (!sm_last(r.ticket + 1, SP, &flag)) return;
-    } else {
-        __threadfence();
-        __syncthreads();
+    __syncthreads();
+    const unsigned mine = have;
+    if (tid == 0) flag = mine ? atomicAdd(&r.ticket[2], mine) : 0u;
+    __syncthreads();
+    const unsigned base = flag;
+    for (unsigned i = tid; i < min(mine, (unsigned)SM_CAP) && base + i < SM_CAP; i += SM_T) {
+        sm_put(&r.list[base + i].x, key[i]);
+        sm_put(&r.list[base + i].y, wt[i]);
     }
+    if (!sm_last(r.ticket + 1, SP, &flag)) return;
     const SmPlan& plan = *r.plan;
-    const int n = (int)r.ticket[2];         // tokens met, listed or not
+    const int n = (int)sm_get(&r.ticket[2]);         // tokens met, listed or not
     if (n > SM_CAP) {
-        sm_by_keys(a, b, h, plan, key, sh);
+        sm_by_keys(a, b, h, plan, key, sh, wtot);
         return;
     }
-    // the list in descending order of its keys (a bitonic network)
-    int n2 = 2;
-    while (n2 < n) n2 <<= 1;
-    for (int i = tid; i < n2; i += SM_T) {
-        const ulonglong2 x = i < n ? r.list[i] : make_ulonglong2(0ull, 0ull);
-        key[i] = x.x;
-        wt[i] = x.y;
+    // The list in descending order of its keys: a bucket for each part of each
+    // marked bin, then each token's rank in its bucket.  (Equal parts of the
+    // keys' range would put a bin into one bucket where the range spans 0: 50 us
+    // for 2000 tokens.)
+    constexpr int E = SM_CAP / SM_T, NB = 2 * SM_T;
+    if (tid == 0) {
+        unsigned t = 0;
+        for (int i = 0; i < SM_BINS / 32; i++) {
+            mbefore[i] = t;
+            t += (unsigned)__popc(mark[i]);
+        }
+        mbefore[SM_BINS / 32] = t;
     }
-    for (int k = 2; k <= n2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int i = tid; i < n2 / 2; i += SM_T) {
-                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                const unsigned long long x = key[lo], y = key[hi];
-                if ((x < y) == ((lo & k) == 0)) {
-                    key[lo] = y;
-                    key[hi] = x;
-                    const unsigned long long t = wt[lo];
-                    wt[lo] = wt[hi];
-                    wt[hi] = t;
-                }
-            }
+    bucket[tid] = bucket[tid + SM_T] = 0;
+    __syncthreads();
+    const int parts = NB / (int)mbefore[SM_BINS / 32];
+    ulonglong2 x[E];
+    unsigned at[E], bk[E];
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (tid + e * SM_T < n) {
+            x[e] = make_ulonglong2(sm_get(&r.list[tid + e * SM_T].x), sm_get(&r.list[tid + e * SM_T].y));
+            const float l = sm_unkey((uint32_t)(x[e].x >> 32));
+            const int bin = sm_bin(h, l);
+            // where in its bin (exact: monotone as the bin itself is)
+            const float z = l == h.mx ? 0.0f : __fmul_rn(__fsub_rn(h.mx, l), h.cb);
+            const int part = (int)fminf(__fmul_rn(__fsub_rn(z, (float)bin), (float)parts), (float)(parts - 1));
+            bk[e] = (mbefore[bin >> 5] + (unsigned)__popc(mark[bin >> 5] & ((1u << (bin & 31)) - 1))) * parts + part;
+            at[e] = atomicAdd(&bucket[bk[e]], 1u);
+        }
+    __syncthreads();
+    const unsigned b0 = bucket[2 * tid], b1 = bucket[2 * tid + 1];
+    const unsigned upto_b = (unsigned)sm_block_scan(b0 + b1, wtot);
+    bucket[2 * tid] = upto_b - b0 - b1;         // the buckets' first places
+    bucket[2 * tid + 1] = upto_b - b1;
+    if (tid == 0) bucket[NB] = (unsigned)n;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (tid + e * SM_T < n) key[bucket[bk[e]] + at[e]] = x[e].x;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (tid + e * SM_T < n) {
+            const unsigned first = bucket[bk[e]], end = bucket[bk[e] + 1];
+            at[e] = first;
+            for (unsigned i = first; i < end; i++) at[e] += key[i] > x[e].x;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (tid + e * SM_T < n) {
+            key[at[e]] = x[e].x;
+            wt[at[e]] = x[e].y;
         }
     __syncthreads();
     // running sums: 4 consecutive entries a thread
-    constexpr int E = SM_CAP / SM_T;
     unsigned long long run[E], t = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         if (E * tid + e < n) t += wt[E * tid + e];
         run[e] = t;
     }
-    unsigned long long upto = t;
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long x = __shfl_up(upto, o, JM_WAVE);
-        if (lane >= o) upto += x;
-    }
-    if (lane == 63) wtot[tid >> 6] = upto;
-    __syncthreads();
-    for (int i = 0; i < (tid >> 6); i++) upto += wtot[i];
+    const unsigned long long upto = sm_block_scan(t, wtot);
+    const bool counts = h.k > 0 && h.k < a.V;
     unsigned cnt[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
@@ -630,18 +704,18 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
         if (i >= n) continue;
         const int bin = sm_bin(h, sm_unkey((uint32_t)(key[i] >> 32)));
         run[e] += upto - t + r.umass[bin];
-        cnt[e] = i + 1 + r.ucnt[bin];
+        cnt[e] = i + 1 + (counts ? r.ucnt[bin] : 0u);
     }
-    sm_finish(a, b, h, plan, [&](auto f) {
+    sm_finish(a, b, h, plan, n, [&](auto f) {
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (E * tid + e < n) f(key[E * tid + e], wt[E * tid + e], run[e], cnt[e]);
-    }, sh);
+            if (E * tid + e < n) f(E * tid + e, key[E * tid + e], wt[E * tid + e], run[e], cnt[e]);
+    }, sh, wtot);
 }
 
-// Chunks of a row: two blocks a CU over all rows, at least 16 tokens a thread.
+// Chunks of a row: two blocks a CU over all rows, at least 8 tokens a thread.
 static int sm_chunks(int B, int V) {
-    return std::max(1, std::min(512 / B, (V + 16 * SM_T - 1) / (16 * SM_T)));
+    return std::max(1, std::min(512 / B, (V + 8 * SM_T - 1) / (8 * SM_T)));
 }
 
 size_t sample_ws_bytes(int B, int V) { return (size_t)B * sm_row_bytes(sm_chunks(B, V)); }
