@@ -1658,7 +1658,7 @@ hipError_t launch_attn(const AttnArgs& a, int qpk, float* att, hipStream_t st) {
         hipError_t e0 = hipGetLastError();
         if (e0 != hipSuccess) return e0;
         // (the partial outputs' buffers hold a.S ranges, one per 128 rows of the longest prefix)
-        Q4AttnPlan p = q4_attn_plan(c, a.H);
+        Q4AttnPlan p = q4_attn_plan(c, a.H, false, !a.append && a.shared);
         p.S = p.S < a.S ? p.S : a.S;
         return launch_q4_attn(c, p, att, false, (long long)a.H * 128, 128, a.H, a.rsdiv, att, a.part_o, a.part_ml, st);
     }

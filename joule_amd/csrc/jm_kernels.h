@@ -361,12 +361,14 @@ hipError_t launch_q4_write(const Q4KvArgs& c, const void* k, const void* v, bool
 // the same rows back, k, v [N][KH][128]
 hipError_t launch_q4_read(const Q4KvArgs& c, void* k, void* v, bool bf, hipStream_t st);
 // How an attention call is cut (jm_kvq4.hip): tokens a unit, units, ranges of
-// rows, and the floats of the partial outputs (0: none).
+// rows, row groups of the kernel for prompts (0: the one for few tokens), and the
+// floats of the partial outputs (0: none).  shared: the decoder's form with one
+// prompt's tokens, which all have the first one's planes.
 struct Q4AttnPlan {
-    int tp, units, S;
+    int tp, units, S, rg;
     size_t o_floats, ml_floats;
 };
-Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H);
+Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared);
 // out [N][H][128] = attention of q [N][H][128] over rows 0 .. the token's own
 hipError_t launch_q4_attn(const Q4KvArgs& c, const Q4AttnPlan& p, const void* q, bool bf, long long qts, long long qhs,
                           int H, float scale, void* out, float* part_o, float* part_ml, hipStream_t st);

@@ -91,8 +91,8 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 // to only 2^-14 of a sum: 7e-5 of the output instead of 5e-7.)
 //
 //   scores   v_mfma_f32_16x16x32_f16, 16 cache rows as A, the 8 query rows as B
-//            in columns n < 8, q brought to [1, 2) by a power of two and rounded
-//            to fp16, the rest of it times 2^11 in columns n + 8; one product a
+//            in columns n < 8, q brought to [2^10, 2^11) by a power of two and
+//            rounded to fp16, the rest of it in columns n + 8; one product a
 //            32 dimensions, one scale a group.  Lane (g, n) gets column n of rows
 //            4 g + i: with the two halves added (one DPP move), the scores of
 //            query row n % 8 at 8 rows of the tile.
@@ -102,7 +102,7 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 //            need no exchange between lanes.  Each lane sums its own weights.
 //   P . V    16 dimensions a product (dimension 16 j + m is row m of product j,
 //            nibble j of the lane's V dwords) as A, weight x scale in fp16, the
-//            rest times 2^11 in columns n + 8, as B, from the lanes that formed
+//            rest in columns n + 8, as B, from the lanes that formed
 //            them: contraction index 8 g + e is row 16 (e / 4) + 4 g + e % 4.
 // q and the weights carry 21 bits so; for bf16 queries (BF) q is exact without
 // the second half, and the weights are rounded to fp16 once (2^-11 of each).
@@ -178,14 +178,11 @@ struct Q4AttnArgs {
     float* part_ml;             // [units][KH][S][qpk tp][2]: ref, sum
 };
 
-constexpr float Q4_LO = 2048.0f;        // what the second halves are times
-
-// The two fp16 halves of a and b: the values rounded towards 0, and the rest
-// times 2^11.
+// The two fp16 halves of a and b: the values rounded towards 0, and the rest.
 __device__ __forceinline__ void split_f16x2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const float ra = __builtin_fmaf((float)h[0], -Q4_LO, __fmul_rn(a, Q4_LO));
-    const float rb = __builtin_fmaf((float)h[1], -Q4_LO, __fmul_rn(b, Q4_LO));
+    const float ra = __builtin_fmaf((float)h[0], -1.0f, a);
+    const float rb = __builtin_fmaf((float)h[1], -1.0f, b);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
 }
@@ -276,11 +273,10 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[st][e]));
         top = fmaxf(top, swz_xor16_f(top));
         top = fmaxf(top, __shfl_xor(top, 32, JM_WAVE));
-        // the power of two below the column's largest value
-        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 2u), 252u);
-        const float f = __uint_as_float((254u - ex) << 23);
-        // q's power of two, the scale and the halves' factor
-        lf = __fmul_rn(__fmul_rn(__uint_as_float(ex << 23), a.scale2), lo_col ? 1.0f / Q4_LO : 1.0f);
+        // q times a power of two, its largest value in [2^10, 2^11)
+        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 12u), 252u);
+        const float f = __uint_as_float((264u - ex) << 23);
+        lf = __fmul_rn(__uint_as_float((ex - 10u) << 23), a.scale2);
 #pragma unroll
         for (int st = 0; st < 4; st++) {
             uint32_t b[4];
@@ -418,7 +414,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float v = O[j][i] * (j & 1 ? 0.0625f : 1.0f);
-            o[i] = BF ? v : __builtin_fmaf(dpp_f<DPP_ROR8>(v), 1.0f / Q4_LO, v);
+            o[i] = BF ? v : __fadd_rn(v, dpp_f<DPP_ROR8>(v));
         }
         if (n < 8) *(float4*)&ow[w][n][16 * j + 4 * g] = make_float4(o[0], o[1], o[2], o[3]);
     }
@@ -492,6 +488,545 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }
 
+// ------------------------------------------------------- many query tokens
+//
+// The same for prompts: block (KV head, unit of RG x 32 QB query rows), 8 waves =
+// RG row groups x PS position strides; in a step wave (rg, ps) takes the 32 cache
+// rows ps of the step's 32 PS for its 32 QB query rows, with an online softmax,
+// and the PS waves of a row group merge once at the end.  The step's codes are
+// turned into fp16 once for all of them, in LDS, while the step before is
+// multiplied (two buffers, one barrier a step; the codes of the step after are on
+// their way).
+//
+//   scores   v_mfma_f32_32x32x16_f16, cache rows as A (lane l: row l % 32, the 8
+//            dimensions of the row's code dword 4 c + s with s = kk / 2, c = 2 (kk % 2)
+//            + l / 32), query rows as B: lane l holds query row l % 32 at cache
+//            rows 8 (v / 4) + 4 (l / 32) + v % 4
+//   P . V    V^T as A (lane l: dimension 32 nt + l % 32) from the rows' blocks of 4
+//            as the plane has them, the weights as B from the lanes that formed
+//            them: contraction index j of half h in step s is row 16 s + 8 (j / 4) +
+//            4 h + j % 4
+//
+// Two forms.  float32 queries: the codes less 8 are exact in LDS, q and the
+// weights are two fp16 halves each, every group's scores are scaled on their own
+// and the V scale goes into the weights, as in k_q4_attn.  bf16 queries (BF): K and
+// V are scaled in LDS and rounded to fp16 (2^-11 of the value, 2^-24 of the step's
+// largest), relative to the step's largest scale, whose exponent goes into the
+// scores and the weights; q is exact, the weights are fp16 once.  That is one
+// product where the other form takes two, no arithmetic on scales between them,
+// and 64 query rows a wave (QB = 2), which halves the LDS reads a product.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Byte offsets in a step's LDS: chunk p (16 bytes, one code dword) of cache row r
+// of K; chunk (s, h) of dimension d of V^T of 32-row tile t.  Spread over the
+// banks for the reads of 16 lanes.
+__device__ __forceinline__ int q4t_k(int r, int p) { return r * 256 + 16 * (p ^ (r & 15)); }
+__device__ __forceinline__ int q4t_v(int t, int d, int sh) { return t * 8192 + d * 64 + 16 * (sh ^ ((d >> 2) & 3)); }
+
+// 2^e as fp16, twice, for e in [-15, 15]
+__device__ __forceinline__ f16x2 q4t_pow2(int e) {
+    const _Float16 f = (_Float16)__uint_as_float((uint32_t)(127 + e) << 23);
+    return f16x2{f, f};
+}
+
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, JM_WAVE));
+    return v;
+}
+
+template <int NG, bool BF, int RG>
+__global__ void __launch_bounds__(512, 2)
+k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
+    constexpr int HD = 128, QB = BF ? 2 : 1, PS = 8 / RG, STEP = 32 * PS, ROWS = 32 * QB * RG;
+    constexpr int NI = STEP / 64;               // 16-byte code chunks a thread and step
+    constexpr int PB = STEP * 512;              // bytes of a step's K and V
+    __shared__ __align__(16) unsigned char kv[2][PB];
+    __shared__ __align__(16) uint16_t sc[BF ? 1 : 2][2][BF ? 8 : STEP * NG];     // the step's scales (float32 queries)
+    __shared__ float mls[8][32 * QB][2];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
+    const int kh = blockIdx.x % c.KH, u = a.units - 1 - (int)(blockIdx.x / c.KH);      // the longest prefixes first
+    Q4Unit un;
+    if (c.pos) {                                // the decoder's form: one prompt's tokens
+        un.seq = 0;
+        un.tok = u * a.tp;
+        un.n = min(a.tp, c.N - un.tok);
+        un.pos = 0;
+    } else if (!q4_unit(c, u, a.tp, un)) {
+        return;
+    }
+    // this lane's query rows, and the last cache row that each sees
+    int tok[QB], prow[QB], head[QB];
+    bool live[QB];
+    int pmax = -1, pmin = c.maxT;
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const int r = 32 * (QB * rg + b) + n, t = r / a.qpk;
+        live[b] = t < un.n;
+        tok[b] = un.tok + min(t, un.n - 1);
+        head[b] = kh * a.qpk + r % a.qpk;
+        prow[b] = c.pos ? c.pos[tok[b]] : un.pos + (tok[b] - un.tok);
+        live[b] = live[b] && prow[b] < c.maxT;
+        prow[b] = min(prow[b], c.maxT - 1);
+    }
+    for (int t = lane; t < un.n; t += 64) {     // (over the unit's tokens, the same in every wave)
+        const int p = min(c.pos ? c.pos[un.tok + t] : un.pos + t, c.maxT - 1);
+        pmax = max(pmax, p);
+        pmin = min(pmin, p);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        pmax = max(pmax, __shfl_xor(pmax, o, JM_WAVE));
+        pmin = min(pmin, __shfl_xor(pmin, o, JM_WAVE));
+    }
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    const int nstep = (pmax + STEP) / STEP;     // (0 where no token sees a row)
+    const Q4Head<NG> kk(q4_plane(c, un.seq, 0), kh, c.KH, c.R), vv(q4_plane(c, un.seq, 1), kh, c.KH, c.R);
+
+    // ---- a step's codes and scales on their way, and into LDS
+    struct Stage {
+        u32x4_t code[NI];
+        u32x4_t scl[NI][NG / 2];                // V: 4 rows' scales; K: the row's in the first words
+        uint32_t mk[STEP / 64][NG / 2], mv[STEP / 64][NG / 2];      // BF: one row a lane, for the step's largest
+    } sg;
+    auto request = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            const int item = tid + 512 * j;
+            if (item < STEP * 4) {
+                const int r = min(i * STEP + (item >> 2), c.R - 1);
+                sg.code[j] = *(gptr<const u32x4_t>)(kk.codes + (size_t)r * 16 + 4 * (item & 3));
+                const gptr<const uint32_t> s = (gptr<const uint32_t>)(kk.scales + (size_t)r * NG);
+#pragma unroll
+                for (int e = 0; e < NG / 2; e++) sg.scl[j][0][e] = s[e];
+            } else {
+                const int r = min(i * STEP + 4 * ((item - STEP * 4) >> 4), c.R - 4);
+                sg.code[j] = *(gptr<const u32x4_t>)(vv.codes + (size_t)r * 16 + 4 * (item & 15));
+#pragma unroll
+                for (int e = 0; e < NG / 2; e++) sg.scl[j][e] = ((gptr<const u32x4_t>)(vv.scales + (size_t)r * NG))[e];
+            }
+        }
+        if (BF) {
+#pragma unroll
+            for (int j = 0; j < STEP / 64; j++) {
+                const int r = min(i * STEP + 64 * j + lane, c.R - 1);
+#pragma unroll
+                for (int e = 0; e < NG / 2; e++) {
+                    sg.mk[j][e] = ((gptr<const uint32_t>)(kk.scales + (size_t)r * NG))[e];
+                    sg.mv[j][e] = ((gptr<const uint32_t>)(vv.scales + (size_t)r * NG))[e];
+                }
+            }
+        }
+    };
+    // BF: the exponents of the step's largest scales, and whether one that a
+    // token sees is not finite (its rows are then 0 in LDS and `taint` has them)
+    int ek[2] = {}, ev[2] = {};
+    uint32_t taint[QB] = {};
+    auto stage = [&](int i, int buf) __attribute__((always_inline)) {
+        unsigned char* const kb = kv[buf];
+        unsigned char* const vb = kv[buf] + STEP * 256;
+        f16x2 fk, fv;
+        if constexpr (BF) {
+            uint32_t bk = 0, bv = 0, bad = 0;
+#pragma unroll
+            for (int j = 0; j < STEP / 64; j++) {
+                const bool in = i * STEP + 64 * j + lane <= pmax;
+#pragma unroll
+                for (int e = 0; e < NG; e++) {
+                    const uint32_t sk = in ? (sg.mk[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu : 0u;
+                    const uint32_t sv = in ? (sg.mv[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu : 0u;
+                    bad |= (uint32_t)(sk >= 0x7C00u) | (uint32_t)(sv >= 0x7C00u);
+                    bk = max(bk, sk >= 0x7C00u ? 0u : sk);
+                    bv = max(bv, sv >= 0x7C00u ? 0u : sv);
+                }
+            }
+            ek[buf] = __builtin_amdgcn_readfirstlane((int)(wave_max_u(bk) >> 10) - 15);
+            ev[buf] = __builtin_amdgcn_readfirstlane((int)(wave_max_u(bv) >> 10) - 15);
+            fk = q4t_pow2(-ek[buf]);
+            fv = q4t_pow2(-ev[buf]);
+            if (__any(bad != 0)) {
+                // row by row: which of this lane's query rows see it
+#pragma unroll 1
+                for (int r = 0; r < STEP; r++) {
+                    const int row = i * STEP + r;
+                    if (row > pmax) break;
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int e = 0; e < NG; e++) {
+                        if ((*kk.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits = (1u << NG) - 1;
+                        if ((*vv.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits |= 1u << e;
+                    }
+#pragma unroll
+                    for (int b = 0; b < QB; b++) taint[b] |= row <= prow[b] ? bits : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            const int item = tid + 512 * j;
+            if (item < STEP * 4) {
+                const int r = item >> 2, cc = item & 3;
+                f16x2 s2[NG];
+                if constexpr (BF) {
+                    const bool in = i * STEP + r <= pmax;
+#pragma unroll
+                    for (int e = 0; e < NG; e++) {
+                        const uint32_t b = (sg.scl[j][0][e / 2] >> (16 * (e & 1))) & 0xFFFFu;
+                        const uint32_t x = in && (b & 0x7FFFu) < 0x7C00u ? b : 0u;
+                        s2[e] = __builtin_bit_cast(f16x2, x | x << 16) * fk;
+                    }
+                } else if (cc == 0) {
+#pragma unroll
+                    for (int e = 0; e < NG / 2; e++) *(uint32_t*)&sc[buf][0][r * NG + 2 * e] = sg.scl[j][0][e];
+                }
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const uint32_t d = sg.code[j][s], d8 = d >> 8;
+                    uint32_t o[4] = {q4_even(d), q4_odd(d), q4_even(d8), q4_odd(d8)};
+                    if constexpr (BF) {
+                        const f16x2 se = s2[s * NG / 4], so = se * (_Float16)0.0625f;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, o[e]) * (e & 1 ? so : se));
+                    }
+                    *(uint4*)(kb + q4t_k(r, 4 * cc + s)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            } else {
+                const int it = item - STEP * 4, blk = it >> 4, nn = it & 15;
+                // rows (0, 1) and (2, 3) of the block
+                uint32_t lo[2], hi[2];
+                f16x2 s2[2][NG];
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const uint32_t d0 = sg.code[j][2 * q], d1 = sg.code[j][2 * q + 1];
+                    lo[q] = __builtin_amdgcn_perm(d1, d0, 0x05040100u);
+                    hi[q] = __builtin_amdgcn_perm(d1, d0, 0x07060302u);
+                    if constexpr (BF) {
+#pragma unroll
+                        for (int e = 0; e < NG; e++) {
+                            uint32_t x = 0;
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const int at = (2 * q + k) * NG + e;
+                                const uint32_t b = (sg.scl[j][at / 8][(at % 8) / 2] >> (16 * (at & 1))) & 0xFFFFu;
+                                const bool in = i * STEP + 4 * blk + 2 * q + k <= pmax && (b & 0x7FFFu) < 0x7C00u;
+                                x |= (in ? b : 0u) << (16 * k);
+                            }
+                            s2[q][e] = __builtin_bit_cast(f16x2, x) * fv;
+                        }
+                    }
+                }
+                if constexpr (!BF) {
+                    if (nn == 0) {
+#pragma unroll
+                        for (int e = 0; e < NG / 2; e++) *(u32x4_t*)&sc[buf][1][4 * blk * NG + 8 * e] = sg.scl[j][e];
+                    }
+                }
+                // block b of the tile's 8: chunk (s, h) = (b / 4, b % 2), its half (b / 2) % 2
+                const int t = blk >> 3, b8 = blk & 7, sh = 2 * (b8 >> 2) + (b8 & 1), half = 8 * ((b8 >> 1) & 1);
+#pragma unroll
+                for (int jn = 0; jn < 8; jn++) {
+                    uint32_t o[2];
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const uint32_t d = (jn < 4 ? lo[q] : hi[q]) >> (jn & 2 ? 8 : 0);
+                        o[q] = jn & 1 ? q4_odd(d) : q4_even(d);
+                        if constexpr (BF) {
+                            const f16x2 s = s2[q][jn * NG / 8];
+                            o[q] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, o[q]) * (jn & 1 ? s * (_Float16)0.0625f : s));
+                        }
+                    }
+                    *(uint2*)(vb + q4t_v(t, 16 * jn + nn, sh) + half) = make_uint2(o[0], o[1]);
+                }
+            }
+        }
+    };
+
+    if (nstep > 0) request(0);
+
+    // ---- the query rows
+    f16x8 qh[QB][8], ql[BF ? 1 : 8];
+    float cs[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const size_t qi = (size_t)(tok[b] * a.qts + head[b] * a.qhs);
+        float x[8][8], top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int d = 32 * (k / 2) + 8 * (2 * (k % 2) + h);
+            float y[4];
+            load4<BF>(a.q, qi + d, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[k][e] = y[e];
+            load4<BF>(a.q, qi + d + 4, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[k][4 + e] = y[e];
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[k][e]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, JM_WAVE));
+        // its largest value in [2^10, 2^11), with the score scale's sign
+        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 12u), 252u);
+        const float f = __builtin_copysignf(__uint_as_float((264u - ex) << 23), a.scale2);
+        cs[b] = __fmul_rn(__uint_as_float((ex - 10u) << 23), fabsf(a.scale2));
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                split_f16x2(__fmul_rn(x[k][e], f), __fmul_rn(x[k][e + 4], f), hi[e], lo[e]);
+                if (!BF && (e & 1)) {           // codes 16 times too large
+                    hi[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, hi[e]) * (_Float16)0.0625f);
+                    lo[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo[e]) * (_Float16)0.0625f);
+                }
+            }
+            qh[b][k] = as_f16x8(hi[0], hi[1], hi[2], hi[3]);
+            if (!BF) ql[k] = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+
+    f32x16 O[QB][4];
+    float ref[QB], l[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        ref[b] = -INFINITY;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) O[b][nt][v] = 0.0f;
+    }
+    // raise a column's reference so that z (the largest exponent met) is at most
+    // 2^14 above it
+    auto raise = [&](int b, float z) __attribute__((always_inline)) {
+        if (__any(z > ref[b] + 14.0f)) {
+            z = fmaxf(z, __shfl_xor(z, 32, JM_WAVE));
+            const float nref = fmaxf(ref[b], z - 6.0f);
+            const float f = ref[b] == -INFINITY ? 0.0f : pow2f(ref[b] - nref);
+            l[b] *= f;
+#pragma unroll
+            for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) O[b][nt][v] *= f;
+            ref[b] = nref;
+        }
+    };
+
+    auto compute = [&](int i, int buf) __attribute__((always_inline)) {
+        const unsigned char* const kb = kv[buf] + ps * 8192;
+        const unsigned char* const vb = kv[buf] + STEP * 256;
+        const int t0 = i * STEP + 32 * ps;
+        if (t0 > pmax) return;
+        auto kop = [&](int k) __attribute__((always_inline)) {
+            return *(const f16x8*)(kb + q4t_k(n, 4 * (2 * (k % 2) + h) + k / 2));
+        };
+        auto vop = [&](int nt, int s) __attribute__((always_inline)) {
+            return *(const f16x8*)(vb + q4t_v(ps, 32 * nt + n, 2 * s + h));
+        };
+        if constexpr (BF) {
+            f32x16 S[QB];
+#pragma unroll
+            for (int b = 0; b < QB; b++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) S[b][v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const f16x8 x = kop(k);
+#pragma unroll
+                for (int b = 0; b < QB; b++) S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[b][k], S[b], 0, 0, 0);
+            }
+            const float fe = __uint_as_float((uint32_t)(127 + ek[buf]) << 23);
+            const float einv = __uint_as_float((uint32_t)(127 - ev[buf]) << 23);
+            f16x8 P[QB][2];
+#pragma unroll
+            for (int b = 0; b < QB; b++) {
+                if (t0 + 31 > pmin) {
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (t0 + 8 * (v / 4) + 4 * h + v % 4 > prow[b]) S[b][v] = -INFINITY;
+                }
+                float m = S[b][0];
+#pragma unroll
+                for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
+                const float cf = __fmul_rn(cs[b], fe);
+                raise(b, __builtin_fmaf(m, cf, (float)ev[buf]));
+                const float add = ref[b] == -INFINITY ? 0.0f : (float)ev[buf] - ref[b];
+                float x[16], t = 0.0f;
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    x[v] = pow2f(__builtin_fmaf(S[b][v], cf, add));
+                    t = __fadd_rn(t, x[v]);
+                }
+                l[b] = __builtin_fmaf(t, einv, l[b]);
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        p[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x[8 * s + 2 * e], (_Float16)x[8 * s + 2 * e + 1]});
+                    P[b][s] = as_f16x8(p[0], p[1], p[2], p[3]);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++) {
+                    const f16x8 x = vop(nt, s);
+#pragma unroll
+                    for (int b = 0; b < QB; b++) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, P[b][s], O[b][nt], 0, 0, 0);
+                }
+        } else {
+            // scales of cache row 8 q + 4 h + e, group g
+            auto scale = [&](int which, int q, int e, int g) __attribute__((always_inline)) {
+                return fp16_hw(sc[buf][which][(32 * ps + 8 * q + 4 * h + e) * NG + g]);
+            };
+            float y[16];
+#pragma unroll
+            for (int v = 0; v < 16; v++) y[v] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                f32x16 acc;
+#pragma unroll
+                for (int v = 0; v < 16; v++) acc[v] = 0.0f;
+#pragma unroll
+                for (int k = g * (8 / NG); k < (g + 1) * (8 / NG); k++) {
+                    const f16x8 x = kop(k);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[k], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[0][k], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int v = 0; v < 16; v++) y[v] = __builtin_fmaf(scale(0, v / 4, v % 4, g), acc[v], y[v]);
+            }
+            const bool edge = t0 + 31 > pmin;
+            float sv[16][NG];
+            float m = -INFINITY, sm = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const bool in = !edge || t0 + 8 * (v / 4) + 4 * h + v % 4 <= prow[0];
+                y[v] = in ? __fmul_rn(y[v], cs[0]) : -INFINITY;
+                m = fmaxf(m, y[v]);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    sv[v][g] = in ? scale(1, v / 4, v % 4, g) : 0.0f;
+                    sm = fmaxf(sm, sv[v][g]);
+                }
+            }
+            raise(0, m + (float)((int)(__float_as_uint(fmaxf(sm, 5.9604645e-8f)) >> 23) - 126));
+            const float r0 = ref[0] == -INFINITY ? 0.0f : ref[0];
+            float p[16];
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                p[v] = pow2f(__fsub_rn(y[v], r0));
+                l[0] = __fadd_rn(l[0], p[v]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        split_f16x2(__fmul_rn(p[8 * s + 2 * e], sv[8 * s + 2 * e][g]),
+                                    __fmul_rn(p[8 * s + 2 * e + 1], sv[8 * s + 2 * e + 1][g]), hi[e], lo[e]);
+                    const f16x8 ph = as_f16x8(hi[0], hi[1], hi[2], hi[3]), pl = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                    for (int nt = g * (4 / NG); nt < (g + 1) * (4 / NG); nt++) {
+                        const f16x8 x = vop(nt, s);
+                        O[0][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl, O[0][nt], 0, 0, 0);
+                        O[0][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph, O[0][nt], 0, 0, 0);
+                    }
+                }
+        }
+    };
+
+    if (nstep > 0) {
+        stage(0, 0);
+        if (nstep > 1) request(1);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < nstep; i += 2) {
+        if (i + 1 < nstep) {
+            stage(i + 1, 1);
+            if (i + 2 < nstep) request(i + 2);
+        }
+        compute(i, 0);
+        __syncthreads();
+        if (i + 1 >= nstep) break;
+        if (i + 2 < nstep) {
+            stage(i + 2, 0);
+            if (i + 3 < nstep) request(i + 3);
+        }
+        compute(i + 1, 1);
+        __syncthreads();
+    }
+
+    // ---- the PS waves of each row group merged, 32 dimensions at a time
+    float f[QB], inv[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        l[b] = __fadd_rn(l[b], __shfl_xor(l[b], 32, JM_WAVE));
+        if (h == 0) {
+            mls[w][32 * b + n][0] = ref[b];
+            mls[w][32 * b + n][1] = l[b];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int q = 0; q < PS; q++) M = fmaxf(M, mls[q * RG + rg][32 * b + n][0]);
+        const float m0 = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int q = 0; q < PS; q++)
+            L = __builtin_fmaf(mls[q * RG + rg][32 * b + n][1], pow2f(mls[q * RG + rg][32 * b + n][0] - m0), L);
+        f[b] = pow2f(ref[b] - m0);
+        inv[b] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);           // no row to see: 0
+        if constexpr (BF) {
+            // (every wave has staged every step: the masks are the same)
+            if (taint[b] != 0 && M == -INFINITY) inv[b] = 1.0f;
+        }
+    }
+    float4* const mb = (float4*)&kv[0][0];                                 // [wave][QB][4][64 lanes]
+    static_assert(8 * QB * 4 * 64 * 16 <= 2 * PB, "the outputs of 32 dimensions fit");
+#pragma unroll
+    for (int nt = 0; nt < 4; nt++) {
+        if (nt) __syncthreads();
+#pragma unroll
+        for (int b = 0; b < QB; b++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                // float32: the odd nibbles' dimensions (the upper 16 of 32) are 16 times too large
+                const float s = !BF && q >= 2 ? f[b] * 0.0625f : f[b];
+                mb[((w * QB + b) * 4 + q) * 64 + lane] = make_float4(O[b][nt][4 * q] * s, O[b][nt][4 * q + 1] * s,
+                                                                     O[b][nt][4 * q + 2] * s, O[b][nt][4 * q + 3] * s);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < QB; b++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if ((b * 4 + q) % PS != ps || !live[b]) continue;
+                float4 s = mb[((rg * QB + b) * 4 + q) * 64 + lane];
+#pragma unroll
+                for (int p = 1; p < PS; p++) {
+                    const float4 x = mb[(((p * RG + rg) * QB + b) * 4 + q) * 64 + lane];
+                    s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
+                }
+                s = make_float4(s.x * inv[b], s.y * inv[b], s.z * inv[b], s.w * inv[b]);
+                if (BF && (taint[b] >> ((32 * nt) / (HD / NG)) & 1)) {
+                    const float x = __uint_as_float(0x7FC00000u);
+                    s = make_float4(x, x, x, x);
+                }
+                store_out<BF>(a.out, ((size_t)tok[b] * a.H + head[b]) * HD + 32 * nt + 8 * q + 4 * h, s);
+            }
+    }
+}
+
 #define JM_Q4_CASE(NGV, BFV, KERNEL, GRID, BLK, ...)                                              \
     if (c.group == 128 / NGV && bf == BFV)                                                        \
         hipLaunchKernelGGL((KERNEL<NGV, BFV>), GRID, BLK, 0, st, __VA_ARGS__)
@@ -515,13 +1050,23 @@ hipError_t launch_q4_read(const Q4KvArgs& c, void* k, void* v, bool bf, hipStrea
     return hipGetLastError();
 }
 
-// How the attention of a call is cut: tokens a unit, units, ranges of rows.
-Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H) {
-    Q4AttnPlan p;
+// How the attention of a call is cut: tokens a unit, units, ranges of rows;
+// whether it takes k_q4_tile, and with how many row groups.
+Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared) {
+    Q4AttnPlan p{};
     const int qpk = H / c.KH;
+    const int n_seq = c.cu ? c.n_seq : shared ? 1 : c.N;
+    p.S = 1;
+    if ((long long)c.N * qpk >= 64ll * n_seq) {
+        for (p.rg = 4;; p.rg = 2) {
+            p.tp = 32 * (bf ? 2 : 1) * p.rg / qpk;
+            p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (p.tp - 1)) / p.tp);
+            if (p.rg == 2 || (long long)p.units * c.KH >= 256) return p;
+        }
+    }
     p.tp = c.cu ? 8 / qpk : 1;
     // (every sequence's tokens are rounded up to whole units)
-    p.units = (int)std::min<long long>(c.N, (long long)c.N / p.tp + c.n_seq);
+    p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (p.tp - 1)) / p.tp);
     const long long blocks = (long long)p.units * c.KH;
     // enough blocks for 4 a CU, at least 128 rows (a tile a wave) each
     p.S = (int)std::max<long long>(1, std::min<long long>((1024 + blocks - 1) / blocks, (c.maxT + 127) / 128));
@@ -539,6 +1084,16 @@ hipError_t launch_q4_attn(const Q4KvArgs& c, const Q4AttnPlan& p, const void* q,
     a.scale2 = scale * 1.4426950408889634f;
     a.out = out; a.units = p.units; a.S = p.S; a.part_o = part_o; a.part_ml = part_ml;
     const dim3 grid((unsigned)c.KH * p.units * p.S);
+    if (p.rg) {
+#define JM_Q4_TILE(NGV, BFV) \
+        if (c.group == 128 / NGV && bf == BFV) { \
+            if (p.rg == 4) hipLaunchKernelGGL((k_q4_tile<NGV, BFV, 4>), grid, dim3(512), 0, st, c, a); \
+            else hipLaunchKernelGGL((k_q4_tile<NGV, BFV, 2>), grid, dim3(512), 0, st, c, a); \
+        }
+        JM_Q4_TILE(2, false) JM_Q4_TILE(2, true) JM_Q4_TILE(4, false) JM_Q4_TILE(4, true)
+#undef JM_Q4_TILE
+        return hipGetLastError();
+    }
     JM_Q4_EACH(k_q4_attn, grid, dim3(256), c, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.S == 1) return e;

@@ -96,7 +96,7 @@ int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
     if (int rc = q4_tensor("q", q, dtype, q_token, q_head)) return rc;
     if (int rc = q4_tensor("out", out, dtype, 0, 0)) return rc;
     hipStream_t st = (hipStream_t)stream;
-    const jm::Q4AttnPlan p = jm::q4_attn_plan(a, n_heads);
+    const jm::Q4AttnPlan p = jm::q4_attn_plan(a, n_heads, dtype == JM_DTYPE_BF16, false);
     jm::PluginWs ws;
     if (p.o_floats)
         if (int rc = jm::plugin_ws(st, (p.o_floats + p.ml_floats) * 4, &ws)) return rc;
