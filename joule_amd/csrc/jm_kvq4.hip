@@ -110,22 +110,36 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(f16x8, make_uint4(a, b, c, d));
 }
 
 // The codes less 8 of nibbles 0 and 4 of w, and 16 times those of nibbles 1 and 5.
-__device__ __forceinline__ uint32_t q4_even(uint32_t w) {
-    const f16x2 h = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
-    return __builtin_bit_cast(uint32_t, h);
-}
-__device__ __forceinline__ uint32_t q4_odd(uint32_t w) {
-    const f16x2 h = __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
-    return __builtin_bit_cast(uint32_t, h);
-}
+// The constants come from registers (one of them a vector register), so that
+// each mask and exponent is one v_and_or_b32.
+struct Q4Bits {
+    uint32_t even = 0x000F000Fu, odd = 0x00F000F0u, one = 0x64006400u;
+    __device__ __forceinline__ Q4Bits() { __asm__("" : "+s"(even), "+s"(odd), "+v"(one)); }
+    __device__ __forceinline__ uint32_t lo(uint32_t w) const {
+        const f16x2 h = __builtin_bit_cast(f16x2, (w & even) | one) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    __device__ __forceinline__ uint32_t hi(uint32_t w) const {
+        const f16x2 h = __builtin_bit_cast(f16x2, (w & odd) | one) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+        return __builtin_bit_cast(uint32_t, h);
+    }
+};
 
 __device__ __forceinline__ float pow2f(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Above the exponent of the largest of some scales, given as fp16 bits (which
+// are in order): x < 2^q4_scale_exp(x).  At least that of 2^-14 (0 and the
+// subnormals; the largest of an infinity or NaN is above every finite one's).
+__device__ __forceinline__ float q4_scale_exp(uint32_t bits) {
+    return (float)((int)max((bits & 0x7FFFu) >> 10, 1u) - 14);
+}
 
 // The KV head's query rows of one unit: which sequence, its first token, how
 // many tokens, the first token's cache row.
@@ -170,7 +184,7 @@ __device__ __forceinline__ bool q4_unit(const Q4KvArgs& c, int u, int tp, Q4Unit
 struct Q4AttnArgs {
     const void* q;              // strides qts, qhs
     long long qts, qhs;
-    int H, qpk, tp;             // tp tokens a unit
+    int H, qpk, lq, tp;         // qpk = 2^lq; tp tokens a unit
     float scale2;               // score scale times log2(e)
     void* out;                  // [N][H][128]
     int units, S;
@@ -238,7 +252,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     Q4Unit un;
     if (!q4_unit(c, u, a.tp, un)) return;                   // (block-uniform)
     const int ncol = a.qpk * un.n;
-    const int ct = min(col / a.qpk, un.n - 1), head = kh * a.qpk + col % a.qpk;
+    const int ct = min(col >> a.lq, un.n - 1), head = kh * a.qpk + (col & (a.qpk - 1));
     const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
     const int crow = min(un.pos + ct, c.maxT - 1);          // and this column's
     const int NT = (last + 32) / 32;                        // (0 where last < 0)
@@ -296,6 +310,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; j++) O[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float ref = -INFINITY, l = 0.0f;
+    const Q4Bits bits;
 
     for (; t < t_end; t += 4) {
         if (t + 4 < t_end) q4_load_tile(nxt, kk, vv, t + 4, lane);
@@ -311,7 +326,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
                 for (int st = e * GS; st < (e + 1) * GS; st++) {
                     const uint32_t d = cur.k[rt][st], d8 = d >> 8;
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        as_f16x8(q4_even(d), q4_odd(d), q4_even(d8), q4_odd(d8)), qb[st], acc, 0, 0, 0);
+                        as_f16x8(bits.lo(d), bits.hi(d), bits.lo(d8), bits.hi(d8)), qb[st], acc, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[i] = __builtin_fmaf(q4_scale(cur.ks, rt, i, e), acc[i], S[i]);
@@ -395,9 +410,9 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             for (int b8 = 0; b8 < 2; b8++) {
                 const int j = 4 * h + 2 * b8, e = 16 * j / (HD / NG);
                 O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    as_f16x8(q4_even(v[0]), q4_even(v[1]), q4_even(v[2]), q4_even(v[3])), pb[e], O[j], 0, 0, 0);
+                    as_f16x8(bits.lo(v[0]), bits.lo(v[1]), bits.lo(v[2]), bits.lo(v[3])), pb[e], O[j], 0, 0, 0);
                 O[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    as_f16x8(q4_odd(v[0]), q4_odd(v[1]), q4_odd(v[2]), q4_odd(v[3])), pb[e], O[j + 1], 0, 0, 0);
+                    as_f16x8(bits.hi(v[0]), bits.hi(v[1]), bits.hi(v[2]), bits.hi(v[3])), pb[e], O[j + 1], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[i] >>= 8;
             }
@@ -442,9 +457,9 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
         L = __builtin_fmaf(mls[i][oc][1], f, L);
     }
     if (a.S == 1) {
-        if (un.pos + oc / a.qpk >= c.maxT) return;
+        if (un.pos + (oc >> a.lq) >= c.maxT) return;
         const float inv = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);       // no row to see: 0
-        const size_t oi = ((size_t)(un.tok + oc / a.qpk) * a.H + kh * a.qpk + oc % a.qpk) * HD + od;
+        const size_t oi = ((size_t)(un.tok + (oc >> a.lq)) * a.H + kh * a.qpk + (oc & (a.qpk - 1))) * HD + od;
         store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         return;
     }
@@ -465,7 +480,7 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     Q4Unit un;
     if (!q4_unit(c, u, a.tp, un)) return;
     const int oc = threadIdx.x >> 5, od = 4 * (threadIdx.x & 31), nc = a.qpk * a.tp;
-    if (oc >= a.qpk * un.n || un.pos + oc / a.qpk >= c.maxT) return;
+    if (oc >= a.qpk * un.n || un.pos + (oc >> a.lq) >= c.maxT) return;
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
     float M = -INFINITY;
     for (int s = 0; s < a.S; s++) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * nc)]);
@@ -484,7 +499,7 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
         L = __builtin_fmaf(a.part_ml[2 * pi + 1], f, L);
     }
     const float inv = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);
-    const size_t oi = ((size_t)(un.tok + oc / a.qpk) * a.H + kh * a.qpk + oc % a.qpk) * HD + od;
+    const size_t oi = ((size_t)(un.tok + (oc >> a.lq)) * a.H + kh * a.qpk + (oc & (a.qpk - 1))) * HD + od;
     store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }
 
@@ -530,10 +545,38 @@ __device__ __forceinline__ f16x2 q4t_pow2(int e) {
     return f16x2{f, f};
 }
 
+// Two codes times their scales, (q - 8) s 2^-10, in one fused multiply-add: the
+// codes' bits are the subnormals q 2^-24 (or 16 times that), and -8 s 2^-10 is
+// exact.  s is at most 2 (one scale of each half's row).
+struct Q4Scaled {
+    f16x2 even, odd, off;
+    __device__ __forceinline__ void set(f16x2 s) {
+        even = s * (_Float16)16384.0f;
+        odd = s * (_Float16)1024.0f;
+        off = s * (_Float16)-0.0078125f;
+    }
+    __device__ __forceinline__ uint32_t lo(uint32_t w) const {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, w & 0x000F000Fu), even, off));
+    }
+    __device__ __forceinline__ uint32_t hi(uint32_t w) const {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, w & 0x00F000F0u), odd, off));
+    }
+};
+
+// the largest over the wave, the same in every lane (DPP: within rows of 16, then
+// the row ends onto the rows behind)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, JM_WAVE));
-    return v;
+    v = dpp_max_u<0x111>(v);                // row_shr 1, 2, 4, 8
+    v = dpp_max_u<0x112>(v);
+    v = dpp_max_u<0x114>(v);
+    v = dpp_max_u<0x118>(v);
+    v = dpp_max_u<0x142>(v);                // row_bcast 15 and 31
+    v = dpp_max_u<0x143>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 template <int NG, bool BF, int RG>
@@ -545,6 +588,9 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     __shared__ __align__(16) unsigned char kv[2][PB];
     __shared__ __align__(16) uint16_t sc[BF ? 1 : 2][2][BF ? 8 : STEP * NG];     // the step's scales (float32 queries)
     __shared__ float mls[8][32 * QB][2];
+    // the second block of query rows of each row group (BF): with it in
+    // registers too, the compiler spills
+    __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % c.KH, u = a.units - 1 - (int)(blockIdx.x / c.KH);      // the longest prefixes first
@@ -563,10 +609,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     int pmax = -1, pmin = c.maxT;
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        const int r = 32 * (QB * rg + b) + n, t = r / a.qpk;
+        const int r = 32 * (QB * rg + b) + n, t = r >> a.lq;
         live[b] = t < un.n;
         tok[b] = un.tok + min(t, un.n - 1);
-        head[b] = kh * a.qpk + r % a.qpk;
+        head[b] = kh * a.qpk + (r & (a.qpk - 1));
         prow[b] = c.pos ? c.pos[tok[b]] : un.pos + (tok[b] - un.tok);
         live[b] = live[b] && prow[b] < c.maxT;
         prow[b] = min(prow[b], c.maxT - 1);
@@ -625,29 +671,43 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     // token sees is not finite (its rows are then 0 in LDS and `taint` has them)
     int ek[2] = {}, ev[2] = {};
     uint32_t taint[QB] = {};
+    const Q4Bits bits;
     auto stage = [&](int i, int buf) __attribute__((always_inline)) {
-        unsigned char* const kb = kv[buf];
-        unsigned char* const vb = kv[buf] + STEP * 256;
         f16x2 fk, fv;
         if constexpr (BF) {
-            uint32_t bk = 0, bv = 0, bad = 0;
+            // two scales a word; as whole numbers, in order
+            u16x2_t bk = 0, bv = 0;
 #pragma unroll
             for (int j = 0; j < STEP / 64; j++) {
-                const bool in = i * STEP + 64 * j + lane <= pmax;
+                const uint32_t in = i * STEP + 64 * j + lane <= pmax ? 0x7FFF7FFFu : 0u;
 #pragma unroll
-                for (int e = 0; e < NG; e++) {
-                    const uint32_t sk = in ? (sg.mk[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu : 0u;
-                    const uint32_t sv = in ? (sg.mv[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu : 0u;
-                    bad |= (uint32_t)(sk >= 0x7C00u) | (uint32_t)(sv >= 0x7C00u);
-                    bk = max(bk, sk >= 0x7C00u ? 0u : sk);
-                    bv = max(bv, sv >= 0x7C00u ? 0u : sv);
+                for (int e = 0; e < NG / 2; e++) {
+                    bk = __builtin_elementwise_max(bk, __builtin_bit_cast(u16x2_t, sg.mk[j][e] & in));
+                    bv = __builtin_elementwise_max(bv, __builtin_bit_cast(u16x2_t, sg.mv[j][e] & in));
                 }
             }
-            ek[buf] = __builtin_amdgcn_readfirstlane((int)(wave_max_u(bk) >> 10) - 15);
-            ev[buf] = __builtin_amdgcn_readfirstlane((int)(wave_max_u(bv) >> 10) - 15);
+            uint32_t mk = wave_max_u(max(bk.x, bk.y)), mv = wave_max_u(max(bv.x, bv.y));
+            const bool bad = mk >= 0x7C00u || mv >= 0x7C00u;       // (wave-uniform)
+            if (bad) {
+                // the largest finite ones
+                uint32_t fk1 = 0, fv1 = 0;
+#pragma unroll
+                for (int j = 0; j < STEP / 64; j++)
+#pragma unroll
+                    for (int e = 0; e < NG; e++) {
+                        const bool in = i * STEP + 64 * j + lane <= pmax;
+                        const uint32_t x = (sg.mk[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu, y = (sg.mv[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu;
+                        fk1 = max(fk1, in && x < 0x7C00u ? x : 0u);
+                        fv1 = max(fv1, in && y < 0x7C00u ? y : 0u);
+                    }
+                mk = wave_max_u(fk1);
+                mv = wave_max_u(fv1);
+            }
+            ek[buf] = (int)(mk >> 10) - 15;
+            ev[buf] = (int)(mv >> 10) - 15;
             fk = q4t_pow2(-ek[buf]);
             fv = q4t_pow2(-ev[buf]);
-            if (__any(bad != 0)) {
+            if (bad) {
                 // row by row: which of this lane's query rows see it
 #pragma unroll 1
                 for (int r = 0; r < STEP; r++) {
@@ -666,17 +726,18 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            const int item = tid + 512 * j;
+            int item = tid + 512 * j;
+            __asm__ volatile("" : "+v"(item));      // (its addresses anew each step)
             if (item < STEP * 4) {
                 const int r = item >> 2, cc = item & 3;
-                f16x2 s2[NG];
+                Q4Scaled s2[NG];
                 if constexpr (BF) {
                     const bool in = i * STEP + r <= pmax;
 #pragma unroll
                     for (int e = 0; e < NG; e++) {
                         const uint32_t b = (sg.scl[j][0][e / 2] >> (16 * (e & 1))) & 0xFFFFu;
                         const uint32_t x = in && (b & 0x7FFFu) < 0x7C00u ? b : 0u;
-                        s2[e] = __builtin_bit_cast(f16x2, x | x << 16) * fk;
+                        s2[e].set(__builtin_bit_cast(f16x2, x | x << 16) * fk);
                     }
                 } else if (cc == 0) {
 #pragma unroll
@@ -685,20 +746,20 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
                     const uint32_t d = sg.code[j][s], d8 = d >> 8;
-                    uint32_t o[4] = {q4_even(d), q4_odd(d), q4_even(d8), q4_odd(d8)};
+                    uint32_t o[4];
                     if constexpr (BF) {
-                        const f16x2 se = s2[s * NG / 4], so = se * (_Float16)0.0625f;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            o[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, o[e]) * (e & 1 ? so : se));
+                        const Q4Scaled& x = s2[s * NG / 4];
+                        o[0] = x.lo(d); o[1] = x.hi(d); o[2] = x.lo(d8); o[3] = x.hi(d8);
+                    } else {
+                        o[0] = bits.lo(d); o[1] = bits.hi(d); o[2] = bits.lo(d8); o[3] = bits.hi(d8);
                     }
-                    *(uint4*)(kb + q4t_k(r, 4 * cc + s)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *(uint4*)(kv[buf] + (q4t_k(r, 4 * cc) ^ (16 * s))) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
             } else {
                 const int it = item - STEP * 4, blk = it >> 4, nn = it & 15;
                 // rows (0, 1) and (2, 3) of the block
                 uint32_t lo[2], hi[2];
-                f16x2 s2[2][NG];
+                Q4Scaled s2[2][NG];
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
                     const uint32_t d0 = sg.code[j][2 * q], d1 = sg.code[j][2 * q + 1];
@@ -715,7 +776,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                                 const bool in = i * STEP + 4 * blk + 2 * q + k <= pmax && (b & 0x7FFFu) < 0x7C00u;
                                 x |= (in ? b : 0u) << (16 * k);
                             }
-                            s2[q][e] = __builtin_bit_cast(f16x2, x) * fv;
+                            s2[q][e].set(__builtin_bit_cast(f16x2, x) * fv);
                         }
                     }
                 }
@@ -733,13 +794,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
                         const uint32_t d = (jn < 4 ? lo[q] : hi[q]) >> (jn & 2 ? 8 : 0);
-                        o[q] = jn & 1 ? q4_odd(d) : q4_even(d);
-                        if constexpr (BF) {
-                            const f16x2 s = s2[q][jn * NG / 8];
-                            o[q] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, o[q]) * (jn & 1 ? s * (_Float16)0.0625f : s));
-                        }
+                        if constexpr (BF) o[q] = jn & 1 ? s2[q][jn * NG / 8].hi(d) : s2[q][jn * NG / 8].lo(d);
+                        else o[q] = jn & 1 ? bits.hi(d) : bits.lo(d);
                     }
-                    *(uint2*)(vb + q4t_v(t, 16 * jn + nn, sh) + half) = make_uint2(o[0], o[1]);
+                    *(uint2*)(kv[buf] + STEP * 256 + q4t_v(t, nn, sh) + half + 1024 * jn) = make_uint2(o[0], o[1]);
                 }
             }
         }
@@ -748,7 +806,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     if (nstep > 0) request(0);
 
     // ---- the query rows
-    f16x8 qh[QB][8], ql[BF ? 1 : 8];
+    f16x8 qh[8], ql[BF ? 1 : 8];
     float cs[QB];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
@@ -783,7 +841,8 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     lo[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo[e]) * (_Float16)0.0625f);
                 }
             }
-            qh[b][k] = as_f16x8(hi[0], hi[1], hi[2], hi[3]);
+            if (b == 0) qh[k] = as_f16x8(hi[0], hi[1], hi[2], hi[3]);
+            else if (ps == 0) q1[rg][k][lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if (!BF) ql[k] = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
         }
     }
@@ -816,17 +875,23 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     };
 
     auto compute = [&](int i, int buf) __attribute__((always_inline)) {
-        const unsigned char* const kb = kv[buf] + ps * 8192;
-        const unsigned char* const vb = kv[buf] + STEP * 256;
         const int t0 = i * STEP + 32 * ps;
         if (t0 > pmax) return;
+        // the operands' addresses from one each, an XOR at a time: kept in
+        // registers over the steps, the compiler spills others for them
+        int ka = ps * 8192 + q4t_k(n, 4 * h), va = q4t_v(ps, n, h);
+        __asm__ volatile("" : "+v"(ka), "+v"(va));
         auto kop = [&](int k) __attribute__((always_inline)) {
-            return *(const f16x8*)(kb + q4t_k(n, 4 * (2 * (k % 2) + h) + k / 2));
+            return *(const f16x8*)(kv[buf] + (ka ^ (16 * (8 * (k % 2) + k / 2))));
         };
         auto vop = [&](int nt, int s) __attribute__((always_inline)) {
-            return *(const f16x8*)(vb + q4t_v(ps, 32 * nt + n, 2 * s + h));
+            return *(const f16x8*)(kv[buf] + STEP * 256 + 2048 * nt + (va ^ (32 * s)));
         };
         if constexpr (BF) {
+            // 2^10 of the codes in LDS goes into the scores here, and that of V
+            // into the end
+            const float fe = __uint_as_float((uint32_t)(137 + ek[buf]) << 23);
+            const float einv = __uint_as_float((uint32_t)(127 - ev[buf]) << 23);
             f32x16 S[QB];
 #pragma unroll
             for (int b = 0; b < QB; b++)
@@ -834,12 +899,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 for (int v = 0; v < 16; v++) S[b][v] = 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const f16x8 x = kop(k);
-#pragma unroll
-                for (int b = 0; b < QB; b++) S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[b][k], S[b], 0, 0, 0);
+                const f16x8 x = kop(k), y = *(const f16x8*)&q1[rg][k][lane];
+                S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[k], S[0], 0, 0, 0);
+                S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, S[1], 0, 0, 0);
             }
-            const float fe = __uint_as_float((uint32_t)(127 + ek[buf]) << 23);
-            const float einv = __uint_as_float((uint32_t)(127 - ev[buf]) << 23);
             f16x8 P[QB][2];
 #pragma unroll
             for (int b = 0; b < QB; b++) {
@@ -854,21 +917,20 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 const float cf = __fmul_rn(cs[b], fe);
                 raise(b, __builtin_fmaf(m, cf, (float)ev[buf]));
                 const float add = ref[b] == -INFINITY ? 0.0f : (float)ev[buf] - ref[b];
-                float x[16], t = 0.0f;
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    x[v] = pow2f(__builtin_fmaf(S[b][v], cf, add));
-                    t = __fadd_rn(t, x[v]);
-                }
-                l[b] = __builtin_fmaf(t, einv, l[b]);
+                float t = 0.0f;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     uint32_t p[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        p[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x[8 * s + 2 * e], (_Float16)x[8 * s + 2 * e + 1]});
+                    for (int e = 0; e < 4; e++) {
+                        const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cf, add));
+                        const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cf, add));
+                        t = __fadd_rn(__fadd_rn(t, x0), x1);
+                        p[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x0, (_Float16)x1});
+                    }
                     P[b][s] = as_f16x8(p[0], p[1], p[2], p[3]);
                 }
+                l[b] = __builtin_fmaf(t, einv, l[b]);
             }
 #pragma unroll
             for (int s = 0; s < 2; s++)
@@ -879,10 +941,23 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     for (int b = 0; b < QB; b++) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, P[b][s], O[b][nt], 0, 0, 0);
                 }
         } else {
-            // scales of cache row 8 q + 4 h + e, group g
-            auto scale = [&](int which, int q, int e, int g) __attribute__((always_inline)) {
-                return fp16_hw(sc[buf][which][(32 * ps + 8 * q + 4 * h + e) * NG + g]);
+            // the scales of the lane's cache rows 8 q + 4 h + e, two a word
+            const uint16_t* const s0 = &sc[buf][0][(32 * ps + 4 * h) * NG];
+            auto load_scales = [&](int which, uint32_t (&x)[4][2 * NG]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int e = 0; e < NG / 2; e++) {
+                        const uint4 y = *(const uint4*)(s0 + which * STEP * NG + 8 * q * NG + 8 * e);
+                        x[q][4 * e] = y.x; x[q][4 * e + 1] = y.y; x[q][4 * e + 2] = y.z; x[q][4 * e + 3] = y.w;
+                    }
             };
+            auto scale = [&](const uint32_t (&x)[4][2 * NG], int v, int g) __attribute__((always_inline)) {
+                const int at = (v % 4) * NG + g;
+                return (float)__builtin_bit_cast(f16x2, x[v / 4][at / 2])[at % 2];
+            };
+            uint32_t sx[4][2 * NG];
+            load_scales(0, sx);
             float y[16];
 #pragma unroll
             for (int v = 0; v < 16; v++) y[v] = 0.0f;
@@ -895,32 +970,37 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 for (int k = g * (8 / NG); k < (g + 1) * (8 / NG); k++) {
                     const f16x8 x = kop(k);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[k], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[0][k], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[k], acc, 0, 0, 0);
                 }
 #pragma unroll
-                for (int v = 0; v < 16; v++) y[v] = __builtin_fmaf(scale(0, v / 4, v % 4, g), acc[v], y[v]);
+                for (int v = 0; v < 16; v++) y[v] = __builtin_fmaf(scale(sx, v, g), acc[v], y[v]);
             }
-            const bool edge = t0 + 31 > pmin;
-            float sv[16][NG];
-            float m = -INFINITY, sm = 0.0f;
+            load_scales(1, sx);
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const bool in = !edge || t0 + 8 * (v / 4) + 4 * h + v % 4 <= prow[0];
-                y[v] = in ? __fmul_rn(y[v], cs[0]) : -INFINITY;
-                m = fmaxf(m, y[v]);
+            for (int v = 0; v < 16; v++) y[v] = __fmul_rn(y[v], cs[0]);
+            if (t0 + 31 > pmin) {
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    sv[v][g] = in ? scale(1, v / 4, v % 4, g) : 0.0f;
-                    sm = fmaxf(sm, sv[v][g]);
+                for (int v = 0; v < 16; v++) {
+                    const bool in = t0 + 8 * (v / 4) + 4 * h + v % 4 <= prow[0];
+                    y[v] = in ? y[v] : -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < NG / 2; e++) sx[v / 4][(v % 4) * NG / 2 + e] = in ? sx[v / 4][(v % 4) * NG / 2 + e] : 0u;
                 }
             }
-            raise(0, m + (float)((int)(__float_as_uint(fmaxf(sm, 5.9604645e-8f)) >> 23) - 126));
+            float m = y[0];
+            u16x2_t sm = 0;
+#pragma unroll
+            for (int v = 1; v < 16; v++) m = fmaxf(m, y[v]);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int e = 0; e < 2 * NG; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sx[q][e]));
+            raise(0, m + q4_scale_exp(max(sm.x, sm.y)));
             const float r0 = ref[0] == -INFINITY ? 0.0f : ref[0];
-            float p[16];
 #pragma unroll
             for (int v = 0; v < 16; v++) {
-                p[v] = pow2f(__fsub_rn(y[v], r0));
-                l[0] = __fadd_rn(l[0], p[v]);
+                y[v] = pow2f(__fsub_rn(y[v], r0));
+                l[0] = __fadd_rn(l[0], y[v]);
             }
 #pragma unroll
             for (int g = 0; g < NG; g++)
@@ -928,9 +1008,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 for (int s = 0; s < 2; s++) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        split_f16x2(__fmul_rn(p[8 * s + 2 * e], sv[8 * s + 2 * e][g]),
-                                    __fmul_rn(p[8 * s + 2 * e + 1], sv[8 * s + 2 * e + 1][g]), hi[e], lo[e]);
+                    for (int e = 0; e < 4; e++) {
+                        const int v = 8 * s + 2 * e;
+                        split_f16x2(__fmul_rn(y[v], scale(sx, v, g)), __fmul_rn(y[v + 1], scale(sx, v + 1, g)), hi[e], lo[e]);
+                    }
                     const f16x8 ph = as_f16x8(hi[0], hi[1], hi[2], hi[3]), pl = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
                     for (int nt = g * (4 / NG); nt < (g + 1) * (4 / NG); nt++) {
@@ -1000,8 +1081,9 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         for (int b = 0; b < QB; b++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                // float32: the odd nibbles' dimensions (the upper 16 of 32) are 16 times too large
-                const float s = !BF && q >= 2 ? f[b] * 0.0625f : f[b];
+                // BF: 2^10 of V's codes; float32: the odd nibbles' dimensions (the
+                // upper 16 of 32) are 16 times too large
+                const float s = BF ? f[b] * 1024.0f : q >= 2 ? f[b] * 0.0625f : f[b];
                 mb[((w * QB + b) * 4 + q) * 64 + lane] = make_float4(O[b][nt][4 * q] * s, O[b][nt][4 * q + 1] * s,
                                                                      O[b][nt][4 * q + 2] * s, O[b][nt][4 * q + 3] * s);
             }
@@ -1080,7 +1162,7 @@ hipError_t launch_q4_attn(const Q4KvArgs& c, const Q4AttnPlan& p, const void* q,
                           int H, float scale, void* out, float* part_o, float* part_ml, hipStream_t st) {
     if (c.N == 0) return hipSuccess;
     Q4AttnArgs a{};
-    a.q = q; a.qts = qts; a.qhs = qhs; a.H = H; a.qpk = H / c.KH; a.tp = p.tp;
+    a.q = q; a.qts = qts; a.qhs = qhs; a.H = H; a.qpk = H / c.KH; a.lq = __builtin_ctz((unsigned)a.qpk); a.tp = p.tp;
     a.scale2 = scale * 1.4426950408889634f;
     a.out = out; a.units = p.units; a.S = p.S; a.part_o = part_o; a.part_ml = part_ml;
     const dim3 grid((unsigned)c.KH * p.units * p.S);
