@@ -638,42 +638,49 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         u32x4_t scl[NI][NG / 2];                // V: 4 rows' scales; K: the row's in the first words
         uint32_t mk[STEP / 64][NG / 2], mv[STEP / 64][NG / 2];      // BF: one row a lane, for the step's largest
     } sg;
+    // (rows of a step by halves of 64, which lie in the plane as wholes: past the
+    // end the last one again, whose rows are masked)
+    auto half_row = [&](int i, int half) __attribute__((always_inline)) { return min(i * STEP + 64 * half, c.R - 64); };
     auto request = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            const int item = tid + 512 * j;
-            if (item < STEP * 4) {
-                const int r = min(i * STEP + (item >> 2), c.R - 1);
-                sg.code[j] = *(gptr<const u32x4_t>)(kk.codes + (size_t)r * 16 + 4 * (item & 3));
-                const gptr<const uint32_t> s = (gptr<const uint32_t>)(kk.scales + (size_t)r * NG);
+            // (wave-uniform: which of K and V, and which half)
+            const int w8 = w + 8 * j;
+            if (w8 < STEP / 16) {
+                const int r0 = half_row(i, w8 / 4), r = 16 * (w8 % 4) + (lane >> 2);
+                sg.code[j] = *(gptr<const u32x4_t>)(kk.codes + (size_t)r0 * 16 + (uint32_t)(16 * r + 4 * (lane & 3)));
+                const gptr<const uint32_t> s = (gptr<const uint32_t>)(kk.scales + (size_t)r0 * NG) + (uint32_t)(r * NG / 2);
 #pragma unroll
                 for (int e = 0; e < NG / 2; e++) sg.scl[j][0][e] = s[e];
             } else {
-                const int r = min(i * STEP + 4 * ((item - STEP * 4) >> 4), c.R - 4);
-                sg.code[j] = *(gptr<const u32x4_t>)(vv.codes + (size_t)r * 16 + 4 * (item & 15));
+                const int wv = w8 - STEP / 16, r0 = half_row(i, wv / 4), r = 16 * (wv % 4) + 4 * (lane >> 4);
+                sg.code[j] = *(gptr<const u32x4_t>)(vv.codes + (size_t)r0 * 16 + (uint32_t)(16 * r + 4 * (lane & 15)));
 #pragma unroll
-                for (int e = 0; e < NG / 2; e++) sg.scl[j][e] = ((gptr<const u32x4_t>)(vv.scales + (size_t)r * NG))[e];
+                for (int e = 0; e < NG / 2; e++)
+                    sg.scl[j][e] = ((gptr<const u32x4_t>)(vv.scales + (size_t)r0 * NG + (uint32_t)(r * NG)))[e];
             }
         }
         if (BF) {
 #pragma unroll
             for (int j = 0; j < STEP / 64; j++) {
-                const int r = min(i * STEP + 64 * j + lane, c.R - 1);
+                const int r0 = half_row(i, j);
 #pragma unroll
                 for (int e = 0; e < NG / 2; e++) {
-                    sg.mk[j][e] = ((gptr<const uint32_t>)(kk.scales + (size_t)r * NG))[e];
-                    sg.mv[j][e] = ((gptr<const uint32_t>)(vv.scales + (size_t)r * NG))[e];
+                    sg.mk[j][e] = ((gptr<const uint32_t>)(kk.scales + (size_t)r0 * NG))[(uint32_t)(lane * NG / 2 + e)];
+                    sg.mv[j][e] = ((gptr<const uint32_t>)(vv.scales + (size_t)r0 * NG))[(uint32_t)(lane * NG / 2 + e)];
                 }
             }
         }
     };
     // BF: the exponents of the step's largest scales, and whether one that a
     // token sees is not finite (its rows are then 0 in LDS and `taint` has them)
-    int ek[2] = {}, ev[2] = {};
+    int ek = 0, ev = 0;
     uint32_t taint[QB] = {};
     const Q4Bits bits;
-    auto stage = [&](int i, int buf) __attribute__((always_inline)) {
+    auto stage = [&](int i) __attribute__((always_inline)) {
+        const int buf = i & 1;
         f16x2 fk, fv;
+        bool bad = false;
         if constexpr (BF) {
             // two scales a word; as whole numbers, in order
             u16x2_t bk = 0, bv = 0;
@@ -687,7 +694,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 }
             }
             uint32_t mk = wave_max_u(max(bk.x, bk.y)), mv = wave_max_u(max(bv.x, bv.y));
-            const bool bad = mk >= 0x7C00u || mv >= 0x7C00u;       // (wave-uniform)
+            bad = mk >= 0x7C00u || mv >= 0x7C00u;       // (wave-uniform)
             if (bad) {
                 // the largest finite ones
                 uint32_t fk1 = 0, fv1 = 0;
@@ -703,10 +710,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 mk = wave_max_u(fk1);
                 mv = wave_max_u(fv1);
             }
-            ek[buf] = (int)(mk >> 10) - 15;
-            ev[buf] = (int)(mv >> 10) - 15;
-            fk = q4t_pow2(-ek[buf]);
-            fv = q4t_pow2(-ev[buf]);
+            ek = (int)(mk >> 10) - 15;
+            ev = (int)(mv >> 10) - 15;
+            fk = q4t_pow2(-ek);
+            fv = q4t_pow2(-ev);
             if (bad) {
                 // row by row: which of this lane's query rows see it
 #pragma unroll 1
@@ -724,25 +731,45 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 }
             }
         }
+        if constexpr (BF) {
+            // scales that are not to be used are 0: rows behind pmax, and those
+            // that are not finite
+            if (bad || (i + 1) * STEP - 1 > pmax) {
+#pragma unroll
+                for (int j = 0; j < NI; j++) {
+                    const int w8 = w + 8 * j;
+                    const bool isk = w8 < STEP / 16;
+                    const int row = i * STEP + 64 * ((isk ? w8 : w8 - STEP / 16) / 4) + 16 * (w8 % 4) + (isk ? lane >> 2 : 4 * (lane >> 4));
+#pragma unroll
+                    for (int e = 0; e < 2 * NG; e++) {          // words, NG / 2 a row
+                        uint32_t x = sg.scl[j][e / 4][e % 4];
+                        if (row + 2 * e / NG > pmax) x = 0;
+                        if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
+                        if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu;
+                        sg.scl[j][e / 4][e % 4] = x;
+                    }
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            int item = tid + 512 * j;
-            __asm__ volatile("" : "+v"(item));      // (its addresses anew each step)
-            if (item < STEP * 4) {
-                const int r = item >> 2, cc = item & 3;
+            const int w8 = w + 8 * j;                           // (wave-uniform)
+            int ln = lane;
+            __asm__ volatile("" : "+v"(ln));                    // (the addresses anew each step)
+            if (w8 < STEP / 16) {
+                const int r = 16 * w8 + (ln >> 2), cc = ln & 3;
                 Q4Scaled s2[NG];
                 if constexpr (BF) {
-                    const bool in = i * STEP + r <= pmax;
 #pragma unroll
                     for (int e = 0; e < NG; e++) {
-                        const uint32_t b = (sg.scl[j][0][e / 2] >> (16 * (e & 1))) & 0xFFFFu;
-                        const uint32_t x = in && (b & 0x7FFFu) < 0x7C00u ? b : 0u;
-                        s2[e].set(__builtin_bit_cast(f16x2, x | x << 16) * fk);
+                        const uint32_t x = sg.scl[j][0][e / 2];
+                        s2[e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x, x, e & 1 ? 0x03020302u : 0x01000100u)) * fk);
                     }
                 } else if (cc == 0) {
 #pragma unroll
                     for (int e = 0; e < NG / 2; e++) *(uint32_t*)&sc[buf][0][r * NG + 2 * e] = sg.scl[j][0][e];
                 }
+                const int at = q4t_k(r, 4 * cc);
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
                     const uint32_t d = sg.code[j][s], d8 = d >> 8;
@@ -753,10 +780,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     } else {
                         o[0] = bits.lo(d); o[1] = bits.hi(d); o[2] = bits.lo(d8); o[3] = bits.hi(d8);
                     }
-                    *(uint4*)(kv[buf] + (q4t_k(r, 4 * cc) ^ (16 * s))) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *(uint4*)(kv[buf] + (at ^ (16 * s))) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
             } else {
-                const int it = item - STEP * 4, blk = it >> 4, nn = it & 15;
+                const int blk = 4 * (w8 - STEP / 16) + (ln >> 4), nn = ln & 15;
                 // rows (0, 1) and (2, 3) of the block
                 uint32_t lo[2], hi[2];
                 Q4Scaled s2[2][NG];
@@ -768,15 +795,9 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     if constexpr (BF) {
 #pragma unroll
                         for (int e = 0; e < NG; e++) {
-                            uint32_t x = 0;
-#pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                const int at = (2 * q + k) * NG + e;
-                                const uint32_t b = (sg.scl[j][at / 8][(at % 8) / 2] >> (16 * (at & 1))) & 0xFFFFu;
-                                const bool in = i * STEP + 4 * blk + 2 * q + k <= pmax && (b & 0x7FFFu) < 0x7C00u;
-                                x |= (in ? b : 0u) << (16 * k);
-                            }
-                            s2[q][e].set(__builtin_bit_cast(f16x2, x) * fv);
+                            const int a0 = (2 * q) * NG + e, a1 = a0 + NG;          // fp16 indices of the two rows
+                            const uint32_t x0 = sg.scl[j][a0 / 8][(a0 % 8) / 2], x1 = sg.scl[j][a1 / 8][(a1 % 8) / 2];
+                            s2[q][e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x1, x0, e & 1 ? 0x07060302u : 0x05040100u)) * fv);
                         }
                     }
                 }
@@ -788,6 +809,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                 }
                 // block b of the tile's 8: chunk (s, h) = (b / 4, b % 2), its half (b / 2) % 2
                 const int t = blk >> 3, b8 = blk & 7, sh = 2 * (b8 >> 2) + (b8 & 1), half = 8 * ((b8 >> 1) & 1);
+                unsigned char* const at = kv[buf] + STEP * 256 + q4t_v(t, nn, sh) + half;
 #pragma unroll
                 for (int jn = 0; jn < 8; jn++) {
                     uint32_t o[2];
@@ -797,7 +819,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                         if constexpr (BF) o[q] = jn & 1 ? s2[q][jn * NG / 8].hi(d) : s2[q][jn * NG / 8].lo(d);
                         else o[q] = jn & 1 ? bits.hi(d) : bits.lo(d);
                     }
-                    *(uint2*)(kv[buf] + STEP * 256 + q4t_v(t, nn, sh) + half + 1024 * jn) = make_uint2(o[0], o[1]);
+                    *(uint2*)(at + 1024 * jn) = make_uint2(o[0], o[1]);
                 }
             }
         }
@@ -874,29 +896,26 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
     };
 
-    auto compute = [&](int i, int buf) __attribute__((always_inline)) {
+    auto compute = [&](int i, int ek, int ev) __attribute__((always_inline)) {
+        const int buf = i & 1;
         const int t0 = i * STEP + 32 * ps;
         if (t0 > pmax) return;
         // the operands' addresses from one each, an XOR at a time: kept in
         // registers over the steps, the compiler spills others for them
-        int ka = ps * 8192 + q4t_k(n, 4 * h), va = q4t_v(ps, n, h);
+        int ka = buf * PB + ps * 8192 + q4t_k(n, 4 * h), va = buf * PB + STEP * 256 + q4t_v(ps, n, h);
         __asm__ volatile("" : "+v"(ka), "+v"(va));
         auto kop = [&](int k) __attribute__((always_inline)) {
-            return *(const f16x8*)(kv[buf] + (ka ^ (16 * (8 * (k % 2) + k / 2))));
+            return *(const f16x8*)(&kv[0][0] + (ka ^ (16 * (8 * (k % 2) + k / 2))));
         };
         auto vop = [&](int nt, int s) __attribute__((always_inline)) {
-            return *(const f16x8*)(kv[buf] + STEP * 256 + 2048 * nt + (va ^ (32 * s)));
+            return *(const f16x8*)(&kv[0][0] + 2048 * nt + (va ^ (32 * s)));
         };
         if constexpr (BF) {
             // 2^10 of the codes in LDS goes into the scores here, and that of V
             // into the end
-            const float fe = __uint_as_float((uint32_t)(137 + ek[buf]) << 23);
-            const float einv = __uint_as_float((uint32_t)(127 - ev[buf]) << 23);
-            f32x16 S[QB];
-#pragma unroll
-            for (int b = 0; b < QB; b++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) S[b][v] = 0.0f;
+            const float fe = __uint_as_float((uint32_t)(137 + ek) << 23);
+            const float einv = __uint_as_float((uint32_t)(127 - ev) << 23);
+            f32x16 S[QB] = {f32x16(0.0f), f32x16(0.0f)};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const f16x8 x = kop(k), y = *(const f16x8*)&q1[rg][k][lane];
@@ -915,8 +934,8 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
                 for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
                 const float cf = __fmul_rn(cs[b], fe);
-                raise(b, __builtin_fmaf(m, cf, (float)ev[buf]));
-                const float add = ref[b] == -INFINITY ? 0.0f : (float)ev[buf] - ref[b];
+                raise(b, __builtin_fmaf(m, cf, (float)ev));
+                const float add = ref[b] == -INFINITY ? 0.0f : (float)ev - ref[b];
                 float t = 0.0f;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
@@ -925,8 +944,9 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     for (int e = 0; e < 4; e++) {
                         const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cf, add));
                         const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cf, add));
-                        t = __fadd_rn(__fadd_rn(t, x0), x1);
-                        p[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x0, (_Float16)x1});
+                        const f16x2 x2 = {(_Float16)x0, (_Float16)x1};
+                        t = __builtin_amdgcn_fdot2(x2, f16x2{(_Float16)1.0f, (_Float16)1.0f}, t, false);
+                        p[e] = __builtin_bit_cast(uint32_t, x2);
                     }
                     P[b][s] = as_f16x8(p[0], p[1], p[2], p[3]);
                 }
@@ -1023,27 +1043,36 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
     };
 
-    if (nstep > 0) {
-        stage(0, 0);
+    // Step k is staged before the barrier that all waves pass before they multiply
+    // it.  Of the two waves of a SIMD (w and w + 4) one stages step k + 1 before it
+    // multiplies step k, the other after, so that the one's vector work falls to
+    // the other's products; in its code the second meets the barrier between
+    // staging k and multiplying it.
+    const bool ahead = w < 4;
+    auto meet = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    };
+    int ck = 0, cv = 0;                         // the exponents of the step to multiply
+    if (ahead) {
+        if (nstep > 0) stage(0);
         if (nstep > 1) request(1);
+        meet();
     }
-    __syncthreads();
 #pragma unroll 1
-    for (int i = 0; i < nstep; i += 2) {
-        if (i + 1 < nstep) {
-            stage(i + 1, 1);
-            if (i + 2 < nstep) request(i + 2);
+    for (int k = 0; k < nstep; k++) {
+        const int sk = ahead ? k + 1 : k;
+        if (ahead) { ck = ek; cv = ev; }
+        if (sk < nstep) {
+            stage(sk);
+            if (sk + 1 < nstep) request(sk + 1);
         }
-        compute(i, 0);
-        __syncthreads();
-        if (i + 1 >= nstep) break;
-        if (i + 2 < nstep) {
-            stage(i + 2, 0);
-            if (i + 3 < nstep) request(i + 3);
-        }
-        compute(i + 1, 1);
-        __syncthreads();
+        if (!ahead) { ck = ek; cv = ev; meet(); }
+        compute(k, ck, cv);
+        if (ahead) meet();
     }
+    if (!ahead) meet();
 
     // ---- the PS waves of each row group merged, 32 dimensions at a time
     float f[QB], inv[QB];
