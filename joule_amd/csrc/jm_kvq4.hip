@@ -525,11 +525,19 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
 // Two forms.  float32 queries: the codes less 8 are exact in LDS, q and the
 // weights are two fp16 halves each, every group's scores are scaled on their own
 // and the V scale goes into the weights, as in k_q4_attn.  bf16 queries (BF): K and
-// V are scaled in LDS and rounded to fp16 (2^-11 of the value, 2^-24 of the step's
-// largest), relative to the step's largest scale, whose exponent goes into the
-// scores and the weights; q is exact, the weights are fp16 once.  That is one
-// product where the other form takes two, no arithmetic on scales between them,
-// and 64 query rows a wave (QB = 2), which halves the LDS reads a product.
+// V are scaled in LDS and rounded to fp16 (2^-11 of the value, 2^-24 of the largest
+// of 16 rows), relative to the 16 rows' largest scale, whose exponent goes into the
+// scores and the weights; q is exact, the weights are fp16 once (their sum is of
+// the float32 ones: where 16 rows of V are far below the others, fp16 no longer
+// holds weights that count).  That is one product where the other form takes two,
+// no arithmetic on scales between them, and 64 query rows a wave (QB = 2), which
+// halves the LDS reads a product.
+//
+// Measured at 2047 tokens behind 4099 rows, 32 query heads on 8 (172 GFLOP, 147 us
+// at the rate of a large library product): 254 - 264 us.  Vector work bounds it:
+// a wave has some 300 vector instructions beside the step's 32 products, and two
+// waves of a SIMD, half a step apart, hide most but not all of it (270 us with
+// both in step).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -591,6 +599,8 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     // the second block of query rows of each row group (BF): with it in
     // registers too, the compiler spills
     __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
+    __shared__ int eb[2][STEP / 16][2];         // (BF) exponents of the 16-row blocks' scales, K and V
+    __shared__ uint32_t tn[8][32 * QB];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % c.KH, u = a.units - 1 - (int)(blockIdx.x / c.KH);      // the longest prefixes first
@@ -636,7 +646,6 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     struct Stage {
         u32x4_t code[NI];
         u32x4_t scl[NI][NG / 2];                // V: 4 rows' scales; K: the row's in the first words
-        uint32_t mk[STEP / 64][NG / 2], mv[STEP / 64][NG / 2];      // BF: one row a lane, for the step's largest
     } sg;
     // (rows of a step by halves of 64, which lie in the plane as wholes: past the
     // end the last one again, whose rows are masked)
@@ -660,110 +669,68 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     sg.scl[j][e] = ((gptr<const u32x4_t>)(vv.scales + (size_t)r0 * NG + (uint32_t)(r * NG)))[e];
             }
         }
-        if (BF) {
-#pragma unroll
-            for (int j = 0; j < STEP / 64; j++) {
-                const int r0 = half_row(i, j);
-#pragma unroll
-                for (int e = 0; e < NG / 2; e++) {
-                    sg.mk[j][e] = ((gptr<const uint32_t>)(kk.scales + (size_t)r0 * NG))[(uint32_t)(lane * NG / 2 + e)];
-                    sg.mv[j][e] = ((gptr<const uint32_t>)(vv.scales + (size_t)r0 * NG))[(uint32_t)(lane * NG / 2 + e)];
-                }
-            }
-        }
     };
-    // BF: the exponents of the step's largest scales, and whether one that a
-    // token sees is not finite (its rows are then 0 in LDS and `taint` has them)
-    int ek = 0, ev = 0;
+    // BF: the 16 rows of K or V that a wave stages are scaled by a power of two of
+    // their own, which goes to the step's multipliers through eb: 2^e just above
+    // their largest scale, and whether one of their scales is not finite (such
+    // scales are 0 in LDS; `taint` has which of this lane's query rows saw one)
     uint32_t taint[QB] = {};
     const Q4Bits bits;
     auto stage = [&](int i) __attribute__((always_inline)) {
         const int buf = i & 1;
-        f16x2 fk, fv;
-        bool bad = false;
-        if constexpr (BF) {
-            // two scales a word; as whole numbers, in order
-            u16x2_t bk = 0, bv = 0;
 #pragma unroll
-            for (int j = 0; j < STEP / 64; j++) {
-                const uint32_t in = i * STEP + 64 * j + lane <= pmax ? 0x7FFF7FFFu : 0u;
+        for (int j = 0; j < NI; j++) {
+            const int w8 = w + 8 * j;                           // (wave-uniform)
+            const bool isk = w8 < STEP / 16;
+            const int rb = isk ? w8 : w8 - STEP / 16;           // the 16-row block
+            int ln = lane;
+            __asm__ volatile("" : "+v"(ln));                    // (the addresses anew each step)
+            f16x2 fe;
+            if constexpr (BF) {
+                constexpr int NW = 2 * NG;                      // V: words of scales, NG / 2 a row; K: the first NG / 2
+                if (i * STEP + 16 * rb + 15 > pmax) {           // rows that nobody sees
+                    const int row = i * STEP + 16 * rb + (isk ? ln >> 2 : 4 * (ln >> 4));
 #pragma unroll
-                for (int e = 0; e < NG / 2; e++) {
-                    bk = __builtin_elementwise_max(bk, __builtin_bit_cast(u16x2_t, sg.mk[j][e] & in));
-                    bv = __builtin_elementwise_max(bv, __builtin_bit_cast(u16x2_t, sg.mv[j][e] & in));
+                    for (int e = 0; e < NW; e++)
+                        if (row + (isk ? 0 : 2 * e / NG) > pmax) sg.scl[j][e / 4][e % 4] = 0;
                 }
-            }
-            uint32_t mk = wave_max_u(max(bk.x, bk.y)), mv = wave_max_u(max(bv.x, bv.y));
-            bad = mk >= 0x7C00u || mv >= 0x7C00u;       // (wave-uniform)
-            if (bad) {
-                // the largest finite ones
-                uint32_t fk1 = 0, fv1 = 0;
+                auto largest = [&]() __attribute__((always_inline)) {
+                    u16x2_t m = 0;
+                    if (isk) {
 #pragma unroll
-                for (int j = 0; j < STEP / 64; j++)
+                        for (int e = 0; e < NG / 2; e++)
+                            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, sg.scl[j][0][e] & 0x7FFF7FFFu));
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < NG; e++) {
-                        const bool in = i * STEP + 64 * j + lane <= pmax;
-                        const uint32_t x = (sg.mk[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu, y = (sg.mv[j][e / 2] >> (16 * (e & 1))) & 0x7FFFu;
-                        fk1 = max(fk1, in && x < 0x7C00u ? x : 0u);
-                        fv1 = max(fv1, in && y < 0x7C00u ? y : 0u);
+                        for (int e = 0; e < NW; e++)
+                            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, sg.scl[j][e / 4][e % 4] & 0x7FFF7FFFu));
                     }
-                mk = wave_max_u(fk1);
-                mv = wave_max_u(fv1);
-            }
-            ek = (int)(mk >> 10) - 15;
-            ev = (int)(mv >> 10) - 15;
-            fk = q4t_pow2(-ek);
-            fv = q4t_pow2(-ev);
-            if (bad) {
-                // row by row: which of this lane's query rows see it
-#pragma unroll 1
-                for (int r = 0; r < STEP; r++) {
-                    const int row = i * STEP + r;
-                    if (row > pmax) break;
-                    uint32_t bits = 0;
+                    return wave_max_u(max(m.x, m.y));
+                };
+                uint32_t m = largest();
+                const bool bad = m >= 0x7C00u;
+                if (bad) {
 #pragma unroll
-                    for (int e = 0; e < NG; e++) {
-                        if ((*kk.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits = (1u << NG) - 1;
-                        if ((*vv.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits |= 1u << e;
-                    }
-#pragma unroll
-                    for (int b = 0; b < QB; b++) taint[b] |= row <= prow[b] ? bits : 0u;
-                }
-            }
-        }
-        if constexpr (BF) {
-            // scales that are not to be used are 0: rows behind pmax, and those
-            // that are not finite
-            if (bad || (i + 1) * STEP - 1 > pmax) {
-#pragma unroll
-                for (int j = 0; j < NI; j++) {
-                    const int w8 = w + 8 * j;
-                    const bool isk = w8 < STEP / 16;
-                    const int row = i * STEP + 64 * ((isk ? w8 : w8 - STEP / 16) / 4) + 16 * (w8 % 4) + (isk ? lane >> 2 : 4 * (lane >> 4));
-#pragma unroll
-                    for (int e = 0; e < 2 * NG; e++) {          // words, NG / 2 a row
+                    for (int e = 0; e < NW; e++) {
                         uint32_t x = sg.scl[j][e / 4][e % 4];
-                        if (row + 2 * e / NG > pmax) x = 0;
                         if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
                         if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu;
                         sg.scl[j][e / 4][e % 4] = x;
                     }
+                    m = largest();
                 }
+                const int e = (int)(m >> 10) - 15;
+                fe = q4t_pow2(-e);
+                if (lane == 0) eb[buf][rb][isk ? 0 : 1] = e + (bad ? 64 : 0);
             }
-        }
-#pragma unroll
-        for (int j = 0; j < NI; j++) {
-            const int w8 = w + 8 * j;                           // (wave-uniform)
-            int ln = lane;
-            __asm__ volatile("" : "+v"(ln));                    // (the addresses anew each step)
-            if (w8 < STEP / 16) {
-                const int r = 16 * w8 + (ln >> 2), cc = ln & 3;
+            if (isk) {
+                const int r = 16 * rb + (ln >> 2), cc = ln & 3;
                 Q4Scaled s2[NG];
                 if constexpr (BF) {
 #pragma unroll
                     for (int e = 0; e < NG; e++) {
                         const uint32_t x = sg.scl[j][0][e / 2];
-                        s2[e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x, x, e & 1 ? 0x03020302u : 0x01000100u)) * fk);
+                        s2[e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x, x, e & 1 ? 0x03020302u : 0x01000100u)) * fe);
                     }
                 } else if (cc == 0) {
 #pragma unroll
@@ -783,7 +750,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     *(uint4*)(kv[buf] + (at ^ (16 * s))) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
             } else {
-                const int blk = 4 * (w8 - STEP / 16) + (ln >> 4), nn = ln & 15;
+                const int blk = 4 * rb + (ln >> 4), nn = ln & 15;
                 // rows (0, 1) and (2, 3) of the block
                 uint32_t lo[2], hi[2];
                 Q4Scaled s2[2][NG];
@@ -797,7 +764,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                         for (int e = 0; e < NG; e++) {
                             const int a0 = (2 * q) * NG + e, a1 = a0 + NG;          // fp16 indices of the two rows
                             const uint32_t x0 = sg.scl[j][a0 / 8][(a0 % 8) / 2], x1 = sg.scl[j][a1 / 8][(a1 % 8) / 2];
-                            s2[q][e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x1, x0, e & 1 ? 0x07060302u : 0x05040100u)) * fv);
+                            s2[q][e].set(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(x1, x0, e & 1 ? 0x07060302u : 0x05040100u)) * fe);
                         }
                     }
                 }
@@ -896,7 +863,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
     };
 
-    auto compute = [&](int i, int ek, int ev) __attribute__((always_inline)) {
+    auto compute = [&](int i) __attribute__((always_inline)) {
         const int buf = i & 1;
         const int t0 = i * STEP + 32 * ps;
         if (t0 > pmax) return;
@@ -911,55 +878,84 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
             return *(const f16x8*)(&kv[0][0] + 2048 * nt + (va ^ (32 * s)));
         };
         if constexpr (BF) {
-            // 2^10 of the codes in LDS goes into the scores here, and that of V
-            // into the end
-            const float fe = __uint_as_float((uint32_t)(137 + ek) << 23);
-            const float einv = __uint_as_float((uint32_t)(127 - ev) << 23);
+            // the exponents of the tile's two 16-row blocks (2^10 of the codes in LDS
+            // goes into the scores here, and that of V into the end)
+            int ek[2], ev[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                ek[q] = __builtin_amdgcn_readfirstlane(eb[buf][2 * ps + q][0]);
+                ev[q] = __builtin_amdgcn_readfirstlane(eb[buf][2 * ps + q][1]);
+            }
+            if (max(max(ek[0], ek[1]), max(ev[0], ev[1])) > 31) {
+                // row by row: which of this lane's query rows see what is not finite
+#pragma unroll 1
+                for (int row = t0; row < t0 + 32 && row <= pmax; row++) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int e = 0; e < NG; e++) {
+                        if ((*kk.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits = (1u << NG) - 1;
+                        if ((*vv.scale(row, e) & 0x7FFFu) >= 0x7C00u) bits |= 1u << e;
+                    }
+#pragma unroll
+                    for (int b = 0; b < QB; b++) taint[b] |= row <= prow[b] ? bits : 0u;
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    if (ek[q] > 31) ek[q] -= 64;
+                    if (ev[q] > 31) ev[q] -= 64;
+                }
+            }
             f32x16 S[QB] = {f32x16(0.0f), f32x16(0.0f)};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const f16x8 x = kop(k), y = *(const f16x8*)&q1[rg][k][lane];
-                S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[k], S[0], 0, 0, 0);
-                S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, S[1], 0, 0, 0);
+                const f16x8 xk = kop(k);
+                S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xk, qh[k], S[0], 0, 0, 0);
+                S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xk, *(const f16x8*)&q1[rg][k][lane], S[1], 0, 0, 0);
             }
             f16x8 P[QB][2];
 #pragma unroll
             for (int b = 0; b < QB; b++) {
                 if (t0 + 31 > pmin) {
+                    const int lim = prow[b] - t0 - 4 * h;
 #pragma unroll
                     for (int v = 0; v < 16; v++)
-                        if (t0 + 8 * (v / 4) + 4 * h + v % 4 > prow[b]) S[b][v] = -INFINITY;
+                        if (8 * (v / 4) + v % 4 > lim) S[b][v] = -INFINITY;
                 }
-                float m = S[b][0];
+                // lane registers 0..7 are rows of the first block, 8..15 of the second
+                float cf[2], z[2];
 #pragma unroll
-                for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
-                const float cf = __fmul_rn(cs[b], fe);
-                raise(b, __builtin_fmaf(m, cf, (float)ev));
-                const float add = ref[b] == -INFINITY ? 0.0f : (float)ev - ref[b];
-                float t = 0.0f;
+                for (int q = 0; q < 2; q++) {
+                    float m = S[b][8 * q];
+#pragma unroll
+                    for (int v = 1; v < 8; v++) m = fmaxf(m, S[b][8 * q + v]);
+                    cf[q] = __fmul_rn(cs[b], __uint_as_float((uint32_t)(137 + ek[q]) << 23));
+                    z[q] = __builtin_fmaf(m, cf[q], (float)ev[q]);
+                }
+                raise(b, fmaxf(z[0], z[1]));
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
+                    const float add = ref[b] == -INFINITY ? 0.0f : (float)ev[s] - ref[b];
+                    float t = 0.0f;
                     uint32_t p[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cf, add));
-                        const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cf, add));
+                        const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cf[s], add));
+                        const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cf[s], add));
+                        t = __fadd_rn(t, __fadd_rn(x0, x1));
                         const f16x2 x2 = {(_Float16)x0, (_Float16)x1};
-                        t = __builtin_amdgcn_fdot2(x2, f16x2{(_Float16)1.0f, (_Float16)1.0f}, t, false);
                         p[e] = __builtin_bit_cast(uint32_t, x2);
                     }
                     P[b][s] = as_f16x8(p[0], p[1], p[2], p[3]);
+                    l[b] = __builtin_fmaf(t, __uint_as_float((uint32_t)(127 - ev[s]) << 23), l[b]);
                 }
-                l[b] = __builtin_fmaf(t, einv, l[b]);
             }
 #pragma unroll
-            for (int s = 0; s < 2; s++)
+            for (int k = 0; k < 8; k++) {
+                const int s = k / 4, nt = k % 4;
+                const f16x8 xv = vop(nt, s);
 #pragma unroll
-                for (int nt = 0; nt < 4; nt++) {
-                    const f16x8 x = vop(nt, s);
-#pragma unroll
-                    for (int b = 0; b < QB; b++) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, P[b][s], O[b][nt], 0, 0, 0);
-                }
+                for (int b = 0; b < QB; b++) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xv, P[b][s], O[b][nt], 0, 0, 0);
+            }
         } else {
             // the scales of the lane's cache rows 8 q + 4 h + e, two a word
             const uint16_t* const s0 = &sc[buf][0][(32 * ps + 4 * h) * NG];
@@ -999,9 +995,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
             for (int v = 0; v < 16; v++) y[v] = __fmul_rn(y[v], cs[0]);
             if (t0 + 31 > pmin) {
+                const int lim = prow[0] - t0 - 4 * h;
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
-                    const bool in = t0 + 8 * (v / 4) + 4 * h + v % 4 <= prow[0];
+                    const bool in = 8 * (v / 4) + v % 4 <= lim;
                     y[v] = in ? y[v] : -INFINITY;
 #pragma unroll
                     for (int e = 0; e < NG / 2; e++) sx[v / 4][(v % 4) * NG / 2 + e] = in ? sx[v / 4][(v % 4) * NG / 2 + e] : 0u;
@@ -1054,7 +1051,6 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     };
-    int ck = 0, cv = 0;                         // the exponents of the step to multiply
     if (ahead) {
         if (nstep > 0) stage(0);
         if (nstep > 1) request(1);
@@ -1063,13 +1059,12 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll 1
     for (int k = 0; k < nstep; k++) {
         const int sk = ahead ? k + 1 : k;
-        if (ahead) { ck = ek; cv = ev; }
         if (sk < nstep) {
             stage(sk);
             if (sk + 1 < nstep) request(sk + 1);
         }
-        if (!ahead) { ck = ek; cv = ev; meet(); }
-        compute(k, ck, cv);
+        if (!ahead) meet();
+        compute(k);
         if (ahead) meet();
     }
     if (!ahead) meet();
@@ -1082,6 +1077,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         if (h == 0) {
             mls[w][32 * b + n][0] = ref[b];
             mls[w][32 * b + n][1] = l[b];
+            if (BF) tn[w][32 * b + n] = taint[b];
         }
     }
     __syncthreads();
@@ -1097,8 +1093,8 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         f[b] = pow2f(ref[b] - m0);
         inv[b] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);           // no row to see: 0
         if constexpr (BF) {
-            // (every wave has staged every step: the masks are the same)
-            if (taint[b] != 0 && M == -INFINITY) inv[b] = 1.0f;
+#pragma unroll
+            for (int q = 0; q < PS; q++) taint[b] |= tn[q * RG + rg][32 * b + n];
         }
     }
     float4* const mb = (float4*)&kv[0][0];                                 // [wave][QB][4][64 lanes]

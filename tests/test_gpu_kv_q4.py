@@ -333,6 +333,25 @@ def test_small_rows_after_a_large_one():
     assert np.abs(got - want)[0, 0].max() <= (2.0 ** -18 * A[0, 0, 0] + 2.0 ** -17) * rest
 
 
+@pytest.mark.parametrize("counts", [[1], [130]])
+def test_a_few_rows_of_v_far_above_the_others(counts):
+    """The others hold no more than the weights' sum, which has to be whole: an
+    output is the few rows' share of it times their value, and relative to that
+    off by the weights' errors alone (2^-9 A of each score and 2^-11 of each weight
+    on both sides of the quotient) and the output's rounding."""
+    H, KH, n = 2, 1, 400
+    for first in (0, 128, 384):
+        c = _cache(1, 600, KH, H=H)
+        k, v = _rows(31, n, KH, torch.bfloat16), torch.zeros(n, KH, HD, dtype=torch.bfloat16, device="cuda")
+        v[first:first + 4] = 3e4
+        c.write(0, k, v, _int([0]), _int([0, n]))
+        st = [n - counts[0]]
+        q = (_randn(32, counts[0], H, HD) * 0.05).to(torch.bfloat16)
+        got = c.attention(0, q, _int(st), _int([0, counts[0]])).double().cpu().numpy()
+        want, A, _ = _want(c, q, st, counts, H)
+        assert (np.abs(got - want) <= (2.0 ** -8 * A + 2.0 ** -8 + 2.0 ** -10) * np.abs(want)).all()
+
+
 def test_strided_q_in_place_and_scale():
     H, KH, T = 8, 2, 90
     c = _cache(2, T, KH, H)
