@@ -21,57 +21,71 @@ __device__ __forceinline__ void load4(const void* p, size_t i, float (&v)[4]) {
     }
 }
 
+// 8 of them (aligned to 4).
+typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
 template <bool BF>
-__device__ __forceinline__ void store4(void* p, size_t i, const float (&v)[4]) {
-    if (BF) *(uint2*)((uint16_t*)p + i) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    else *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
+    if (BF) {
+        const u32x4_a8 u = *(const u32x4_a8*)((const uint16_t*)p + i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[2 * e] = __uint_as_float(u[e] << 16);
+            v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 u = *(const float4*)((const float*)p + i + e);
+            v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
+        }
+    }
 }
 
-// One wave per (token, KV head): lanes 0..31 the k row, 32..63 the v row.
+template <bool BF>
+__device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
+    if (BF) {
+        u32x4_a8 u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) u[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+        *(u32x4_a8*)((uint16_t*)p + i) = u;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) *(float4*)((float*)p + i + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    }
+}
+
+// Rows in and out: one wave per (KV head, 4 consecutive tokens), 16 lanes a row,
+// 8 dimensions a lane, so that a row moves in 16-byte pieces (the v codes change
+// hands between 8 lanes in registers); both are bound by memory.
 template <int NG, bool BF>
 __global__ void __launch_bounds__(256)
 k_q4_write(Q4KvArgs c, const void* __restrict__ k, const void* __restrict__ v, long long kts, long long khs,
            long long vts, long long vhs) {
-    const int lane = threadIdx.x & 63, j = lane & 31;
     const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = item / c.KH, kh = item % c.KH;
-    if (t >= c.N) return;
+    const int t0 = 4 * (item / c.KH), kh = item % c.KH, t = t0 + ((threadIdx.x & 63) >> 4);
     int seq, r;
-    if (!q4_place(c, t, seq, r)) return;
-    const bool isk = lane < 32;
-    float x[4];
-    load4<BF>(isk ? k : v, (size_t)(isk ? t * kts + kh * khs : t * vts + kh * vhs) + 4 * j, x);
-    const Q4Head<NG> h(q4_plane(c, seq, isk ? 0 : 1), kh, c.KH, c.R);
-    q4_store_row<NG>(x, isk, r, j, h);
+    if (t0 >= c.N || !q4_places(c, t0, seq, r)) return;
+    float x[8], y[8];
+    load8<BF>(k, (size_t)(t * kts + kh * khs) + 8 * q4_chunk(), x);
+    load8<BF>(v, (size_t)(t * vts + kh * vhs) + 8 * q4_chunk(), y);
+    q4_store_chunk<NG>(x, true, r, Q4Head<NG>(q4_plane(c, seq, 0), kh, c.KH, c.R));
+    q4_store_chunk<NG>(y, false, r, Q4Head<NG>(q4_plane(c, seq, 1), kh, c.KH, c.R));
 }
 
-// The rows back, one wave per (token, KV head): the exact values, bf16 rounded.
+// (the exact values, bf16 rounded)
 template <int NG, bool BF>
 __global__ void __launch_bounds__(256)
 k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
-    const int lane = threadIdx.x & 63, j = lane & 31;
     const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = item / c.KH, kh = item % c.KH;
-    if (t >= c.N) return;
+    const int t0 = 4 * (item / c.KH), kh = item % c.KH, t = t0 + ((threadIdx.x & 63) >> 4);
     int seq, r;
-    if (!q4_place(c, t, seq, r)) return;
-    const bool isk = lane < 32;
-    const Q4Head<NG> h(q4_plane(c, seq, isk ? 0 : 1), kh, c.KH, c.R);
-    const float s = fp16_hw(*h.scale(r, j / (32 / NG)));
-    float x[4];
-    if (isk) {
-        const int o = j >> 1;
-        const uint32_t w = *h.k_dword(r, 4 * (o & 3) + (o >> 2)) >> (16 * (j & 1));
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __fmul_rn((float)((int)((w >> (4 * e)) & 15u) - 8), s);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t w = *h.v_dword(r, 4 * (j & 3) + e) >> (4 * (j >> 2));
-            x[e] = __fmul_rn((float)((int)(w & 15u) - 8), s);
-        }
-    }
-    store4<BF>(isk ? k : v, (size_t)item * 128 + 4 * j, x);
+    if (t0 >= c.N || !q4_places(c, t0, seq, r)) return;
+    float x[8], y[8];
+    q4_load_chunk<NG>(x, true, r, Q4Head<NG>(q4_plane(c, seq, 0), kh, c.KH, c.R));
+    q4_load_chunk<NG>(y, false, r, Q4Head<NG>(q4_plane(c, seq, 1), kh, c.KH, c.R));
+    const size_t at = ((size_t)t * c.KH + kh) * 128 + 8 * q4_chunk();
+    store8<BF>(k, at, x);
+    store8<BF>(v, at, y);
 }
 
 // ---------------------------------------------------------------- attention
@@ -1145,14 +1159,14 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 hipError_t launch_q4_write(const Q4KvArgs& c, const void* k, const void* v, bool bf, const long long (&st4)[4],
                            hipStream_t st) {
     if (c.N == 0) return hipSuccess;
-    const dim3 grid((unsigned)(((long long)c.N * c.KH + 3) / 4));
+    const dim3 grid((unsigned)((((long long)c.N + 3) / 4 * c.KH + 3) / 4));
     JM_Q4_EACH(k_q4_write, grid, dim3(256), c, k, v, st4[0], st4[1], st4[2], st4[3]);
     return hipGetLastError();
 }
 
 hipError_t launch_q4_read(const Q4KvArgs& c, void* k, void* v, bool bf, hipStream_t st) {
     if (c.N == 0) return hipSuccess;
-    const dim3 grid((unsigned)(((long long)c.N * c.KH + 3) / 4));
+    const dim3 grid((unsigned)((((long long)c.N + 3) / 4 * c.KH + 3) / 4));
     JM_Q4_EACH(k_q4_read, grid, dim3(256), c, k, v);
     return hipGetLastError();
 }

@@ -68,39 +68,124 @@ __device__ __forceinline__ bool q4_place(const Q4KvArgs& c, int t, int& seq, int
     return p >= 0 && p < c.maxT;
 }
 
+// The same for the four tokens t0 .. t0 + 3 of a call (not the decoder's form) in
+// the wave's four rows of 16 lanes: each lane's row has its token's.
+__device__ __forceinline__ bool q4_places(const Q4KvArgs& c, int t0, int& seq, int& pos) {
+    const int lane = threadIdx.x & 63, i = lane >> 4, t = t0 + i;
+    seq = t;
+    int first = t;
+    if (c.cu) {
+        int n = 0;
+        for (int s = 0; s <= c.n_seq; s += 64) {
+            const int x = c.cu[min(s + lane, c.n_seq)];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int upto = __popcll(__ballot(s + lane <= c.n_seq && x <= t0 + q));
+                n += i == q ? upto : 0;
+            }
+        }
+        seq = n - 1;
+        if (t >= c.N || seq < 0 || seq >= c.n_seq) return false;
+        first = c.cu[seq];
+    } else if (t >= c.N || t >= c.n_seq) {
+        return false;
+    }
+    const long long p = (long long)c.start[seq] + (t - first);
+    pos = (int)(p < 0 ? -1 : p >= c.maxT ? c.maxT : p);
+    return p >= 0 && p < c.maxT;
+}
+
 __device__ __forceinline__ unsigned long long q4_plane(const Q4KvArgs& c, int seq, int which) {
     if (c.pos) return c.tab[((size_t)seq * c.L + c.layer) * 2 + which];
     return (unsigned long long)(uintptr_t)(which ? c.v : c.k) + (unsigned long long)seq * c.seq_stride;
 }
 
-// One head's 128 values of one row encoded by 32 lanes (an aligned half of the
-// wave; lane j holds dimensions 4 j .. + 3), k (isk) or v.  The quotient is the
-// correctly rounded fp32 one: scale's reciprocal rounded, then one Newton step
-// on the quotient with the exact remainder.
+// A group's scale from the bits of its largest magnitude (a NaN's are the
+// largest of all), and its values' codes + 8.  The quotient is the correctly
+// rounded fp32 one: the scale's reciprocal rounded, then one Newton step on the
+// quotient with the exact remainder.
+struct Q4Group {
+    uint32_t m;
+    _Float16 s16;
+    float s, inv;
+    __device__ __forceinline__ explicit Q4Group(uint32_t largest) : m(largest) {
+        const float top = m > 0x2B8CBCCCu ? __uint_as_float(m) : 1e-12f;       // (the bits of 1e-12f)
+        s16 = (_Float16)__fdiv_rn(top, 7.0f);
+        s = (float)s16;
+        inv = __fdiv_rn(1.0f, s);
+    }
+    __device__ __forceinline__ uint32_t code(float x) const {
+        const float a = __fmul_rn(x, inv);
+        const float f = __builtin_fmaf(__builtin_fmaf(-a, s, x), inv, a);
+        float n = fminf(fmaxf(rintf(f), -8.0f), 7.0f);
+        // a scale of 0 (a group below 7 * 2^-25): +-inf or NaN over 0
+        if (s == 0.0f) n = x > 0.0f ? 7.0f : x < 0.0f ? -8.0f : 0.0f;
+        // NaN, or an infinite scale: 0, and the scale makes the value non-finite
+        if (m >= 0x7F800000u || s == INFINITY) n = 0.0f;
+        return (uint32_t)((int)n + 8);
+    }
+};
+
+// 8 codes a lane and 8 lanes: nibble e of lane m against nibble m of lane e.
+__device__ __forceinline__ uint32_t q4_transpose(uint32_t d, int m) {
+    constexpr int XOR3 = 0x1B;              // quad_perm(3,2,1,0)
+    uint32_t o = (uint32_t)dpp_i<XOR3>(dpp_i<DPP_HALF_MIRROR>((int)d));     // lane ^ 4
+    d = __builtin_amdgcn_perm(o, d, m & 4 ? 0x03020706u : 0x05040100u);
+    o = (uint32_t)dpp_i<DPP_XOR2>((int)d);
+    d = __builtin_amdgcn_perm(o, d, m & 2 ? 0x03070105u : 0x06020400u);
+    o = (uint32_t)dpp_i<DPP_XOR1>((int)d);
+    const uint32_t keep = m & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+    return (d & keep) | ((m & 1 ? o >> 4 : o << 4) & ~keep);
+}
+
+// One head's 128 values of one row by 16 lanes (a row of the wave), lane 8 g + m
+// with the 8 dimensions from 8 q4_chunk() on; k (isk) or v.
+__device__ __forceinline__ int q4_chunk() { return 2 * (threadIdx.x & 7) + ((threadIdx.x >> 3) & 1); }
+__device__ __forceinline__ int q4_k_at(int chunk) { return 4 * (chunk & 3) + (chunk >> 2); }    // its dword of a k row
+
+template <int NG>
+__device__ __forceinline__ void q4_store_chunk(const float (&x)[8], bool isk, int r, const Q4Head<NG>& h) {
+    const int o = q4_chunk();
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    m = max(m, (uint32_t)dpp_i<DPP_XOR1>((int)m));
+    if (NG == 2) m = max(m, (uint32_t)dpp_i<DPP_XOR2>((int)m));
+    m = max(m, (uint32_t)dpp_i<DPP_ROR8>((int)m));
+    const Q4Group q(m);
+    uint32_t d = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) d |= q.code(x[e]) << (4 * e);
+    if (o % (16 / NG) == 0) *h.scale(r, o / (16 / NG)) = __builtin_bit_cast(uint16_t, q.s16);
+    const uint32_t y = q4_transpose(d, threadIdx.x & 7);
+    *(isk ? h.k_dword(r, q4_k_at(o)) : h.v_dword(r, threadIdx.x & 15)) = isk ? d : y;
+}
+
+template <int NG>
+__device__ __forceinline__ void q4_load_chunk(float (&x)[8], bool isk, int r, const Q4Head<NG>& h) {
+    const int o = q4_chunk();
+    uint32_t d = *(isk ? h.k_dword(r, q4_k_at(o)) : h.v_dword(r, threadIdx.x & 15));
+    const float s = fp16_hw(*h.scale(r, o / (16 / NG)));
+    const uint32_t y = q4_transpose(d, threadIdx.x & 7);
+    d = isk ? d : y;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = __fmul_rn((float)((int)((d >> (4 * e)) & 15u) - 8), s);
+}
+
+// The same store by 32 lanes (an aligned half of the wave; lane j holds
+// dimensions 4 j .. + 3), as the decoder's append has them.
 template <int NG>
 __device__ __forceinline__ void q4_store_row(const float (&x)[4], bool isk, int r, int j, const Q4Head<NG>& h) {
-    // the largest magnitude by its bits: a NaN is the largest of all
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
 #pragma unroll
     for (int o = 1; o < 32 / NG; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, JM_WAVE));
-    const float top = m > 0x2B8CBCCCu ? __uint_as_float(m) : 1e-12f;       // (the bits of 1e-12f)
-    const _Float16 s16 = (_Float16)__fdiv_rn(top, 7.0f);
-    const float s = (float)s16, inv = __fdiv_rn(1.0f, s);
+    const Q4Group g(m);
     uint32_t q[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const float a = __fmul_rn(x[e], inv);
-        const float f = __builtin_fmaf(__builtin_fmaf(-a, s, x[e]), inv, a);
-        float n = fminf(fmaxf(rintf(f), -8.0f), 7.0f);
-        // a scale of 0 (a group below 7 * 2^-25): +-inf or NaN over 0
-        if (s == 0.0f) n = x[e] > 0.0f ? 7.0f : x[e] < 0.0f ? -8.0f : 0.0f;
-        // NaN, or an infinite scale: 0, and the scale makes the value non-finite
-        if (m >= 0x7F800000u || s == INFINITY) n = 0.0f;
-        q[e] = (uint32_t)((int)n + 8);
-    }
-    if (j % (32 / NG) == 0) *h.scale(r, j / (32 / NG)) = __builtin_bit_cast(uint16_t, s16);
+    for (int e = 0; e < 4; e++) q[e] = g.code(x[e]);
+    if (j % (32 / NG) == 0) *h.scale(r, j / (32 / NG)) = __builtin_bit_cast(uint16_t, g.s16);
     if (isk) {
         const uint32_t half = q[0] | (q[1] << 4) | (q[2] << 8) | (q[3] << 12);
         const uint32_t other = (uint32_t)__shfl_xor((int)half, 1, JM_WAVE);
