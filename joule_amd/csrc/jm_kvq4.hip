@@ -496,22 +496,40 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     const int oc = threadIdx.x >> 5, od = 4 * (threadIdx.x & 31), nc = a.qpk * a.tp;
     if (oc >= a.qpk * un.n || un.pos + (oc >> a.lq) >= c.maxT) return;
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
+    // lane j of the 32 has the factors of ranges j, j + 32, ..; the ranges' outputs
+    // are on their way four at a time
+    const int j = threadIdx.x & 31, half = threadIdx.x & 32;
     float M = -INFINITY;
-    for (int s = 0; s < a.S; s++) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * nc)]);
+    for (int s = j; s < a.S; s += 32) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * nc)]);
+    M = seg_max<32>(M);
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float L = 0.0f;
-    for (int s = 0; s < a.S; s++) {
-        const size_t pi = p0 + (size_t)s * nc;
-        const float m = a.part_ml[2 * pi];
-        if (m == -INFINITY) continue;
-        const float f = pow2f(m - M);
-        const float4 x = *(const float4*)(a.part_o + pi * HD + od);
-        v.x = __builtin_fmaf(x.x, f, v.x);
-        v.y = __builtin_fmaf(x.y, f, v.y);
-        v.z = __builtin_fmaf(x.z, f, v.z);
-        v.w = __builtin_fmaf(x.w, f, v.w);
-        L = __builtin_fmaf(a.part_ml[2 * pi + 1], f, L);
+    for (int s0 = 0; s0 < a.S; s0 += 32) {
+        float f = 0.0f;
+        if (s0 + j < a.S) {
+            const float2 x = *(const float2*)(a.part_ml + 2 * (p0 + (size_t)(s0 + j) * nc));
+            if (x.x != -INFINITY) {
+                f = pow2f(x.x - M);
+                L = __builtin_fmaf(x.y, f, L);
+            }
+        }
+        for (int e = s0; e < min(s0 + 32, a.S); e += 4) {
+            float4 x[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                x[q] = *(const float4*)(a.part_o + (p0 + (size_t)min(e + q, a.S - 1) * nc) * HD + od);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float y = __shfl(f, half + e - s0 + q, JM_WAVE);
+                if (y == 0.0f) continue;        // (a range without a row has no output; past the end too)
+                v.x = __builtin_fmaf(x[q].x, y, v.x);
+                v.y = __builtin_fmaf(x[q].y, y, v.y);
+                v.z = __builtin_fmaf(x[q].z, y, v.z);
+                v.w = __builtin_fmaf(x[q].w, y, v.w);
+            }
+        }
     }
+    L = seg_sum<32>(L);
     const float inv = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);
     const size_t oi = ((size_t)(un.tok + (oc >> a.lq)) * a.H + kh * a.qpk + (oc & (a.qpk - 1))) * HD + od;
     store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));

@@ -14,7 +14,6 @@ are read and written only through these calls.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -46,6 +45,7 @@ class Q4KVCacheSet:
                 or data.data_ptr() % 16:
             raise ValueError(f"cache must be a contiguous 16-byte aligned uint8 CUDA tensor {full}")
         self.shape, self.B, self.group, self.data = shape, B, group, data
+        self._device = data.device
         base, seq = data.data_ptr(), L * 2 * plane
         self.table = (KVCache * (B * L))()
         for b in range(B):
@@ -54,53 +54,45 @@ class Q4KVCacheSet:
                 self.table[b * L + l].v = base + b * seq + l * 2 * plane + plane
         self._layers = [_lib.KvQ4(base + l * 2 * plane, base + l * 2 * plane + plane, seq, B, shape.maxT, shape.n_kv, group)
                         for l in range(L)]
+        self._refs = [ctypes.byref(x) for x in self._layers]
 
     # ------------------------------------------------------------ arguments
 
     def _layer(self, l: int):
         if not 0 <= l < len(self._layers):
             raise ValueError(f"layer {l} outside [0, {len(self._layers)})")
-        return ctypes.byref(self._layers[l])
+        return self._refs[l]
 
     def _tokens(self, start, cu, n: int) -> None:
         """start [B] and cu [B + 1] (or None: one token a sequence)."""
         for t, name, size in ((start, "start", self.B), (cu, "cu", self.B + 1)):
             if t is None and name == "cu":
                 continue
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.data.device \
-                    or tuple(t.shape) != (size,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous int32 tensor [{size}] on {self.data.device}")
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self._device \
+                    or t.shape != (size,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 tensor [{size}] on {self._device}")
         if cu is None and n != self.B:
             raise ValueError(f"without cu there is one token a sequence: {n} tokens, {self.B} sequences")
 
     def _heads(self, t, name: str, n: int, heads: int, dtype=None) -> None:
         """t is [n, heads, 128] in float32 or bfloat16, its rows contiguous."""
-        if not isinstance(t, torch.Tensor) or t.device != self.data.device or t.dtype not in _DTYPES \
+        if not isinstance(t, torch.Tensor) or t.device != self._device or t.dtype not in _DTYPES \
                 or (dtype is not None and t.dtype != dtype):
             raise ValueError(f"{name} must be a {'float32 or bfloat16' if dtype is None else dtype} tensor "
-                             f"on {self.data.device}")
-        if tuple(t.shape) != (n, heads, HD):
+                             f"on {self._device}")
+        if t.shape != (n, heads, HD):
             raise ValueError(f"{name} must be [{n}, {heads}, {HD}], got {list(t.shape)}")
-        if t.numel() and (t.stride(2) != 1 or t.stride(0) % 4 or t.stride(1) % 4
-                          or t.data_ptr() % (4 * t.element_size())):
+        ts, hs, one = t.stride()
+        if n and (one != 1 or ts % 4 or hs % 4 or t.data_ptr() % (16 if t.dtype == torch.float32 else 8)):
             raise ValueError(f"{name}: rows of {HD} contiguous values, strides and address multiples of 4 elements")
 
     def _out(self, t, name: str, shape: tuple, dtype):
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=self.data.device)
+            return torch.empty(shape, dtype=dtype, device=self._device)
         self._heads(t, name, shape[0], shape[1], dtype)
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         return t
-
-    def _on(self, stream):
-        """The cache's device, with `stream` (or its current one) current: the
-        outputs are allocated there."""
-        ctx = contextlib.ExitStack()
-        ctx.enter_context(torch.cuda.device(self.data.device))
-        if stream is not None:
-            ctx.enter_context(torch.cuda.stream(stream))
-        return ctx
 
     # ------------------------------------------------------------ operators
 
@@ -118,10 +110,10 @@ class Q4KVCacheSet:
         self._heads(k, "k", n, self.shape.n_kv)
         self._heads(v, "v", n, self.shape.n_kv, k.dtype)
         self._tokens(start, cu, n)
-        with self._on(stream):
+        with _lib.on(self._device, stream):
             _lib.check(_lib.lib().jm_kv_q4_write(
-                self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, _lib.ptr(k), k.stride(0), k.stride(1),
-                _lib.ptr(v), v.stride(0), v.stride(1), _DTYPES[k.dtype], _lib.stream_handle()), "jm_kv_q4_write")
+                self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, _lib.ptr(k), *k.stride()[:2],
+                _lib.ptr(v), *v.stride()[:2], _DTYPES[k.dtype], _lib.stream_handle()), "jm_kv_q4_write")
 
     def read(self, l: int, start: torch.Tensor, cu: torch.Tensor | None = None, n: int | None = None,
              dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None, v: torch.Tensor | None = None,
@@ -139,7 +131,7 @@ class Q4KVCacheSet:
         if dtype not in _DTYPES:
             raise ValueError("dtype must be float32 or bfloat16")
         self._tokens(start, cu, n)
-        with self._on(stream):
+        with _lib.on(self._device, stream):
             k = self._out(k, "k", (n, self.shape.n_kv, HD), dtype)
             v = self._out(v, "v", (n, self.shape.n_kv, HD), dtype)
             _lib.check(_lib.lib().jm_kv_q4_read(
@@ -157,10 +149,10 @@ class Q4KVCacheSet:
         n, H = (q.shape[0], q.shape[1]) if isinstance(q, torch.Tensor) and q.dim() == 3 else (-1, self.shape.n_heads)
         self._heads(q, "q", n, H)
         self._tokens(start, cu, n)
-        with self._on(stream):
+        with _lib.on(self._device, stream):
             out = self._out(out, "out", (n, H, HD), q.dtype)
             _lib.check(_lib.lib().jm_kv_q4_attn(
-                self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, _lib.ptr(q), q.stride(0), q.stride(1), H,
+                self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, _lib.ptr(q), *q.stride()[:2], H,
                 HD ** -0.5 if scale is None else float(scale), _DTYPES[q.dtype], _lib.ptr(out),
                 _lib.stream_handle()), "jm_kv_q4_attn")
         return out

@@ -5,7 +5,6 @@ order of summation)."""
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -52,16 +51,15 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Ten
             how.top_k = int(value)
         else:
             setattr(how, name, float(value))
-    with contextlib.ExitStack() as on:
-        on.enter_context(torch.cuda.device(dev))
-        if stream is not None:
-            on.enter_context(torch.cuda.stream(stream))
+    with _lib.on(dev, stream):
         if out_tok is None:
             out_tok = torch.empty(B, dtype=torch.int32, device=dev)
-        check_tensor(out_tok, "out_tok", (B,), torch.int32, dev)
+        else:
+            check_tensor(out_tok, "out_tok", (B,), torch.int32, dev)
         if out_p is None:
             out_p = torch.empty(B, dtype=torch.float32, device=dev)
-        check_tensor(out_p, "out_p", (B,), torch.float32, dev)
+        else:
+            check_tensor(out_p, "out_p", (B,), torch.float32, dev)
         _lib.check(_lib.lib().jm_sample(_lib.ptr(logits), _DTYPES[logits.dtype], max(V, logits.stride(0)), B, V,
                                         ctypes.byref(how), _lib.ptr(u), _lib.ptr(out_tok), _lib.ptr(out_p),
                                         _lib.stream_handle()), "jm_sample")
