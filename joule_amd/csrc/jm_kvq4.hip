@@ -1207,8 +1207,16 @@ Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared) {
     // (every sequence's tokens are rounded up to whole units)
     p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (p.tp - 1)) / p.tp);
     const long long blocks = (long long)p.units * c.KH;
-    // enough blocks for 4 a CU, at least 128 rows (a tile a wave) each
-    p.S = (int)std::max<long long>(1, std::min<long long>((1024 + blocks - 1) / blocks, (c.maxT + 127) / 128));
+    // Ranges: a block a CU while each has 128 rows (a tile a wave), up to 4 a CU
+    // while each has 512.  (Measured with float32 queries, both kernels: one
+    // sequence of 777 rows 10.3 us, with 256 rows a block 10.4; 8 sequences of 2048
+    // 11.6 us on 256 blocks, 14.6 on 1024; 6 sequences' drafts over up to 5000 rows
+    // 22.0 us on 256 blocks, 19.4 on 1024; bfloat16, 32 sequences of 16384: 115 us
+    // without a split, 104 with 1024 blocks.)
+    auto ranges = [&](long long want, int rows) {
+        return std::min((want + blocks - 1) / blocks, ((long long)c.maxT + rows - 1) / rows);
+    };
+    p.S = (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
     const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;
     p.ml_floats = p.S > 1 ? cols * 2 : 0;
