@@ -21,9 +21,13 @@
 // A row whose marked bins hold more than SM_CAP tokens (many equal logits, a
 // very high temperature) is selected by its keys instead, in the last kernel.
 //
-// Bound: the logits are read three times, the first time from memory, and 20
-// float64 operations a token in the histogram; a row takes three launches and
-// two hand-overs between its chunks however short it is.
+// Bound: the logits are read three times, the first time from memory, 20 float64
+// operations and a 64-bit LDS addition a token in the histogram; a row takes three
+// launches and two hand-overs between its chunks however short it is.  Measured
+// (151936 float32 logits a row; kernels alone): one row 3.2 + 10.0 + 10.5 us, 7
+// rows of 50304 3.4 + 13.3 + 8.0, 128 rows with settings of their own 13.3 + 43 + 35
+// (read once at the rate of a copy: 16); at 128 rows, both hand-overs taken off,
+// the histogram is three and the list two times as long as the reading.
 #include <algorithm>
 
 #include "jm_device.h"
@@ -51,6 +55,7 @@ struct SmPlan {
 struct SmRow {
     unsigned* ticket;           // [2] chunks done of the two kernels that hand over; [2]: the list's length
     float2* cmm;                // [SP] largest and smallest logit of the chunk
+    float* wmx;                 // [SP][SM_T / 64] largest of each wave's
     SmPlan* plan;
     unsigned long long* umass;  // [SM_BINS] weight of the unmarked bins before a bin
     unsigned* ucnt;             // [SM_BINS]
@@ -60,7 +65,7 @@ struct SmRow {
 };
 
 __host__ __device__ __forceinline__ size_t sm_row_bytes(int SP) {
-    return 16 + ((size_t)SP * 8 + 15) / 16 * 16 + (sizeof(SmPlan) + 15) / 16 * 16 + (size_t)SM_BINS * 12 * (1 + SP) +
+    return 16 + ((size_t)SP * 8 + 15) / 16 * 16 + (size_t)SP * (SM_T / 16) + (sizeof(SmPlan) + 15) / 16 * 16 + (size_t)SM_BINS * 12 * (1 + SP) +
            (size_t)SM_CAP * 16;
 }
 
@@ -69,6 +74,7 @@ __device__ __forceinline__ SmRow sm_row(char* ws, int b, int SP) {
     char* p = ws + (size_t)b * sm_row_bytes(SP);
     r.ticket = (unsigned*)p; p += 16;
     r.cmm = (float2*)p; p += ((size_t)SP * 8 + 15) / 16 * 16;
+    r.wmx = (float*)p; p += (size_t)SP * (SM_T / 16);
     r.plan = (SmPlan*)p; p += (sizeof(SmPlan) + 15) / 16 * 16;
     r.list = (ulonglong2*)p; p += (size_t)SM_CAP * 16;
     r.umass = (unsigned long long*)p; p += (size_t)SM_BINS * 8;
@@ -214,8 +220,9 @@ k_sample_max(SampleArgs a, char* ws, int SP, int chunk) {
         red[0][tid >> 6] = mx;
         red[1][tid >> 6] = mn;
     }
-    __syncthreads();
     const SmRow r = sm_row(ws, b, SP);
+    if ((tid & 63) == 0) r.wmx[s * (SM_T / 64) + (tid >> 6)] = mx;
+    __syncthreads();
     if (tid == 0) {
         for (int i = 1; i < SM_T / 64; i++) {
             mx = fmaxf(mx, red[0][i]);
@@ -266,11 +273,27 @@ __device__ __forceinline__ void sm_find(F pass, int* out) {
 }
 static_assert(SM_BINS == SM_T, "a bin a thread");
 
+// A logit that at least k <= 64 of the row's are not below: the k-th of the
+// maxima of 64 parts of it (or fewer); by one wave.
+__device__ __forceinline__ float sm_kth_part(const SmRow& r, int SP, int k) {
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY;
+    for (int i = lane; i < SP * (SM_T / 64); i += 64) m = fmaxf(m, r.wmx[i]);
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i++) {
+        const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), i));
+        above += x > m || (x == m && i < lane);
+    }
+    return __shfl(m, __builtin_ctzll(__ballot(above == k - 1)), JM_WAVE);
+}
+
 __global__ void __launch_bounds__(SM_T, 8)
 k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     __shared__ unsigned long long mass[SM_BINS], incl[SM_BINS], wtot[16];
     __shared__ unsigned cnt[SM_BINS], cincl[SM_BINS], flag, mark[SM_BINS / 32];
     __shared__ int found[5];
+    __shared__ float least;
     const int b = blockIdx.x / SP, s = blockIdx.x % SP, tid = threadIdx.x, lane = tid & 63;
     const size_t row = (size_t)b * a.ld;
     const int i1 = min((s + 1) * chunk, a.V);
@@ -282,6 +305,13 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     const bool counts = h.k > 0 && h.k < a.V, few = counts && h.k <= SM_CAP / 4;
     mass[tid] = 0;
     cnt[tid] = 0;
+    // What is below the k-th largest need not be counted: worth its finding, 1.5 us,
+    // where a thread has many tokens (top-k 50 of 151936: 128 rows 64 us without, 60
+    // with it; one row, 8 tokens a thread, 24.7 and 27.0).
+    if (few && tid < 64) {
+        const float x = h.k <= 64 && chunk >= 16 * SM_T ? sm_kth_part(r, SP, h.k) : -INFINITY;
+        if (tid == 0) least = x;
+    }
     __syncthreads();
     if (h.mx > -INFINITY)
         for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
@@ -295,6 +325,7 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
                 for (int e = 0; e < 8; e++) {
                     // (the last bin, where everything far below piles up, is
                     // what is taken if the others do not reach k)
+                    if (!(v[e] >= least)) continue;
                     const int bin = sm_bin(h, v[e]);
                     if (bin < SM_BINS - 1) atomicAdd(&cnt[bin], 1u);
                 }
@@ -593,12 +624,22 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
     if (tid < SM_BINS / 32) mark[tid] = r.plan->mark[tid];
     if (tid == 0) have = 0;
     __syncthreads();
+    // the first and the end of the marked bins; most tokens are outside
+    const uint32_t mw = lane < SM_BINS / 32 ? mark[lane] : 0u;
+    const unsigned long long mb = __ballot(mw != 0);
+    const int wa = mb ? __builtin_ctzll(mb) : 0, wz = mb ? 63 - __builtin_clzll(mb) : 0;
+    const uint32_t ma = (uint32_t)__builtin_amdgcn_readlane((int)mw, wa), mz = (uint32_t)__builtin_amdgcn_readlane((int)mw, wz);
+    const float za = ma ? (float)(32 * wa + __builtin_ctz(ma)) : 0.0f;
+    const int be = mz ? 32 * wz + 32 - __builtin_clz(mz) : 0;
+    const float zz = be < SM_BINS ? (float)be : __uint_as_float(0x7FC00000u);     // (the last bin has no end)
     for (int i0 = s * chunk + tid; i0 - tid < i1; i0 += 8 * SM_T) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
 #pragma unroll
         for (int e = 0; e < 8; e++) {
+            const float z = __fmul_rn(__fsub_rn(h.mx, v[e]), h.cb);
+            if (!__any(!(z < za || z >= zz))) continue;
             const int bin = sm_bin(h, v[e]);
             bool in = i0 + e * SM_T < i1 && (mark[bin >> 5] >> (bin & 31) & 1);
             if (!__any(in)) continue;
@@ -713,7 +754,8 @@ k_sample_pick(SampleArgs a, char* ws, int SP, int chunk) {
     }, sh, wtot);
 }
 
-// Chunks of a row: two blocks a CU over all rows, at least 8 tokens a thread.
+// Chunks of a row: two blocks a CU over all rows (128 rows: 94 us; one 105, four
+// 98, eight 115), at least 8 tokens a thread.
 static int sm_chunks(int B, int V) {
     return std::max(1, std::min(512 / B, (V + 8 * SM_T - 1) / (8 * SM_T)));
 }
