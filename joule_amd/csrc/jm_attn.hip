@@ -1657,9 +1657,11 @@ hipError_t launch_attn(const AttnArgs& a, int qpk, float* att, hipStream_t st) {
         else hipLaunchKernelGGL(k_kv_append_q4<4>, ga, gb, 0, st, a, c, att);
         hipError_t e0 = hipGetLastError();
         if (e0 != hipSuccess) return e0;
-        // (the partial outputs' buffers hold a.S ranges, one per 128 rows of the longest prefix)
+        // (the partial outputs' buffers hold a.S ranges of the tokens, one per 128 rows
+        // of the longest prefix; units may round the tokens up)
         Q4AttnPlan p = q4_attn_plan(c, a.H, false, !a.append && a.shared);
-        p.S = p.S < a.S ? p.S : a.S;
+        const long long fit = (long long)a.S * a.B / ((long long)p.units * p.tp);
+        p.S = fit < 1 ? 1 : p.S < fit ? p.S : (int)fit;
         return launch_q4_attn(c, p, att, false, (long long)a.H * 128, 128, a.H, a.rsdiv, att, a.part_o, a.part_ml, st);
     }
     if (!a.append) {

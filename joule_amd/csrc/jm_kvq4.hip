@@ -226,6 +226,10 @@ __device__ __forceinline__ void store_out(void* p, size_t i, float4 v) {
     else *(float4*)((float*)p + i) = v;
 }
 
+// Whether a running maximum and sum are those of no row at all (a NaN among the
+// scores leaves the maximum, but not the sum).
+__device__ __forceinline__ bool q4_dead(float ref, float sum) { return ref == -INFINITY && sum == 0.0f; }
+
 // One tile of 32 cache rows as a lane gets it: 16 bytes of K codes of rows
 // 16 t + l % 16, of V codes of the row blocks 4 t + l / 16, and the scales of
 // rows 16 t + 4 (l / 16) .. + 3.
@@ -468,7 +472,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     float L = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if (mls[i][oc][0] == -INFINITY) continue;
+        if (q4_dead(mls[i][oc][0], mls[i][oc][1])) continue;
         const float f = pow2f(mls[i][oc][0] - M);
         const float4 x = *(const float4*)&ow[i][oc][od];
         v.x = __builtin_fmaf(x.x, f, v.x);
@@ -485,23 +489,29 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
         return;
     }
     const size_t pi = (((size_t)u * c.KH + kh) * a.S + s) * (a.qpk * a.tp) + oc;
-    if (M != -INFINITY) *(float4*)(a.part_o + pi * HD + od) = v;
+    if (!q4_dead(M, L)) *(float4*)(a.part_o + pi * HD + od) = v;
     if ((threadIdx.x & 31) == 0) {
         a.part_ml[2 * pi] = M;
         a.part_ml[2 * pi + 1] = L;
     }
 }
 
-// The ranges of one (KV head, unit) merged into the output.
+// The ranges of one (KV head, unit) merged into the output, 8 query rows a block.
 template <bool BF>
 __global__ void __launch_bounds__(256)
 k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     constexpr int HD = 128;
-    const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH;
+    const int nc = a.qpk * a.tp, nb = (nc + 7) / 8;
+    const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH / nb;
     Q4Unit un;
-    if (!q4_unit(c, u, a.tp, un)) return;
-    const int oc = threadIdx.x >> 5, od = 4 * (threadIdx.x & 31), nc = a.qpk * a.tp;
-    if (oc >= a.qpk * un.n || un.pos + (oc >> a.lq) >= c.maxT) return;
+    if (c.pos) {
+        un.tok = u * a.tp;
+        un.n = min(a.tp, c.N - un.tok);
+    } else if (!q4_unit(c, u, a.tp, un)) {
+        return;
+    }
+    const int oc = 8 * (blockIdx.x / c.KH % nb) + (threadIdx.x >> 5), od = 4 * (threadIdx.x & 31);
+    if (oc >= a.qpk * un.n || (c.pos ? c.pos[un.tok + (oc >> a.lq)] : un.pos + (oc >> a.lq)) >= c.maxT) return;
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
     // lane j of the 32 has the factors of ranges j, j + 32, ..; the ranges' outputs
     // are on their way four at a time
@@ -512,10 +522,10 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float L = 0.0f;
     for (int s0 = 0; s0 < a.S; s0 += 32) {
-        float f = 0.0f;
+        float f = -1.0f;                // (a range without a row: it has no output; and past the end)
         if (s0 + j < a.S) {
             const float2 x = *(const float2*)(a.part_ml + 2 * (p0 + (size_t)(s0 + j) * nc));
-            if (x.x != -INFINITY) {
+            if (!q4_dead(x.x, x.y)) {
                 f = pow2f(x.x - M);
                 L = __builtin_fmaf(x.y, f, L);
             }
@@ -528,7 +538,7 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const float y = __shfl(f, half + e - s0 + q, JM_WAVE);
-                if (y == 0.0f) continue;        // (a range without a row has no output; past the end too)
+                if (y < 0.0f) continue;         // (0 counts: it may meet a NaN)
                 v.x = __builtin_fmaf(x[q].x, y, v.x);
                 v.y = __builtin_fmaf(x[q].y, y, v.y);
                 v.z = __builtin_fmaf(x[q].z, y, v.z);
@@ -642,7 +652,8 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     __shared__ uint32_t tn[8][32 * QB];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
-    const int kh = blockIdx.x % c.KH, u = a.units - 1 - (int)(blockIdx.x / c.KH);      // the longest prefixes first
+    const int kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH;
+    const int u = a.units - 1 - rs % a.units, sr = rs / a.units;        // the longest prefixes first
     Q4Unit un;
     if (c.pos) {                                // the decoder's form: one prompt's tokens
         un.seq = 0;
@@ -678,7 +689,9 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     }
     pmax = __builtin_amdgcn_readfirstlane(pmax);
     pmin = __builtin_amdgcn_readfirstlane(pmin);
-    const int nstep = (pmax + STEP) / STEP;     // (0 where no token sees a row)
+    // this block's range of the steps (none where no token sees a row)
+    const int steps = (pmax + STEP) / STEP;
+    const int step0 = (int)((long long)steps * sr / a.S), nstep = (int)((long long)steps * (sr + 1) / a.S);
     const Q4Head<NG> kk(q4_plane(c, un.seq, 0), kh, c.KH, c.R), vv(q4_plane(c, un.seq, 1), kh, c.KH, c.R);
 
     // ---- a step's codes and scales on their way, and into LDS
@@ -831,7 +844,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
     };
 
-    if (nstep > 0) request(0);
+    if (step0 < nstep) request(step0);
 
     // ---- the query rows
     f16x8 qh[8], ql[BF ? 1 : 8];
@@ -1091,12 +1104,12 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     };
     if (ahead) {
-        if (nstep > 0) stage(0);
-        if (nstep > 1) request(1);
+        if (step0 < nstep) stage(step0);
+        if (step0 + 1 < nstep) request(step0 + 1);
         meet();
     }
 #pragma unroll 1
-    for (int k = 0; k < nstep; k++) {
+    for (int k = step0; k < nstep; k++) {
         const int sk = ahead ? k + 1 : k;
         if (sk < nstep) {
             stage(sk);
@@ -1131,6 +1144,11 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
             L = __builtin_fmaf(mls[q * RG + rg][32 * b + n][1], pow2f(mls[q * RG + rg][32 * b + n][0] - m0), L);
         f[b] = pow2f(ref[b] - m0);
         inv[b] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);           // no row to see: 0
+        if (a.S > 1) {
+            inv[b] = 1.0f;
+            float* const ml = a.part_ml + 2 * (((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n);
+            if (ps == 0 && h == 0 && live[b]) *(float2*)ml = make_float2(M, L);
+        }
         if constexpr (BF) {
 #pragma unroll
             for (int q = 0; q < PS; q++) taint[b] |= tn[q * RG + rg][32 * b + n];
@@ -1168,7 +1186,13 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     const float x = __uint_as_float(0x7FC00000u);
                     s = make_float4(x, x, x, x);
                 }
-                store_out<BF>(a.out, ((size_t)tok[b] * a.H + head[b]) * HD + 32 * nt + 8 * q + 4 * h, s);
+                const int d = 32 * nt + 8 * q + 4 * h;
+                if (a.S == 1) {
+                    store_out<BF>(a.out, ((size_t)tok[b] * a.H + head[b]) * HD + d, s);
+                } else {
+                    const size_t row = ((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n;
+                    *(float4*)(a.part_o + row * HD + d) = s;
+                }
             }
     }
 }
@@ -1202,28 +1226,47 @@ Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared) {
     Q4AttnPlan p{};
     const int qpk = H / c.KH;
     const int n_seq = c.cu ? c.n_seq : shared ? 1 : c.N;
-    p.S = 1;
-    if ((long long)c.N * qpk >= 64ll * n_seq) {
-        for (p.rg = 4;; p.rg = 2) {
-            p.tp = 32 * (bf ? 2 : 1) * p.rg / qpk;
-            p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (p.tp - 1)) / p.tp);
-            if (p.rg == 2 || (long long)p.units * c.KH >= 256) return p;
-        }
-    }
-    p.tp = c.cu ? 8 / qpk : 1;
-    // (every sequence's tokens are rounded up to whole units)
-    p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (p.tp - 1)) / p.tp);
-    const long long blocks = (long long)p.units * c.KH;
-    // Ranges: a block a CU while each has 128 rows (a tile a wave), up to 4 a CU
-    // while each has 512.  (Measured with float32 queries, both kernels: one
-    // sequence of 777 rows 10.3 us, with 256 rows a block 10.4; 8 sequences of 2048
-    // 11.6 us on 256 blocks, 14.6 on 1024; 6 sequences' drafts over up to 5000 rows
-    // 22.0 us on 256 blocks, 19.4 on 1024; bfloat16, 32 sequences of 16384: 115 us
-    // without a split, 104 with 1024 blocks.)
+    auto cut = [&](int tp) {
+        p.tp = tp;
+        // (every sequence's tokens are rounded up to whole units)
+        p.units = (int)std::min<long long>(c.N, ((long long)c.N + (long long)n_seq * (tp - 1)) / tp);
+        return (long long)p.units * c.KH;
+    };
+    long long blocks;
+    // up to `want` blocks while each has `rows` cache rows
     auto ranges = [&](long long want, int rows) {
         return std::min((want + blocks - 1) / blocks, ((long long)c.maxT + rows - 1) / rows);
     };
-    p.S = (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+    // Tiles from 64 query rows a sequence (bf16: 96).  Both ways, us, float32 and
+    // bf16, 8 query heads a KV head: 8 tokens behind 30000 rows (8 KV heads) tiles
+    // 42 and 46, else 54 and 47; 16 tokens 57 and 48, else 93 and 80; 8 tokens behind
+    // 2000 (4 sequences, 4 heads) 20 and 22, else 17 and 15; 16 tokens 27 and 24, else 25
+    // and 22; 64 tokens behind 4000 (8 heads) 36 and 30, else 56 and 48.
+    const long long rows = (long long)c.N * qpk;
+    if (rows >= (bf ? 96ll : 64ll) * n_seq) {
+        // 4 row groups share what a step stages, but take twice the rows for a block:
+        // where the blocks are enough, or the prefixes may be long enough to be cut.
+        // (us, with 2 and with 4, bf16, 8 KV heads: 64 tokens behind 4000 rows 30 and
+        // 33, 256 tokens 69 and 64; behind 30000 rows 107 and 94, 358 and 296)
+        const int unit = bf ? 256 : 128;
+        p.rg = 4;
+        blocks = cut(unit / qpk);
+        if (rows < (long long)unit * n_seq || (blocks < 256 && blocks * c.maxT < 160000)) {
+            p.rg = 2;
+            blocks = cut(unit / 2 / qpk);
+        }
+        // (a block fills a CU; 256 tokens behind 30000 rows, bf16: 682 us uncut with 2)
+        p.S = (int)std::max(std::min(256 / blocks, ((long long)c.maxT + 255) / 256), 1ll);
+    } else {
+        blocks = cut(c.cu ? 8 / qpk : 1);
+        // Ranges: a block a CU while each has 128 rows (a tile a wave), up to 4 a CU
+        // while each has 512.  (Measured with float32 queries, both kernels: one
+        // sequence of 777 rows 10.3 us, with 256 rows a block 10.4; 8 sequences of 2048
+        // 11.6 us on 256 blocks, 14.6 on 1024; 6 sequences' drafts over up to 5000 rows
+        // 22.0 us on 256 blocks, 19.4 on 1024; bfloat16, 32 sequences of 16384: 115 us
+        // without a split, 104 with 1024 blocks.)
+        p.S = (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+    }
     const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;
     p.ml_floats = p.S > 1 ? cols * 2 : 0;
@@ -1246,12 +1289,12 @@ hipError_t launch_q4_attn(const Q4KvArgs& c, const Q4AttnPlan& p, const void* q,
         }
         JM_Q4_TILE(2, false) JM_Q4_TILE(2, true) JM_Q4_TILE(4, false) JM_Q4_TILE(4, true)
 #undef JM_Q4_TILE
-        return hipGetLastError();
+    } else {
+        JM_Q4_EACH(k_q4_attn, grid, dim3(256), c, a);
     }
-    JM_Q4_EACH(k_q4_attn, grid, dim3(256), c, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.S == 1) return e;
-    const dim3 mg((unsigned)c.KH * p.units);
+    const dim3 mg((unsigned)c.KH * p.units * ((a.qpk * a.tp + 7) / 8));
     if (bf) hipLaunchKernelGGL(k_q4_merge<true>, mg, dim3(256), 0, st, c, a);
     else hipLaunchKernelGGL(k_q4_merge<false>, mg, dim3(256), 0, st, c, a);
     return hipGetLastError();

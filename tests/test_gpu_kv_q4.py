@@ -233,6 +233,12 @@ def test_prompts(H, KH, counts, start, dt, group):
     _check(H, KH, counts, start, group, dt)
 
 
+@pytest.mark.parametrize("dt,group", [("f32", 64), ("bf16", 32)])
+@pytest.mark.parametrize("H,KH,counts,start", [(8, 1, [64], [1500]), (4, 2, [40, 0, 90], [900, 5, 1800]), (2, 2, [129], [2000]), (8, 8, [70], [700])])
+def test_prompts_behind_long_prefixes(H, KH, counts, start, dt, group):
+    _check(H, KH, counts, start, group, dt, maxT=4000)
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [3, 2], [40, 70]])
 def test_rows_below_zero_see_nothing(counts):
     """A token whose row is below 0 gets 0; the sequence's later ones see what
@@ -300,6 +306,38 @@ def test_a_row_of_nan_reaches_those_that_see_it(counts):
     got = c.attention(0, q, _int([s]), _int([0, n]))
     assert torch.equal(got[:n // 2], clean[:n // 2])
     assert bool(got[n // 2:].isnan().all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1], [3], [100]])
+def test_a_row_of_nan_counts_however_small_its_weight(counts, dt):
+    """A visible V of NaN makes the output NaN, also where float32 has no weight
+    as small as the row's, and far from the rows with weight."""
+    H, KH, n = 2, 1, 1500
+    for at in (3, 700, 1300):
+        c = _cache(1, 2000, KH, H=H)
+        k, v = torch.ones(n, KH, HD, device="cuda"), _rows(8, n, KH, DT["f32"])
+        k[at] = -1.0
+        v[at, :, 5] = float("nan")
+        c.write(0, k.to(DT[dt]), v.to(DT[dt]), _int([0]), _int([0, n]))
+        q = torch.full((counts[0], H, HD), 40.0, dtype=DT[dt], device="cuda")   # scores of 450 and -450
+        got = c.attention(0, q, _int([n - counts[0]]), _int([0, counts[0]]))
+        assert bool(got[..., :64].isnan().all())
+        assert not bool(got[..., 64:].isnan().any())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1], [3], [100]])
+def test_a_query_of_nan_gives_nan(counts, dt):
+    H, KH, n = 2, 1, 1500
+    c = _cache(1, 2000, KH, H=H)
+    _fill(c, [n], dt)
+    q = _randn(12, counts[0], H, HD).to(DT[dt])
+    q[0, 1, 77] = float("nan")
+    got = c.attention(0, q, _int([n - counts[0]]), _int([0, counts[0]]))
+    assert bool(got[0, 1].isnan().all())
+    got[0, 1] = 0.0
+    assert bool(got.isfinite().all())
 
 
 @pytest.mark.parametrize("qscale", [1e-30, 1e-4, 30.0, 1e4])
