@@ -760,16 +760,36 @@ static int sm_chunks(int B, int V) {
     return std::max(1, std::min(512 / B, (V + 8 * SM_T - 1) / (8 * SM_T)));
 }
 
-size_t sample_ws_bytes(int B, int V) { return (size_t)B * sm_row_bytes(sm_chunks(B, V)); }
+// Rows a launch takes: more would fill the card no better, and the workspace is
+// some 90 KB a row.
+constexpr int SM_ROWS = 1024;
 
-hipError_t launch_sample(const SampleArgs& a, void* ws, hipStream_t st) {
-    if (a.B == 0) return hipSuccess;
-    const int SP = sm_chunks(a.B, a.V), chunk = (a.V + SP - 1) / SP;
-    const dim3 grid((unsigned)a.B * SP);
-    hipLaunchKernelGGL(k_sample_max, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
-    hipLaunchKernelGGL(k_sample_hist, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
-    hipLaunchKernelGGL(k_sample_pick, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
-    return hipGetLastError();
+size_t sample_ws_bytes(int B, int V) {
+    B = std::min(B, SM_ROWS);
+    return (size_t)B * sm_row_bytes(sm_chunks(B, V));
+}
+
+hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t st) {
+    for (int b0 = 0; b0 < all.B; b0 += SM_ROWS) {
+        SampleArgs a = all;
+        a.B = std::min(all.B - b0, SM_ROWS);
+        a.logits = (const char*)all.logits + (size_t)b0 * all.ld * (all.bf ? 2 : 4);
+        a.u += b0;
+        a.out_tok += b0;
+        if (a.out_p) a.out_p += b0;
+        if (a.temperature_b) a.temperature_b += b0;
+        if (a.top_k_b) a.top_k_b += b0;
+        if (a.top_p_b) a.top_p_b += b0;
+        if (a.min_p_b) a.min_p_b += b0;
+        // (as many chunks as the workspace has room for)
+        const int SP = sm_chunks(std::min(all.B, SM_ROWS), a.V), chunk = (a.V + SP - 1) / SP;
+        const dim3 grid((unsigned)a.B * SP);
+        hipLaunchKernelGGL(k_sample_max, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
+        hipLaunchKernelGGL(k_sample_hist, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
+        hipLaunchKernelGGL(k_sample_pick, grid, dim3(SM_T), 0, st, a, (char*)ws, SP, chunk);
+        if (const hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace jm

@@ -91,6 +91,37 @@ def test_settings_of_each_row():
            pick([1.0, 2.0, 0.9, 0.3, 0.0, -1.0]), pick([0.0, -1.0, 0.05, 0.5, 1.0, 3.0]))
 
 
+def test_small_top_k_of_many_rows():
+    """Rows in chunks of many tokens a thread, of which few are counted: sorted
+    either way, tied, with all that is kept in one place, and mostly -infinity."""
+    B, V = 258, 40001
+    x = _logits(21, B, V)
+    rng = np.random.default_rng(22)
+    for b in range(B):
+        if b % 6 == 1:
+            x[b] = np.sort(x[b])
+        elif b % 6 == 2:
+            x[b] = -np.sort(-x[b])
+        elif b % 6 == 3:
+            x[b] = np.rint(x[b] * 0.5)
+        elif b % 6 == 4:
+            x[b, 64 * 1024 // 4:64 * 1024 // 4 + 80] += 30.0
+        elif b % 6 == 5:
+            x[b, rng.random(V) < 0.999] = -np.inf
+    k = rng.choice(np.asarray([1, 2, 20, 63, 64, 65, 400], np.int32), B)
+    _check(x, rng.random(B).astype(np.float32), temperature=0.9, top_k=k, top_p=rng.choice(np.asarray([1.0, 0.9], np.float32), B))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_one_launch_takes(dtype):
+    B, V = 2100, 77
+    rng = np.random.default_rng(23)
+    x = torch.from_numpy(_logits(24, B, V)).to(dtype).float().numpy()
+    pick = lambda v, t: rng.choice(np.asarray(v, t), B)  # noqa: E731
+    _check(x, rng.random(B).astype(np.float32), pick([0.0, 0.7, 1.3], np.float32), pick([0, 1, 9], np.int32),
+           pick([1.0, 0.8], np.float32), pick([0.0, 0.1], np.float32), dtype)
+
+
 @pytest.mark.parametrize("how", [dict(), dict(top_k=5), dict(top_p=0.6), dict(min_p=0.5), dict(top_k=700, top_p=0.9)])
 @pytest.mark.parametrize("V", [5, 1000, 40001])
 def test_ties_go_to_the_lower_index(V, how):
