@@ -226,10 +226,10 @@ class HipNativeDecoder:
                             min_p=0.0) -> list[int]:
         """The next token per sequence, drawn with the random numbers u (one a
         sequence, in [0, 1)); settings as sampling.sample takes them."""
-        dev = self.kv.data.device
-        out, _ = self.dec.decode_layers_batch_sample(
-            self._embed(tokens), positions, self.kv, torch.as_tensor(np.asarray(u, dtype=np.float32), device=dev),
-            temperature, top_k, top_p, min_p)
+        if not isinstance(u, torch.Tensor):
+            u = torch.as_tensor(np.asarray(u, dtype=np.float32))
+        out, _ = self.dec.decode_layers_batch_sample(self._embed(tokens), positions, self.kv, u.to(self.kv.data.device),
+                                                     temperature, top_k, top_p, min_p)
         for b, p in enumerate(positions):
             self._seq_pos[f"seq{b}"] = p + 1
         return [int(v) for v in out.cpu().tolist()]

@@ -211,11 +211,21 @@ struct Q4AttnArgs {
     float* part_ml;             // [units][KH][S][qpk tp][2]: ref, sum
 };
 
+// Constants from registers, unknown to the compiler: a fused multiply-add with
+// an fp16 factor is one v_fma_mix_f32, where it would make a product or a
+// difference of it (exactly as good) two instructions.
+struct Q4Mix {
+    float zero = 0.0f, minus1 = -1.0f;
+    __device__ __forceinline__ Q4Mix() { __asm__("" : "+s"(zero), "+s"(minus1)); }
+    __device__ __forceinline__ float mul(float a, _Float16 b) const { return __builtin_fmaf(a, (float)b, zero); }
+    __device__ __forceinline__ float sub(float a, _Float16 b) const { return __builtin_fmaf((float)b, minus1, a); }
+};
+
 // The two fp16 halves of a and b: the values rounded towards 0, and the rest.
-__device__ __forceinline__ void split_f16x2(float a, float b, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void split_f16x2(const Q4Mix& mix, float a, float b, uint32_t& hi, uint32_t& lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const float ra = __builtin_fmaf((float)h[0], -1.0f, a);
-    const float rb = __builtin_fmaf((float)h[1], -1.0f, b);
+    const float ra = mix.sub(a, (_Float16)h[0]);
+    const float rb = mix.sub(b, (_Float16)h[1]);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
 }
@@ -285,6 +295,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     int t = (int)((long long)NT * s / a.S) + w;
 
     const Q4Head<NG> kk(q4_plane(c, un.seq, 0), kh, c.KH, c.R), vv(q4_plane(c, un.seq, 1), kh, c.KH, c.R);
+    const Q4Mix mix;
     Q4Tile<NG> cur, nxt;
     if (t < t_end) q4_load_tile(cur, kk, vv, t, lane);
 
@@ -322,7 +333,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t hi, lo;
-                split_f16x2(__fmul_rn(x[st][e], f), __fmul_rn(x[st][e + 4], f), hi, lo);
+                split_f16x2(mix, __fmul_rn(x[st][e], f), __fmul_rn(x[st][e + 4], f), hi, lo);
                 const f16x2 h = __builtin_bit_cast(f16x2, lo_col ? lo : hi);
                 // codes of nibbles 1, 3, 5 and 7 come 16 times too large
                 b[e] = __builtin_bit_cast(uint32_t, e & 1 ? h * (_Float16)0.0625f : h);
@@ -362,30 +373,33 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
                 y[4 * rt + i] = BF ? v : __fadd_rn(v, dpp_f<DPP_ROR8>(v));
             }
         }
-        float sv[8][NG];
+        uint32_t sv[8][NG / 2];                             // V's scales, two a word
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int e = 0; e < NG; e++) sv[i][e] = q4_scale(cur.vs, i >> 2, i & 3, e);
+            for (int e = 0; e < NG / 2; e++) {
+                const int at = (i & 3) * (NG / 2) + e;
+                sv[i][e] = cur.vs[(i >> 2) * (NG / 2) + at / 4][at % 4];
+            }
         if (32 * t + 31 > un.pos) {                         // some column does not see the whole tile
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const bool in = 32 * t + 16 * (i >> 2) + 4 * g + (i & 3) <= crow;
                 y[i] = in ? y[i] : -INFINITY;
 #pragma unroll
-                for (int e = 0; e < NG; e++) sv[i][e] = in ? sv[i][e] : 0.0f;
+                for (int e = 0; e < NG / 2; e++) sv[i][e] = in ? sv[i][e] : 0u;
             }
         }
         // ---- the reference: the largest weight x scale, to the exponent
-        float ym = y[0], sm = 0.0f;
+        float ym = y[0];
+        u16x2_t sm = 0;
 #pragma unroll
         for (int i = 1; i < 8; i++) ym = fmaxf(ym, y[i]);
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int e = 0; e < NG; e++) sm = fmaxf(sm, sv[i][e]);
-        // (sm < 2^(exponent + 1); 0, which no scale that counts is below, as 2^-24)
-        float z = ym + (float)((int)(__float_as_uint(fmaxf(sm, 5.9604645e-8f)) >> 23) - 126);
+            for (int e = 0; e < NG / 2; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sv[i][e]));
+        float z = ym + q4_scale_exp(max(sm.x, sm.y));
         if (__any(z > ref + 14.0f)) {
             z = fmaxf(z, swz_xor16_f(z));
             z = fmaxf(z, __shfl_xor(z, 32, JM_WAVE));
@@ -409,12 +423,13 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
             uint32_t b[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x0 = __fmul_rn(p[2 * i], sv[2 * i][e]), x1 = __fmul_rn(p[2 * i + 1], sv[2 * i + 1][e]);
+                const float x0 = mix.mul(p[2 * i], __builtin_bit_cast(f16x2, sv[2 * i][e / 2])[e % 2]);
+                const float x1 = mix.mul(p[2 * i + 1], __builtin_bit_cast(f16x2, sv[2 * i + 1][e / 2])[e % 2]);
                 if (BF) {
                     b[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x0, (_Float16)x1});
                 } else {
                     uint32_t hi, lo;
-                    split_f16x2(x0, x1, hi, lo);
+                    split_f16x2(mix, x0, x1, hi, lo);
                     b[i] = lo_col ? lo : hi;
                 }
             }
@@ -728,6 +743,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     // scales are 0 in LDS; `taint` has which of this lane's query rows saw one)
     uint32_t taint[QB] = {};
     const Q4Bits bits;
+    const Q4Mix mix;
     auto stage = [&](int i) __attribute__((always_inline)) {
         const int buf = i & 1;
 #pragma unroll
@@ -876,7 +892,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                split_f16x2(__fmul_rn(x[k][e], f), __fmul_rn(x[k][e + 4], f), hi[e], lo[e]);
+                split_f16x2(mix, __fmul_rn(x[k][e], f), __fmul_rn(x[k][e + 4], f), hi[e], lo[e]);
                 if (!BF && (e & 1)) {           // codes 16 times too large
                     hi[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, hi[e]) * (_Float16)0.0625f);
                     lo[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo[e]) * (_Float16)0.0625f);
@@ -1079,7 +1095,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int v = 8 * s + 2 * e;
-                        split_f16x2(__fmul_rn(y[v], scale(sx, v, g)), __fmul_rn(y[v + 1], scale(sx, v + 1, g)), hi[e], lo[e]);
+                        split_f16x2(mix, __fmul_rn(y[v], scale(sx, v, g)), __fmul_rn(y[v + 1], scale(sx, v + 1, g)), hi[e], lo[e]);
                     }
                     const f16x8 ph = as_f16x8(hi[0], hi[1], hi[2], hi[3]), pl = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
