@@ -61,7 +61,8 @@ __device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
 // hands between 8 lanes in registers).  Bound by memory where there is much: 112016
 // tokens of 8 heads read back as bf16 in 40 us, 5.7 TB/s of codes and values.  What
 // is read back is stored past the caches, which it would only go through: with
-// ordinary stores, into outputs that were not there before, 65 us.
+// ordinary stores, into outputs that were not there before, 65 us.  3 prompts of up
+// to 1531 bf16 tokens written in 6.6 us; 8 tokens of 4 heads in 3.5 (the launch).
 template <int NG, bool BF>
 __global__ void __launch_bounds__(256)
 k_q4_write(Q4KvArgs c, const void* __restrict__ k, const void* __restrict__ v, long long kts, long long khs,
@@ -125,6 +126,13 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 //            them: contraction index 8 g + e is row 16 (e / 4) + 4 g + e % 4.
 // q and the weights carry 21 bits so; for bf16 queries (BF) q is exact without
 // the second half, and the weights are rounded to fp16 once (2^-11 of each).
+//
+// Measured, this kernel and k_q4_merge: 1 token behind 777 rows of 4 KV heads 6.5 +
+// 3.4 us, 8 tokens behind 2048 rows each 7.8 + 3.1 (a tile a wave takes 6.4 us: the
+// launch, the unit's place, q and the tile, the waves joined); 6 drafts of 5 tokens
+// behind 3001 rows of 16 heads (26 MB) 15.6 + 3.2, on 576 blocks of 4 tiles a wave,
+// the same with a tenth of the vector instructions less; 32 bf16 tokens behind 16003
+// rows each of 8 heads (441 MB, groups of 32) 94 + 4.4 us, 4.7 TB/s: memory.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -598,8 +606,9 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
 // halves the LDS reads a product.
 //
 // Measured at 2047 tokens behind 4099 rows, 32 query heads on 8 (172 GFLOP, 147 us
-// at the rate of a large library product): 254 - 264 us.  Vector work bounds it:
-// a wave has some 300 vector instructions beside the step's 32 products, and two
+// at the rate of a large library product): 227 us a call, 250 - 264 under a
+// profiler.  Vector work bounds it:
+// a wave has some 300 vector instructions beside the step's 32 products, and the two
 // waves of a SIMD, half a step apart, hide most but not all of it (270 us with
 // both in step).
 
