@@ -116,6 +116,22 @@ def test_prompts_match_oracle(H, KH, qk, group, T, p0):
     dec.store.close()
 
 
+@pytest.mark.parametrize("H,KH,group,T", [(8, 1, 64, 24), (8, 4, 32, 90)])
+def test_a_prompt_behind_a_long_prefix(H, KH, group, T):
+    """Its cache rows are cut into ranges, whose partial outputs the step's
+    workspace holds."""
+    p0 = 900
+    print(f"[q4 prompt] H={H} KH={KH} T={T} p0={p0}", flush=True)
+    dec, oracle, kv, kv_h = _model(H, KH, 1, 1100, 1, group, 1)
+    _preload(kv, kv_h, p0)
+    x = activations(T, DIM, seed=T)
+    got = dec.decode_layers_batch(torch.from_numpy(x).cuda(), list(range(p0, p0 + T)), kv, seqs=[0] * T).cpu().numpy()
+    want = np.concatenate([oracle.decode_layers_batch(x[i:i + 1], [p0 + i], [kv_h[0]]) for i in range(T)])
+    assert _rel(got, want) <= TOL
+    _rows_agree(kv, kv_h, 0, 0, p0, T)
+    dec.store.close()
+
+
 def test_caches_of_each_kind_in_turn_over_one_graph():
     """A store's decoder goes from bf16 caches to 4-bit ones and back: the
     recorded step is not replayed over the wrong kind."""
