@@ -41,35 +41,10 @@ struct Q4Head {
     __device__ __forceinline__ gptr<uint16_t> scale(int r, int g) const { return scales + (size_t)r * NG + g; }
 };
 
-// The sequence and cache row of token t of a call, the same in every lane of
-// the wave; false for a token that has none (behind the last sequence, or a row
+// The sequence and cache row of the four tokens t0 .. t0 + 3 of a call (not the
+// decoder's form) in the wave's four rows of 16 lanes: each lane gets its row's
+// token's; false for a token that has none (behind the last sequence, or a row
 // outside the cache).
-__device__ __forceinline__ bool q4_place(const Q4KvArgs& c, int t, int& seq, int& pos) {
-    if (c.pos) {                            // the decoder: token t is entry t of the table
-        seq = t;
-        pos = c.pos[t];
-        return pos >= 0 && pos < c.maxT;
-    }
-    seq = t;
-    int first = t;
-    if (c.cu) {
-        const int lane = threadIdx.x & 63;
-        int n = 0;
-        for (int i = 0; i <= c.n_seq; i += 64)
-            n += __popcll(__ballot(i + lane <= c.n_seq && c.cu[min(i + lane, c.n_seq)] <= t));
-        seq = n - 1;
-        if (seq < 0 || seq >= c.n_seq) return false;
-        first = c.cu[seq];
-    } else if (t >= c.n_seq) {
-        return false;
-    }
-    const long long p = (long long)c.start[seq] + (t - first);
-    pos = (int)(p < 0 ? -1 : p >= c.maxT ? c.maxT : p);
-    return p >= 0 && p < c.maxT;
-}
-
-// The same for the four tokens t0 .. t0 + 3 of a call (not the decoder's form) in
-// the wave's four rows of 16 lanes: each lane's row has its token's.
 __device__ __forceinline__ bool q4_places(const Q4KvArgs& c, int t0, int& seq, int& pos) {
     const int lane = threadIdx.x & 63, i = lane >> 4, t = t0 + i;
     seq = t;
