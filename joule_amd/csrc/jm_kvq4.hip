@@ -127,9 +127,10 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 // q and the weights carry 21 bits so; for bf16 queries (BF) q is exact without
 // the second half, and the weights are rounded to fp16 once (2^-11 of each).
 //
-// Measured, this kernel and k_q4_merge: 1 token behind 777 rows of 4 KV heads 6.5 +
-// 3.4 us, 8 tokens behind 2048 rows each 7.8 + 3.1 (a tile a wave takes 6.4 us: the
-// launch, the unit's place, q and the tile, the waves joined); 6 drafts of 5 tokens
+// Measured: 1 token behind 777 rows of 4 KV heads 10.0 us, in one range; with
+// k_q4_merge, 8 tokens behind 2048 rows each 7.8 + 3.1 (a tile a wave takes 6.4 us:
+// the launch, the unit's place, q and the tile, the waves joined; each further
+// tile 0.6); 6 drafts of 5 tokens
 // behind 3001 rows of 16 heads (26 MB) 15.6 + 3.2, on 576 blocks of 4 tiles a wave,
 // the same with a tenth of the vector instructions less; 32 bf16 tokens behind 16003
 // rows each of 8 heads (441 MB, groups of 32) 94 + 4.4 us, 4.7 TB/s: memory.
@@ -1284,13 +1285,16 @@ Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared) {
         p.S = (int)std::max(std::min(256 / blocks, ((long long)c.maxT + 255) / 256), 1ll);
     } else {
         blocks = cut(c.cu ? 8 / qpk : 1);
-        // Ranges: a block a CU while each has 128 rows (a tile a wave), up to 4 a CU
-        // while each has 512.  (Measured with float32 queries, both kernels: one
-        // sequence of 777 rows 10.3 us, with 256 rows a block 10.4; 8 sequences of 2048
-        // 11.6 us on 256 blocks, 14.6 on 1024; 6 sequences' drafts over up to 5000 rows
-        // 22.0 us on 256 blocks, 19.4 on 1024; bfloat16, 32 sequences of 16384: 115 us
-        // without a split, 104 with 1024 blocks.)
-        p.S = (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+        // Ranges, for caches of more than 1024 rows: a block a CU while each has 128
+        // rows (a tile a wave), up to 4 a CU while each has 512.  Up to there one
+        // range is faster than a second launch and its workspace: 1 or 8 tokens behind
+        // 777 float32 rows (4 KV heads) 10.0 us against 12.6, 23 in a captured graph,
+        // where the workspace is a node; 1000 rows 10.9 and 12.8, 1500 rows 14.2 and
+        // 12.6.  (Above, both kernels alone: 8 sequences of 2048 rows 11.6 us on 256
+        // blocks, 14.6 on 1024; 6 sequences' drafts over up to 5000 rows 22.0 us on 256
+        // blocks, 19.4 on 1024; bfloat16, 32 sequences of 16384: 115 us without a
+        // split, 104 with 1024 blocks.)
+        p.S = c.maxT <= 1024 ? 1 : (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
     }
     const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;

@@ -233,6 +233,14 @@ def test_prompts(H, KH, counts, start, dt, group):
     _check(H, KH, counts, start, group, dt)
 
 
+@pytest.mark.parametrize("dt,group", [("f32", 64), ("bf16", 64), ("f32", 32), ("bf16", 32)])
+@pytest.mark.parametrize("H,KH,counts,start", [(8, 2, [1, 1, 1, 1], [0, 31, 1027, 2900]), (2, 2, [1], [40]), (4, 1, [3, 0, 2, 5], [0, 7, 1500, 2040]),
+                                               (8, 8, [7, 1], [900, 2600])])
+def test_few_tokens_of_long_caches(H, KH, counts, start, dt, group):
+    """Caches whose rows are cut into ranges, some of them without a row."""
+    _check(H, KH, counts, start, group, dt, maxT=3001)
+
+
 @pytest.mark.parametrize("dt,group", [("f32", 64), ("bf16", 32)])
 @pytest.mark.parametrize("H,KH,counts,start", [(8, 1, [64], [1500]), (4, 2, [40, 0, 90], [900, 5, 1800]), (2, 2, [129], [2000]), (8, 8, [70], [700])])
 def test_prompts_behind_long_prefixes(H, KH, counts, start, dt, group):
