@@ -296,9 +296,8 @@ class HipDecoder:
             dt = _lib.JM_DTYPE_Q4 if kv.group == 64 else _lib.JM_DTYPE_Q4_G32
         else:
             dt = _lib.JM_DTYPE_F32 if kv.data.dtype == torch.float32 else _lib.JM_DTYPE_BF16
-        if getattr(self, "_kvdt", None) != dt:
-            _lib.check(_lib.lib().jm_store_set_kv_dtype(self.store._h, dt), "jm_store_set_kv_dtype")
-            self._kvdt = dt
+        # (every call: another decoder over the same store may have set its own)
+        _lib.check(_lib.lib().jm_store_set_kv_dtype(self.store._h, dt), "jm_store_set_kv_dtype")
 
     def _positions(self, positions, B):
         pos = np.ascontiguousarray(np.asarray(positions, dtype=np.int32).reshape(-1))
