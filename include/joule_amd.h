@@ -447,7 +447,9 @@ int jm_q4_gemv_f32(float* out, const float* x, const uint8_t* packed, const uint
  * blocks are fewer than 256, the contraction is split over up to 8 blocks
  * and the partial sums are added in split order), below on the v_dot8 digit
  * kernel.  Workspace: one buffer per (device, stream), kept and grown; a
- * call under stream capture takes a stream-ordered allocation instead. */
+ * call under stream capture takes a stream-ordered allocation instead.  A call
+ * holds the buffer until its kernels are enqueued, so that calls of several
+ * host threads on one stream follow one another whole. */
 int jm_q4_gemm_f32(float* out, const float* X, int T, const uint8_t* packed, const uint16_t* scales,
                    int m, int d, int group, void* stream);
 

@@ -13,10 +13,10 @@
 #include <cstdio>
 #include <atomic>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <vector>
 
-#include "jm_plugin_ws.h"
 #include "jm_store.h"
 
 namespace jm {
@@ -39,20 +39,11 @@ int hip_fail(hipError_t e, const char* what) {
 
 namespace {
 
-// Workspace of the calls without a store (the plugin products, the 4-bit
-// cache's attention, sampling): one buffer per (device, stream), the policy of
-// jm_plugin_ws.h (reuse, grow with the old buffer retired, or a stream-ordered
-// allocation under capture, freed after the call).
-struct PluginBuf {
-    int dev;
-    hipStream_t st;
-    void* p;
-    size_t bytes;
-};
-
-std::mutex g_pws_mu;
-std::vector<PluginBuf> g_pws;
-std::vector<void*> g_pws_retired;           // replaced buffers, kept until the process ends
+// Buffers of the calls without a store, by device and stream.
+jm::PluginBufs& plugin_bufs() {
+    static jm::PluginBufs* const bufs = new jm::PluginBufs;     // (never destroyed: calls may come until the process ends)
+    return *bufs;
+}
 
 }  // namespace
 
@@ -63,31 +54,34 @@ int plugin_ws(hipStream_t st, size_t bytes, PluginWs* out) {
     JM_HIP(hipGetDevice(&dev), "hipGetDevice");
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     JM_HIP(hipStreamIsCapturing(st, &cs), "hipStreamIsCapturing");
-    std::lock_guard<std::mutex> lk(g_pws_mu);
+    const bool capturing = cs != hipStreamCaptureStatusNone;
     PluginBuf* b = nullptr;
-    for (auto& x : g_pws)
-        if (x.dev == dev && x.st == st) b = &x;
-    switch (jm::plugin_ws_action(b ? b->bytes : 0, bytes, cs != hipStreamCaptureStatusNone)) {
-        case jm::WsAction::StreamOrdered:
+    if (!capturing) {
+        try {
+            b = &plugin_bufs().of(dev, st);
+            out->held = std::unique_lock<std::mutex>(b->mu);
+            b->retired.reserve(b->retired.size() + 1);
+        } catch (const std::exception& x) {
+            return fail(JM_ERR_HIP, "workspace of the stream: %s", x.what());
+        }
+    }
+    switch (plugin_ws_action(b ? b->bytes : 0, bytes, capturing)) {
+        case WsAction::StreamOrdered:
             JM_HIP(hipMallocAsync(&out->p, bytes, st), "hipMallocAsync plugin workspace");
             out->async = true;
             return 0;
-        case jm::WsAction::Reuse:
+        case WsAction::Reuse:
             out->p = b->p;
             return 0;
-        case jm::WsAction::Grow:
+        case WsAction::Grow:
             break;
     }
-    const size_t grow = jm::plugin_ws_grow(b ? b->bytes : 0, bytes);
+    const size_t grow = plugin_ws_grow(b->bytes, bytes);
     void* p = nullptr;
     JM_HIP(hipMalloc(&p, grow), "hipMalloc plugin workspace");
-    if (b) {
-        if (b->p) g_pws_retired.push_back(b->p);
-        b->p = p;
-        b->bytes = grow;
-    } else {
-        g_pws.push_back(PluginBuf{dev, st, p, grow});
-    }
+    if (b->p) b->retired.push_back(b->p);
+    b->p = p;
+    b->bytes = grow;
     out->p = p;
     return 0;
 }

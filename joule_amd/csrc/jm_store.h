@@ -8,6 +8,7 @@
 
 #include "../../include/joule_amd.h"
 #include "jm_kernels.h"
+#include "jm_plugin_ws.h"
 
 namespace jm {
 
@@ -142,12 +143,8 @@ int fail(int code, const char* fmt, ...);
 int hip_fail(hipError_t e, const char* what);
 
 // Workspace of `bytes` for one call's kernels on st, on the current device
-// (jm_plugin_ws.h has the policy); async: free it with hipFreeAsync(p, st)
-// once they are enqueued.
-struct PluginWs {
-    void* p = nullptr;
-    bool async = false;
-};
+// (jm_plugin_ws.h has the policy).  *out lives until they are all enqueued;
+// async: free it with hipFreeAsync(p, st) then.
 int plugin_ws(hipStream_t st, size_t bytes, PluginWs* out);
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
