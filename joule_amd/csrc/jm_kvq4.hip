@@ -896,7 +896,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         // its largest value in [2^10, 2^11), with the score scale's sign
         const uint32_t ex = min(max(__float_as_uint(top) >> 23, 12u), 252u);
         const float f = __builtin_copysignf(__uint_as_float((264u - ex) << 23), a.scale2);
+        // (a scale of 0, or one that underflows with q, as 2^-100: scores below 2^-48, as
+        // they are, and masked ones still -inf behind it)
         cs[b] = __fmul_rn(__uint_as_float((ex - 10u) << 23), fabsf(a.scale2));
+        if (BF) cs[b] = fmaxf(cs[b], 0x1p-100f);
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             uint32_t hi[4], lo[4];
