@@ -507,7 +507,9 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     }
     if (a.S == 1) {
         if (un.pos + (oc >> a.lq) >= c.maxT) return;
-        const float inv = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);       // no row to see: 0
+        // a row below 0 sees none: 0.  (A sum of 0 elsewhere is that of scores that are
+        // all -infinity, as an infinite query makes them: NaN.)
+        const float inv = un.pos + (oc >> a.lq) < 0 ? 0.0f : __fdiv_rn(1.0f, L);
         const size_t oi = ((size_t)(un.tok + (oc >> a.lq)) * a.H + kh * a.qpk + (oc & (a.qpk - 1))) * HD + od;
         store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         return;
@@ -535,7 +537,9 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
         return;
     }
     const int oc = 8 * (blockIdx.x / c.KH % nb) + (threadIdx.x >> 5), od = 4 * (threadIdx.x & 31);
-    if (oc >= a.qpk * un.n || (c.pos ? c.pos[un.tok + (oc >> a.lq)] : un.pos + (oc >> a.lq)) >= c.maxT) return;
+    if (oc >= a.qpk * un.n) return;
+    const int pos = c.pos ? c.pos[un.tok + (oc >> a.lq)] : un.pos + (oc >> a.lq);
+    if (pos >= c.maxT) return;
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
     // lane j of the 32 has the factors of ranges j, j + 32, ..; the ranges' outputs
     // are on their way four at a time
@@ -571,7 +575,7 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
         }
     }
     L = seg_sum<32>(L);
-    const float inv = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);
+    const float inv = pos < 0 ? 0.0f : __fdiv_rn(1.0f, L);                  // (as in k_q4_attn)
     const size_t oi = ((size_t)(un.tok + (oc >> a.lq)) * a.H + kh * a.qpk + (oc & (a.qpk - 1))) * HD + od;
     store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }
@@ -1172,7 +1176,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         for (int q = 0; q < PS; q++)
             L = __builtin_fmaf(mls[q * RG + rg][32 * b + n][1], pow2f(mls[q * RG + rg][32 * b + n][0] - m0), L);
         f[b] = pow2f(ref[b] - m0);
-        inv[b] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);           // no row to see: 0
+        inv[b] = prow[b] < 0 ? 0.0f : __fdiv_rn(1.0f, L);              // (as in k_q4_attn)
         if (a.S > 1) {
             inv[b] = 1.0f;
             float* const ml = a.part_ml + 2 * (((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n);

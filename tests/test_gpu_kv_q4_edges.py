@@ -2,8 +2,9 @@
 
 import numpy as np
 import pytest
+import torch
 
-from test_gpu_kv_q4_bound import cache, check, rows, run, write
+from test_gpu_kv_q4_bound import cache, check, ints, queries, rows, run, write
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,40 @@ def test_queries_of_zero_and_of_the_smallest_values(counts, start, dt):
         q = np.random.default_rng(3).standard_normal((sum(counts), 4, HD)).astype(np.float32) * np.float32(value)
         for scale in (HD ** -0.5, 1e-8, 0.0):
             check(c, q, start, counts, dt, scale)
+
+
+@pytest.mark.parametrize("maxT", [0, 3000])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n,start", [(1, 0), (1, 700), (3, 0), (5, 700), (130, 0), (130, 333)])
+def test_an_infinite_query_gives_nan(n, start, dt, maxT):
+    """Also where every score that it makes is -infinity, whose softmax is
+    undefined: never the 0 of a token that sees no row."""
+    H, KH, T = 4, 2, start + n
+    c = cache(1, maxT or T, KH, H)
+    k, v = rows(5, T, KH)
+    k[:, :, 77] = -2.0                  # an infinity there makes every score -infinity
+    k[:, :, 78] = 2.0                   # ... +infinity
+    write(c, 0, k, v)
+    for at, value in ((77, np.inf), (78, np.inf), (78, -np.inf), (5, np.inf)):
+        q = queries(6, k, start, n, H)
+        q[:, 1, at] = value
+        q[n // 2, 2, at] = value
+        got = c.attention(0, torch.from_numpy(q).cuda().to({"f32": torch.float32, "bf16": torch.bfloat16}[dt]), ints([start]), ints([0, n]))
+        assert bool(got[:, 1].isnan().all()) and bool(got[n // 2, 2].isnan().all())
+        got[:, 1] = 0.0
+        got[n // 2, 2] = 0.0
+        assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("maxT", [200, 3000])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 130])
+def test_a_token_without_rows_gets_0_whatever_its_query(n, dt, maxT):
+    c = cache(2, maxT, 2, 8)
+    k, v = rows(5, 180, 2)
+    write(c, 0, k, v)
+    q = torch.from_numpy(queries(6, k, 0, 2 * n, 8)).cuda().to(dt)
+    q[0, 0], q[0, 1, 5], q[0, 2, 5], q[n, 3] = float("nan"), float("inf"), -float("inf"), float("nan")
+    got = c.attention(0, q, ints([-1, -200]), ints([0, n, 2 * n]))
+    assert not bool(got[0].any()) and not bool(got[n:].any())
+    assert bool(got.isfinite().all())
