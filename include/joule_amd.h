@@ -528,8 +528,9 @@ int jm_kv_q4_read(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
  * own, which are in the cache already (jm_kv_q4_write); n_heads / n_kv is 1, 2, 4
  * or 8.  A token whose row is below 0 sees none: its output is 0 (the one
  * exception to the above).  Scores and sums are float32; float32 q and its weights
- * enter the products with 21 bits, with bf16 q the weights (and, for prompts, the
- * scaled K and V) are rounded to fp16.  A NaN or an infinity in a row that a token
+ * enter the products with 21 bits (weights times V to 2^-29 of the largest such
+ * product, q to 2^-30 of its largest value), with bf16 q the weights (and, for
+ * prompts, the scaled K and V) are rounded to fp16.  A NaN or an infinity in a row that a token
  * sees makes its output NaN; rows that it does not see may hold anything.  out may
  * be q where q is contiguous.  Workspace: as jm_q4_gemm_f32's. */
 int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,

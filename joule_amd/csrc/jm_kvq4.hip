@@ -119,7 +119,10 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 //   weights  exp2(score - ref), ref common to a column's lanes and chosen so that
 //            weight x V scale stays below 2^15: raised only when a lane meets a
 //            product above 2^14, to where the largest is 2^6, so that most tiles
-//            need no exchange between lanes.  Each lane sums its own weights.
+//            need no exchange between lanes.  Each row's weight counts with its own
+//            scale: a large V without weight must not raise ref, under which the
+//            other products would fall out of fp16's range (5 % of the output for a
+//            V 10^8 times the others').  Each lane sums its own weights.
 //   P . V    16 dimensions a product (dimension 16 j + m is row m of product j,
 //            nibble j of the lane's V dwords) as A, weight x scale in fp16, the
 //            rest in columns n + 8, as B, from the lanes that formed
@@ -162,11 +165,15 @@ struct Q4Bits {
 
 __device__ __forceinline__ float pow2f(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Above the exponent of the largest of some scales, given as fp16 bits (which
-// are in order): x < 2^q4_scale_exp(x).  At least that of 2^-14 (0 and the
-// subnormals; the largest of an infinity or NaN is above every finite one's).
-__device__ __forceinline__ float q4_scale_exp(uint32_t bits) {
-    return (float)((int)max((bits & 0x7FFFu) >> 10, 1u) - 14);
+// y + log2(a row's largest V scale) + 15, the scale's logarithm read off its fp16
+// bits (at most 0.09 below the logarithm, and at least -15; an infinity's and a
+// NaN's are above every finite one's).  w: the row's scales, two a word.
+template <int NG>
+__device__ __forceinline__ float q4_weight_exp(float y, const uint32_t* w) {
+    u16x2_t m = __builtin_bit_cast(u16x2_t, w[0]);
+#pragma unroll
+    for (int e = 1; e < NG / 2; e++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[e]));
+    return __builtin_fmaf((float)max(m.x, m.y), 0x1p-10f, y);
 }
 
 // The KV head's query rows of one unit: which sequence, its first token, how
@@ -399,16 +406,11 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
                 for (int e = 0; e < NG / 2; e++) sv[i][e] = in ? sv[i][e] : 0u;
             }
         }
-        // ---- the reference: the largest weight x scale, to the exponent
-        float ym = y[0];
-        u16x2_t sm = 0;
+        // ---- the reference: the largest weight x scale, row by row, to the exponent
+        float z = q4_weight_exp<NG>(y[0], sv[0]);
 #pragma unroll
-        for (int i = 1; i < 8; i++) ym = fmaxf(ym, y[i]);
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int e = 0; e < NG / 2; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sv[i][e]));
-        float z = ym + q4_scale_exp(max(sm.x, sm.y));
+        for (int i = 1; i < 8; i++) z = fmaxf(z, q4_weight_exp<NG>(y[i], sv[i]));
+        z -= 15.0f;
         if (__any(z > ref + 14.0f)) {
             z = fmaxf(z, swz_xor16_f(z));
             z = fmaxf(z, __shfl_xor(z, 32, JM_WAVE));
@@ -1089,15 +1091,10 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     for (int e = 0; e < NG / 2; e++) sx[v / 4][(v % 4) * NG / 2 + e] = in ? sx[v / 4][(v % 4) * NG / 2 + e] : 0u;
                 }
             }
-            float m = y[0];
-            u16x2_t sm = 0;
+            float z = -INFINITY;
 #pragma unroll
-            for (int v = 1; v < 16; v++) m = fmaxf(m, y[v]);
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int e = 0; e < 2 * NG; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sx[q][e]));
-            raise(0, m + q4_scale_exp(max(sm.x, sm.y)));
+            for (int v = 0; v < 16; v++) z = fmaxf(z, q4_weight_exp<NG>(y[v], &sx[v / 4][(v % 4) * NG / 2]));
+            raise(0, z - 15.0f);
             const float r0 = ref[0] == -INFINITY ? 0.0f : ref[0];
 #pragma unroll
             for (int v = 0; v < 16; v++) {

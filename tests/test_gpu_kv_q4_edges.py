@@ -69,3 +69,30 @@ def test_a_token_without_rows_gets_0_whatever_its_query(n, dt, maxT):
     got = c.attention(0, q, ints([-1, -200]), ints([0, n, 2 * n]))
     assert not bool(got[0].any()) and not bool(got[n:].any())
     assert bool(got.isfinite().all())
+
+
+def _without_weight(T, big, at):
+    """Rows of 1e-3 that share the weight, and row `at` of `big` with none."""
+    rng = np.random.default_rng(4)
+    q = rng.standard_normal((1, 2, HD)).astype(np.float32)
+    k, v = rows(9, T, 1)
+    v *= 1e-3
+    k[at, 0] = -30.0 * (q[0, 0] + q[0, 1])
+    v[at, 0] = big
+    return q, k, v
+
+
+@pytest.mark.parametrize("big", [1.0, 1e3, 1e5, 4e5])
+@pytest.mark.parametrize("at", [0, 37, 390])
+@pytest.mark.parametrize("maxT", [400, 3000])
+def test_a_large_v_without_weight_leaves_the_others_whole(maxT, at, big):
+    """Single tokens, float32 and bf16, and prompts, float32: the weights of the
+    others keep their bits, next to the large row and after it."""
+    T = 400
+    q, k, v = _without_weight(T, big, at)
+    c = cache(1, maxT, 1, 2)
+    write(c, 0, k, v)
+    for dt in ("f32", "bf16"):
+        check(c, q, [T - 1], [1], dt)
+    # 100 tokens with the last one's query
+    check(c, np.repeat(q, 100, axis=0), [T - 100], [100], "f32", only=[70, 99] if at > 300 else [0, 70, 99])
