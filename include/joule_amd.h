@@ -529,10 +529,13 @@ int jm_kv_q4_read(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
  * or 8.  A token whose row is below 0 sees none: its output is 0 (the one
  * exception to the above).  Scores and sums are float32; float32 q and its weights
  * enter the products with 21 bits (weights times V to 2^-29 of the largest such
- * product, q to 2^-30 of its largest value), with bf16 q the weights (and, for
- * prompts, the scaled K and V) are rounded to fp16.  A NaN or an infinity in a row that a token
- * sees makes its output NaN; rows that it does not see may hold anything.  out may
- * be q where q is contiguous.  Workspace: as jm_q4_gemm_f32's. */
+ * product, q to 2^-30 of its largest value).  With bf16 q the weights are rounded to
+ * fp16, and, from 96 query rows a KV head and sequence on, K and V too (2^-11 of the
+ * value, or 2^-15 of the largest scale of 16 consecutive rows, where no row's is
+ * below 2^-8 of that; such rows are kept whole, at several times the cost of the
+ * call).  A NaN or an infinity in K in a row that a token sees, or in q, makes its
+ * output NaN, one in V that group's part of it.  Rows that it does not see may hold
+ * anything.  out may be q where q is contiguous.  Workspace: as jm_q4_gemm_f32's. */
 int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
                   int64_t q_head, int n_heads, float scale, int dtype, void* out, void* stream);
 

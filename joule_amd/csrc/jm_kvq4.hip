@@ -265,23 +265,41 @@ struct Q4Tile {
     u32x4_t ks[NG], vs[NG];     // (NG / 2 words of 16 bytes a row group t)
 };
 
+// Where a lane's share of a tile lies, and of the tiles after it.
 template <int NG>
-__device__ __forceinline__ void q4_load_tile(Q4Tile<NG>& x, const Q4Head<NG>& k, const Q4Head<NG>& v, int tile, int lane) {
-    const int g = lane >> 4, n = lane & 15;
+struct Q4TileAt {
+    gptr<const u32x4_t> k, v, ks, vs;
+    __device__ __forceinline__ Q4TileAt(const Q4Head<NG>& kk, const Q4Head<NG>& vv, int tile, int lane) {
+        const int g = lane >> 4, n = lane & 15;
+        const size_t r = (size_t)32 * tile;
+        k = (gptr<const u32x4_t>)(kk.codes + (r + n) * 16 + 4 * g);
+        v = (gptr<const u32x4_t>)(vv.codes + r * 16 + 64 * g + 4 * n);
+        ks = (gptr<const u32x4_t>)(kk.scales + (r + 4 * g) * NG);
+        vs = (gptr<const u32x4_t>)(vv.scales + (r + 4 * g) * NG);
+    }
+    __device__ __forceinline__ void skip(int tiles) {
+        k += tiles * 128;       // (16 bytes of a row's 64, 32 rows a tile)
+        v += tiles * 128;
+        ks += tiles * 4 * NG;
+        vs += tiles * 4 * NG;
+        // (from registers: left to the compiler, the additions come ahead of the loads)
+        __asm__("" : "+v"(k), "+v"(v), "+v"(ks), "+v"(vs));
+    }
+    __device__ __forceinline__ void load(Q4Tile<NG>& x) const {
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const size_t r = (size_t)32 * tile + 16 * t;
-        // (past the caches: 32 sequences of 16384 rows 105 -> 101 us, and no slower
-        // where units share rows)
-        x.k[t] = __builtin_nontemporal_load((gptr<const u32x4_t>)(k.codes + (r + n) * 16 + 4 * g));
-        x.v[t] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v.codes + r * 16 + 64 * g + 4 * n));
+        for (int t = 0; t < 2; t++) {
+            // (past the caches: 32 sequences of 16384 rows 105 -> 101 us, and no slower
+            // where units share rows)
+            x.k[t] = __builtin_nontemporal_load(k + 64 * t);
+            x.v[t] = __builtin_nontemporal_load(v + 64 * t);
 #pragma unroll
-        for (int i = 0; i < NG / 2; i++) {
-            x.ks[t * (NG / 2) + i] = ((gptr<const u32x4_t>)(k.scales + (r + 4 * g) * NG))[i];
-            x.vs[t * (NG / 2) + i] = ((gptr<const u32x4_t>)(v.scales + (r + 4 * g) * NG))[i];
+            for (int i = 0; i < NG / 2; i++) {
+                x.ks[t * (NG / 2) + i] = ks[2 * NG * t + i];
+                x.vs[t * (NG / 2) + i] = vs[2 * NG * t + i];
+            }
         }
     }
-}
+};
 
 // scale of row i (0..3) of row group t, group e
 template <int NG>
@@ -291,29 +309,26 @@ __device__ __forceinline__ float q4_scale(const u32x4_t (&s)[NG], int t, int i, 
     return (float)__builtin_bit_cast(f16x2, w)[h % 2];
 }
 
-template <int NG, bool BF>
-__global__ void __launch_bounds__(256, 2)
-k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
+// The 8 query rows of one unit over tiles t0 .. t_end - 1, a wave taking every W-th;
+// all W waves joined, and the output, or (several ranges) the partial outputs of
+// unit u and range s from their row row0 on.  ow and mls: LDS for the W waves.
+template <int NG, bool BF, int W>
+__device__ __forceinline__ void q4_attn_unit(const Q4KvArgs& c, const Q4AttnArgs& a, const Q4Unit& un, int kh, int t0,
+                                             int t_end, int u, int s, int row0, float (*ow)[8][128], float (*mls)[8][2]) {
     constexpr int HD = 128, GS = 4 / NG;                    // contraction steps a group
-    __shared__ __align__(16) float ow[4][8][HD];
-    __shared__ float mls[4][8][2];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15, col = n & 7;
-    const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH % a.units, s = blockIdx.x / c.KH / a.units;
-    Q4Unit un;
-    if (!q4_unit(c, u, a.tp, un)) return;                   // (block-uniform)
     const int ncol = a.qpk * un.n;
+    int t = t0 + w;
     const int ct = min(col >> a.lq, un.n - 1), head = kh * a.qpk + (col & (a.qpk - 1));
-    const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
-    const int crow = min(un.pos + ct, c.maxT - 1);          // and this column's
-    const int NT = (last + 32) / 32;                        // (0 where last < 0)
-    const int t_end = (int)((long long)NT * (s + 1) / a.S);
-    int t = (int)((long long)NT * s / a.S) + w;
+    const int crow = min(un.pos + ct, c.maxT - 1);          // the last row that this column sees
 
     const Q4Head<NG> kk(q4_plane(c, un.seq, 0), kh, c.KH, c.R), vv(q4_plane(c, un.seq, 1), kh, c.KH, c.R);
     const Q4Mix mix;
     Q4Tile<NG> cur, nxt;
-    if (t < t_end) q4_load_tile(cur, kk, vv, t, lane);
+    Q4TileAt<NG> at(kk, vv, t, lane);
+    if (t < t_end) at.load(cur);
+    at.skip(W);
 
     // the query columns: dimensions 32 st + 8 g + e, pairs (e, e + 4)
     const bool lo_col = !BF && n >= 8;
@@ -364,8 +379,9 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     float ref = -INFINITY, l = 0.0f;
     const Q4Bits bits;
 
-    for (; t < t_end; t += 4) {
-        if (t + 4 < t_end) q4_load_tile(nxt, kk, vv, t + 4, lane);
+    for (; t < t_end; t += W) {
+        if (t + W < t_end) at.load(nxt);
+        at.skip(W);
         // ---- scores
         float y[8];
 #pragma unroll
@@ -493,11 +509,13 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     // ---- the block's: thread = column tid / 32, dimensions 4 (tid % 32) ..
     const int oc = threadIdx.x >> 5, od = 4 * (threadIdx.x & 31);
     if (oc >= ncol) return;
-    const float M = fmaxf(fmaxf(mls[0][oc][0], mls[1][oc][0]), fmaxf(mls[2][oc][0], mls[3][oc][0]));
+    float M = mls[0][oc][0];
+#pragma unroll
+    for (int i = 1; i < W; i++) M = fmaxf(M, mls[i][oc][0]);
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float L = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < W; i++) {
         if (q4_dead(mls[i][oc][0], mls[i][oc][1])) continue;
         const float f = pow2f(mls[i][oc][0] - M);
         const float4 x = *(const float4*)&ow[i][oc][od];
@@ -516,12 +534,25 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
         store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         return;
     }
-    const size_t pi = (((size_t)u * c.KH + kh) * a.S + s) * (a.qpk * a.tp) + oc;
+    const size_t pi = (((size_t)u * c.KH + kh) * a.S + s) * (a.qpk * a.tp) + row0 + oc;
     if (!q4_dead(M, L)) *(float4*)(a.part_o + pi * HD + od) = v;
     if ((threadIdx.x & 31) == 0) {
         a.part_ml[2 * pi] = M;
         a.part_ml[2 * pi + 1] = L;
     }
+}
+
+template <int NG, bool BF>
+__global__ void __launch_bounds__(256, 2)
+k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
+    __shared__ __align__(16) float ow[4][8][128];
+    __shared__ float mls[4][8][2];
+    const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH % a.units, s = blockIdx.x / c.KH / a.units;
+    Q4Unit un;
+    if (!q4_unit(c, u, a.tp, un)) return;                   // (block-uniform)
+    const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
+    const int NT = (last + 32) / 32;                        // (0 where last < 0)
+    q4_attn_unit<NG, BF, 4>(c, a, un, kh, (int)((long long)NT * s / a.S), (int)((long long)NT * (s + 1) / a.S), u, s, 0, ow, mls);
 }
 
 // The ranges of one (KV head, unit) merged into the output, 8 query rows a block.
@@ -604,13 +635,20 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
 // Two forms.  float32 queries: the codes less 8 are exact in LDS, q and the
 // weights are two fp16 halves each, every group's scores are scaled on their own
 // and the V scale goes into the weights, as in k_q4_attn.  bf16 queries (BF): K and
-// V are scaled in LDS and rounded to fp16 (2^-11 of the value, 2^-24 of the largest
-// of 16 rows), relative to the 16 rows' largest scale, whose exponent goes into the
-// scores and the weights; q is exact, the weights are fp16 once (their sum is of
-// the float32 ones: where 16 rows of V are far below the others, fp16 no longer
-// holds weights that count).  That is one product where the other form takes two,
-// no arithmetic on scales between them, and 64 query rows a wave (QB = 2), which
+// V are scaled in LDS and rounded to fp16 (2^-11 of the value, or 2^-15 of the
+// largest scale of 16 rows), relative to the 16 rows' largest scale, whose exponent
+// goes into the scores and the weights; q is exact, the weights are fp16 once (their
+// sum is of the float32 ones: where 16 rows of V are far below the others, fp16 no
+// longer holds weights that count).  That is one product where the other form takes
+// two, no arithmetic on scales between them, and 64 query rows a wave (QB = 2), which
 // halves the LDS reads a product.
+//
+// Rows of which one is below 2^-8 of the largest of its 16 do not bear that: a later
+// token's row would take the bits of an earlier token's.  A block that finds such
+// among the scales of its range does the range as k_q4_attn does.  Looking takes some
+// 1.3 us (509 tokens 25.7 -> 27.0 us, 2047 behind 4099 rows 224 -> 227); looking while
+// staging, or branching behind the loop, spilled the loop's registers.  Where there
+// are such rows these take 90 and 1070 us.
 //
 // Measured at 2047 tokens behind 4099 rows, 32 query heads on 8 (172 GFLOP, 147 us
 // at the rate of a large library product): 227 us a call, 250 - 264 under a
@@ -667,6 +705,65 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// Whether of rows r0 .. r1 - 1 (r0 a multiple of 16) one's largest scale is below 2^-8
+// of the largest of its 16 (rows of zeros, exact at any exponent, and scales that
+// are not finite do not count): this thread's share of the 512 threads'.
+template <int NG>
+__device__ __forceinline__ bool q4_rows_apart(const Q4Head<NG>& k, const Q4Head<NG>& v, int r0, int r1) {
+    constexpr int RPL = 8 / NG;                 // rows a lane: 16 bytes of scales
+    bool far = false;
+    auto look = [&](u32x4_t x, int r) __attribute__((always_inline)) {
+        uint32_t m[RPL], top = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            u16x2_t h = 0;
+#pragma unroll
+            for (int e = 0; e < NG / 2; e++) {
+                uint32_t y = x[i * (NG / 2) + e] & 0x7FFF7FFFu;
+                if ((y & 0x7C00u) == 0x7C00u) y &= 0xFFFF0000u;
+                if ((y & 0x7C000000u) == 0x7C000000u) y &= 0xFFFFu;
+                h = __builtin_elementwise_max(h, __builtin_bit_cast(u16x2_t, y));
+            }
+            m[i] = r + i < r1 ? max(h.x, h.y) : 0u;
+            top = max(top, m[i]);
+            least = min(least, m[i] - 1u);      // (0 last of all)
+        }
+        top = max(top, (uint32_t)dpp_i<DPP_XOR1>((int)top));
+        top = max(top, (uint32_t)dpp_i<DPP_XOR2>((int)top));
+        if (NG == 4) top = max(top, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)top));
+        const _Float16 lim = __builtin_bit_cast(_Float16, (uint16_t)top) * (_Float16)0x1p-8f;
+        far |= least < max((uint32_t)__builtin_bit_cast(uint16_t, lim), 1u) - 1u;
+    };
+    for (int r = r0 + RPL * (int)threadIdx.x; r - RPL * (int)threadIdx.x < r1; r += RPL * 512) {
+        const int at = min(r, (r1 - 1) / RPL * RPL);            // (inside the plane; rows past the end count as 0)
+        const u32x4_t x = *(gptr<const u32x4_t>)(k.scales + (size_t)at * NG);
+        const u32x4_t y = *(gptr<const u32x4_t>)(v.scales + (size_t)at * NG);
+        look(x, r);
+        look(y, r);
+    }
+    return far;
+}
+
+// A block's range of k_q4_tile<BF> from the codes, 8 query rows at a time.
+template <int NG, int STEP>
+__device__ __forceinline__ void q4_tile_again(const Q4KvArgs& c, const Q4AttnArgs& a, float (*ow)[8][128], float (*mls)[8][2]) {
+    uint32_t bx = blockIdx.x;
+    __asm__ volatile("" : "+s"(bx));
+    const int kh = bx % c.KH, rs = bx / c.KH, u = a.units - 1 - rs % a.units, sr = rs / a.units;
+    Q4Unit un;
+    if (!q4_unit(c, u, a.tp, un)) return;
+    const int steps = (min(un.pos + un.n - 1, c.maxT - 1) + STEP) / STEP;
+    const int t0 = (int)((long long)steps * sr / a.S) * (STEP / 32), t1 = (int)((long long)steps * (sr + 1) / a.S) * (STEP / 32);
+    const int tp = 8 >> a.lq;
+#pragma unroll 1
+    for (int t = 0; t < un.n; t += tp) {
+        const Q4Unit x = {un.seq, un.tok + t, min(tp, un.n - t), un.pos + t};
+        const int NT = (min(x.pos + x.n - 1, c.maxT - 1) + 32) / 32;
+        q4_attn_unit<NG, true, 8>(c, a, x, kh, t0, min(t1, NT), u, sr, t << a.lq, ow, mls);
+        __syncthreads();
+    }
+}
+
 template <int NG, bool BF, int RG>
 __global__ void __launch_bounds__(512, 2)
 k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
@@ -681,6 +778,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
     __shared__ int eb[2][STEP / 16][2];         // (BF) exponents of the 16-row blocks' scales, K and V
     __shared__ uint32_t tn[8][32 * QB];
+    __shared__ uint32_t apart[8];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH;
@@ -877,6 +975,19 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     };
 
     if (step0 < nstep) request(step0);
+    if constexpr (BF) {
+        const bool far = q4_rows_apart<NG>(kk, vv, step0 * STEP, min(nstep * STEP, pmax + 1));
+        const bool any = __any(far);
+        if (lane == 0) apart[w] = any;
+        __syncthreads();
+        uint32_t f = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) f |= apart[i];
+        if (__builtin_amdgcn_readfirstlane(f)) {
+            q4_tile_again<NG, STEP>(c, a, (float (*)[8][HD])&kv[0][0], (float (*)[8][2])&mls[0][0][0]);
+            return;
+        }
+    }
 
     // ---- the query rows
     f16x8 qh[8], ql[BF ? 1 : 8];
@@ -1185,7 +1296,7 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
         }
     }
     float4* const mb = (float4*)&kv[0][0];                                 // [wave][QB][4][64 lanes]
-    static_assert(8 * QB * 4 * 64 * 16 <= 2 * PB, "the outputs of 32 dimensions fit");
+    static_assert(8 * QB * 4 * 64 * 16 <= 2 * PB && 8 * 8 * HD * 4 <= 2 * PB, "the outputs of 32 dimensions, and of 8 rows, fit");
 #pragma unroll
     for (int nt = 0; nt < 4; nt++) {
         if (nt) __syncthreads();

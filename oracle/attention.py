@@ -43,8 +43,10 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, seen: int, scale: float)
 
 
 def _rows16(x: np.ndarray, seen: int) -> np.ndarray:
-    """2^-15 of the largest scale of each row's 16 rows, or of 2^8 times its own."""
+    """2^-15 of the largest scale of each row's 16 rows, or of 2^8 times its own
+    (rows that are not finite, behind those seen, do not count)."""
     s = np.abs(x).max(axis=1) / 6.9
+    s = np.where(np.isfinite(s), s, 0.0)
     n = -(-len(s) // 16) * 16
     block = np.concatenate([s, np.zeros(n - len(s))]).reshape(-1, 16).max(axis=1).repeat(16)[:len(s)]
     return 2.0 ** -15 * np.minimum(block, 2.0 ** 8 * s)[:seen]

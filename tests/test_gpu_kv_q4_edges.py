@@ -96,3 +96,69 @@ def test_a_large_v_without_weight_leaves_the_others_whole(maxT, at, big):
         check(c, q, [T - 1], [1], dt)
     # 100 tokens with the last one's query
     check(c, np.repeat(q, 100, axis=0), [T - 100], [100], "f32", only=[70, 99] if at > 300 else [0, 70, 99])
+
+
+@pytest.mark.parametrize("group", [64, 32])
+@pytest.mark.parametrize("maxT", [400, 3000, 40000])
+@pytest.mark.parametrize("big", [3.0, 1e3, 1e5, 4e5])
+def test_a_large_v_without_weight_in_bf16_prompts(big, maxT, group):
+    T = 400
+    for at in (0, 37, 390):
+        q, k, v = _without_weight(T, big, at)
+        c = cache(1, maxT, 1, 2, group)
+        write(c, 0, k, v)
+        check(c, np.repeat(q, 100, axis=0), [T - 100], [100], "bf16", only=[70, 99] if at > 300 else [0, 70, 99])
+
+
+@pytest.mark.parametrize("H,KH,n,start", [(2, 1, 100, 0), (8, 1, 60, 333), (8, 2, 150, 10), (4, 4, 130, 64)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("maxT", [0, 3000, 40000])
+def test_rows_of_later_tokens_may_hold_anything(H, KH, n, start, dt, maxT):
+    """A prompt's row with a K or V far above the others: tokens before it are
+    as exact as without it."""
+    for which, big in (("v", 3e5), ("k", 3e5), ("v", 300.0), ("k", 300.0)):
+        k, v = rows(17, start + n + 1, KH)
+        at = start + n // 2
+        (v if which == "v" else k)[at] *= big / 3
+        c = cache(1, maxT or start + n, KH, H)
+        write(c, 0, k[:start + n], v[:start + n])
+        q = queries(18, rows(17, start + n + 1, KH)[0], start, n, H)
+        check(c, q, [start], [n], dt, only=sorted({0, n // 4, n // 2 - 2, n // 2 - 1}))
+
+
+@pytest.mark.parametrize("group", [64, 32])
+@pytest.mark.parametrize("maxT", [0, 3000, 40000])
+def test_rows_of_every_magnitude_in_bf16_prompts(maxT, group):
+    """K and V from 1e-7 to 1e5 within 16 rows, subnormal scales among them, and
+    sequences without such rows beside."""
+    H, KH, counts, start = 4, 2, [120, 0, 90, 100], [50, 3, 400, 0]
+    c = cache(4, maxT or 490, KH, H, group)
+    q = []
+    for b, (s, n) in enumerate(zip(start, counts)):
+        k, v = rows(b + 40, s + n + 1, KH)
+        if b != 3:
+            v *= 10.0 ** (np.arange(s + n + 1) % 13 - 7.0)[:, None, None]
+        if b == 2:
+            k *= 10.0 ** (np.arange(s + n + 1) % 5 - 3.0)[:, None, None]
+        write(c, b, k[:s + n], v[:s + n])
+        q.append(queries(b + 60, rows(b + 40, s + n + 1, KH)[0], s, n, H))
+    check(c, np.concatenate(q), start, counts, "bf16")
+
+
+def test_non_finite_rows_beside_large_ones_in_bf16_prompts():
+    """A NaN in V reaches the group's outputs of those that see it, also where rows
+    differ far; the others are as they were."""
+    H, KH, n, s = 4, 1, 100, 60
+    k, v = rows(71, s + n + 1, KH)
+    v[s + 10] *= 1e5
+    clean = cache(1, s + n, KH, H)
+    write(clean, 0, k[:s + n], v[:s + n])
+    q = queries(72, k, s, n, H)
+    want = check(clean, q, [s], [n], "bf16", only=[0, 9, 50])
+    bad = v.copy()
+    bad[s + 40, 0, 3] = np.nan
+    c = cache(1, s + n, KH, H)
+    write(c, 0, k[:s + n], bad[:s + n])
+    got = c.attention(0, torch.from_numpy(q).cuda().bfloat16(), ints([s]), ints([0, n]))
+    assert torch.equal(got[:40], want[:40]) and bool(got[40:, :, 64:].isfinite().all())
+    assert bool(got[40:, :, :64].isnan().all())
