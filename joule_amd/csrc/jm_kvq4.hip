@@ -165,15 +165,18 @@ struct Q4Bits {
 
 __device__ __forceinline__ float pow2f(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// y + log2(a row's largest V scale) + 15, the scale's logarithm read off its fp16
-// bits (at most 0.09 below the logarithm, and at least -15; an infinity's and a
-// NaN's are above every finite one's).  w: the row's scales, two a word.
+// y + log2(the largest of some V scales, given as fp16 bits) + 15, the logarithm read
+// off the bits (at most 0.09 below it, and at least -15; an infinity's and a NaN's
+// are above every finite one's).
+__device__ __forceinline__ float q4_weight_exp(float y, u16x2_t m) { return __builtin_fmaf((float)max(m.x, m.y), 0x1p-10f, y); }
+
+// ... of a row's scales, two a word
 template <int NG>
 __device__ __forceinline__ float q4_weight_exp(float y, const uint32_t* w) {
     u16x2_t m = __builtin_bit_cast(u16x2_t, w[0]);
 #pragma unroll
     for (int e = 1; e < NG / 2; e++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[e]));
-    return __builtin_fmaf((float)max(m.x, m.y), 0x1p-10f, y);
+    return q4_weight_exp(y, m);
 }
 
 // The KV head's query rows of one unit: which sequence, its first token, how
@@ -422,20 +425,31 @@ __device__ __forceinline__ void q4_attn_unit(const Q4KvArgs& c, const Q4AttnArgs
                 for (int e = 0; e < NG / 2; e++) sv[i][e] = in ? sv[i][e] : 0u;
             }
         }
-        // ---- the reference: the largest weight x scale, row by row, to the exponent
-        float z = q4_weight_exp<NG>(y[0], sv[0]);
+        // ---- the reference: the largest weight x scale, to the exponent; row by row
+        // only where the largest weight times the largest scale passes it
+        float ym = y[0];
+        u16x2_t sm = 0;
 #pragma unroll
-        for (int i = 1; i < 8; i++) z = fmaxf(z, q4_weight_exp<NG>(y[i], sv[i]));
-        z -= 15.0f;
-        if (__any(z > ref + 14.0f)) {
-            z = fmaxf(z, swz_xor16_f(z));
-            z = fmaxf(z, __shfl_xor(z, 32, JM_WAVE));
-            const float nref = fmaxf(ref, z - 6.0f);
-            const float f = ref == -INFINITY ? 0.0f : pow2f(ref - nref);
-            l *= f;
+        for (int i = 1; i < 8; i++) ym = fmaxf(ym, y[i]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) O[j] *= f;
-            ref = nref;
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < NG / 2; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sv[i][e]));
+        const float pass = ref + 29.0f;                     // (q4_weight_exp's 15 among it)
+        if (__any(q4_weight_exp(ym, sm) > pass)) {
+            float z = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) z = fmaxf(z, q4_weight_exp<NG>(y[i], sv[i]));
+            if (__any(z > pass)) {
+                z = fmaxf(z, swz_xor16_f(z));
+                z = fmaxf(z, __shfl_xor(z, 32, JM_WAVE));
+                const float nref = fmaxf(ref, z - 21.0f);
+                const float f = ref == -INFINITY ? 0.0f : pow2f(ref - nref);
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) O[j] *= f;
+                ref = nref;
+            }
         }
         const float r0 = ref == -INFINITY ? 0.0f : ref;     // (a column that has seen nothing yet)
         float p[8];
@@ -1202,10 +1216,20 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
                     for (int e = 0; e < NG / 2; e++) sx[v / 4][(v % 4) * NG / 2 + e] = in ? sx[v / 4][(v % 4) * NG / 2 + e] : 0u;
                 }
             }
-            float z = -INFINITY;
+            float m = y[0];
+            u16x2_t sm = 0;
 #pragma unroll
-            for (int v = 0; v < 16; v++) z = fmaxf(z, q4_weight_exp<NG>(y[v], &sx[v / 4][(v % 4) * NG / 2]));
-            raise(0, z - 15.0f);
+            for (int v = 1; v < 16; v++) m = fmaxf(m, y[v]);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int e = 0; e < 2 * NG; e++) sm = __builtin_elementwise_max(sm, __builtin_bit_cast(u16x2_t, sx[q][e]));
+            if (__any(q4_weight_exp(m, sm) > ref[0] + 29.0f)) {     // (as in q4_attn_unit)
+                float z = -INFINITY;
+#pragma unroll
+                for (int v = 0; v < 16; v++) z = fmaxf(z, q4_weight_exp<NG>(y[v], &sx[v / 4][(v % 4) * NG / 2]));
+                raise(0, z - 15.0f);
+            }
             const float r0 = ref[0] == -INFINITY ? 0.0f : ref[0];
 #pragma unroll
             for (int v = 0; v < 16; v++) {
