@@ -126,7 +126,7 @@ struct SmHow {
     float mx;                   // the largest logit
     double c;                   // log2(e) / T
     float cb;                   // bins a unit of l
-    float zb;                   // bins a unit of (max - l) / T
+    float T;
     int k;                      // 0: all
     float p, mp, u;
 };
@@ -149,7 +149,7 @@ __device__ __forceinline__ void sm_how(SmHow& h, const SampleArgs& a, int b, con
     // (0 / 0 where all are alike: no span)
     const float span = fminf(__fsub_rn(h.mx, -seg_max<64>(-mn)), __fmul_rn(SM_SPAN, T));
     h.cb = fminf(__fdiv_rn((float)SM_BINS, span), 3.0e38f);
-    h.zb = __fmul_rn(T, h.cb);
+    h.T = T;
 }
 
 __device__ __forceinline__ unsigned long long sm_weight(const SmHow& h, float l) {
@@ -432,13 +432,16 @@ k_sample_hist(SampleArgs a, char* ws, int SP, int chunk) {
     }
     int mbin = 0;
     if (h.mp > 0.0f) {
-        // the bin where weights pass the border (rounded ones: half a unit
-        // below it), and its neighbours, which rounding here may mean
+        // the bin where weights pass the border (rounded ones: half a unit below it),
+        // and its neighbours, which rounding here may mean; in float64, as next to a
+        // min_p of 1 the border is 2^-41 of (max - l) / T, and the last bin where a high
+        // temperature puts it past all logits.  (cb is 0 where logits differ by more
+        // than float32 holds: two bins for all, the border in either.)
         const double wmin = fmin(ceil((double)h.mp * (double)SM_ONE), (double)SM_ONE);
-        const float z = -__logf((float)((wmin - 0.5) / (double)SM_ONE)) * h.zb;
-        const int i = (int)fminf(fmaxf(z, 0.0f), (float)(SM_BINS - 1));
-        mbin = max(i - 1, 0);
-        const int mh = min(i + 1, SM_BINS - 1);
+        const double z = -log((wmin - 0.5) / (double)SM_ONE) * (double)h.T * (double)h.cb;
+        const int i = z < (double)(SM_BINS - 1) ? (int)z : SM_BINS - 1;
+        mbin = h.cb > 0.0f ? max(i - 1, 0) : 0;
+        const int mh = h.cb > 0.0f ? min(i + 1, SM_BINS - 1) : SM_BINS - 1;
         set(mbin, mh);
         lo = min(lo, before(mbin));
         hi = min(hi, incl[mh]);
