@@ -210,8 +210,10 @@ k_sample_max(SampleArgs a, char* ws, int SP, int chunk) {
         for (int e = 0; e < 8; e++) v[e] = sm_logit(a, row, min(i0 + e * SM_T, i1 - 1));
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            mx = fmaxf(mx, v[e]);
-            mn = fminf(mn, v[e] > -INFINITY ? v[e] : INFINITY);
+            // (each logit counts once: sm_kth_part takes the waves' maxima for parts)
+            const bool in = i0 + e * SM_T < i1;
+            mx = fmaxf(mx, in ? v[e] : -INFINITY);
+            mn = fminf(mn, in && v[e] > -INFINITY ? v[e] : INFINITY);
         }
     }
     mx = seg_max<64>(mx);

@@ -51,3 +51,25 @@ def test_a_border_among_logits_that_differ_beyond_float32(min_p):
     for T in (3e37, 1e38, 3e38):
         for u in (0.0, 0.4, 0.97):
             _check(x, [u] * 3, temperature=T, min_p=min_p)
+
+
+def test_small_top_k_with_the_largest_logit_at_a_chunks_end():
+    """The last token of a chunk belongs to one part of the row, from whose maxima
+    the bound on the k-th logit comes; where it counted for several, the bound
+    passed all but that token and the row was selected by its keys."""
+    B, V = 128, 151936
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(B, V, generator=g, device="cuda") * 2
+    chunk = V // 4
+    for at in (chunk - 1, 2 * chunk - 1, V - 1, 0):
+        y = x.clone()
+        y[:, at] = 40.0
+        u = torch.rand(B, generator=g, device="cuda")
+        for k in (2, 16, 50):
+            tok, p = sample(y, u, 30.0, k)
+            w, order = y.double().topk(k, dim=1)
+            w = torch.round(torch.exp((w - w[:, :1]) / 30.0) * 2.0 ** 40)
+            run = w.cumsum(dim=1)
+            i = (run <= torch.floor(u.double()[:, None] * run[:, -1:])).sum(dim=1, keepdim=True)
+            assert torch.equal(order.gather(1, i).squeeze(1).int(), tok)
+            assert torch.allclose((w.gather(1, i) / run[:, -1:]).squeeze(1).float(), p, rtol=2.0 ** -22, atol=0)
