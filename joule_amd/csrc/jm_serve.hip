@@ -11,6 +11,13 @@ namespace {
 
 constexpr int HD = 128;
 
+// Threads of a launch.
+constexpr long long MAX_THREADS = UINT32_MAX;
+
+// Rows of a cache: cache rows and tiles of them are counted in 32 bits, up to a
+// block's step past the last.
+constexpr int Q4_MAX_T = INT32_MAX - 1023;
+
 int check_group(int group) {
     if (group != 32 && group != 64) return fail(JM_ERR_SHAPE, "group must be 64 or 32, got %d", group);
     return 0;
@@ -24,7 +31,9 @@ int q4_args(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, j
         return fail(JM_ERR_SHAPE, "n_seq=%d must be >= 0, maxT=%d and n_kv=%d positive", c->n_seq, c->maxT, c->n_kv);
     if (N < 0) return fail(JM_ERR_ARG, "N must be >= 0");
     if (!cu && N != c->n_seq) return fail(JM_ERR_SHAPE, "without cu there is one token a sequence: N=%d, n_seq=%d", N, c->n_seq);
-    if ((long long)N * c->n_kv > INT32_MAX) return fail(JM_ERR_SHAPE, "N * n_kv = %lld is too large", (long long)N * c->n_kv);
+    // rows are written and read by 16 threads each, a wave 4 tokens of a head
+    if (((long long)N + 3) / 4 * c->n_kv * 64 > MAX_THREADS - 256)
+        return fail(JM_ERR_SHAPE, "N=%d tokens of %d KV heads are more than one launch takes", N, c->n_kv);
     const int64_t bytes = jm_kv_q4_bytes(c->maxT, c->n_kv, c->group);
     if (bytes < 0) return (int)bytes;
     if (N == 0 || c->n_seq == 0) return 0;
@@ -56,7 +65,7 @@ extern "C" {
 
 int64_t jm_kv_q4_bytes(int maxT, int n_kv, int group) {
     if (maxT <= 0 || n_kv <= 0) return fail(JM_ERR_SHAPE, "maxT=%d and n_kv=%d must be positive", maxT, n_kv);
-    if (maxT > INT32_MAX - 64) return fail(JM_ERR_SHAPE, "maxT=%d is too large", maxT);
+    if (maxT > Q4_MAX_T) return fail(JM_ERR_SHAPE, "maxT=%d is too large", maxT);
     if (int rc = check_group(group)) return rc;
     return (int64_t)jm::q4_plane_rows(maxT) * n_kv * (HD / 2 + 2 * HD / group);
 }
@@ -97,6 +106,9 @@ int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
     if (int rc = q4_tensor("out", out, dtype, 0, 0)) return rc;
     hipStream_t st = (hipStream_t)stream;
     const jm::Q4AttnPlan p = jm::q4_attn_plan(a, n_heads, dtype == JM_DTYPE_BF16, false);
+    // (ranges are for few units, so that the kernel that joins them has fewer threads)
+    const long long threads = (long long)c->n_kv * p.units * p.S * (p.rg ? 512 : 256);
+    if (threads > MAX_THREADS) return fail(JM_ERR_SHAPE, "attention of N=%d tokens and %d KV heads is more than one launch takes", N, c->n_kv);
     jm::PluginWs ws;
     if (p.o_floats)
         if (int rc = jm::plugin_ws(st, (p.o_floats + p.ml_floats) * 4, &ws)) return rc;
