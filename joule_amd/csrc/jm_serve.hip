@@ -100,7 +100,8 @@ int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
     const int qpk = n_heads > 0 && n_heads % c->n_kv == 0 ? n_heads / c->n_kv : 0;
     if (qpk != 1 && qpk != 2 && qpk != 4 && qpk != 8)
         return fail(JM_ERR_SHAPE, "n_heads / n_kv must be 1, 2, 4 or 8 (got %d / %d)", n_heads, c->n_kv);
-    if (!std::isfinite(scale)) return fail(JM_ERR_ARG, "scale must be finite");
+    // (the kernels take it times log2(e))
+    if (!std::isfinite(scale * 1.4426950408889634f)) return fail(JM_ERR_ARG, "scale must be finite, and below 2.3e38 in magnitude");
     if (a.N == 0) return 0;
     if (int rc = q4_tensor("q", q, dtype, q_token, q_head)) return rc;
     if (int rc = q4_tensor("out", out, dtype, 0, 0)) return rc;

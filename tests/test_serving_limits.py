@@ -39,3 +39,9 @@ def test_more_rows_than_a_launch_takes():
     assert L.jm_kv_q4_attn(_cache(N), P, None, N, P, 1024, 128, 8, 0.1, 0, P, None) == -2
     assert b"launch" in L.jm_last_error()
     assert L.jm_kv_q4_attn(_cache(1 << 20), P, P, (1 << 26) - 64, P, 1024, 128, 4, 0.1, 1, P, None) == -2
+
+
+def test_scales_that_overflow_with_the_exponentials_base():
+    L = _lib.lib()
+    for scale in (3e38, -3e38, float("inf"), float("nan")):
+        assert L.jm_kv_q4_attn(_cache(2), P, None, 2, P, 1024, 128, 8, scale, 0, P, None) == -1
