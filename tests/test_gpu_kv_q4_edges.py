@@ -162,3 +162,92 @@ def test_non_finite_rows_beside_large_ones_in_bf16_prompts():
     got = c.attention(0, torch.from_numpy(q).cuda().bfloat16(), ints([s]), ints([0, n]))
     assert torch.equal(got[:40], want[:40]) and bool(got[40:, :, 64:].isfinite().all())
     assert bool(got[40:, :, :64].isnan().all())
+
+
+@pytest.mark.parametrize("counts,start", [([1, 1], [37, 90]), ([4, 2], [37, 90]), ([70, 66], [37, 90]), ([200], [37])])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("maxT", [237, 3000])
+def test_infinite_and_other_scales_behind_a_tokens_own_row(counts, start, dt, maxT):
+    """What rows that were never written hold, as fp16: infinities, the largest
+    values, the smallest; over caches just filled and with room."""
+    res = []
+    for bits in (0x7C00, 0x7BFF, 0x0001, 0xFC00, 0x0000):
+        c = cache(len(counts), maxT, 2, 8)
+        c.data.view(torch.int16).fill_(bits - 0x10000 if bits & 0x8000 else bits)
+        q = []
+        for b, (s, n) in enumerate(zip(start, counts)):
+            k, v = rows(b + 90, s + n + 1, 2)
+            write(c, b, k[:s + n], v[:s + n])
+            q.append(queries(b + 95, k, s, n, 8))
+        res.append(check(c, np.concatenate(q), start, counts, dt))
+    for r in res[1:]:
+        assert torch.equal(r, res[0])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 5, 130])
+def test_rows_moved_into_a_wider_cache(n, dt):
+    """Read from a cache of 300 rows and written into one of 5000: the same values,
+    in planes laid out otherwise, and attention over them."""
+    k, v = rows(3, 300, 2)
+    a, b = cache(2, 300, 2, 8), cache(2, 5000, 2, 8)
+    write(a, 0, k, v)
+    write(a, 1, k[:200] * 3, v[:200])
+    cu = ints([0, 300, 500])
+    zero = ints([0, 0])
+    ka, va = a.read(0, zero, cu, 500)
+    b.write(0, ka, va, zero, cu)
+    for x, y in zip(b.read(0, zero, cu, 500), (ka, va)):
+        assert torch.equal(x, y)
+    q = np.concatenate([queries(4, k, 299 - n, n, 8), queries(5, k, 199 - n, n, 8)])
+    check(b, q, [300 - n, 200 - n], [n, n], dt)
+
+
+@pytest.mark.parametrize("counts,start", [([1] * 5, [900, 3, 250, 64, 511]), ([5], [900]), ([200], [300])])
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_the_same_call_gives_the_same_bits(counts, start, apart, dt):
+    c = cache(len(counts), 1100, 2, 8)
+    for b, (s, n) in enumerate(zip(start, counts)):
+        k, v = rows(b + 7, s + n, 2)
+        if apart:
+            v[::50] *= 1e4
+        write(c, b, k, v)
+    q = torch.from_numpy(np.random.default_rng(2).standard_normal((sum(counts), 8, HD)).astype(np.float32)).cuda().to(dt)
+    cu = ints(np.concatenate([[0], np.cumsum(counts)]).tolist())
+    want = c.attention(0, q, ints(start), cu)
+    for _ in range(5):
+        assert torch.equal(c.attention(0, q, ints(start), cu), want)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("maxT", [400, 5000])
+def test_prompts_in_place_and_captured(maxT, dt, apart):
+    """The output over q, and two graphs replayed in turn between eager calls."""
+    H, KH, n, s = 8, 2, 150, 240
+    c = cache(1, maxT, KH, H)
+    k, v = rows(7, s + n, KH)
+    if apart:
+        v[::50] *= 1e4
+    write(c, 0, k, v)
+    start, cu = ints([s]), ints([0, n])
+    new = lambda seed: torch.from_numpy(np.random.default_rng(seed).standard_normal((n, H, HD)).astype(np.float32)).cuda().to(dt)  # noqa: E731
+    q = new(1)
+    want = c.attention(0, q, start, cu)
+    same = q.clone()
+    assert torch.equal(c.attention(0, same, start, cu, out=same), want) and torch.equal(same, want)
+    out = torch.empty_like(q)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.attention(0, q, start, cu, out=out)
+        graphs.append(g)
+    for i in range(6):
+        q.copy_(new(10 + i))
+        out.zero_()
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(c.attention(0, q, start, cu), got)
