@@ -476,8 +476,8 @@ int jm_gemm_plan(int rows0, int rows1, int rows2, int K, int B, int* slices);
  * is held in the expert store's Q4 format (q4_store.py:40-67): groups of 64 or
  * 32 values, each with the scale fp16(fp32(absmax / 7)), the codes
  * clip(round_half_even(x / scale), -8, 7) + 8: 68 or 72 bytes instead of
- * bf16's 256.  A group that holds a NaN or an infinity, or a magnitude above
- * 7 * 65504, reads back as NaN.
+ * bf16's 256.  A group that holds a NaN or an infinity, or a magnitude of
+ * 7 * 65520 or more (whose scale is infinite in fp16), reads back as NaN.
  *
  * A plane (the k or the v rows of one sequence and layer) is
  * jm_kv_q4_bytes(maxT, n_kv, group) bytes: rows are kept head by head, the codes
@@ -499,8 +499,8 @@ typedef struct jm_kv_q4 {
     int group;
 } jm_kv_q4;
 
-/* Bytes of one plane; a negative code for maxT or n_kv <= 0 or a group other
- * than 64 and 32. */
+/* Bytes of one plane; a negative code for maxT or n_kv <= 0, a maxT above
+ * 2^31 - 1024, or a group other than 64 and 32. */
 int64_t jm_kv_q4_bytes(int maxT, int n_kv, int group);
 
 /* The N tokens of a call: sequence s has the tokens cu[s] .. cu[s + 1] - 1 at
@@ -513,7 +513,9 @@ int64_t jm_kv_q4_bytes(int maxT, int n_kv, int group);
  * Tensors are [N][heads][128] in dtype JM_DTYPE_F32 or JM_DTYPE_BF16; the
  * strides (in elements, multiples of 4) are those of tokens and heads, the last
  * dimension is contiguous; pointers are aligned to 4 elements.  Outputs are
- * contiguous.  The calls run on the current device. */
+ * contiguous.  The calls run on the current device.  N * n_kv is at most some 2^28
+ * (a launch's threads); attention takes some 2^24 KV heads of single tokens, more
+ * where units hold several. */
 
 /* k and v of the tokens into their cache rows. */
 int jm_kv_q4_write(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* k, int64_t k_token,

@@ -105,7 +105,7 @@ class Q4KVCacheSet:
         start[s] + 1, ... (int32 CUDA tensors, cu ascending); without cu every
         sequence has one token.  Tokens from cu[B] on, and rows outside
         [0, maxT), are skipped.  A group with a NaN, an infinity or a magnitude
-        above 458528 reads back as NaN."""
+        of 458640 or more reads back as NaN."""
         n = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else -1
         self._heads(k, "k", n, self.shape.n_kv)
         self._heads(v, "v", n, self.shape.n_kv, k.dtype)

@@ -251,3 +251,40 @@ def test_prompts_in_place_and_captured(maxT, dt, apart):
         torch.cuda.synchronize()
         got = out.clone()
         assert torch.equal(c.attention(0, q, start, cu), got)
+
+
+@pytest.mark.parametrize("group", [64, 32])
+def test_the_largest_magnitude_that_a_group_holds(group):
+    """Scales round to 65504 below 65520, to infinity from there: 7 times that
+    is the first magnitude that reads back as NaN."""
+    x = torch.zeros(6, 1, HD, device="cuda")
+    x[:, 0, 1] = torch.tensor([458528.0, 458600.0, 458639.96875, 458640.0, 458700.0, -458640.0], device="cuda")
+    x[:, 0, 2] = -65504.0
+    c = cache(1, 6, 1, 1, group)
+    c.write(0, x, -x, ints([0]), ints([0, 6]))
+    for got, sign in zip(c.read(0, ints([0]), ints([0, 6]), 6), (1.0, -1.0)):
+        assert bool((got[:3, 0, 1] == sign * 458528.0).all()) and bool((got[:3, 0, 2] == -sign * 65504.0).all())
+        assert bool(got[3:, 0, :group].isnan().all()) and bool((got[3:, 0, group:] == 0.0).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[2, 3], [90, 60]])
+def test_tokens_before_the_first_sequence_are_skipped(counts, dt):
+    """cu may begin behind 0, as the ends of a packed batch's padding do."""
+    lead, N = 5, 5 + sum(counts)
+    start, cu = [20, 3], [lead, lead + counts[0], N]
+    k, v = rows(33, N, 2)
+    c = cache(2, 200, 2, 8)
+    for b in range(2):
+        write(c, b, *rows(b + 60, start[b], 2))
+    c.write(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), ints(start), ints(cu))
+    out = torch.full((N, 2, HD), 7.0, device="cuda")
+    c.read(0, ints(start), ints(cu), N, k=out, v=out.clone())
+    assert bool((out[:lead] == 7.0).all()) and not bool((out[lead:] == 7.0).all(dim=2).any())
+    q = np.random.default_rng(1).standard_normal((N, 8, HD)).astype(np.float32)
+    d = {"f32": torch.float32, "bf16": torch.bfloat16}[dt]
+    got = torch.full((N, 8, HD), 7.0, dtype=d, device="cuda")
+    c.attention(0, torch.from_numpy(q).cuda().to(d), ints(start), ints(cu), out=got)
+    assert bool((got[:lead] == 7.0).all())
+    want = check(c, q[lead:], start, counts, dt)
+    assert torch.equal(got[lead:], want)
