@@ -62,7 +62,7 @@ __device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
 // tokens of 8 heads read back as bf16 in 40 us, 5.7 TB/s of codes and values.  What
 // is read back is stored past the caches, which it would only go through: with
 // ordinary stores, into outputs that were not there before, 65 us.  3 prompts of up
-// to 1531 bf16 tokens written in 6.6 us; 8 tokens of 4 heads in 3.5 (the launch).
+// to 1531 bf16 tokens written in 6.7 us; 8 tokens of 4 heads in 3.4 (the launch).
 template <int NG, bool BF>
 __global__ void __launch_bounds__(256)
 k_q4_write(Q4KvArgs c, const void* __restrict__ k, const void* __restrict__ v, long long kts, long long khs,
@@ -130,13 +130,12 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
 // q and the weights carry 21 bits so; for bf16 queries (BF) q is exact without
 // the second half, and the weights are rounded to fp16 once (2^-11 of each).
 //
-// Measured: 1 token behind 777 rows of 4 KV heads 10.0 us, in one range; with
-// k_q4_merge, 8 tokens behind 2048 rows each 7.8 + 3.1 (a tile a wave takes 6.4 us:
-// the launch, the unit's place, q and the tile, the waves joined; each further
-// tile 0.6); 6 drafts of 5 tokens
-// behind 3001 rows of 16 heads (26 MB) 15.6 + 3.2, on 576 blocks of 4 tiles a wave,
-// the same with a tenth of the vector instructions less; 32 bf16 tokens behind 16003
-// rows each of 8 heads (441 MB, groups of 32) 94 + 4.4 us, 4.7 TB/s: memory.
+// Measured, kernels alone, caches as long as their rows: 1 token behind 777 rows of 4
+// KV heads 9.8 us, in one range; with k_q4_merge, 8 tokens behind 2048 rows each 7.7 +
+// 2.9 (a tile a wave takes 6.4 us: the launch, the unit's place, q and the tile, the
+// waves joined; each further tile 0.6); 6 drafts of 5 tokens behind 3001 rows of 16
+// heads (26 MB) 15.4 + 3.1, on 576 blocks of 4 tiles a wave; 32 bf16 tokens behind
+// 16003 rows each of 8 heads (441 MB, groups of 32) 93.4 + 4.8 us, 4.7 TB/s: memory.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -291,7 +290,7 @@ struct Q4TileAt {
     __device__ __forceinline__ void load(Q4Tile<NG>& x) const {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            // (past the caches: 32 sequences of 16384 rows 105 -> 101 us, and no slower
+            // (past the caches: 32 sequences of 16384 rows 4% faster, and no slower
             // where units share rows)
             x.k[t] = __builtin_nontemporal_load(k + 64 * t);
             x.v[t] = __builtin_nontemporal_load(v + 64 * t);
@@ -665,11 +664,12 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
 // are such rows these take 90 and 1070 us.
 //
 // Measured at 2047 tokens behind 4099 rows, 32 query heads on 8 (172 GFLOP, 147 us
-// at the rate of a large library product): 227 us a call, 250 - 264 under a
-// profiler.  Vector work bounds it:
-// a wave has some 300 vector instructions beside the step's 32 products, and the two
-// waves of a SIMD, half a step apart, hide most but not all of it (270 us with
-// both in step).
+// at the rate of a large library product): 222 us a call in a run of them, 245 alone
+// under a profiler, whose clock is lower.  Vector work bounds it: 49.2 million vector
+// instructions beside 5.3 million products, 296 a wave and step beside 32, and the
+// two waves of a SIMD, half a step apart, hide most but not all of it (225 us with
+// both in step; for the 509 float32 tokens, of which a block has 4 steps at most,
+// 20.7 in step and 21.0 apart).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -1420,11 +1420,16 @@ Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared) {
             p.rg = 2;
             blocks = cut(unit / 2 / qpk);
         }
-        // (a block fills a CU; 256 tokens behind 30000 rows, bf16: 682 us uncut with 2)
+        // (a block fills a CU; 256 tokens behind 30000 rows, bf16: 682 us uncut with 2.
+        // By the rows that a cache has room for, here too: 509 float32 tokens in a cache
+        // of 509 rows 21 us, of 4096 or 32768 28)
         p.S = (int)std::max(std::min(256 / blocks, ((long long)c.maxT + 255) / 256), 1ll);
     } else {
         blocks = cut(c.cu ? 8 / qpk : 1);
-        // Ranges, for caches of more than 1024 rows: a block a CU while each has 128
+        // Ranges, for caches of more than 1024 rows (those it has room for: how many are
+        // in use is in device memory.  1 token behind 777 rows 9.6 us in a cache of
+        // 1024, 11.7 in one of 4096, 14.7 of 32768, 34 of 131072; 8 behind 2048 rows 11.4
+        // in caches of 2049 and 4096, 15.8 of 32768): a block a CU while each has 128
         // rows (a tile a wave), up to 4 a CU while each has 512.  Up to there one
         // range is faster than a second launch and its workspace: 1 or 8 tokens behind
         // 777 float32 rows (4 KV heads) 10.0 us against 12.6, 23 in a captured graph,

@@ -24,10 +24,9 @@
 // Bound: the logits are read three times, the first time from memory, 20 float64
 // operations and a 64-bit LDS addition a token in the histogram; a row takes three
 // launches and two hand-overs between its chunks however short it is.  Measured
-// (151936 float32 logits a row; kernels alone): one row 3.2 + 10.0 + 10.5 us, 7
-// rows of 50304 3.4 + 13.3 + 8.0, 128 rows with settings of their own 13.3 + 43 + 35
-// (read once at the rate of a copy: 16); at 128 rows, both hand-overs taken off,
-// the histogram is three and the list two times as long as the reading.
+// (151936 float32 logits a row; kernels alone): one row 3.4 + 9.7 + 9.6 us, 7 rows of
+// 50304 3.4 + 12.8 + 8.8, 128 rows with settings of their own 13.7 + 42.6 + 34.1 (read
+// once at the rate of a copy: 16).
 #include <algorithm>
 
 #include "jm_device.h"
