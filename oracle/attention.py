@@ -1,7 +1,7 @@
 """softmax(scale q . K) V in float64 over the values that a 4-bit cache holds,
 and how far an output may be from it.
 
-TEST INFRASTRUCTURE ONLY: imported by tests/, as the checker.  The product path
+TEST INFRASTRUCTURE ONLY: the oracle of the tests.  The product path
 (joule_amd) never imports it.
 
 The bound is a sum over the rows that a token sees, each row weighted as the
