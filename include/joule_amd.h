@@ -541,6 +541,74 @@ int jm_kv_q4_read(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
 int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
                   int64_t q_head, int n_heads, float scale, int dtype, void* out, void* stream);
 
+/* ---- paged KV caches ----
+ *
+ * No counterpart in the reference, whose KVCache is one array of maxT rows a sequence
+ * (decode_kernel.c:328-331).  Here the rows of all sequences in a layer share a pool of
+ * pages, and a table in DEVICE memory says which pages a sequence has: its row r is row
+ * r % page of page table[s][r / page].  A page holds [n_kv][page][128] values of k and as
+ * many of v, bf16 or float32.  Sequences may have pages in common (a shared prefix).
+ *
+ * A table entry outside [0, n_pages) is no page: rows there are not written, and
+ * attention does not see them, whether the page is still to come or was given back
+ * (the first pages of a long conversation, say). */
+typedef struct jm_kv_paged {
+    void* k;                        /* page p's k rows at k + p * page_stride, v's at v + p * page_stride */
+    void* v;                        /* (16-byte aligned, page_stride a multiple of 16 bytes) */
+    uint64_t page_stride;
+    const int32_t* table;           /* device [n_seq][table_stride]; ceil(maxT / page) entries a sequence are read */
+    int64_t table_stride;
+    int n_pages;
+    int page;                       /* rows a page: a power of two from 16 to 1024 */
+    int n_seq;
+    int maxT;                       /* rows a sequence may have */
+    int n_kv;
+    int dtype;                      /* JM_DTYPE_BF16 or JM_DTYPE_F32 */
+} jm_kv_paged;
+
+/* The new tokens' heads, [N][heads][128] each in dtype JM_DTYPE_F32 or JM_DTYPE_BF16 (of
+ * the caches' own or not); strides and alignment as for jm_kv_q4_write. */
+typedef struct jm_kv_rows {
+    const void* q;                  /* NULL: k and v only */
+    const void* k;
+    const void* v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int n_heads;                    /* of q */
+    int dtype;
+    void* q_out;                    /* [N][n_heads][128], contiguous; may be q where q is */
+    const float* cos;               /* [maxT][128], 16-byte aligned, or both NULL: no rotation */
+    const float* sin;
+    const uint16_t* q_norm;         /* bf16 [128], 16-byte aligned, or NULL: no norm */
+    const uint16_t* k_norm;
+    float eps;
+} jm_kv_rows;
+
+/* The tokens' rows into their sequences' pages.  The tokens and their rows are said as
+ * for jm_kv_q4_write (start, cu, N; tokens from cu[n_seq] on and rows outside [0, maxT)
+ * are skipped, in q_out too).
+ *   q_norm, k_norm  each q and k head becomes x / sqrt(mean(x^2) + eps) times the weight
+ *   cos, sin        then each q and k head is rotated by halves to its row r: dimension
+ *                   d < 64 becomes x[d] cos[r][d] - x[d + 64] sin[r][d], d + 64 becomes
+ *                   x[d + 64] cos[r][d + 64] + x[d] sin[r][d + 64]
+ * in float32, rounded once (to nearest even) to the caches' type, and to q's in q_out.  Of
+ * two tokens of a call with one row in one page either may stay. */
+int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const jm_kv_rows* rows,
+                       void* stream);
+
+/* out [N][n_heads][128] = softmax(scale q . K) V over the rows 0 .. the token's own that
+ * the table has pages for, which are in the cache already; n_heads / n_kv is a whole
+ * number from 1 to 16.  A token that sees no row (its own below 0, or none with a page)
+ * gets 0; other skipped tokens keep what out held.  A NaN or an infinity counts only in
+ * rows that a token sees, and in q: it makes of the output what the formula makes of it.
+ *   max_rows  at least as many rows as the longest sequence has after this call, where
+ *             the caller knows (0: maxT): the call is cut by it.  A smaller number is
+ *             slower, not wrong.
+ * float32 q: scores, weights and sums hold float32's 24 bits.  bf16 q: q and the weights
+ * are exact to 2^-16 of the weight; sums are float32.  out may be q where q is
+ * contiguous.  The magnitudes of V stay below 2^100.  Workspace: as jm_q4_gemm_f32's. */
+int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
+                     int64_t q_head, int n_heads, float scale, int max_rows, int dtype, void* out, void* stream);
+
 /* ---- sampling ----
  *
  * Beside jm_decode_layers_batch_argmax; no counterpart in the native reference.

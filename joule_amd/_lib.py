@@ -68,6 +68,8 @@ SIGNATURES = {
     "jm_kv_q4_write": ([_vp] * 3 + [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _vp], _i),
     "jm_kv_q4_read": ([_vp] * 3 + [_i, _vp, _vp, _i, _vp], _i),
     "jm_kv_q4_attn": ([_vp] * 3 + [_i, _vp, _i64, _i64, _i, _c.c_float, _i, _vp, _vp], _i),
+    "jm_kv_paged_append": ([_vp] * 3 + [_i, _vp, _vp], _i),
+    "jm_kv_paged_attn": ([_vp] * 3 + [_i, _vp, _i64, _i64, _i, _c.c_float, _i, _i, _vp, _vp], _i),
     "jm_sample": ([_vp, _i, _i64, _i, _i] + [_vp] * 5, _i),
 }
 
@@ -91,6 +93,19 @@ class ExpertJob(ctypes.Structure):
 class KvQ4(ctypes.Structure):
     """jm_kv_q4: the 4-bit caches of n_seq sequences in one layer."""
     _fields_ = [("k", _vp), ("v", _vp), ("seq_stride", _u64), ("n_seq", _i), ("maxT", _i), ("n_kv", _i), ("group", _i)]
+
+
+class KvPaged(ctypes.Structure):
+    """jm_kv_paged: the pages of n_seq sequences in one layer."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _u64), ("table", _vp), ("table_stride", _i64), ("n_pages", _i),
+                ("page", _i), ("n_seq", _i), ("maxT", _i), ("n_kv", _i), ("dtype", _i)]
+
+
+class KvRows(ctypes.Structure):
+    """jm_kv_rows: the new tokens' heads, and what is done to them on the way into the pages."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_token", _i64), ("q_head", _i64), ("k_token", _i64), ("k_head", _i64),
+                ("v_token", _i64), ("v_head", _i64), ("n_heads", _i), ("dtype", _i), ("q_out", _vp), ("cos", _vp), ("sin", _vp),
+                ("q_norm", _vp), ("k_norm", _vp), ("eps", _c.c_float)]
 
 
 class Sampling(ctypes.Structure):

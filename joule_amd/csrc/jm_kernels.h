@@ -373,6 +373,46 @@ Q4AttnPlan q4_attn_plan(const Q4KvArgs& c, int H, bool bf, bool shared);
 hipError_t launch_q4_attn(const Q4KvArgs& c, const Q4AttnPlan& p, const void* q, bool bf, long long qts, long long qhs,
                           int H, float scale, void* out, float* part_o, float* part_ml, hipStream_t st);
 
+// ---- paged KV caches (jm_paged.hip)
+
+struct PagedArgs {
+    const void* k;            // page p's rows [KH][1 << lp][128] at k + p * page_stride bytes
+    const void* v;
+    unsigned long long page_stride;
+    const int* table;         // [n_seq][table_stride] page numbers; outside [0, n_pages): no page
+    long long table_stride;
+    int n_pages, lp, f32;     // lp: log2 of a page's rows; f32: float32 rows (else bf16)
+    int n_seq, maxT, KH;
+    const int* start;         // as in Q4KvArgs
+    const int* cu;
+    int N;
+    const int* pos;           // NULL (the decoder's form)
+};
+// q, k and v of the tokens as the projections give them, and what is done to them on
+// the way.
+struct PagedRows {
+    const void* x[3];         // q (or NULL), k, v [N][heads][128], bf16 or float32
+    long long ts[3], hs[3];   // strides of tokens and heads
+    int H;                    // q heads (0: no q)
+    int bf;
+    void* q_out;              // [N][H][128]
+    const float* cos;         // [maxT][128], or NULL: no rotation
+    const float* sin;
+    const uint16_t* w[2];     // bf16 [128] RMSNorm weights of q and k heads, or NULL
+    float eps;
+};
+hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream_t st);
+// How an attention call is cut: tokens a unit, units, ranges of rows, and the floats of
+// the partial outputs (0: none).  rows: how many rows the longest sequence may have.
+struct PagedPlan {
+    int tp, units, S;
+    size_t o_floats, ml_floats;
+};
+PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows);
+// out [N][H][128] = attention of q [N][H][128] over rows 0 .. the token's own
+hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void* q, bool bf, long long qts, long long qhs,
+                             int H, float scale, void* out, float* part_o, float* part_ml, hipStream_t st);
+
 // ---- sampling (jm_sample.hip)
 #define JM_SAMPLE_MAX_V (1 << 20)
 struct SampleArgs {

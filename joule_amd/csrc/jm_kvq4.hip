@@ -6,56 +6,6 @@
 
 namespace jm {
 
-// 4 consecutive values of a float32 or bf16 tensor.
-template <bool BF>
-__device__ __forceinline__ void load4(const void* p, size_t i, float (&v)[4]) {
-    if (BF) {
-        const uint2 u = *(const uint2*)((const uint16_t*)p + i);
-        v[0] = bf16_bits_to_f32(u.x & 0xFFFFu);
-        v[1] = __uint_as_float(u.x & 0xFFFF0000u);
-        v[2] = bf16_bits_to_f32(u.y & 0xFFFFu);
-        v[3] = __uint_as_float(u.y & 0xFFFF0000u);
-    } else {
-        const float4 u = *(const float4*)((const float*)p + i);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-    }
-}
-
-// 8 of them (aligned to 4).
-typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
-template <bool BF>
-__device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
-    if (BF) {
-        const u32x4_a8 u = *(const u32x4_a8*)((const uint16_t*)p + i);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[2 * e] = __uint_as_float(u[e] << 16);
-            v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const float4 u = *(const float4*)((const float*)p + i + e);
-            v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
-        }
-    }
-}
-
-template <bool BF>
-__device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
-    if (BF) {
-        u32x4_a8 u;
-#pragma unroll
-        for (int e = 0; e < 4; e++) u[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-        __builtin_nontemporal_store(u, (u32x4_a8*)((uint16_t*)p + i));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 4)
-            __builtin_nontemporal_store(u32x4_t{__float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]),
-                                                __float_as_uint(v[e + 3])}, (u32x4_t*)((float*)p + i + e));
-    }
-}
-
 // Rows in and out: one wave per (KV head, 4 consecutive tokens), 16 lanes a row,
 // 8 dimensions a lane, so that a row moves in 16-byte pieces (the v codes change
 // hands between 8 lanes in registers).  Bound by memory where there is much: 112016
@@ -70,7 +20,7 @@ k_q4_write(Q4KvArgs c, const void* __restrict__ k, const void* __restrict__ v, l
     const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t0 = 4 * (item / c.KH), kh = item % c.KH, t = t0 + ((threadIdx.x & 63) >> 4);
     int seq, r;
-    if (t0 >= c.N || !q4_places(c, t0, seq, r)) return;
+    if (t0 >= c.N || !call_places(c, t0, seq, r)) return;
     float x[8], y[8];
     load8<BF>(k, (size_t)(t * kts + kh * khs) + 8 * q4_chunk(), x);
     load8<BF>(v, (size_t)(t * vts + kh * vhs) + 8 * q4_chunk(), y);
@@ -85,7 +35,7 @@ k_q4_read(Q4KvArgs c, void* __restrict__ k, void* __restrict__ v) {
     const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t0 = 4 * (item / c.KH), kh = item % c.KH, t = t0 + ((threadIdx.x & 63) >> 4);
     int seq, r;
-    if (t0 >= c.N || !q4_places(c, t0, seq, r)) return;
+    if (t0 >= c.N || !call_places(c, t0, seq, r)) return;
     float x[8], y[8];
     q4_load_chunk<NG>(x, true, r, Q4Head<NG>(q4_plane(c, seq, 0), kh, c.KH, c.R));
     q4_load_chunk<NG>(y, false, r, Q4Head<NG>(q4_plane(c, seq, 1), kh, c.KH, c.R));
@@ -180,46 +130,6 @@ __device__ __forceinline__ float q4_weight_exp(float y, const uint32_t* w) {
     return q4_weight_exp(y, m);
 }
 
-// The KV head's query rows of one unit: which sequence, its first token, how
-// many tokens, the first token's cache row.
-struct Q4Unit {
-    int seq, tok, n, pos;
-};
-
-// Unit u of the call for tp tokens a unit (without cu and in the decoder's form:
-// token u alone); false if there is none.  The same in every lane.
-__device__ __forceinline__ bool q4_unit(const Q4KvArgs& c, int u, int tp, Q4Unit& q) {
-    if (!c.cu) {
-        q.seq = q.tok = u;
-        q.n = 1;
-        q.pos = c.pos ? c.pos[u] : c.start[u];
-        return true;
-    }
-    const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        const int t0 = c.cu[min(s, c.n_seq)], t1 = c.cu[min(s + 1, c.n_seq)];
-        const int n = s < c.n_seq ? max(t1 - t0, 0) : 0;
-        const unsigned units = (unsigned)((n + tp - 1) / tp), upto = wave_inclusive_scan(units);
-        const unsigned long long below = __ballot(base + (int)upto <= u);
-        const int all = base + (int)__builtin_amdgcn_readlane((int)upto, 63);
-        if (u < all) {
-            const int l = __popcll(below);                  // the first sequence whose units pass u
-            const int k = u - base - (int)__builtin_amdgcn_readlane((int)(upto - units), l);
-            q.seq = s0 + l;
-            q.tok = __builtin_amdgcn_readlane(t0, l) + k * tp;
-            q.n = min(tp, __builtin_amdgcn_readlane(n, l) - k * tp);
-            q.n = min(q.n, c.N - q.tok);
-            const long long p = (long long)c.start[q.seq] + k * tp;
-            q.pos = (int)(p < -c.N ? -c.N : p > c.maxT ? c.maxT : p);
-            return q.n > 0 && q.tok >= 0;
-        }
-        base = all;
-    }
-    return false;
-}
-
 struct Q4AttnArgs {
     const void* q;              // strides qts, qhs
     long long qts, qhs;
@@ -248,12 +158,6 @@ __device__ __forceinline__ void split_f16x2(const Q4Mix& mix, float a, float b, 
     const float rb = mix.sub(b, (_Float16)h[1]);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
-}
-
-template <bool BF>
-__device__ __forceinline__ void store_out(void* p, size_t i, float4 v) {
-    if (BF) *(uint2*)((uint16_t*)p + i) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-    else *(float4*)((float*)p + i) = v;
 }
 
 // Whether a running maximum and sum are those of no row at all (a NaN among the
@@ -317,7 +221,7 @@ __device__ __forceinline__ float q4_scale(const u32x4_t (&s)[NG], int t, int i, 
 // all W waves joined, and the output, or (several ranges) the partial outputs of
 // unit u and range s from their row row0 on.  ow and mls: LDS for the W waves.
 template <int NG, bool BF, int W>
-__device__ __forceinline__ void q4_attn_unit(const Q4KvArgs& c, const Q4AttnArgs& a, const Q4Unit& un, int kh, int t0,
+__device__ __forceinline__ void q4_attn_unit(const Q4KvArgs& c, const Q4AttnArgs& a, const CallUnit& un, int kh, int t0,
                                              int t_end, int u, int s, int row0, float (*ow)[8][128], float (*mls)[8][2]) {
     constexpr int HD = 128, GS = 4 / NG;                    // contraction steps a group
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -563,8 +467,8 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     __shared__ __align__(16) float ow[4][8][128];
     __shared__ float mls[4][8][2];
     const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH % a.units, s = blockIdx.x / c.KH / a.units;
-    Q4Unit un;
-    if (!q4_unit(c, u, a.tp, un)) return;                   // (block-uniform)
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;                   // (block-uniform)
     const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
     const int NT = (last + 32) / 32;                        // (0 where last < 0)
     q4_attn_unit<NG, BF, 4>(c, a, un, kh, (int)((long long)NT * s / a.S), (int)((long long)NT * (s + 1) / a.S), u, s, 0, ow, mls);
@@ -577,11 +481,11 @@ k_q4_merge(Q4KvArgs c, Q4AttnArgs a) {
     constexpr int HD = 128;
     const int nc = a.qpk * a.tp, nb = (nc + 7) / 8;
     const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH / nb;
-    Q4Unit un;
+    CallUnit un;
     if (c.pos) {
         un.tok = u * a.tp;
         un.n = min(a.tp, c.N - un.tok);
-    } else if (!q4_unit(c, u, a.tp, un)) {
+    } else if (!call_unit(c, u, a.tp, un)) {
         return;
     }
     const int oc = 8 * (blockIdx.x / c.KH % nb) + (threadIdx.x >> 5), od = 4 * (threadIdx.x & 31);
@@ -766,14 +670,14 @@ __device__ __forceinline__ void q4_tile_again(const Q4KvArgs& c, const Q4AttnArg
     uint32_t bx = blockIdx.x;
     __asm__ volatile("" : "+s"(bx));
     const int kh = bx % c.KH, rs = bx / c.KH, u = a.units - 1 - rs % a.units, sr = rs / a.units;
-    Q4Unit un;
-    if (!q4_unit(c, u, a.tp, un)) return;
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;
     const int steps = (min(un.pos + un.n - 1, c.maxT - 1) + STEP) / STEP;
     const int t0 = (int)((long long)steps * sr / a.S) * (STEP / 32), t1 = (int)((long long)steps * (sr + 1) / a.S) * (STEP / 32);
     const int tp = 8 >> a.lq;
 #pragma unroll 1
     for (int t = 0; t < un.n; t += tp) {
-        const Q4Unit x = {un.seq, un.tok + t, min(tp, un.n - t), un.pos + t};
+        const CallUnit x = {un.seq, un.tok + t, min(tp, un.n - t), un.pos + t};
         const int NT = (min(x.pos + x.n - 1, c.maxT - 1) + 32) / 32;
         q4_attn_unit<NG, true, 8>(c, a, x, kh, t0, min(t1, NT), u, sr, t << a.lq, ow, mls);
         __syncthreads();
@@ -799,13 +703,13 @@ k_q4_tile(Q4KvArgs c, Q4AttnArgs a) {
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH;
     const int u = a.units - 1 - rs % a.units, sr = rs / a.units;        // the longest prefixes first
-    Q4Unit un;
+    CallUnit un;
     if (c.pos) {                                // the decoder's form: one prompt's tokens
         un.seq = 0;
         un.tok = u * a.tp;
         un.n = min(a.tp, c.N - un.tok);
         un.pos = 0;
-    } else if (!q4_unit(c, u, a.tp, un)) {
+    } else if (!call_unit(c, u, a.tp, un)) {
         return;
     }
     // this lane's query rows, and the last cache row that each sees

@@ -1,0 +1,602 @@
+// Paged KV caches: new rows finished (norm, rotation) and written to their
+// sequences' pages, and attention over the pages.
+//
+// The rows of a (page, KV head) are contiguous, [page][128]; pages hold at least 16
+// rows, so 16 aligned rows always lie in one page.
+#include <algorithm>
+#include <climits>
+
+#include "jm_kernels.h"
+#include "jm_tokens.h"
+
+namespace jm {
+
+// ---------------------------------------------------------------- new rows
+
+// 16 lanes a head, 8 dimensions a lane (dimension d and its partner d + 64 lie 8 lanes
+// apart), 16 heads of one token a block: q heads, then k heads, then v heads.
+template <bool BF>
+__global__ void __launch_bounds__(256)
+k_paged_append(PagedArgs c, PagedRows r, int chunks) {
+    constexpr int HD = 128;
+    const int t = blockIdx.x / chunks, hr = blockIdx.x % chunks * 16 + (threadIdx.x >> 4);
+    const int j = threadIdx.x & 15;
+    int seq, pos;
+    if (!call_place(c, t, seq, pos)) return;                // (block-uniform)
+    if (hr >= r.H + 2 * c.KH) return;                       // (whole rows of 16 lanes)
+    const int what = hr < r.H ? 0 : hr < r.H + c.KH ? 1 : 2;
+    const int head = what == 0 ? hr : what == 1 ? hr - r.H : hr - r.H - c.KH;
+    float x[8];
+    load8<BF>(r.x[what], (size_t)(t * r.ts[what] + head * r.hs[what]) + 8 * j, x);
+    const uint16_t* w = what < 2 ? r.w[what] : nullptr;
+    if (w) {
+        const uint4 u = *(const uint4*)(w + 8 * j);
+        const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
+        ss = seg_sum<16>(ss);
+        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(ss * (1.0f / HD), r.eps)));
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[2 * e] = x[2 * e] * inv * __uint_as_float(ww[e] << 16);
+            x[2 * e + 1] = x[2 * e + 1] * inv * __uint_as_float(ww[e] & 0xFFFF0000u);
+        }
+    }
+    if (r.cos && what < 2) {
+        const size_t at = (size_t)pos * HD + 8 * j;
+        float cs[8], sn[8];
+        load8<false>(r.cos, at, cs);
+        load8<false>(r.sin, at, sn);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = dpp_f<DPP_ROR8>(x[e]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(j < 8 ? -y[e] : y[e], sn[e], x[e] * cs[e]);
+    }
+    if (what == 0) {
+        store8<BF>(r.q_out, ((size_t)t * r.H + head) * HD + 8 * j, x);
+        return;
+    }
+    const int page = c.table[seq * c.table_stride + (pos >> c.lp)];
+    if ((unsigned)page >= (unsigned)c.n_pages) return;
+    char* const base = (char*)(what == 1 ? c.k : c.v) + (size_t)page * c.page_stride;
+    const size_t at = (((size_t)head << c.lp) + (pos & ((1 << c.lp) - 1))) * HD + 8 * j;
+    if (c.f32) store8<false>(base, at, x);
+    else store8<true>(base, at, x);
+}
+
+hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream_t st) {
+    if (c.N == 0) return hipSuccess;
+    const int chunks = (r.H + 2 * c.KH + 15) / 16;
+    const dim3 grid((unsigned)((long long)c.N * chunks));
+    if (r.bf) hipLaunchKernelGGL(k_paged_append<true>, grid, dim3(256), 0, st, c, r, chunks);
+    else hipLaunchKernelGGL(k_paged_append<false>, grid, dim3(256), 0, st, c, r, chunks);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------- few query tokens
+//
+// Block (KV head, unit of up to 16 query rows: tokens x heads of the KV head, range of
+// the unit's rows), W waves that take the range's tiles in turn, with a softmax each,
+// joined at the end; the ranges of a unit are joined by a second launch
+// (k_paged_merge).  A tile (8 KB of K and of V: 32 bf16 rows, 16 float32 ones) goes
+// straight to the lanes' registers in the order in which the matrix cores take it, the
+// next tile's while one is multiplied; nothing passes through LDS.
+//
+//   scores  16 rows as A (lane l: row 4 (l % 4) + l % 16 / 4 of them and the dimensions
+//           of its group l / 16), the query rows as B: lane (g, n) holds query row n
+//           at rows 4 i + g, i = 0 .. 3.  bf16: v_mfma_f32_16x16x32, group g of step s
+//           dimensions 32 s + 8 g ..; float32: v_mfma_f32_16x16x4, group g of step
+//           (s, e) dimension 16 s + 4 g + e.
+//   P . V   V^T as A, the weights as B from the lanes that formed them: of its
+//           contraction, group g has the rows 4 i + g.  Product j has the dimensions 8 m
+//           + j in its rows m, so that lane (g, m) wants 8 consecutive dimensions of each
+//           of its rows, 16 or 32 bytes as they lie in memory: in float32 these are the
+//           operands of the 8 products; in bf16 pairs of rows change places, one
+//           v_perm_b32 a register.
+//
+// bf16 pages: float32 q and weights are three bf16 parts (24 bits, one product each),
+// bf16 q is exact in one, its weights two parts; all their products with K and V are
+// exact, sums float32.  float32 pages: float32 products.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float pow2f(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ bf16x8 as_bf16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(bf16x8, make_uint4(a, b, c, d));
+}
+
+// a and b as NP bf16 parts, each the rest of those before it.  (An infinity's rest is
+// NaN: so is every output that it enters.)
+template <int NP>
+__device__ __forceinline__ void parts_bf16(float a, float b, uint32_t (&p)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        p[i] = pack_bf16x2(a, b);
+        a = __fsub_rn(a, __uint_as_float(p[i] << 16));
+        b = __fsub_rn(b, __uint_as_float(p[i] & 0xFFFF0000u));
+    }
+}
+
+struct PagedAttnArgs {
+    const void* q;              // strides qts, qhs
+    long long qts, qhs;
+    int H, qpk, tp;             // tp tokens a unit
+    float scale2;               // score scale times log2(e)
+    void* out;                  // [N][H][128]
+    int units, S;
+    float* part_o;              // [units][KH][S][qpk tp][128]: not divided by the sum
+    float* part_ml;             // [units][KH][S][qpk tp][2]: reference, sum (-1: no row seen)
+};
+
+// The pages of a sequence in one KV head.
+struct PagedSeq {
+    const int* table;
+    const char* k;              // this head's rows of page 0
+    const char* v;
+    __device__ __forceinline__ PagedSeq(const PagedArgs& c, int seq, int kh) {
+        const size_t head = ((size_t)kh << c.lp) * (c.f32 ? 512 : 256);
+        table = c.table + seq * c.table_stride;
+        k = (const char*)c.k + head;
+        v = (const char*)c.v + head;
+    }
+};
+
+// Where a tile's 16-row groups lie (wave-uniform): bytes from page 0's rows, and the last
+// row of the group that may be read.  A group without a page, or past the last row that
+// anyone sees, reads the tile's other group in its place; a tile without either is not
+// read (live false).
+template <int NG>
+struct PagedTile {
+    size_t at[NG];
+    int lim[NG];
+    bool ok[NG];
+    bool live;
+};
+
+// The pages of the wave's tiles: lane i holds those of its group i of the next 64.
+template <bool F32>
+struct PagedWalk {
+    static constexpr int NG = F32 ? 1 : 2, TR = 16 * NG, ROWB = F32 ? 512 : 256, AHEAD = 64 / NG;
+    const PagedArgs& c;
+    const int* table;
+    int last, t0, W;            // the last row anyone sees, the wave's first tile, tiles between
+    int page, next;             // the batch at hand and the one behind it
+    __device__ __forceinline__ int fetch(int batch) const {
+        const int lane = threadIdx.x & 63;
+        const long long row = ((long long)t0 + (long long)(batch * AHEAD + lane / NG) * W) * TR + 16 * (lane % NG);
+        const int p = row <= last ? table[row >> c.lp] : -1;
+        return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+    }
+    __device__ __forceinline__ PagedWalk(const PagedArgs& c_, const int* tb, int last_, int t, int w)
+        : c(c_), table(tb), last(last_), t0(t), W(w) {
+        page = fetch(0);
+        next = fetch(1);
+    }
+    // the wave's i-th tile (each i once, in order)
+    __device__ __forceinline__ void tile(int i, PagedTile<NG>& x) {
+        if (i && i % AHEAD == 0) {
+            page = next;
+            next = fetch(i / AHEAD + 1);
+        }
+        const int row0 = (t0 + i * W) * TR;
+        x.live = false;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const int p = __builtin_amdgcn_readlane(page, i % AHEAD * NG + g);
+            const int row = row0 + 16 * g;
+            x.ok[g] = p >= 0;
+            x.lim[g] = min(last - row, 15);
+            x.at[g] = (size_t)(p >= 0 ? p : 0) * c.page_stride + (size_t)(row & ((1 << c.lp) - 1)) * ROWB;
+            x.live |= x.ok[g];
+        }
+        if (NG == 2) {
+            if (!x.ok[0]) { x.at[0] = x.at[NG - 1]; x.lim[0] = x.lim[NG - 1]; }
+            else if (!x.ok[NG - 1]) { x.at[NG - 1] = x.at[0]; x.lim[NG - 1] = x.lim[0]; }
+        }
+    }
+};
+
+// A tile as a lane gets it.
+struct PagedRegs {
+    u32x4_t k[8], v[8];
+};
+
+template <bool F32>
+__device__ __forceinline__ void paged_load(const PagedSeq& s, const PagedTile<F32 ? 1 : 2>& x, PagedRegs& r) {
+    constexpr int ROWB = F32 ? 512 : 256;
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    if (!x.live) return;
+    if (F32) {
+        const gptr<const char> k = (gptr<const char>)(s.k + x.at[0]), v = (gptr<const char>)(s.v + x.at[0]);
+        const uint32_t kr = (uint32_t)min(4 * (n & 3) + (n >> 2), x.lim[0]) * ROWB + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.k[i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(k + kr + 64 * i));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t vr = (uint32_t)min(4 * i + g, x.lim[0]) * ROWB + 32 * n;
+            r.v[2 * i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + vr));
+            r.v[2 * i + 1] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + vr + 16));
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const gptr<const char> k = (gptr<const char>)(s.k + x.at[F32 ? 0 : h]), v = (gptr<const char>)(s.v + x.at[F32 ? 0 : h]);
+            const int lim = x.lim[F32 ? 0 : h];
+            const uint32_t kr = (uint32_t)min(4 * (n & 3) + (n >> 2), lim) * ROWB + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.k[4 * h + i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(k + kr + 64 * i));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                r.v[4 * h + i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + ((uint32_t)min(4 * i + g, lim) * ROWB + 16 * n)));
+        }
+    }
+}
+
+// O[j] += V^T's product j times the weights p of the lane's rows.
+template <bool F32, int NP>
+__device__ __forceinline__ void paged_pv(const u32x4_t (&v)[8], const float (&p)[8], f32x4 (&O)[8]) {
+    if (F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                O[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[2 * i + j / 4][j % 4]), p[i], O[j], 0, 0, 0);
+    } else {
+        uint32_t w[NP][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t x[NP];
+            parts_bf16<NP>(p[2 * i], p[2 * i + 1], x);
+#pragma unroll
+            for (int k = 0; k < NP; k++) w[k][i] = x[k];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint32_t a[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                a[i] = __builtin_amdgcn_perm(v[2 * i + 1][j / 2], v[2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+            const bf16x8 x = as_bf16x8(a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int k = NP - 1; k >= 0; k--)
+                O[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(w[k][0], w[k][1], w[k][2], w[k][3]), O[j], 0, 0, 0);
+        }
+    }
+}
+
+constexpr int PAGED_OW = 132;               // floats between the columns of a wave's outputs in LDS
+
+// The query rows of one unit over tiles t0 .. t_end - 1 of its sequence; the waves joined,
+// and the output, or (several ranges) the partial outputs.
+template <bool F32, bool BF, int W>
+__global__ void __launch_bounds__(64 * W, W >= 8 ? 1 : 2)
+k_paged_attn(PagedArgs c, PagedAttnArgs a) {
+    constexpr int HD = 128, NG = F32 ? 1 : 2, TR = 16 * NG, NY = 4 * NG;
+    constexpr int NQ = BF ? 1 : 3, NP = BF ? 2 : 3;         // parts of q, of the weights
+    __shared__ __align__(16) float ow[W][16][PAGED_OW];
+    __shared__ float mls[W][16][2];
+    const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH % a.units, s = blockIdx.x / c.KH / a.units;
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;                 // (block-uniform)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
+    const int NT = last < 0 ? 0 : last / TR + 1;
+    const int t0 = (int)((long long)NT * s / a.S), t_end = (int)((long long)NT * (s + 1) / a.S);
+    const int ncol = a.qpk * un.n;
+    const int ct = min(n / a.qpk, un.n - 1), head = kh * a.qpk + n % a.qpk;
+    const int crow = min(un.pos + ct, c.maxT - 1);          // the last row that this column sees
+
+    const PagedSeq seq(c, un.seq, kh);
+    const int mine = t_end - t0 > w ? (t_end - t0 - w + W - 1) / W : 0;     // this wave's tiles
+    PagedWalk<F32> walk(c, seq.table, mine ? last : -1, t0 + w, W);
+    PagedTile<NG> x, xn;
+    PagedRegs cur, nxt;
+    x.live = false;
+    if (mine) {
+        walk.tile(0, x);
+        paged_load<F32>(seq, x, cur);
+    }
+
+    // the query columns
+    const size_t qi = (size_t)((un.tok + ct) * a.qts + head * a.qhs);
+    float qf[F32 ? 32 : 1];
+    bf16x8 qb[F32 ? 1 : NQ][4];
+    if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float y[4];
+            load4<BF>(a.q, qi + 16 * i + 4 * g, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) qf[4 * i + e] = y[e];
+        }
+    } else {
+#pragma unroll
+        for (int st = 0; st < 4; st++) {
+            float y[8];
+            load8<BF>(a.q, qi + 32 * st + 8 * g, y);
+            uint32_t b[NQ][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t p[NQ];
+                parts_bf16<NQ>(y[2 * e], y[2 * e + 1], p);
+#pragma unroll
+                for (int k = 0; k < NQ; k++) b[k][e] = p[k];
+            }
+#pragma unroll
+            for (int k = 0; k < NQ; k++) qb[k][st] = as_bf16x8(b[k][0], b[k][1], b[k][2], b[k][3]);
+        }
+    }
+
+    f32x4 O[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) O[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = -INFINITY, l = 0.0f;
+    bool seen = false;
+
+    for (int i = 0; i < mine; i++) {
+        if (i + 1 < mine) {
+            walk.tile(i + 1, xn);
+            paged_load<F32>(seq, xn, nxt);
+        }
+        if (x.live) {
+            const int row0 = (t0 + w + i * W) * TR;
+            // ---- scores
+            float y[8];
+#pragma unroll
+            for (int h = 0; h < NG; h++) {
+                f32x4 S = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (F32) {
+                    f32x4 S2 = S;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        S = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[k / 4][k % 4]), qf[k], S, 0, 0, 0);
+                        S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[k / 4][k % 4 + 1]), qf[k + 1], S2, 0, 0, 0);
+                    }
+                    S += S2;
+                } else {
+#pragma unroll
+                    for (int k = NQ - 1; k >= 0; k--)
+#pragma unroll
+                        for (int st = 0; st < 4; st++)
+                            S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, cur.k[4 * h + st]), qb[k][st], S, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[4 * h + e] = __fmul_rn(S[e], a.scale2);
+            }
+            // rows that the column does not see: past its own, or without a page
+            bool whole = row0 + TR - 1 <= un.pos;
+#pragma unroll
+            for (int h = 0; h < NG; h++) {
+                whole &= x.ok[h];
+                seen |= x.ok[h] && row0 + 16 * h <= crow;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < NY; e++)
+                    if (!x.ok[e / 4] || row0 + 16 * (e / 4) + 4 * (e % 4) + g > crow) y[e] = -INFINITY;
+            }
+            // ---- the reference: raised to the largest score when one passes it by 2^10
+            float ym = y[0];
+#pragma unroll
+            for (int e = 1; e < NY; e++) ym = fmaxf(ym, y[e]);
+            if (__any(ym > ref + 10.0f)) {
+                ym = fmaxf(ym, swz_xor16_f(ym));
+                ym = fmaxf(ym, __shfl_xor(ym, 32, JM_WAVE));
+                const float nref = fmaxf(ref, ym);
+                const float f = nref == -INFINITY ? 1.0f : pow2f(ref - nref);
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) O[j] *= f;
+                ref = nref;
+            }
+            const float r0 = ref == -INFINITY ? 0.0f : ref;     // (a column that has seen nothing yet)
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < NY; e++) {
+                p[e] = pow2f(__fsub_rn(y[e], r0));
+                l = __fadd_rn(l, p[e]);
+            }
+            // ---- P . V.  A weight of 0 does not hide a value that is not finite: where
+            // some column does not see such a row, token by token, each with the rows that
+            // it sees.
+            bool apart = false;
+            auto row_of = [&](int e) __attribute__((always_inline)) {       // of v[e]; a group without a page holds another's
+                const int h = F32 ? 0 : e / 4;
+                return x.ok[h] ? row0 + 16 * h + 4 * (F32 ? e / 2 : e % 4) + g : INT_MAX;
+            };
+            if (!whole && un.n > 1) {
+                uint32_t bad = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    uint32_t b = 0;
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        b |= (cur.v[e][d] & 0x7F800000u) == 0x7F800000u;
+                        if (!F32) b |= (cur.v[e][d] & 0x7F80u) == 0x7F80u;
+                    }
+                    bad |= row_of(e) > un.pos ? b : 0u;
+                }
+                apart = __any(bad != 0);
+            }
+            if (!apart) {
+                paged_pv<F32, NP>(cur.v, p, O);
+            } else {
+#pragma unroll 1
+                for (int t = 0; t < un.n; t++) {
+                    u32x4_t v[8];
+                    float pt[8];
+                    f32x4 T[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        v[e] = row_of(e) <= un.pos + t ? cur.v[e] : u32x4_t{0u, 0u, 0u, 0u};
+                        T[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (e < NY) pt[e] = ct == t ? p[e] : 0.0f;
+                    }
+                    paged_pv<F32, NP>(v, pt, T);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (ct == t) O[j] += T[j];
+                }
+            }
+        }
+        x = xn;
+        cur = nxt;
+    }
+
+    // ---- the wave's outputs: dimensions 32 g + 8 i + j of column n
+    l += swz_xor16_f(l);
+    l += __shfl_xor(l, 32, JM_WAVE);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        *(float4*)&ow[w][n][32 * g + 8 * i] = make_float4(O[0][i], O[1][i], O[2][i], O[3][i]);
+        *(float4*)&ow[w][n][32 * g + 8 * i + 4] = make_float4(O[4][i], O[5][i], O[6][i], O[7][i]);
+    }
+    if (g == 0) {
+        mls[w][n][0] = ref;
+        mls[w][n][1] = seen ? l : -1.0f;
+    }
+    __syncthreads();
+
+    // ---- the block's: thread = column, dimensions 4 (tid % 32) ..
+    for (int oc = threadIdx.x >> 5; oc < ncol; oc += 2 * W) {
+        const int od = 4 * (threadIdx.x & 31);
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < W; i++) M = fmaxf(M, mls[i][oc][0]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float L = 0.0f;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            if (mls[i][oc][1] == -1.0f) continue;
+            any = true;
+            const float f = pow2f(mls[i][oc][0] - M);
+            const float4 y = *(const float4*)&ow[i][oc][od];
+            v.x = __builtin_fmaf(y.x, f, v.x);
+            v.y = __builtin_fmaf(y.y, f, v.y);
+            v.z = __builtin_fmaf(y.z, f, v.z);
+            v.w = __builtin_fmaf(y.w, f, v.w);
+            L = __builtin_fmaf(mls[i][oc][1], f, L);
+        }
+        const int to = oc / a.qpk;
+        if (un.pos + to >= c.maxT) continue;
+        if (a.S == 1) {
+            // a token that sees no row: 0.  (A sum of 0 elsewhere is that of scores that are
+            // all -infinity: NaN.)
+            const float inv = any ? __fdiv_rn(1.0f, L) : 0.0f;
+            const size_t oi = ((size_t)(un.tok + to) * a.H + kh * a.qpk + oc % a.qpk) * HD + od;
+            store_out<BF>(a.out, oi, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        } else {
+            const size_t pi = (((size_t)u * c.KH + kh) * a.S + s) * (a.qpk * a.tp) + oc;
+            if (any) *(float4*)(a.part_o + pi * HD + od) = v;
+            if ((threadIdx.x & 31) == 0) *(float2*)(a.part_ml + 2 * pi) = make_float2(M, any ? L : -1.0f);
+        }
+    }
+}
+
+// The ranges of one (unit, KV head, query row) joined into the output: 8 groups of 32
+// lanes take the ranges in turn, 4 dimensions a lane, and are added in order.
+template <bool BF>
+__global__ void __launch_bounds__(256)
+k_paged_merge(PagedArgs c, PagedAttnArgs a) {
+    constexpr int HD = 128;
+    __shared__ __align__(16) float4 acc[8][32];
+    __shared__ float ls[8];
+    const int nc = a.qpk * a.tp;
+    const int kh = blockIdx.x % c.KH, oc = blockIdx.x / c.KH % nc, u = blockIdx.x / c.KH / nc;
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;
+    const int to = oc / a.qpk;
+    if (to >= un.n || un.pos + to >= c.maxT) return;        // (block-uniform)
+    const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
+    const int j = threadIdx.x & 31, gr = threadIdx.x >> 5;
+    float M = -INFINITY;
+    bool any = false;
+    for (int s = j; s < a.S; s += 32) {
+        const float2 x = *(const float2*)(a.part_ml + 2 * (p0 + (size_t)s * nc));
+        M = fmaxf(M, x.x);
+        any |= x.y != -1.0f;
+    }
+    M = seg_max<32>(M);
+    any = __any(any);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float L = 0.0f;
+    for (int s0 = gr; s0 < a.S; s0 += 32) {
+        float4 x[4];
+        float2 ml[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const size_t p = p0 + (size_t)min(s0 + 8 * q, a.S - 1) * nc;
+            ml[q] = *(const float2*)(a.part_ml + 2 * p);
+            x[q] = *(const float4*)(a.part_o + p * HD + 4 * j);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (s0 + 8 * q >= a.S || ml[q].y == -1.0f) continue;       // (a range without a row has no output)
+            const float f = pow2f(ml[q].x - M);
+            v.x = __builtin_fmaf(x[q].x, f, v.x);
+            v.y = __builtin_fmaf(x[q].y, f, v.y);
+            v.z = __builtin_fmaf(x[q].z, f, v.z);
+            v.w = __builtin_fmaf(x[q].w, f, v.w);
+            L = __builtin_fmaf(ml[q].y, f, L);
+        }
+    }
+    acc[gr][j] = v;
+    if (j == 0) ls[gr] = L;
+    __syncthreads();
+    if (gr) return;
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        const float4 y = acc[i][j];
+        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+        L += ls[i];
+    }
+    const float inv = any ? __fdiv_rn(1.0f, L) : 0.0f;                  // (as in k_paged_attn)
+    store_out<BF>(a.out, ((size_t)(un.tok + to) * a.H + kh * a.qpk + oc % a.qpk) * HD + 4 * j,
+                  make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+}
+
+PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
+    PagedPlan p{};
+    const int qpk = H / c.KH;
+    rows = std::min(rows, c.maxT);
+    p.tp = c.cu ? 16 / qpk : 1;
+    // (every sequence's tokens are rounded up to whole units)
+    p.units = c.cu ? (int)std::min<long long>(c.N, ((long long)c.N + (long long)c.n_seq * (p.tp - 1)) / p.tp) : c.N;
+    const long long blocks = (long long)p.units * c.KH;
+    // up to `want` blocks while each has `least` rows
+    auto ranges = [&](long long want, int least) {
+        return std::min((want + blocks - 1) / blocks, ((long long)rows + least - 1) / least);
+    };
+    p.S = rows <= 1024 ? 1 : (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+    const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
+    p.o_floats = p.S > 1 ? cols * 128 : 0;
+    p.ml_floats = p.S > 1 ? cols * 2 : 0;
+    return p;
+}
+
+hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void* q, bool bf, long long qts, long long qhs,
+                             int H, float scale, void* out, float* part_o, float* part_ml, hipStream_t st) {
+    if (c.N == 0) return hipSuccess;
+    PagedAttnArgs a{};
+    a.q = q; a.qts = qts; a.qhs = qhs; a.H = H; a.qpk = H / c.KH; a.tp = p.tp;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.out = out; a.units = p.units; a.S = p.S; a.part_o = part_o; a.part_ml = part_ml;
+    const dim3 grid((unsigned)c.KH * p.units * p.S);
+#define JM_PAGED(F32V, BFV) \
+    if ((c.f32 != 0) == F32V && bf == BFV) hipLaunchKernelGGL((k_paged_attn<F32V, BFV, 4>), grid, dim3(256), 0, st, c, a)
+    JM_PAGED(false, false); else JM_PAGED(false, true); else JM_PAGED(true, false); else JM_PAGED(true, true);
+#undef JM_PAGED
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.S == 1) return e;
+    const dim3 mg((unsigned)c.KH * p.units * (unsigned)(a.qpk * a.tp));
+    if (bf) hipLaunchKernelGGL(k_paged_merge<true>, mg, dim3(256), 0, st, c, a);
+    else hipLaunchKernelGGL(k_paged_merge<false>, mg, dim3(256), 0, st, c, a);
+    return hipGetLastError();
+}
+
+}  // namespace jm

@@ -22,6 +22,7 @@
 
 #include "jm_device.h"
 #include "jm_kernels.h"
+#include "jm_tokens.h"
 
 namespace jm {
 
@@ -40,35 +41,6 @@ struct Q4Head {
     }
     __device__ __forceinline__ gptr<uint16_t> scale(int r, int g) const { return scales + (size_t)r * NG + g; }
 };
-
-// The sequence and cache row of the four tokens t0 .. t0 + 3 of a call (not the
-// decoder's form) in the wave's four rows of 16 lanes: each lane gets its row's
-// token's; false for a token that has none (behind the last sequence, or a row
-// outside the cache).
-__device__ __forceinline__ bool q4_places(const Q4KvArgs& c, int t0, int& seq, int& pos) {
-    const int lane = threadIdx.x & 63, i = lane >> 4, t = t0 + i;
-    seq = t;
-    int first = t;
-    if (c.cu) {
-        int n = 0;
-        for (int s = 0; s <= c.n_seq; s += 64) {
-            const int x = c.cu[min(s + lane, c.n_seq)];
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int upto = __popcll(__ballot(s + lane <= c.n_seq && x <= t0 + q));
-                n += i == q ? upto : 0;
-            }
-        }
-        seq = n - 1;
-        if (t >= c.N || seq < 0 || seq >= c.n_seq) return false;
-        first = c.cu[seq];
-    } else if (t >= c.N || t >= c.n_seq) {
-        return false;
-    }
-    const long long p = (long long)c.start[seq] + (t - first);
-    pos = (int)(p < 0 ? -1 : p >= c.maxT ? c.maxT : p);
-    return p >= 0 && p < c.maxT;
-}
 
 __device__ __forceinline__ unsigned long long q4_plane(const Q4KvArgs& c, int seq, int which) {
     if (c.pos) return c.tab[((size_t)seq * c.L + c.layer) * 2 + which];

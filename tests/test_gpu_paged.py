@@ -1,0 +1,223 @@
+"""Paged KV caches: rows appended and attention over the pages, against float64
+(oracle/paged.py, which derives the bounds)."""
+
+import numpy as np
+import pytest
+import torch
+
+from joule_amd.decoder import DecoderShape, rope_tables
+from joule_amd.dense import dense_ffn_shape
+from joule_amd.kv_paged import PagedKVCacheSet
+from oracle.paged import attend, finish
+
+pytestmark = pytest.mark.gpu
+
+HD = 128
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}           # half a step of a value, relative
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cache(B, maxT, KH, page=16, dtype="bf16", layers=1, extra=3, seed=0):
+    """Caches of NaN, every sequence's pages anywhere in the pool."""
+    shape = DecoderShape(n_layers=layers, moe=dense_ffn_shape(1024, 512), n_heads=KH, n_kv=KH, maxT=maxT)
+    width = -(-maxT // page)
+    c = PagedKVCacheSet(shape, B, B * width + extra, page=page, dtype=DT[dtype])
+    c.data.fill_(float("nan"))
+    order = np.random.default_rng(seed).permutation(B * width + extra)[:B * width]
+    c.table.copy_(ints(order.reshape(B, width).tolist()))
+    return c
+
+
+def put(c, b, k, v, l=0, first=0):
+    """Rows first .. of sequence b, by plain indexing."""
+    r = np.arange(first, first + len(k))
+    table = c.table.cpu().numpy()
+    page = torch.from_numpy(table[b, r // c.page].astype(np.int64)).cuda()
+    at = torch.from_numpy(r % c.page).cuda()
+    for i, x in enumerate((k, v)):
+        c.data[l, page, i, :, at] = torch.as_tensor(x, device="cuda").to(c.data.dtype)
+
+
+def held(c, b, n, l=0):
+    """k and v [n, KH, 128] in float32 of rows 0 .. n - 1; NaN without a page."""
+    t = c.table[b, :-(-n // c.page)].long()
+    x = c.data[l, t.clamp(0, c.n_pages - 1)].float()
+    x[(t < 0) | (t >= c.n_pages)] = float("nan")
+    x = x.permute(1, 0, 3, 2, 4).reshape(2, -1, c.shape.n_kv, HD)[:, :n].cpu().numpy()
+    return x[0], x[1]
+
+
+def rows(seed, T, KH):
+    rng = np.random.default_rng(seed)
+    k, v = (rng.standard_normal((T, KH, HD)).astype(np.float32) for _ in range(2))
+    k[:, :, 3::17] *= 2.0
+    return k, v
+
+
+def queries(seed, k, start, n, H):
+    """n tokens from row `start` on, each looking at its own row and the one before."""
+    rng = np.random.default_rng(seed)
+    KH = k.shape[1]
+    q = rng.standard_normal((n, H, HD)).astype(np.float32)
+    for i in range(n):
+        at = max(start + i - 1, 0)
+        for h in range(H):
+            q[i, h] += 0.4 * np.nan_to_num(k[at:start + i + 1, h * KH // H]).sum(axis=0)
+    return q
+
+
+def form_of(dt, n, H, KH, n_seq):
+    return "f32" if dt == "f32" else "bf16"
+
+
+def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=None, one=False):
+    """attention() of tokens q [N, H, 128] (numpy) against float64; returns the output."""
+    H, KH = q.shape[1], c.shape.n_kv
+    qd = torch.from_numpy(q).cuda().to(DT[dt])
+    cu = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    print(f"[paged] H={H} KH={KH} {counts} at {start} of {c.shape.maxT} page {c.page} {dt}/{c.data.dtype} scale {scale} max_rows {max_rows}",
+          flush=True)
+    got = c.attention(0, qd, ints(start), None if one else ints(cu), scale=scale, out=out, max_rows=max_rows)
+    torch.cuda.synchronize()
+    g64, q64 = got.double().cpu().numpy(), qd.float().cpu().numpy()
+    table = c.table.cpu().numpy()
+    for b, (s, n) in enumerate(zip(start, counts)):
+        T = s + n
+        if n == 0 or T <= 0:
+            continue
+        k, v = held(c, b, T)
+        t = np.arange(T)
+        paged = (table[b, t // c.page] >= 0) & (table[b, t // c.page] < c.n_pages)
+        pick = np.array(only if only is not None else sorted({0, n - 1, *np.random.default_rng(n).integers(0, n, 30).tolist()}))
+        pick = pick[s + pick < c.shape.maxT]
+        see = paged & (t <= s + pick[:, None])
+        for h in range(H):
+            want, tol = attend(q64[cu[b] + pick, h], k[:, h * KH // H], v[:, h * KH // H], see, scale, form_of(dt, n, H, KH, len(counts)))
+            off = np.abs(g64[cu[b] + pick, h] - want)
+            worst = np.nanmax(off / np.maximum(tol, 1e-300))
+            assert (off <= tol).all(), f"sequence {b} head {h}: {worst:.3g} bounds off, by {np.nanmax(off):.3g}"
+    return got
+
+
+def run(H, KH, counts, start, dt, cached, page=16, maxT=None, **kw):
+    c = cache(len(counts), maxT or max(s + n for s, n in zip(start, counts)), KH, page, cached)
+    q = []
+    for b, (s, n) in enumerate(zip(start, counts)):
+        k, v = rows(7 * b + 1, max(s + n, 1), KH)
+        if s + n > 0:
+            put(c, b, k[:s + n], v[:s + n])
+        q.append(queries(b + 100, k, s, n, H))
+    return check(c, np.concatenate(q), start, counts, dt, **kw)
+
+
+# ------------------------------------------------------------------ append
+
+
+def append_case(H, KH, counts, start, dt, cached, page, norm, rope, maxT=None, l=0, layers=1, inplace=False, strided=False):
+    T = maxT or max(max(s + n for s, n in zip(start, counts)), 1)
+    c = cache(len(counts), T, KH, page, cached, layers=layers)
+    N = sum(counts)
+    rng = np.random.default_rng(N + H)
+    x = [torch.from_numpy(rng.standard_normal((N, h, HD)).astype(np.float32)).cuda().to(DT[dt]) for h in (H, KH, KH)]
+    if strided:
+        full = torch.zeros((N, H + 2 * KH + 1, HD + 4), dtype=DT[dt], device="cuda")
+        out, at = [], 0
+        for y in x:
+            z = full[:, at:at + y.shape[1], :HD]
+            z.copy_(y)
+            out.append(z)
+            at += y.shape[1]
+        x = out
+    q, k, v = x
+    w = [torch.from_numpy((1 + 0.3 * rng.standard_normal(HD)).astype(np.float32)).cuda().bfloat16() for _ in range(2)] if norm else [None, None]
+    tables = rope_tables(T, HD, 1e4) if rope else (None, None)
+    cos, sin = (None if t is None else torch.from_numpy(t).cuda() for t in tables)
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    before = c.data.clone()
+    want_in = [t.float().cpu().numpy() for t in (q, k, v)]
+    print(f"[append] H={H} KH={KH} {counts} at {start} page {page} {dt}/{cached} norm {norm} rope {rope}", flush=True)
+    got = c.append(l, k, v, ints(start), ints(cu.tolist()), q=q, cos=cos, sin=sin, q_norm=w[0], k_norm=w[1], eps=1e-5,
+                   q_out=q if inplace else None)
+    torch.cuda.synchronize()
+    row = np.concatenate([np.arange(s, s + n) for s, n in zip(start, counts)]).astype(np.int64)
+    seq = np.repeat(np.arange(len(counts)), counts)
+    live = (row >= 0) & (row < T)
+    r = np.clip(row, 0, T - 1)
+    wn = [None if y is None else y.float().cpu().numpy() for y in w]
+    wq, wk = (finish(want_in[i], r, wn[i], tables[0], tables[1], 1e-5) for i in range(2))
+    # 12 float32 roundings of values of at most |x| + |partner|, in the sum of squares half of
+    # 128 more; then the type's own
+    room = [(12 + 64 * norm) * 2.0 ** -24 * (np.abs(y) + np.abs(np.roll(y, HD // 2, axis=-1)) + 1e-30) for y in (wq, wk)]
+    g = got.double().cpu().numpy()
+    assert (np.abs(g - wq) <= room[0] + HALF[dt] * np.abs(wq))[live].all()
+    table = c.table.cpu().numpy()
+    page_of = table[np.where(live, seq, 0), np.where(live, row, 0) // page]
+    ok = live & (page_of >= 0) & (page_of < c.n_pages)
+    idx = (torch.from_numpy(page_of[ok].astype(np.int64)).cuda(), torch.from_numpy(row[ok] % page).cuda())
+    gk, gv = (c.data[l, idx[0], i, :, idx[1]].double().cpu().numpy() for i in range(2))
+    assert (np.abs(gk - wk[ok]) <= room[1][ok] + HALF[cached] * np.abs(wk[ok])).all()
+    assert np.array_equal(gv, torch.from_numpy(want_in[2][ok]).to(DT[cached]).double().numpy())
+    # nothing else was touched
+    for i in range(2):
+        before[l, idx[0], i, :, idx[1]] = c.data[l, idx[0], i, :, idx[1]]
+    assert torch.equal(before.view(torch.uint8), c.data.view(torch.uint8))
+    return c, got
+
+
+@pytest.mark.parametrize("dt,cached", [("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("norm,rope", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("H,KH,counts,start,page", [(1, 1, [1], [0], 16), (8, 2, [3, 0, 40], [14, 7, 0], 16), (28, 4, [17, 33], [31, 64], 32),
+                                                    (16, 16, [1, 1, 1], [5, 100, 31], 64), (5, 1, [130], [60], 128)])
+def test_append(H, KH, counts, start, page, norm, rope, dt, cached):
+    append_case(H, KH, counts, start, dt, cached, page, norm, rope)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_append_in_place_strided_and_in_a_later_layer(dt):
+    append_case(8, 2, [3, 5], [0, 20], dt, "bf16", 16, True, True, inplace=True)
+    append_case(8, 2, [3, 5], [0, 20], dt, "bf16", 16, True, True, strided=True)
+    append_case(7, 1, [9], [11], dt, "f32", 32, False, True, layers=3, l=2)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_append_skips_rows_outside(dt):
+    append_case(4, 2, [5, 6, 3], [-2, 28, 500], dt, "bf16", 16, True, True, maxT=30)
+
+
+# --------------------------------------------------------------- attention
+
+TYPES = [("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")]
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,page", [(1, 1, 16), (8, 2, 32), (28, 4, 16), (16, 1, 64), (12, 4, 128), (5, 5, 16)])
+@pytest.mark.parametrize("start", [[0], [15, 16, 17], [30, 700, 31, 63], [2500, 3]])
+def test_single_tokens(H, KH, page, start, dt, cached):
+    run(H, KH, [1] * len(start), start, dt, cached, page, one=True)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", [(8, 2, [5, 0, 3], [900, 4, 12]), (7, 1, [2, 9], [15, 1300]), (2, 2, [16, 17], [0, 40]),
+                                               (16, 1, [4], [2222])])
+def test_few_tokens(H, KH, counts, start, dt, cached):
+    run(H, KH, counts, start, dt, cached)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start,page", [(8, 1, [64], [1500], 16), (2, 2, [129], [2000], 64), (6, 2, [300], [97], 32),
+                                                    (8, 8, [130], [700], 16), (4, 2, [130, 0, 90], [900, 5, 1800], 128), (7, 1, [201], [0], 16)])
+def test_prompts(H, KH, counts, start, page, dt, cached):
+    run(H, KH, counts, start, dt, cached, page, maxT=4000)
+    run(H, KH, counts, start, dt, cached, page)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("counts,start", [([1], [777]), ([5], [777]), ([70], [700])])
+@pytest.mark.parametrize("max_rows", [1, 700, 1025, 5000, 100000, 2 ** 31 - 1])
+def test_max_rows_only_cuts(counts, start, max_rows, dt, cached):
+    """Any bound gives the same, too small or too large."""
+    run(4, 2, counts, start, dt, cached, maxT=120000, max_rows=max_rows)
