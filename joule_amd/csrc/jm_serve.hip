@@ -64,6 +64,20 @@ int rows_tensor(const char* name, const void* p, int dtype, int64_t ts, int64_t 
     return 0;
 }
 
+// launch_kernels(workspace of `bytes`, NULL for 0) on st, the workspace held until they
+// are enqueued.
+template <class F>
+int with_workspace(hipStream_t st, size_t bytes, const char* what, F launch_kernels) {
+    jm::PluginWs ws;
+    if (bytes)
+        if (int rc = jm::plugin_ws(st, bytes, &ws)) return rc;
+    const hipError_t e = launch_kernels((float*)ws.p);
+    const hipError_t f = ws.async ? hipFreeAsync(ws.p, st) : hipSuccess;
+    if (e != hipSuccess) return jm::hip_fail(e, what);
+    if (f != hipSuccess) return jm::hip_fail(f, "hipFreeAsync");
+    return 0;
+}
+
 // The paged cache and the call's tokens as the kernels take them (a->N stays 0 where
 // there is nothing to do).
 int paged_args(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, jm::PagedArgs* a) {
@@ -152,16 +166,9 @@ int jm_kv_q4_attn(const jm_kv_q4* c, const int32_t* start, const int32_t* cu, in
     // (ranges are for few units, so that the kernel that joins them has fewer threads)
     const long long threads = (long long)c->n_kv * p.units * p.S * (p.rg ? 512 : 256);
     if (threads > MAX_THREADS) return fail(JM_ERR_SHAPE, "attention of N=%d tokens and %d KV heads is more than one launch takes", N, c->n_kv);
-    jm::PluginWs ws;
-    if (p.o_floats)
-        if (int rc = jm::plugin_ws(st, (p.o_floats + p.ml_floats) * 4, &ws)) return rc;
-    float* part = (float*)ws.p;
-    const hipError_t e = jm::launch_q4_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part,
-                                            part + p.o_floats, st);
-    const hipError_t f = ws.async ? hipFreeAsync(ws.p, st) : hipSuccess;
-    if (e != hipSuccess) return jm::hip_fail(e, "4-bit attention launch");
-    if (f != hipSuccess) return jm::hip_fail(f, "hipFreeAsync");
-    return 0;
+    return with_workspace(st, (p.o_floats + p.ml_floats) * 4, "4-bit attention launch", [&](float* part) {
+        return jm::launch_q4_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part, part + p.o_floats, st);
+    });
 }
 
 int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const jm_kv_rows* r,
@@ -212,16 +219,9 @@ int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* 
     const jm::PagedPlan p = jm::paged_plan(a, n_heads, dtype == JM_DTYPE_BF16, max_rows ? max_rows : c->maxT);
     if ((long long)c->n_kv * p.units * p.S * 512 > MAX_THREADS || (long long)p.units * p.tp * n_heads * 256 > MAX_THREADS)
         return fail(JM_ERR_SHAPE, "attention of N=%d tokens and %d heads is more than one launch takes", N, n_heads);
-    jm::PluginWs ws;
-    if (p.o_floats)
-        if (int rc = jm::plugin_ws(st, (p.o_floats + p.ml_floats) * 4, &ws)) return rc;
-    float* part = (float*)ws.p;
-    const hipError_t e = jm::launch_paged_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part,
-                                               part + p.o_floats, st);
-    const hipError_t f = ws.async ? hipFreeAsync(ws.p, st) : hipSuccess;
-    if (e != hipSuccess) return jm::hip_fail(e, "paged attention launch");
-    if (f != hipSuccess) return jm::hip_fail(f, "hipFreeAsync");
-    return 0;
+    return with_workspace(st, (p.o_floats + p.ml_floats) * 4, "paged attention launch", [&](float* part) {
+        return jm::launch_paged_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part, part + p.o_floats, st);
+    });
 }
 
 int jm_sample(const void* logits, int dtype, int64_t ld, int B, int V, const jm_sampling* how, const float* u,
