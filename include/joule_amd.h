@@ -598,8 +598,10 @@ int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t
 /* out [N][n_heads][128] = softmax(scale q . K) V over the rows 0 .. the token's own that
  * the table has pages for, which are in the cache already; n_heads / n_kv is a whole
  * number from 1 to 16.  A token that sees no row (its own below 0, or none with a page)
- * gets 0; other skipped tokens keep what out held.  A NaN or an infinity counts only in
- * rows that a token sees, and in q: it makes of the output what the formula makes of it.
+ * gets 0; other skipped tokens keep what out held.  A NaN or an infinity in q, or in K in
+ * a row that a token sees, makes its output NaN, one in V that dimension NaN or infinite
+ * (products are taken in parts, of which some are 0); rows that it does not see may hold
+ * anything.
  *   max_rows  at least as many rows as the longest sequence has after this call, where
  *             the caller knows (0: maxT): the call is cut by it.  A smaller number is
  *             slower, not wrong.

@@ -402,10 +402,11 @@ struct PagedRows {
     float eps;
 };
 hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream_t st);
-// How an attention call is cut: tokens a unit, units, ranges of rows, and the floats of
-// the partial outputs (0: none).  rows: how many rows the longest sequence may have.
+// How an attention call is cut: tokens a unit, units, ranges of rows, row groups of the
+// kernel for prompts (0: the one for few tokens), and the floats of the partial outputs
+// (0: none).  rows: how many rows the longest sequence may have.
 struct PagedPlan {
-    int tp, units, S;
+    int tp, units, S, rg;
     size_t o_floats, ml_floats;
 };
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows);

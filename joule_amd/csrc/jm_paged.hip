@@ -560,19 +560,402 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
                   make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }
 
+// ------------------------------------------------------ many query tokens
+//
+// Prompts over bf16 pages: block (KV head, unit of 32 QB RG query rows, range of the
+// unit's rows), 8 waves = RG row groups x PS position strides; in a step wave (rg, ps)
+// takes the 32 cache rows ps of the step's 32 PS for its 32 QB query rows, with an online
+// softmax, and the PS waves of a row group are joined at the end.  A step's rows go
+// straight to LDS (global_load_lds), the steps after it on their way.
+//
+//   scores   v_mfma_f32_32x32x16_bf16, cache rows as A (lane l: row l % 32, dimensions 16
+//            kk + 8 (l / 32) ..), query rows as B: lane l holds query row l % 32 at cache
+//            rows 8 (v / 4) + 4 (l / 32) + v % 4
+//   P . V    V^T as A, read transposed from LDS (ds_read_b64_tr_b16: 4 rows of 16
+//            dimensions), the weights as B from the registers that formed them:
+//            contraction index j of half h in step s is row 16 s + 8 (j / 4) + 4 h + j % 4
+//
+// bf16 queries (BF): 64 query rows a wave (QB = 2), so that an operand read from LDS serves
+// two products; q is exact, a weight is rounded to bf16 once, and the sum is of the
+// rounded weights, so that the output stays a mean of values of V.  float32 queries: q and
+// the weights as three bf16 parts each, as in k_paged_attn.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// 4 rows x 16 columns of bf16 in LDS, transposed over 16 lanes: lane i gives the address
+// of 4 columns (4 (i % 4) ..) of row i / 4 and receives column i of rows 0 .. 3
+__device__ __forceinline__ s16x4 paged_tr16(const uint16_t* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(void*)p);
+}
+
+template <bool BF, int RG>
+__global__ void __launch_bounds__(512, 2)
+k_paged_tile(PagedArgs c, PagedAttnArgs a) {
+    constexpr int HD = 128, QB = BF ? 2 : 1, NQ = BF ? 1 : 3, PS = 8 / RG, STEP = 32 * PS, TILE = 32 * HD;
+    constexpr int NS = PS == 2 ? 3 : 2;         // steps in LDS
+    constexpr int GW = PS / 2;                  // 16-row groups that a wave stages a step
+    constexpr int LPS = 4 * GW;                 // its loads
+    constexpr int NROW = 32 * QB * RG;
+    // PS tiles of K, then of V, for each step in LDS (arrays of their own, so that the
+    // compiler sees that a step's reads do not wait for another's rows); at the end the
+    // outputs being joined
+    __shared__ __align__(16) uint16_t kv0[2 * PS * TILE], kv1[2 * PS * TILE], kv2[NS == 3 ? 2 * PS * TILE : 8];
+    // the second block of query rows of each row group (BF)
+    __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
+    __shared__ float mls[8][32 * QB][2];
+    __shared__ uint8_t okf[NS][2 * PS];         // whether a step's 16-row groups have pages
+    // which dimensions met a V value of +inf (bit 0), -inf (bit 1) or NaN (both) that not
+    // every query row sees, 16 dimensions a word
+    __shared__ uint32_t taint[NROW][HD / 16];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
+    const int kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH;
+    const int u = a.units - 1 - rs % a.units, sr = rs / a.units;        // the longest prefixes first
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;
+    const PagedSeq seq(c, un.seq, kh);
+    const int pmax = min(un.pos + un.n - 1, c.maxT - 1), pmin = min(un.pos, c.maxT - 1);
+    // this block's range of the steps (none where no token sees a row)
+    const int steps = pmax < 0 ? 0 : pmax / STEP + 1;
+    const int step0 = (int)((long long)steps * sr / a.S), nstep = (int)((long long)steps * (sr + 1) / a.S);
+
+    // this lane's query rows, and the last cache row that each sees
+    int tok[QB], prow[QB], head[QB];
+    bool live[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const int r = 32 * (QB * rg + b) + n, t = r / a.qpk;
+        live[b] = t < un.n && un.pos + t < c.maxT;
+        tok[b] = min(t, un.n - 1);
+        head[b] = kh * a.qpk + r % a.qpk;
+        prow[b] = min(un.pos + tok[b], c.maxT - 1);
+    }
+    // ... over the wave's rows
+    const int wmin = min(un.pos + min(32 * QB * rg / a.qpk, un.n - 1), c.maxT - 1);
+    const int wmax = min(un.pos + min((32 * QB * (rg + 1) - 1) / a.qpk, un.n - 1), c.maxT - 1);
+
+    // ---- staging: wave w has the 16-row groups GW (w % 4) .. of each step, of K (w < 4) or V
+    const bool isk = w < 4;
+    const char* const src = isk ? seq.k : seq.v;
+    auto fetch = [&](int batch) __attribute__((always_inline)) {        // lane: group lane % GW of the batch's step lane / GW
+        const long long row = (long long)(step0 + batch * (64 / GW) + lane / GW) * STEP + 16 * (GW * (w & 3) + lane % GW);
+        const int p = row <= pmax ? seq.table[row >> c.lp] : -1;
+        return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+    };
+    int page = fetch(0), next = fetch(1);
+    auto stage = [&](int i, uint16_t* kv, int slot) __attribute__((always_inline)) {
+        const int k = i - step0;
+        if (k && k % (64 / GW) == 0) {
+            page = next;
+            next = fetch(k / (64 / GW) + 1);
+        }
+#pragma unroll
+        for (int q = 0; q < GW; q++) {
+            const int gi = GW * (w & 3) + q, row = i * STEP + 16 * gi;
+            const int p = __builtin_amdgcn_readlane(page, k % (64 / GW) * GW + q);
+            uint16_t* const dst = kv + (isk ? 0 : PS * TILE) + gi * 16 * HD;
+            if (isk && lane == 0) okf[slot][gi] = p >= 0;
+            if (p >= 0) {
+                const int lim = min(pmax - row, 15);        // (rows past the prefixes repeat the last one; their weights are 0)
+                const gptr<const char> base = (gptr<const char>)(src + (size_t)p * c.page_stride) + (uint32_t)((row & ((1 << c.lp) - 1)) * 256);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int r = 4 * j + (lane >> 4);
+                    const int x = isk ? r : 4 * (lane >> 4);
+                    __builtin_amdgcn_global_load_lds((gptr<void>)(base + ((uint32_t)min(r, lim) * 256 + 16 * ((lane & 15) ^ x))),
+                                                     (__attribute__((address_space(3))) void*)(dst + 4 * j * HD), 16, 0, 0);
+                }
+            } else if (!isk) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) *(uint4*)(dst + 4 * j * HD + 8 * lane) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    if (step0 < nstep) stage(step0, kv0, 0);
+    if (step0 + 1 < nstep) stage(step0 + 1, kv1, 1);
+
+    // ---- the query rows, with the score scale's sign (a scale of 0, or a smaller one, as
+    // 2^-100: masked scores stay -inf behind it)
+    const float cs = fmaxf(fabsf(a.scale2), 0x1p-100f);
+    const uint32_t sign = a.scale2 < 0.0f ? 0x80008000u : 0u;
+    bf16x8 qr[NQ][8];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const size_t qi = (size_t)((un.tok + tok[b]) * a.qts + head[b] * a.qhs);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            float x[8];
+            load8<BF>(a.q, qi + 16 * k + 8 * h, x);
+            uint32_t y[NQ][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t p[NQ];
+                parts_bf16<NQ>(x[2 * e], x[2 * e + 1], p);
+#pragma unroll
+                for (int i = 0; i < NQ; i++) y[i][e] = p[i] ^ sign;
+            }
+            if (b == 0) {
+#pragma unroll
+                for (int i = 0; i < NQ; i++) qr[i][k] = as_bf16x8(y[i][0], y[i][1], y[i][2], y[i][3]);
+            } else if (ps == 0) {
+                q1[rg][k][lane] = make_uint4(y[0][0], y[0][1], y[0][2], y[0][3]);
+            }
+        }
+    }
+    for (int i = tid; i < NROW * (HD / 16); i += 512) (&taint[0][0])[i] = 0;
+
+    f32x16 O[QB][4];
+    float ref[QB], l[QB];
+    bool seen[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        ref[b] = -INFINITY;
+        l[b] = 0.0f;
+        seen[b] = false;
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) O[b][nt] = f32x16(0.0f);
+    }
+    const int kx = h ^ (n & 15);                // K row n: dimensions 16 kk + 8 h .. at chunk (2 kk) ^ kx
+    // this lane's part of a transposed read: row 4 h + i / 4, 4 columns 16 (l / 16 % 2) + 4 (i
+    // % 4) of a 32-column block, i = l % 16; chunk c of V row r sits at c ^ 4 (r % 4)
+    const int vrow = (lane & 15) >> 2;
+    const int vo = (4 * h + vrow) * HD + 8 * (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 4 * (lane & 1);
+
+    auto step = [&](int i, uint16_t* kv, int slot, uint16_t* kvn, int slotn) __attribute__((always_inline)) {
+        // this wave's rows of step i have arrived (those of step i + 1 may be on their
+        // way), then everyone's
+        if (i + 1 < nstep) __builtin_amdgcn_s_waitcnt(LPS == 4 ? 0x0074 : 0x0078);     // vmcnt(LPS), lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);                                        // vmcnt(0), lgkmcnt(0)
+        wave_meet();
+        if (NS == 3 && i + 2 < nstep) stage(i + 2, kvn, slotn);
+        const int t0 = i * STEP + 32 * ps;
+        uint16_t* const kw = kv + ps * TILE;
+        uint16_t* const vw = kv + (PS + ps) * TILE;
+        if (i * STEP + STEP - 1 > pmin) {
+            // A weight of 0 does not hide a value of V that is not finite.  In a step
+            // whose rows not everyone sees such values go into `taint`, for the rows that
+            // see them, and out of the step.  (Block-uniform.)
+            uint32_t nf = 0;
+#pragma unroll
+            for (int j = 0; j < 8 / RG; j++) {
+                const uint4 y = *(const uint4*)(vw + 8 * ((8 / RG) * 64 * rg + 64 * j + lane));
+                const uint32_t x[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    nf |= (uint32_t)((x[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((x[e] & 0x7F800000u) == 0x7F800000u);
+            }
+            if (__syncthreads_or(nf != 0)) {
+#pragma unroll 1
+                for (int e = lane; e < TILE; e += 64) {
+                    const int r = e / HD, dim = (e % HD) ^ (32 * (r & 3));
+                    const uint32_t x = vw[e];
+                    if ((x & 0x7F80u) != 0x7F80u) continue;
+                    const uint32_t bits = (x & 0x7Fu) ? 3u : (x >> 15) ? 2u : 1u;
+                    // (a row past the prefixes holds the last one again)
+                    if (t0 + r > pmax) continue;
+#pragma unroll 1
+                    for (int q = 0; q < 32 * QB; q++)
+                        if (t0 + r <= un.pos + min((32 * QB * rg + q) / a.qpk, un.n - 1))
+                            atomicOr(&taint[32 * QB * rg + q][dim / 16], bits << (2 * (dim % 16)));
+                }
+                __syncthreads();
+                if (rg == 0) {
+#pragma unroll 1
+                    for (int e = lane; e < TILE; e += 64)
+                        if ((vw[e] & 0x7F80u) == 0x7F80u) vw[e] = 0;
+                }
+                __syncthreads();
+            }
+        }
+        if (t0 <= wmax) {
+            const uint32_t ok = *(const uint16_t*)&okf[slot][2 * ps];
+            const bool ok0 = __builtin_amdgcn_readfirstlane(ok & 0xFFu), ok1 = __builtin_amdgcn_readfirstlane(ok >> 8);
+            f32x16 S[QB];
+#pragma unroll
+            for (int b = 0; b < QB; b++) S[b] = f32x16(0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const bf16x8 x = __builtin_bit_cast(bf16x8, *(const uint4*)(kw + n * HD + 8 * ((2 * k) ^ kx)));
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--) S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qr[p][k], S[0], 0, 0, 0);
+                if (QB == 2) S[QB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, *(const bf16x8*)&q1[rg][k][lane], S[QB - 1], 0, 0, 0);
+            }
+            bf16x8 P[QB][NQ][2];
+            const bool whole = t0 + 31 <= wmin && ok0 && ok1;
+#pragma unroll
+            for (int b = 0; b < QB; b++) {
+                seen[b] |= (ok0 && t0 <= prow[b]) || (ok1 && t0 + 16 <= prow[b]);
+                if (!whole) {
+                    const int lim = prow[b] - t0 - 4 * h;
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (8 * (v / 4) + v % 4 > lim || !(v < 8 ? ok0 : ok1)) S[b][v] = -INFINITY;
+                }
+                float m = S[b][0];
+#pragma unroll
+                for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
+                m *= cs;
+                if (__any(m > ref[b] + 10.0f)) {
+                    m = fmaxf(m, __shfl_xor(m, 32, JM_WAVE));
+                    const float nref = fmaxf(ref[b], m);
+                    const float f = nref == -INFINITY ? 1.0f : pow2f(ref[b] - nref);
+                    l[b] *= f;
+#pragma unroll
+                    for (int nt = 0; nt < 4; nt++) O[b][nt] *= f;
+                    ref[b] = nref;
+                }
+                const float r0 = ref[b] == -INFINITY ? 0.0f : ref[b];
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t y[NQ][4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cs, -r0));
+                        const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cs, -r0));
+                        uint32_t p[NQ];
+                        parts_bf16<NQ>(x0, x1, p);
+#pragma unroll
+                        for (int q = 0; q < NQ; q++) y[q][e] = p[q];
+                        if (BF) l[b] += __uint_as_float(p[0] << 16) + __uint_as_float(p[0] & 0xFFFF0000u);
+                        else l[b] += x0 + x1;
+                    }
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) P[b][q][s] = as_bf16x8(y[q][0], y[q][1], y[q][2], y[q][3]);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++) {
+                    const s16x4 v0 = paged_tr16(vw + vo + 16 * s * HD + 32 * (nt ^ vrow));
+                    const s16x4 v1 = paged_tr16(vw + vo + (16 * s + 8) * HD + 32 * (nt ^ vrow));
+                    const bf16x8 x = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int b = 0; b < QB; b++)
+#pragma unroll
+                        for (int q = NQ - 1; q >= 0; q--) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, P[b][q][s], O[b][nt], 0, 0, 0);
+                }
+        }
+        if (NS == 2) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): this wave's reads of the step, then
+            wave_meet();                            // everyone's, are done
+            if (i + 2 < nstep) stage(i + 2, kvn, slotn);
+        }
+    };
+#pragma unroll 1
+    for (int i = step0; i < nstep; i += NS) {
+        if (NS == 3) {
+            step(i, kv0, 0, kv2, 2);
+            if (i + 1 < nstep) step(i + 1, kv1, 1, kv0, 0);
+            if (i + 2 < nstep) step(i + 2, kv2, 2, kv1, 1);
+        } else {
+            step(i, kv0, 0, kv0, 0);
+            if (i + 1 < nstep) step(i + 1, kv1, 1, kv1, 1);
+        }
+    }
+
+    // ---- the PS waves of each row group joined, 32 dimensions at a time
+    float f[QB], inv[QB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        l[b] += __shfl_xor(l[b], 32, JM_WAVE);
+        if (h == 0) {
+            mls[w][32 * b + n][0] = ref[b];
+            mls[w][32 * b + n][1] = seen[b] ? l[b] : -1.0f;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        float M = -INFINITY, L = 0.0f;
+        bool any = false;
+#pragma unroll
+        for (int q = 0; q < PS; q++) M = fmaxf(M, mls[q * RG + rg][32 * b + n][0]);
+#pragma unroll
+        for (int q = 0; q < PS; q++) {
+            const float lq = mls[q * RG + rg][32 * b + n][1];
+            if (lq == -1.0f) continue;
+            any = true;
+            L = __builtin_fmaf(lq, pow2f(mls[q * RG + rg][32 * b + n][0] - M), L);
+        }
+        f[b] = seen[b] ? pow2f(ref[b] - M) : 0.0f;
+        inv[b] = any ? __fdiv_rn(1.0f, L) : 0.0f;                           // (as in k_paged_attn)
+        if (a.S > 1) {
+            inv[b] = 1.0f;
+            float* const ml = a.part_ml + 2 * (((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n);
+            if (ps == 0 && h == 0 && live[b]) *(float2*)ml = make_float2(M, any ? L : -1.0f);
+        }
+    }
+    float4* const mb = (float4*)&kv0[0];        // [wave][4][64 lanes]
+    static_assert(4 * 8 * 64 * 16 <= sizeof(kv0), "the outputs of 32 rows and dimensions of each wave fit");
+#pragma unroll
+    for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+        for (int b = 0; b < QB; b++) {
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                mb[(w * 4 + q) * 64 + lane] = make_float4(O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b], O[b][nt][4 * q + 2] * f[b],
+                                                          O[b][nt][4 * q + 3] * f[b]);
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (q % PS != ps || !live[b]) continue;
+                float4 s = mb[(rg * 4 + q) * 64 + lane];
+#pragma unroll
+                for (int p = 1; p < PS; p++) {
+                    const float4 x = mb[((p * RG + rg) * 4 + q) * 64 + lane];
+                    s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
+                }
+                const uint32_t tw = taint[32 * (QB * rg + b) + n][2 * nt + q / 2] >> (16 * (q % 2) + 8 * h);     // dimensions 8 q + 4 h ..
+                float o[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t x = (tw >> (2 * e)) & 3u;
+                    const float add = x == 0 ? 0.0f : x == 1 ? INFINITY : x == 2 ? -INFINITY : __int_as_float(0x7FC00000);
+                    o[e] = __fmul_rn(__fadd_rn(o[e], add), inv[b]);
+                }
+                const int d = 32 * nt + 8 * q + 4 * h;
+                if (a.S == 1) {
+                    store_out<BF>(a.out, ((size_t)(un.tok + tok[b]) * a.H + head[b]) * HD + d, make_float4(o[0], o[1], o[2], o[3]));
+                } else {
+                    const size_t row = ((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n;
+                    *(float4*)(a.part_o + row * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+                }
+            }
+        }
+}
+
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     PagedPlan p{};
     const int qpk = H / c.KH;
     rows = std::min(rows, c.maxT);
-    p.tp = c.cu ? 16 / qpk : 1;
-    // (every sequence's tokens are rounded up to whole units)
-    p.units = c.cu ? (int)std::min<long long>(c.N, ((long long)c.N + (long long)c.n_seq * (p.tp - 1)) / p.tp) : c.N;
-    const long long blocks = (long long)p.units * c.KH;
+    long long blocks;
+    auto cut = [&](int tp) {
+        p.tp = tp;
+        // (every sequence's tokens are rounded up to whole units)
+        p.units = c.cu ? (int)std::min<long long>(c.N, ((long long)c.N + (long long)c.n_seq * (tp - 1)) / tp) : c.N;
+        blocks = (long long)p.units * c.KH;
+    };
     // up to `want` blocks while each has `least` rows
     auto ranges = [&](long long want, int least) {
         return std::min((want + blocks - 1) / blocks, ((long long)rows + least - 1) / least);
     };
-    p.S = rows <= 1024 ? 1 : (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+    const long long qrows = (long long)c.N * qpk;
+    if (!c.f32 && c.cu && qrows >= 64ll * c.n_seq) {
+        const int unit = bf ? 256 : 128;
+        p.rg = 4;
+        cut(unit / qpk);
+        if (qrows < (long long)unit * c.n_seq || (blocks < 256 && blocks * rows < 160000)) {
+            p.rg = 2;
+            cut(unit / 2 / qpk);
+        }
+        p.S = (int)std::max(std::min(256 / blocks, ((long long)rows + 255) / 256), 1ll);
+    } else {
+        cut(c.cu ? 16 / qpk : 1);
+        p.S = rows <= 1024 ? 1 : (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+    }
     const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;
     p.ml_floats = p.S > 1 ? cols * 2 : 0;
@@ -587,10 +970,17 @@ hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void*
     a.scale2 = scale * 1.4426950408889634f;
     a.out = out; a.units = p.units; a.S = p.S; a.part_o = part_o; a.part_ml = part_ml;
     const dim3 grid((unsigned)c.KH * p.units * p.S);
+    if (p.rg) {
+#define JM_PAGED_TILE(BFV, RGV) \
+        if (bf == BFV && p.rg == RGV) hipLaunchKernelGGL((k_paged_tile<BFV, RGV>), grid, dim3(512), 0, st, c, a)
+        JM_PAGED_TILE(false, 2); else JM_PAGED_TILE(false, 4); else JM_PAGED_TILE(true, 2); else JM_PAGED_TILE(true, 4);
+#undef JM_PAGED_TILE
+    } else {
 #define JM_PAGED(F32V, BFV) \
-    if ((c.f32 != 0) == F32V && bf == BFV) hipLaunchKernelGGL((k_paged_attn<F32V, BFV, 4>), grid, dim3(256), 0, st, c, a)
-    JM_PAGED(false, false); else JM_PAGED(false, true); else JM_PAGED(true, false); else JM_PAGED(true, true);
+        if ((c.f32 != 0) == F32V && bf == BFV) hipLaunchKernelGGL((k_paged_attn<F32V, BFV, 4>), grid, dim3(256), 0, st, c, a)
+        JM_PAGED(false, false); else JM_PAGED(false, true); else JM_PAGED(true, false); else JM_PAGED(true, true);
 #undef JM_PAGED
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.S == 1) return e;
     const dim3 mg((unsigned)c.KH * p.units * (unsigned)(a.qpk * a.tp));

@@ -70,8 +70,10 @@ def queries(seed, k, start, n, H):
     return q
 
 
-def form_of(dt, n, H, KH, n_seq):
-    return "f32" if dt == "f32" else "bf16"
+def form_of(c, dt, n, H, KH, n_seq):
+    """As the entry point decides: prompts over bf16 pages from 64 query rows a KV head
+    and sequence."""
+    return "f32" if dt == "f32" else "bf16 prompt" if c.data.dtype == torch.bfloat16 and n * (H // KH) >= 64 * n_seq else "bf16"
 
 
 def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=None, one=False):
@@ -92,11 +94,15 @@ def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=
         k, v = held(c, b, T)
         t = np.arange(T)
         paged = (table[b, t // c.page] >= 0) & (table[b, t // c.page] < c.n_pages)
-        pick = np.array(only if only is not None else sorted({0, n - 1, *np.random.default_rng(n).integers(0, n, 30).tolist()}))
+        pick = np.array(sorted({0, n - 1, *np.random.default_rng(n).integers(0, n, 30).tolist()}))
+        if only == "before":                    # tokens in front of the middle one
+            pick = np.array(sorted({*pick[pick < n // 2].tolist(), max(n // 2 - 1, 0)})) if n > 1 else np.array([], int)
+            if len(pick) == 0:
+                continue
         pick = pick[s + pick < c.shape.maxT]
         see = paged & (t <= s + pick[:, None])
         for h in range(H):
-            want, tol = attend(q64[cu[b] + pick, h], k[:, h * KH // H], v[:, h * KH // H], see, scale, form_of(dt, n, H, KH, len(counts)))
+            want, tol = attend(q64[cu[b] + pick, h], k[:, h * KH // H], v[:, h * KH // H], see, scale, form_of(c, dt, len(q), H, KH, len(counts)))
             off = np.abs(g64[cu[b] + pick, h] - want)
             worst = np.nanmax(off / np.maximum(tol, 1e-300))
             assert (off <= tol).all(), f"sequence {b} head {h}: {worst:.3g} bounds off, by {np.nanmax(off):.3g}"
@@ -221,3 +227,125 @@ def test_prompts(H, KH, counts, start, page, dt, cached):
 def test_max_rows_only_cuts(counts, start, max_rows, dt, cached):
     """Any bound gives the same, too small or too large."""
     run(4, 2, counts, start, dt, cached, maxT=120000, max_rows=max_rows)
+
+
+# ------------------------------------------------- what is not finite, what is not there
+
+CALLS = [(4, 2, [1], [40]), (8, 1, [2], [500]), (4, 2, [5, 0, 3], [40, 9, 700]), (2, 2, [100, 130], [0, 333]), (7, 1, [150], [77]),
+         (16, 2, [300], [600])]
+
+
+def prepared(H, KH, counts, start, cached, maxT, page=16, seed=0):
+    c = cache(len(counts), maxT, KH, page, cached, seed=seed)
+    q = []
+    for b, (s, n) in enumerate(zip(start, counts)):
+        k, v = rows(7 * b + 1, max(s + n, 1), KH)
+        if s + n > 0:
+            put(c, b, k[:s + n], v[:s + n])
+        q.append(queries(b + 100, k, s, n, H))
+    return c, np.concatenate(q)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", CALLS)
+@pytest.mark.parametrize("maxT", [0, 1500])
+def test_rows_of_later_tokens_may_hold_anything(H, KH, counts, start, maxT, dt, cached):
+    """NaN and infinities in K and V of a token's row do not reach the tokens before
+    it; the tokens from it on get what the formula gives."""
+    T = maxT or max(s + n for s, n in zip(start, counts))
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    for value in (float("nan"), float("inf"), -float("inf"), 3e38):
+        c, q = prepared(H, KH, counts, start, cached, T)
+        late = []
+        for b, (s, n) in enumerate(zip(start, counts)):
+            if not n:
+                continue
+            k, v = (x[s + n // 2:s + n // 2 + 1].copy() for x in held(c, b, s + n))
+            v[:, :, 5], v[:, 0, 77] = value, -value
+            put(c, b, k, v, first=s + n // 2)
+            late += range(int(cu[b]) + n // 2, int(cu[b]) + n)
+        got = check(c, q, start, counts, dt, only="before")
+        if value != 3e38:
+            x = got[late].float()
+            assert not bool(x[:, :, 5].isfinite().any()) and not bool(x[:, 0, 77].isfinite().any())
+            x[:, :, 5] = 0.0
+            x[:, :, 77] = 0.0
+            assert bool(x.isfinite().all())
+        # the same in K
+        for b, (s, n) in enumerate(zip(start, counts)):
+            if n:
+                k, v = (x[s + n // 2:s + n // 2 + 1].copy() for x in held(c, b, s + n))
+                k[:, :, 3] = value
+                put(c, b, k, v, first=s + n // 2)
+        check(c, q, start, counts, dt, only="before")
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", CALLS)
+def test_pages_that_are_not_there(H, KH, counts, start, dt, cached):
+    """Rows of pages given back, of numbers outside the pool and of pages still to
+    come are not seen; a token that sees none gets 0."""
+    for gone in ([0], [1, 2], [3], [0, 1, 2, 3, 4, 5], list(range(400))):
+        c, q = prepared(H, KH, counts, start, cached, 1500)
+        for b in range(c.B):
+            for i, p in enumerate(gone):
+                if p < c.table.shape[1]:
+                    c.table[b, p] = [-1, c.n_pages, 2 ** 31 - 1, -2 ** 31][i % 4]
+        # (the pages of NaN behind the rows, and those that others hold, are not read in their place)
+        got = check(c, q, start, counts, dt)
+        if len(gone) == 400:
+            assert not bool(got.any())
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", [(4, 2, [1, 1], [-1, 20]), (4, 2, [3, 5], [-2, -9]), (4, 2, [100, 130], [-40, 900]), (4, 2, [70, 70], [-200, 960])])
+def test_tokens_without_rows_and_rows_outside(H, KH, counts, start, dt, cached):
+    """A row below 0: 0.  A row past the cache, and tokens behind the last sequence:
+    left as they were."""
+    T = 1000
+    c, q = prepared(H, KH, counts, [min(s, T - n) for s, n in zip(start, counts)], cached, T)
+    q = np.concatenate([q, q[:3]])
+    out = torch.full((len(q), H, HD), 7.0, dtype=DT[dt], device="cuda")
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    qd = torch.from_numpy(q).cuda().to(DT[dt])
+    qd[0, 0, 5] = float("nan")
+    got = c.attention(0, qd, ints(start), ints(cu.tolist()), out=out)
+    torch.cuda.synchronize()
+    assert got.data_ptr() == out.data_ptr()
+    for b, (s, n) in enumerate(zip(start, counts)):
+        r = torch.arange(s, s + n, device="cuda")
+        x = got[int(cu[b]):int(cu[b + 1])]
+        assert not bool(x[r < 0].any())
+        assert bool((x[r >= T] == 7.0).all())
+        assert bool(x[(r >= 0) & (r < T)].isfinite().all())
+    assert bool((got[int(cu[-1]):] == 7.0).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-38, 1e-9, -0.3, -HD ** -0.5, 1.0])
+@pytest.mark.parametrize("dt,cached", TYPES)
+def test_scales_of_any_sign_and_zero(dt, cached, scale):
+    for H, KH, counts, start in CALLS:
+        run(H, KH, counts, start, dt, cached, scale=scale)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", CALLS)
+def test_an_infinite_query_gives_nan(H, KH, counts, start, dt, cached):
+    c, q = prepared(H, KH, counts, start, cached, 1500)
+    q[:, 1, 77] = np.inf
+    q[0, 0, 5] = -np.inf
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    got = c.attention(0, torch.from_numpy(q).cuda().to(DT[dt]), ints(start), ints(cu.tolist()))
+    assert bool(got[:, 1].isnan().all()) and bool(got[0, 0].isnan().all())
+    got[:, 1] = 0.0
+    got[0, 0] = 0.0
+    assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", CALLS)
+def test_weights_far_apart(H, KH, counts, start, dt, cached):
+    """Scores of hundreds: one row has all the weight, the reference rises often."""
+    c, q = prepared(H, KH, counts, start, cached, 1500)
+    check(c, q * 30.0, start, counts, dt)
+    check(c, q * 1e-4, start, counts, dt)
