@@ -5,6 +5,7 @@
 // rows, so 16 aligned rows always lie in one page.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "jm_kernels.h"
 #include "jm_tokens.h"
@@ -589,24 +590,33 @@ __device__ __forceinline__ s16x4 paged_tr16(const uint16_t* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(void*)p);
 }
 
+#ifndef PAGED_AHEAD
+#define PAGED_AHEAD 1
+#endif
+// The phases of k_paged_tile: what must have completed is waited for explicitly, and
+// nothing moves from one to the next.
+__device__ __forceinline__ void paged_meet() {
+    __builtin_amdgcn_sched_barrier(0);
+    wave_meet();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <bool BF, int RG>
 __global__ void __launch_bounds__(512, 2)
 k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     constexpr int HD = 128, QB = BF ? 2 : 1, NQ = BF ? 1 : 3, PS = 8 / RG, STEP = 32 * PS, TILE = 32 * HD;
+    constexpr int RW = 8 * (PS / 2);            // rows of a step that a wave stages, of K and of V
+    constexpr int LPS = RW / 2;                 // its loads, 4 rows each
+    constexpr int NROW = 32 * QB * RG, AHEAD = PAGED_AHEAD;
     constexpr int NS = PS == 2 ? 3 : 2;         // steps in LDS
-    constexpr int GW = PS / 2;                  // 16-row groups that a wave stages a step
-    constexpr int LPS = 4 * GW;                 // its loads
-    constexpr int NROW = 32 * QB * RG;
-    // PS tiles of K, then of V, for each step in LDS (arrays of their own, so that the
-    // compiler sees that a step's reads do not wait for another's rows); at the end the
-    // outputs being joined
-    __shared__ __align__(16) uint16_t kv0[2 * PS * TILE], kv1[2 * PS * TILE], kv2[NS == 3 ? 2 * PS * TILE : 8];
+    // PS tiles of K and of V of NS steps; at the end the outputs being joined
+    __shared__ __align__(16) uint16_t kt[NS][PS * TILE], vt[NS][PS * TILE];
     // the second block of query rows of each row group (BF)
     __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
     __shared__ float mls[8][32 * QB][2];
-    __shared__ uint8_t okf[NS][2 * PS];         // whether a step's 16-row groups have pages
+    __shared__ uint8_t okf[NS][2 * PS];          // whether a step's 16-row groups have pages
     // which dimensions met a V value of +inf (bit 0), -inf (bit 1) or NaN (both) that not
-    // every query row sees, 16 dimensions a word
+    // every query row of a wave sees, 16 dimensions a word
     __shared__ uint32_t taint[NROW][HD / 16];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w % RG, ps = w / RG, n = lane & 31, h = lane >> 5;
@@ -615,10 +625,10 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     CallUnit un;
     if (!call_unit(c, u, a.tp, un)) return;
     const PagedSeq seq(c, un.seq, kh);
-    const int pmax = min(un.pos + un.n - 1, c.maxT - 1), pmin = min(un.pos, c.maxT - 1);
+    const int pmax = min(un.pos + un.n - 1, c.maxT - 1);
     // this block's range of the steps (none where no token sees a row)
     const int steps = pmax < 0 ? 0 : pmax / STEP + 1;
-    const int step0 = (int)((long long)steps * sr / a.S), nstep = (int)((long long)steps * (sr + 1) / a.S);
+    const int step0 = (int)((long long)steps * sr / a.S), nstep = (int)((long long)steps * (sr + 1) / a.S) - step0;
 
     // this lane's query rows, and the last cache row that each sees
     int tok[QB], prow[QB], head[QB];
@@ -631,49 +641,79 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
         head[b] = kh * a.qpk + r % a.qpk;
         prow[b] = min(un.pos + tok[b], c.maxT - 1);
     }
-    // ... over the wave's rows
+    // ... the first of the wave's
     const int wmin = min(un.pos + min(32 * QB * rg / a.qpk, un.n - 1), c.maxT - 1);
-    const int wmax = min(un.pos + min((32 * QB * (rg + 1) - 1) / a.qpk, un.n - 1), c.maxT - 1);
 
-    // ---- staging: wave w has the 16-row groups GW (w % 4) .. of each step, of K (w < 4) or V
-    const bool isk = w < 4;
-    const char* const src = isk ? seq.k : seq.v;
-    auto fetch = [&](int batch) __attribute__((always_inline)) {        // lane: group lane % GW of the batch's step lane / GW
-        const long long row = (long long)(step0 + batch * (64 / GW) + lane / GW) * STEP + 16 * (GW * (w & 3) + lane % GW);
+    // ---- staging: of the half of a step that its four waves (w < 4, or the others)
+    // multiply, wave w has rows RW (w % 4) ..: 8 or 16 rows of the tile that it multiplies
+    // itself.  Lane 2 i + g of `page` has the page of the tile's 16-row group g in the i-th of
+    // 32 steps.
+    const int srow = STEP / 2 * (w >> 2) + RW * (w & 3), sgroup = (srow >> 4) & 1;
+    auto fetch = [&](int batch) __attribute__((always_inline)) {
+        const long long row = (long long)(step0 + 32 * batch + (lane >> 1)) * STEP + 32 * ps + 16 * (lane & 1);
         const int p = row <= pmax ? seq.table[row >> c.lp] : -1;
         return (unsigned)p < (unsigned)c.n_pages ? p : -1;
     };
     int page = fetch(0), next = fetch(1);
-    auto stage = [&](int i, uint16_t* kv, int slot) __attribute__((always_inline)) {
-        const int k = i - step0;
-        if (k && k % (64 / GW) == 0) {
-            page = next;
-            next = fetch(k / (64 / GW) + 1);
-        }
+    // where a lane's first load of a step lies within its rows (load j: 4 j rows on; of K
+    // another chunk of them)
+    const int r0 = lane >> 4;
+    const int koff = 256 * r0 + 16 * ((lane & 15) ^ ((srow + r0) & 15)), voff = 256 * r0 + 16 * ((lane & 15) ^ (4 * r0));
+    // the wave's rows of K or V of a step into `to`: `at` bytes from page 0's rows, lim + 1 of
+    // them to be read (none: no page)
+    auto request = [&](auto full, const char* src, bool isk, size_t at, int lim, uint16_t* to) __attribute__((always_inline)) {
+        // (as a number: the compiler would have every read of LDS wait for these loads, which
+        // are waited for below; and as a buffer: behind a load from a global address to LDS,
+        // which counts as both, it lets no read of LDS be outstanding when it waits for one)
+        uint32_t num = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(to + srow * HD));
+        __asm__ volatile("" : "+s"(num));
+        const auto dst = (__attribute__((address_space(3))) uint16_t*)(uintptr_t)num;
+        const auto base = __builtin_amdgcn_make_buffer_rsrc((void*)(src + at), 0, RW * 256, 0x00020000);
+        if (decltype(full)::value || lim >= RW - 1) {
 #pragma unroll
-        for (int q = 0; q < GW; q++) {
-            const int gi = GW * (w & 3) + q, row = i * STEP + 16 * gi;
-            const int p = __builtin_amdgcn_readlane(page, k % (64 / GW) * GW + q);
-            uint16_t* const dst = kv + (isk ? 0 : PS * TILE) + gi * 16 * HD;
-            if (isk && lane == 0) okf[slot][gi] = p >= 0;
-            if (p >= 0) {
-                const int lim = min(pmax - row, 15);        // (rows past the prefixes repeat the last one; their weights are 0)
-                const gptr<const char> base = (gptr<const char>)(src + (size_t)p * c.page_stride) + (uint32_t)((row & ((1 << c.lp) - 1)) * 256);
+            for (int j = 0; j < RW / 4; j++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)(dst + 4 * j * HD), 16,
+                                                         isk ? koff ^ (64 * j) : voff, 1024 * j, 0, 0);
+        } else if (lim >= 0) {
+            // (rows past the prefixes repeat the last one; their weights are 0)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int r = 4 * j + (lane >> 4);
-                    const int x = isk ? r : 4 * (lane >> 4);
-                    __builtin_amdgcn_global_load_lds((gptr<void>)(base + ((uint32_t)min(r, lim) * 256 + 16 * ((lane & 15) ^ x))),
-                                                     (__attribute__((address_space(3))) void*)(dst + 4 * j * HD), 16, 0, 0);
-                }
-            } else if (!isk) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) *(uint4*)(dst + 4 * j * HD + 8 * lane) = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < RW / 4; j++) {
+                const int r = 4 * j + r0, x = isk ? (srow + r) & 15 : 4 * r0;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)(dst + 4 * j * HD), 16,
+                                                         min(r, lim) * 256 + 16 * ((lane & 15) ^ x), 0, 0, 0);
             }
+        } else if (!isk) {
+#pragma unroll
+            for (int j = 0; j < RW / 4; j++) *(uint4*)(to + (srow + 4 * j) * HD + 8 * lane) = make_uint4(0, 0, 0, 0);
         }
     };
-    if (step0 < nstep) stage(step0, kv0, 0);
-    if (step0 + 1 < nstep) stage(step0 + 1, kv1, 1);
+    // where the rows of K of the step to be requested next lie, and those of V, of the step
+    // before it; has: whether the tile's groups have pages, two bits a step, the latest lowest
+    int klim = -1, vlim = -1;
+    size_t kat = 0, vat = 0;
+    uint32_t has = 0;
+    auto locate = [&](int t) __attribute__((always_inline)) {
+        vat = kat;
+        vlim = klim;
+        if (t && t % 32 == 0) {
+            page = next;
+            next = fetch(t / 32 + 1);
+        }
+        const int p0 = __builtin_amdgcn_readlane(page, 2 * (t % 32)), p1 = __builtin_amdgcn_readlane(page, 2 * (t % 32) + 1);
+        has = has << 2 | (p0 >= 0 ? 1u : 0u) | (p1 >= 0 ? 2u : 0u);
+        const int p = sgroup ? p1 : p0, row = (step0 + t) * STEP + srow;
+        klim = p >= 0 ? min(pmax - row, RW - 1) : -1;
+        kat = (size_t)(klim >= 0 ? p : 0) * c.page_stride + (uint32_t)((row & ((1 << c.lp) - 1)) * 256);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+#pragma unroll 1
+    for (int t = 0; t < NS; t++) {
+        locate(t);
+        if (t < nstep) request(no, seq.k, true, kat, klim, kt[t]);
+        if (t < nstep && t < NS - 1) request(no, seq.v, false, kat, klim, vt[t]);
+    }
+    locate(NS);
 
     // ---- the query rows, with the score scale's sign (a scale of 0, or a smaller one, as
     // 2^-100: masked scores stay -inf behind it)
@@ -707,158 +747,214 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
 
     f32x16 O[QB][4];
     float ref[QB], l[QB];
-    bool seen[QB];
+    int seen[QB];                               // whether the lane's query rows saw a row; all: all of them did
+    bool all = false;
+    f32x16 S[QB];
+    u32x4_t P[QB][NQ][2];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
         ref[b] = -INFINITY;
         l[b] = 0.0f;
-        seen[b] = false;
+        seen[b] = 0;
 #pragma unroll
         for (int nt = 0; nt < 4; nt++) O[b][nt] = f32x16(0.0f);
     }
-    const int kx = h ^ (n & 15);                // K row n: dimensions 16 kk + 8 h .. at chunk (2 kk) ^ kx
+    const int ko = (32 * ps + n) * HD + 8 * (h ^ (n & 15));     // K row n: dimensions 16 kk + 8 h .. at chunk (2 kk) ^ h ^ (n % 16)
     // this lane's part of a transposed read: row 4 h + i / 4, 4 columns 16 (l / 16 % 2) + 4 (i
     // % 4) of a 32-column block, i = l % 16; chunk c of V row r sits at c ^ 4 (r % 4)
     const int vrow = (lane & 15) >> 2;
-    const int vo = (4 * h + vrow) * HD + 8 * (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 4 * (lane & 1);
+    const int vo = (32 * ps + 4 * h + vrow) * HD + 32 * vrow + 8 * (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 4 * (lane & 1);
 
-    auto step = [&](int i, uint16_t* kv, int slot, uint16_t* kvn, int slotn) __attribute__((always_inline)) {
-        // this wave's rows of step i have arrived (those of step i + 1 may be on their
-        // way), then everyone's
-        if (i + 1 < nstep) __builtin_amdgcn_s_waitcnt(LPS == 4 ? 0x0074 : 0x0078);     // vmcnt(LPS), lgkmcnt(0)
-        else __builtin_amdgcn_s_waitcnt(0x0070);                                        // vmcnt(0), lgkmcnt(0)
-        wave_meet();
-        if (NS == 3 && i + 2 < nstep) stage(i + 2, kvn, slotn);
-        const int t0 = i * STEP + 32 * ps;
-        uint16_t* const kw = kv + ps * TILE;
-        uint16_t* const vw = kv + (PS + ps) * TILE;
-        if (i * STEP + STEP - 1 > pmin) {
-            // A weight of 0 does not hide a value of V that is not finite.  In a step
-            // whose rows not everyone sees such values go into `taint`, for the rows that
-            // see them, and out of the step.  (Block-uniform.)
-            uint32_t nf = 0;
+    // ---- a wave's weights of a step: of lane registers 8 s + 2 e, + 1 of its scores
+    auto weights = [&](int s, int e) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 8 / RG; j++) {
-                const uint4 y = *(const uint4*)(vw + 8 * ((8 / RG) * 64 * rg + 64 * j + lane));
+        for (int b = 0; b < QB; b++) {
+            const float r0 = ref[b] == -INFINITY ? 0.0f : ref[b];
+            const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cs, -r0));
+            const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cs, -r0));
+            uint32_t p[NQ];
+            parts_bf16<NQ>(x0, x1, p);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) P[b][q][s][e] = p[q];
+            if (BF) l[b] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p[0]), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l[b], false);
+            else l[b] += x0 + x1;
+        }
+    };
+    // The vector work of a phase: of step t, the scores that are not seen, the reference, and
+    // the weights of the first half of its rows.
+    auto weigh = [&](int t) __attribute__((always_inline)) {
+        const int t0 = (step0 + t) * STEP + 32 * ps;
+        const uint32_t ok = has >> (2 * NS) & 3u;
+        if (ok == 3u && t0 + 31 <= wmin) {
+            all = true;
+        } else {
+#pragma unroll
+            for (int b = 0; b < QB; b++) {
+                const int lim = prow[b] - t0;
+                seen[b] |= (int)(ok & 1u) & (int)(lim >= 0);
+                seen[b] |= (int)(ok >> 1) & (int)(lim >= 16);
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int see = ok & (v < 8 ? 1u : 2u) ? lim - 4 * h : -1;
+                    S[b][v] = 8 * (v / 4) + v % 4 > see ? -INFINITY : S[b][v];
+                }
+            }
+        }
+        float m[QB];
+        bool high = false;
+#pragma unroll
+        for (int b = 0; b < QB; b++) {
+            m[b] = S[b][0];
+#pragma unroll
+            for (int v = 1; v < 16; v++) m[b] = fmaxf(m[b], S[b][v]);
+            m[b] *= cs;
+            high |= m[b] > ref[b] + 10.0f;
+        }
+        if (__any(high)) {
+#pragma unroll
+            for (int b = 0; b < QB; b++) {
+                m[b] = fmaxf(m[b], __shfl_xor(m[b], 32, JM_WAVE));
+                const float nref = fmaxf(ref[b], m[b]);
+                const float f = nref == -INFINITY ? 1.0f : pow2f(ref[b] - nref);
+                l[b] *= f;
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++) O[b][nt] *= f;
+                ref[b] = nref;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) weights(0, e);
+        // (here and now: the compiler would put them off to where they are used, among the
+        // products)
+#pragma unroll
+        for (int b = 0; b < QB; b++) {
+#pragma unroll
+            for (int q = 0; q < NQ; q++) __asm__ volatile("" : "+v"(P[b][q][0].x), "+v"(P[b][q][0].y), "+v"(P[b][q][0].z), "+v"(P[b][q][0].w));
+            __asm__ volatile("" : "+v"(l[b]));
+        }
+    };
+
+    // ---- the products of a phase: the weights of step t times its V, the scores of the step
+    // after it.  (Operands AHEAD products ahead of their use, in an order
+    // that the compiler keeps: left to it, every product waits for its own.  Their
+    // addresses from one each, an XOR at a time: those of all steps in LDS kept in
+    // registers, others spill.)
+    auto multiply = [&](auto has_v, int t, uint16_t* v, const uint16_t* kk) __attribute__((always_inline)) {
+        constexpr bool V = decltype(has_v)::value;
+        const int t0 = (step0 + t) * STEP + 32 * ps;
+        int va = vo;
+        __asm__ volatile("" : "+v"(va));
+        auto vop = [&](int k) __attribute__((always_inline)) {
+            const uint16_t* const p = v + (va ^ (32 * (k % 4))) + 16 * (k / 4) * HD;
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(paged_tr16(p), paged_tr16(p + 8 * HD), 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        // A weight of 0 does not hide a value that is not finite.  Where not all of the
+        // wave's query rows see the tile, such values go into `taint`, for all of the
+        // block's rows that see them, and out of the tile.  (The other waves that multiply it
+        // find them there or in `taint`: either is right.)
+        if (V && t0 + 31 > wmin) {
+            uint16_t* const tile = v + ps * TILE;
+            uint32_t nf = 0;
+#pragma unroll 2
+            for (int j = 0; j < 8; j++) {
+                const uint4 y = *(const uint4*)(tile + 8 * (64 * j + lane));
                 const uint32_t x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     nf |= (uint32_t)((x[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((x[e] & 0x7F800000u) == 0x7F800000u);
             }
-            if (__syncthreads_or(nf != 0)) {
+            if (__any(nf != 0)) {
 #pragma unroll 1
                 for (int e = lane; e < TILE; e += 64) {
                     const int r = e / HD, dim = (e % HD) ^ (32 * (r & 3));
-                    const uint32_t x = vw[e];
+                    const uint32_t x = tile[e];
                     if ((x & 0x7F80u) != 0x7F80u) continue;
                     const uint32_t bits = (x & 0x7Fu) ? 3u : (x >> 15) ? 2u : 1u;
-                    // (a row past the prefixes holds the last one again)
-                    if (t0 + r > pmax) continue;
+                    if (t0 + r <= pmax) {               // (a row past the prefixes holds the last one again)
 #pragma unroll 1
-                    for (int q = 0; q < 32 * QB; q++)
-                        if (t0 + r <= un.pos + min((32 * QB * rg + q) / a.qpk, un.n - 1))
-                            atomicOr(&taint[32 * QB * rg + q][dim / 16], bits << (2 * (dim % 16)));
-                }
-                __syncthreads();
-                if (rg == 0) {
-#pragma unroll 1
-                    for (int e = lane; e < TILE; e += 64)
-                        if ((vw[e] & 0x7F80u) == 0x7F80u) vw[e] = 0;
-                }
-                __syncthreads();
-            }
-        }
-        if (t0 <= wmax) {
-            const uint32_t ok = *(const uint16_t*)&okf[slot][2 * ps];
-            const bool ok0 = __builtin_amdgcn_readfirstlane(ok & 0xFFu), ok1 = __builtin_amdgcn_readfirstlane(ok >> 8);
-            f32x16 S[QB];
-#pragma unroll
-            for (int b = 0; b < QB; b++) S[b] = f32x16(0.0f);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const bf16x8 x = __builtin_bit_cast(bf16x8, *(const uint4*)(kw + n * HD + 8 * ((2 * k) ^ kx)));
-#pragma unroll
-                for (int p = NQ - 1; p >= 0; p--) S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qr[p][k], S[0], 0, 0, 0);
-                if (QB == 2) S[QB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, *(const bf16x8*)&q1[rg][k][lane], S[QB - 1], 0, 0, 0);
-            }
-            bf16x8 P[QB][NQ][2];
-            const bool whole = t0 + 31 <= wmin && ok0 && ok1;
-#pragma unroll
-            for (int b = 0; b < QB; b++) {
-                seen[b] |= (ok0 && t0 <= prow[b]) || (ok1 && t0 + 16 <= prow[b]);
-                if (!whole) {
-                    const int lim = prow[b] - t0 - 4 * h;
-#pragma unroll
-                    for (int v = 0; v < 16; v++)
-                        if (8 * (v / 4) + v % 4 > lim || !(v < 8 ? ok0 : ok1)) S[b][v] = -INFINITY;
-                }
-                float m = S[b][0];
-#pragma unroll
-                for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
-                m *= cs;
-                if (__any(m > ref[b] + 10.0f)) {
-                    m = fmaxf(m, __shfl_xor(m, 32, JM_WAVE));
-                    const float nref = fmaxf(ref[b], m);
-                    const float f = nref == -INFINITY ? 1.0f : pow2f(ref[b] - nref);
-                    l[b] *= f;
-#pragma unroll
-                    for (int nt = 0; nt < 4; nt++) O[b][nt] *= f;
-                    ref[b] = nref;
-                }
-                const float r0 = ref[b] == -INFINITY ? 0.0f : ref[b];
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    uint32_t y[NQ][4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cs, -r0));
-                        const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cs, -r0));
-                        uint32_t p[NQ];
-                        parts_bf16<NQ>(x0, x1, p);
-#pragma unroll
-                        for (int q = 0; q < NQ; q++) y[q][e] = p[q];
-                        if (BF) l[b] += __uint_as_float(p[0] << 16) + __uint_as_float(p[0] & 0xFFFF0000u);
-                        else l[b] += x0 + x1;
+                        for (int q = 0; q < NROW; q++)
+                            if (t0 + r <= un.pos + min(q / a.qpk, un.n - 1)) atomicOr(&taint[q][dim / 16], bits << (2 * (dim % 16)));
                     }
-#pragma unroll
-                    for (int q = 0; q < NQ; q++) P[b][q][s] = as_bf16x8(y[q][0], y[q][1], y[q][2], y[q][3]);
+                    tile[e] = 0;
                 }
+                __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0)
+                __asm__ volatile("" : : : "memory");
             }
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int nt = 0; nt < 4; nt++) {
-                    const s16x4 v0 = paged_tr16(vw + vo + 16 * s * HD + 32 * (nt ^ vrow));
-                    const s16x4 v1 = paged_tr16(vw + vo + (16 * s + 8) * HD + 32 * (nt ^ vrow));
-                    const bf16x8 x = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int b = 0; b < QB; b++)
-#pragma unroll
-                        for (int q = NQ - 1; q >= 0; q--) O[b][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, P[b][q][s], O[b][nt], 0, 0, 0);
-                }
         }
-        if (NS == 2) {
-            __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): this wave's reads of the step, then
-            wave_meet();                            // everyone's, are done
-            if (i + 2 < nstep) stage(i + 2, kvn, slotn);
+        int ka = ko;
+        __asm__ volatile("" : "+v"(ka));
+        auto kop = [&](int k) __attribute__((always_inline)) { return *(const bf16x8*)(kk + (ka ^ (16 * k))); };
+        auto qop = [&](int k) __attribute__((always_inline)) { return *(const bf16x8*)&q1[BF ? rg : 0][k][lane]; };
+        constexpr int first = V ? 0 : 8, end = 16;
+        bf16x8 x[16], y[16];
+#pragma unroll
+        for (int k = first; k < end + AHEAD; k++) {
+            if (k < end) {
+                x[k] = k < 8 ? vop(k) : kop(k - 8);
+                if (QB == 2 && k >= 8) y[k] = qop(k - 8);
+            }
+            if (k < first + AHEAD) continue;
+            __builtin_amdgcn_sched_barrier(0);
+            const int j = k - AHEAD;
+            if (j == 8) {
+#pragma unroll
+                for (int b = 0; b < QB; b++) S[b] = f32x16(0.0f);
+            }
+            if (j < 8) {
+#pragma unroll
+                for (int b = 0; b < QB; b++)
+#pragma unroll
+                    for (int q = NQ - 1; q >= 0; q--)
+                        O[b][j % 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[j], __builtin_bit_cast(bf16x8, P[b][q][j / 4]), O[b][j % 4], 0, 0, 0);
+                if (j < 4) weights(1, j);       // (in the products' shadow, whose results nobody waits for)
+                if (j == 4) locate(t + 1 + NS);
+            } else {
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--) S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[j], qr[p][j - 8], S[0], 0, 0, 0);
+                if (QB == 2) S[QB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[j], y[j], S[QB - 1], 0, 0, 0);
+            }
         }
     };
+    // ---- the vector work of a phase: the weights of step t
+    // ---- The two waves of a SIMD (w and w + 4) are one phase apart: while one multiplies,
+    // the other weighs.  In the phase in which a wave weighs step t it requests K of step t +
+    // NS and V of step t + NS - 1, into the rows that its half multiplied in the phase
+    // before; it waits for them by the end of the phase in which it weighs step t + NS - 1,
+    // behind which they are multiplied.
+    __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0), lgkmcnt(0)
+    paged_meet();
+    if (w >= 4) paged_meet();
+    multiply(std::false_type{}, 0, vt[0], kt[0]);
+    __builtin_amdgcn_s_waitcnt(0xC07F);         // lgkmcnt(0): this wave's reads are done
+    paged_meet();
+    int slot = 0;                               // t % NS
 #pragma unroll 1
-    for (int i = step0; i < nstep; i += NS) {
-        if (NS == 3) {
-            step(i, kv0, 0, kv2, 2);
-            if (i + 1 < nstep) step(i + 1, kv1, 1, kv0, 0);
-            if (i + 2 < nstep) step(i + 2, kv2, 2, kv1, 1);
+    for (int t = 0; t < nstep; t++) {
+        weigh(t);
+        const int before = slot ? slot - 1 : NS - 1, after = slot < NS - 1 ? slot + 1 : 0;
+        if (t + NS < nstep && min(klim, vlim) == RW - 1) {
+            request(yes, seq.v, false, vat, vlim, vt[before]);
+            request(yes, seq.k, true, kat, klim, kt[slot]);
+            static_assert((NS - 1) * LPS == 8, "the loads that may be on their way");
+            __builtin_amdgcn_s_waitcnt(0x0078); // vmcnt(8), lgkmcnt(0)
         } else {
-            step(i, kv0, 0, kv0, 0);
-            if (i + 1 < nstep) step(i + 1, kv1, 1, kv1, 1);
+            if (t + NS <= nstep) request(no, seq.v, false, vat, vlim, vt[before]);
+            if (t + NS < nstep) request(no, seq.k, true, kat, klim, kt[slot]);
+            __builtin_amdgcn_s_waitcnt(0x0070);
         }
+        paged_meet();
+        multiply(std::true_type{}, t, vt[slot], kt[after]);     // (behind the last step: scores that nobody takes)
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        paged_meet();
+        slot = after;
     }
+    if (w < 4) paged_meet();
 
-    // ---- the PS waves of each row group joined, 32 dimensions at a time
+    // ---- the PS waves of each row group joined, 32 dimensions of 32 rows at a time
     float f[QB], inv[QB];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
+        seen[b] |= all;
         l[b] += __shfl_xor(l[b], 32, JM_WAVE);
         if (h == 0) {
             mls[w][32 * b + n][0] = ref[b];
@@ -887,29 +983,32 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             if (ps == 0 && h == 0 && live[b]) *(float2*)ml = make_float2(M, any ? L : -1.0f);
         }
     }
-    float4* const mb = (float4*)&kv0[0];        // [wave][4][64 lanes]
-    static_assert(4 * 8 * 64 * 16 <= sizeof(kv0), "the outputs of 32 rows and dimensions of each wave fit");
+    // a wave keeps one in PS of the 4 quarters (8 dimensions each) of a piece, which it
+    // finishes, and hands the others on: quarter q of wave p at [p][which(q, p)]
+    auto which = [](int q, int p) { return PS == 2 ? q >> 1 : q - (q > p); };
+    static_assert(8 * (4 - 4 / PS) * 64 * 16 <= sizeof(kt[0]), "what the waves hand on fits");
 #pragma unroll
     for (int nt = 0; nt < 4; nt++)
 #pragma unroll
         for (int b = 0; b < QB; b++) {
-            __syncthreads();
+            float4* const mb = (float4*)&kt[(nt * QB + b) & 1][0] + lane;       // (in turn: one barrier a piece)
 #pragma unroll
             for (int q = 0; q < 4; q++)
-                mb[(w * 4 + q) * 64 + lane] = make_float4(O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b], O[b][nt][4 * q + 2] * f[b],
-                                                          O[b][nt][4 * q + 3] * f[b]);
+                if (q % PS != ps)
+                    mb[(w * (4 - 4 / PS) + which(q, ps)) * 64] = make_float4(O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b],
+                                                                            O[b][nt][4 * q + 2] * f[b], O[b][nt][4 * q + 3] * f[b]);
             __syncthreads();
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 if (q % PS != ps || !live[b]) continue;
-                float4 s = mb[(rg * 4 + q) * 64 + lane];
+                float o[4] = {O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b], O[b][nt][4 * q + 2] * f[b], O[b][nt][4 * q + 3] * f[b]};
 #pragma unroll
-                for (int p = 1; p < PS; p++) {
-                    const float4 x = mb[((p * RG + rg) * 4 + q) * 64 + lane];
-                    s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
+                for (int i = 1; i < PS; i++) {
+                    const int p = (ps + i) % PS;
+                    const float4 x = mb[((p * RG + rg) * (4 - 4 / PS) + which(q, p)) * 64];
+                    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w;
                 }
                 const uint32_t tw = taint[32 * (QB * rg + b) + n][2 * nt + q / 2] >> (16 * (q % 2) + 8 * h);     // dimensions 8 q + 4 h ..
-                float o[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t x = (tw >> (2 * e)) & 3u;
