@@ -591,7 +591,7 @@ __device__ __forceinline__ s16x4 paged_tr16(const uint16_t* p) {
 }
 
 #ifndef PAGED_AHEAD
-#define PAGED_AHEAD 1
+#define PAGED_AHEAD 2
 #endif
 // The phases of k_paged_tile: what must have completed is waited for explicitly, and
 // nothing moves from one to the next.
@@ -610,7 +610,9 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     constexpr int NROW = 32 * QB * RG, AHEAD = PAGED_AHEAD;
     constexpr int NS = PS == 2 ? 3 : 2;         // steps in LDS
     // PS tiles of K and of V of NS steps; at the end the outputs being joined
-    __shared__ __align__(16) uint16_t kt[NS][PS * TILE], vt[NS][PS * TILE];
+    __shared__ __align__(16) uint16_t kv[2][NS][PS * TILE];
+    auto& kt = kv[0];
+    auto& vt = kv[1];
     // the second block of query rows of each row group (BF)
     __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
     __shared__ float mls[8][32 * QB][2];
@@ -655,6 +657,17 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
         return (unsigned)p < (unsigned)c.n_pages ? p : -1;
     };
     int page = fetch(0), next = fetch(1);
+    // ---- the query rows' values on their way
+    u32x4_a8 qv[QB][8][BF ? 1 : 2];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const size_t qi = (size_t)((un.tok + tok[b]) * a.qts + head[b] * a.qhs);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+#pragma unroll
+            for (int i = 0; i < (BF ? 1 : 2); i++)
+                qv[b][k][i] = BF ? *(const u32x4_a8*)((const uint16_t*)a.q + qi + 16 * k + 8 * h) : *(const u32x4_a8*)((const float*)a.q + qi + 16 * k + 8 * h + 4 * i);
+    }
     // where a lane's first load of a step lies within its rows (load j: 4 j rows on; of K
     // another chunk of them)
     const int r0 = lane >> 4;
@@ -721,19 +734,21 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     const uint32_t sign = a.scale2 < 0.0f ? 0x80008000u : 0u;
     bf16x8 qr[NQ][8];
 #pragma unroll
-    for (int b = 0; b < QB; b++) {
-        const size_t qi = (size_t)((un.tok + tok[b]) * a.qts + head[b] * a.qhs);
+    for (int b = 0; b < QB; b++)
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            float x[8];
-            load8<BF>(a.q, qi + 16 * k + 8 * h, x);
             uint32_t y[NQ][4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                uint32_t p[NQ];
-                parts_bf16<NQ>(x[2 * e], x[2 * e + 1], p);
+                if (BF) {
+                    y[0][e] = qv[b][k][0][e] ^ sign;
+                } else {
+                    uint32_t p[NQ];
+                    const u32x4_a8 x = qv[b][k][BF ? 0 : e / 2];
+                    parts_bf16<NQ>(__uint_as_float(x[2 * (e & 1)]), __uint_as_float(x[2 * (e & 1) + 1]), p);
 #pragma unroll
-                for (int i = 0; i < NQ; i++) y[i][e] = p[i] ^ sign;
+                    for (int i = 0; i < NQ; i++) y[i][e] = p[i] ^ sign;
+                }
             }
             if (b == 0) {
 #pragma unroll
@@ -742,7 +757,6 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
                 q1[rg][k][lane] = make_uint4(y[0][0], y[0][1], y[0][2], y[0][3]);
             }
         }
-    }
     for (int i = tid; i < NROW * (HD / 16); i += 512) (&taint[0][0])[i] = 0;
 
     f32x16 O[QB][4];
@@ -780,8 +794,8 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             else l[b] += x0 + x1;
         }
     };
-    // The vector work of a phase: of step t, the scores that are not seen, the reference, and
-    // the weights of the first half of its rows.
+    // The vector work of a phase: of step t, the scores that are not seen, the weights, the
+    // reference.
     auto weigh = [&](int t) __attribute__((always_inline)) {
         const int t0 = (step0 + t) * STEP + 32 * ps;
         const uint32_t ok = has >> (2 * NS) & 3u;
@@ -800,36 +814,40 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
                 }
             }
         }
-        float m[QB];
+        // The weights by the reference as it is, and a new one only where their sum says that one
+        // has passed it by far (or where there is none yet): the largest score is not looked for
+        // otherwise.
+        float before[QB];
+#pragma unroll
+        for (int b = 0; b < QB; b++) before[b] = l[b];
+#pragma unroll
+        for (int e = 0; e < 8; e++) weights(e / 4, e % 4);
         bool high = false;
 #pragma unroll
-        for (int b = 0; b < QB; b++) {
-            m[b] = S[b][0];
-#pragma unroll
-            for (int v = 1; v < 16; v++) m[b] = fmaxf(m[b], S[b][v]);
-            m[b] *= cs;
-            high |= m[b] > ref[b] + 10.0f;
-        }
+        for (int b = 0; b < QB; b++) high |= l[b] > before[b] + 4096.0f || ref[b] == -INFINITY;
         if (__any(high)) {
 #pragma unroll
             for (int b = 0; b < QB; b++) {
-                m[b] = fmaxf(m[b], __shfl_xor(m[b], 32, JM_WAVE));
-                const float nref = fmaxf(ref[b], m[b]);
+                float m = S[b][0];
+#pragma unroll
+                for (int v = 1; v < 16; v++) m = fmaxf(m, S[b][v]);
+                m = fmaxf(m, __shfl_xor(m, 32, JM_WAVE)) * cs;
+                const float nref = fmaxf(ref[b], m);
                 const float f = nref == -INFINITY ? 1.0f : pow2f(ref[b] - nref);
-                l[b] *= f;
+                l[b] = before[b] * f;
 #pragma unroll
                 for (int nt = 0; nt < 4; nt++) O[b][nt] *= f;
                 ref[b] = nref;
             }
-        }
 #pragma unroll
-        for (int e = 0; e < 4; e++) weights(0, e);
+            for (int e = 0; e < 8; e++) weights(e / 4, e % 4);
+        }
         // (here and now: the compiler would put them off to where they are used, among the
         // products)
 #pragma unroll
         for (int b = 0; b < QB; b++) {
 #pragma unroll
-            for (int q = 0; q < NQ; q++) __asm__ volatile("" : "+v"(P[b][q][0].x), "+v"(P[b][q][0].y), "+v"(P[b][q][0].z), "+v"(P[b][q][0].w));
+            for (int q = 0; q < NQ; q++) __asm__ volatile("" : "+v"(P[b][q][0]), "+v"(P[b][q][1]));
             __asm__ volatile("" : "+v"(l[b]));
         }
     };
@@ -906,7 +924,6 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
 #pragma unroll
                     for (int q = NQ - 1; q >= 0; q--)
                         O[b][j % 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[j], __builtin_bit_cast(bf16x8, P[b][q][j / 4]), O[b][j % 4], 0, 0, 0);
-                if (j < 4) weights(1, j);       // (in the products' shadow, whose results nobody waits for)
                 if (j == 4) locate(t + 1 + NS);
             } else {
 #pragma unroll
@@ -983,47 +1000,97 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             if (ps == 0 && h == 0 && live[b]) *(float2*)ml = make_float2(M, any ? L : -1.0f);
         }
     }
-    // a wave keeps one in PS of the 4 quarters (8 dimensions each) of a piece, which it
-    // finishes, and hands the others on: quarter q of wave p at [p][which(q, p)]
-    auto which = [](int q, int p) { return PS == 2 ? q >> 1 : q - (q > p); };
-    static_assert(8 * (4 - 4 / PS) * 64 * 16 <= sizeof(kt[0]), "what the waves hand on fits");
+    // of a row block's 4 pieces of 32 dimensions a wave keeps one in PS, which it finishes, and
+    // hands the others on (piece nt of wave w at [w][which(nt)])
+    constexpr int HAND = 4 - 4 / PS;
+    auto which = [](int nt, int p) { return PS == 2 ? nt >> 1 : nt - (nt > p); };
+    float4* const mb = (float4*)&kt[0][0] + lane;
+    static_assert(8 * HAND * 4096 <= sizeof(kt) + sizeof(vt), "what the waves hand on fits");
 #pragma unroll
-    for (int nt = 0; nt < 4; nt++)
+    for (int b = 0; b < QB; b++) {
+        if (b) __syncthreads();
 #pragma unroll
-        for (int b = 0; b < QB; b++) {
-            float4* const mb = (float4*)&kt[(nt * QB + b) & 1][0] + lane;       // (in turn: one barrier a piece)
+        for (int nt = 0; nt < 4; nt++)
+            if (nt % PS != ps)
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (q % PS != ps)
-                    mb[(w * (4 - 4 / PS) + which(q, ps)) * 64] = make_float4(O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b],
-                                                                            O[b][nt][4 * q + 2] * f[b], O[b][nt][4 * q + 3] * f[b]);
-            __syncthreads();
+                for (int q = 0; q < 4; q++)
+                    mb[((w * HAND + which(nt, ps)) * 4 + q) * 64] = make_float4(O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b],
+                                                                                O[b][nt][4 * q + 2] * f[b], O[b][nt][4 * q + 3] * f[b]);
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            if (nt % PS != ps) continue;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                if (q % PS != ps || !live[b]) continue;
-                float o[4] = {O[b][nt][4 * q] * f[b], O[b][nt][4 * q + 1] * f[b], O[b][nt][4 * q + 2] * f[b], O[b][nt][4 * q + 3] * f[b]};
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int i = 1; i < PS; i++) {
                     const int p = (ps + i) % PS;
-                    const float4 x = mb[((p * RG + rg) * (4 - 4 / PS) + which(q, p)) * 64];
-                    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w;
+                    const float4 y = mb[(((p * RG + rg) * HAND + which(nt, p)) * 4 + q) * 64];
+                    x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
                 }
-                const uint32_t tw = taint[32 * (QB * rg + b) + n][2 * nt + q / 2] >> (16 * (q % 2) + 8 * h);     // dimensions 8 q + 4 h ..
+                O[b][nt][4 * q] = (O[b][nt][4 * q] * f[b] + x.x) * inv[b];
+                O[b][nt][4 * q + 1] = (O[b][nt][4 * q + 1] * f[b] + x.y) * inv[b];
+                O[b][nt][4 * q + 2] = (O[b][nt][4 * q + 2] * f[b] + x.z) * inv[b];
+                O[b][nt][4 * q + 3] = (O[b][nt][4 * q + 3] * f[b] + x.w) * inv[b];
+            }
+            const uint32_t* const tn = &taint[32 * (QB * rg + b) + n][2 * nt];
+            if (__any(tn[0] | tn[1])) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t x = (tw >> (2 * e)) & 3u;
-                    const float add = x == 0 ? 0.0f : x == 1 ? INFINITY : x == 2 ? -INFINITY : __int_as_float(0x7FC00000);
-                    o[e] = __fmul_rn(__fadd_rn(o[e], add), inv[b]);
-                }
-                const int d = 32 * nt + 8 * q + 4 * h;
-                if (a.S == 1) {
-                    store_out<BF>(a.out, ((size_t)(un.tok + tok[b]) * a.H + head[b]) * HD + d, make_float4(o[0], o[1], o[2], o[3]));
-                } else {
-                    const size_t row = ((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n;
-                    *(float4*)(a.part_o + row * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+                for (int v = 0; v < 16; v++) {
+                    // dimension 8 (v / 4) + 4 h + v % 4
+                    const uint32_t x = tn[v / 8] >> (16 * (v / 4 % 2) + 8 * h + 2 * (v % 4)) & 3u;
+                    const uint32_t bits = (x ? 0x7F800000u : 0u) | (x == 2u ? 0x80000000u : 0u) | (x == 3u ? 0x400000u : 0u);
+                    O[b][nt][v] += __uint_as_float(bits);
                 }
             }
         }
+    }
+    if (a.S > 1) {
+#pragma unroll
+        for (int b = 0; b < QB; b++)
+#pragma unroll
+            for (int nt = 0; nt < 4; nt++) {
+                if (nt % PS != ps || !live[b]) continue;
+                const size_t row = ((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + 32 * (QB * rg + b) + n;
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    *(float4*)(a.part_o + row * HD + 32 * nt + 8 * q + 4 * h) =
+                        make_float4(O[b][nt][4 * q], O[b][nt][4 * q + 1], O[b][nt][4 * q + 2], O[b][nt][4 * q + 3]);
+            }
+        return;
+    }
+    // the rows through LDS, so that they leave in whole lines: 16-byte chunk x of row r at x ^ (r
+    // % 8), where each row goes in `to`
+    constexpr int OB = BF ? 2 : 4, CH = HD * OB / 16;
+    static_assert(NROW * HD * OB + NROW * 8 <= sizeof(kt) + sizeof(vt), "the rows fit");
+    char* const rows = (char*)&kt[0][0];
+    long long* const to = (long long*)(rows + NROW * HD * OB);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+        const int r = 32 * (QB * rg + b) + n;
+        if (ps == 0 && h == 0) to[r] = live[b] ? (long long)(un.tok + tok[b]) * a.H + head[b] : -1;
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            if (nt % PS != ps) continue;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float4 v = make_float4(O[b][nt][4 * q], O[b][nt][4 * q + 1], O[b][nt][4 * q + 2], O[b][nt][4 * q + 3]);
+                const int x = BF ? 4 * nt + q : 8 * nt + 2 * q + h;
+                store_out<BF>(rows + (size_t)r * HD * OB + 16 * (x ^ (r & 7)) + (BF ? 8 * h : 0), 0, v);
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < NROW * CH; i += 512) {
+        const int r = i / CH, x = i % CH;
+        const long long row = to[r];
+        if (row >= 0) {
+            const uint4 v = *(const uint4*)(rows + (size_t)r * HD * OB + 16 * (x ^ (r & 7)));
+            *(u32x4_a8*)((char*)a.out + (size_t)row * HD * OB + 16 * x) = u32x4_a8{v.x, v.y, v.z, v.w};
+        }
+    }
 }
 
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {

@@ -134,7 +134,7 @@ __device__ __forceinline__ bool call_unit(const C& c, int u, int tp, CallUnit& q
     for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
         const int s = s0 + lane;
         const int t0 = c.cu[min(s, c.n_seq)], t1 = c.cu[min(s + 1, c.n_seq)];
-        const int n = s < c.n_seq ? max(t1 - t0, 0) : 0;
+        const int n = s < c.n_seq ? max(t1 - t0, 0) : 0, p0 = c.start[min(s, c.n_seq - 1)];
         const unsigned units = (unsigned)((n + tp - 1) / tp), upto = wave_inclusive_scan(units);
         const unsigned long long below = __ballot(base + (int)upto <= u);
         const int all = base + (int)__builtin_amdgcn_readlane((int)upto, 63);
@@ -145,7 +145,7 @@ __device__ __forceinline__ bool call_unit(const C& c, int u, int tp, CallUnit& q
             q.tok = __builtin_amdgcn_readlane(t0, l) + k * tp;
             q.n = min(tp, __builtin_amdgcn_readlane(n, l) - k * tp);
             q.n = min(q.n, c.N - q.tok);
-            const long long p = (long long)c.start[q.seq] + k * tp;
+            const long long p = (long long)__builtin_amdgcn_readlane(p0, l) + k * tp;
             q.pos = (int)(p < -c.N ? -c.N : p > c.maxT ? c.maxT : p);
             return q.n > 0 && q.tok >= 0;
         }
