@@ -200,80 +200,80 @@ struct PagedWalk {
     }
 };
 
-// A tile as a lane gets it.
-struct PagedRegs {
-    u32x4_t k[8], v[8];
-};
-
+// A tile as a lane gets it: 8 pieces of 16 bytes of K and of V.
 template <bool F32>
-__device__ __forceinline__ void paged_load(const PagedSeq& s, const PagedTile<F32 ? 1 : 2>& x, PagedRegs& r) {
-    constexpr int ROWB = F32 ? 512 : 256;
+__device__ __forceinline__ void paged_load_k(const PagedSeq& s, const PagedTile<F32 ? 1 : 2>& x, u32x4_t (&k)[8]) {
+    constexpr int ROWB = F32 ? 512 : 256, NG = F32 ? 1 : 2;
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     if (!x.live) return;
-    if (F32) {
-        const gptr<const char> k = (gptr<const char>)(s.k + x.at[0]), v = (gptr<const char>)(s.v + x.at[0]);
-        const uint32_t kr = (uint32_t)min(4 * (n & 3) + (n >> 2), x.lim[0]) * ROWB + 16 * g;
 #pragma unroll
-        for (int i = 0; i < 8; i++) r.k[i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(k + kr + 64 * i));
+    for (int h = 0; h < NG; h++) {
+        const gptr<const char> p = (gptr<const char>)(s.k + x.at[h]);
+        const uint32_t r = (uint32_t)min(4 * (n & 3) + (n >> 2), x.lim[h]) * ROWB + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 8 / NG; i++) k[8 / NG * h + i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(p + r + 64 * i));
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void paged_load_v(const PagedSeq& s, const PagedTile<F32 ? 1 : 2>& x, u32x4_t (&v)[8]) {
+    constexpr int ROWB = F32 ? 512 : 256, NG = F32 ? 1 : 2;
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    if (!x.live) return;
+#pragma unroll
+    for (int h = 0; h < NG; h++) {
+        const gptr<const char> p = (gptr<const char>)(s.v + x.at[h]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint32_t vr = (uint32_t)min(4 * i + g, x.lim[0]) * ROWB + 32 * n;
-            r.v[2 * i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + vr));
-            r.v[2 * i + 1] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + vr + 16));
-        }
-    } else {
+            const uint32_t r = (uint32_t)min(4 * i + g, x.lim[h]) * ROWB + ROWB / 16 * n;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const gptr<const char> k = (gptr<const char>)(s.k + x.at[F32 ? 0 : h]), v = (gptr<const char>)(s.v + x.at[F32 ? 0 : h]);
-            const int lim = x.lim[F32 ? 0 : h];
-            const uint32_t kr = (uint32_t)min(4 * (n & 3) + (n >> 2), lim) * ROWB + 16 * g;
-#pragma unroll
-            for (int i = 0; i < 4; i++) r.k[4 * h + i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(k + kr + 64 * i));
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                r.v[4 * h + i] = __builtin_nontemporal_load((gptr<const u32x4_t>)(v + ((uint32_t)min(4 * i + g, lim) * ROWB + 16 * n)));
+            for (int j = 0; j < 2 / NG; j++) v[4 * h + 2 / NG * i + j] = __builtin_nontemporal_load((gptr<const u32x4_t>)(p + r + 16 * j));
         }
     }
 }
 
-// O[j] += V^T's product j times the weights p of the lane's rows.
+// The weights p of the lane's rows as operands.
 template <bool F32, int NP>
-__device__ __forceinline__ void paged_pv(const u32x4_t (&v)[8], const float (&p)[8], f32x4 (&O)[8]) {
-    if (F32) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                O[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[2 * i + j / 4][j % 4]), p[i], O[j], 0, 0, 0);
-    } else {
-        uint32_t w[NP][4];
+struct PagedWeights {
+    uint32_t w[NP][4];
+    __device__ __forceinline__ explicit PagedWeights(const float (&p)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+            if (F32) {
+                w[0][i] = __float_as_uint(p[i]);
+                continue;
+            }
             uint32_t x[NP];
             parts_bf16<NP>(p[2 * i], p[2 * i + 1], x);
 #pragma unroll
             for (int k = 0; k < NP; k++) w[k][i] = x[k];
         }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint32_t a[4];
+    }
+    // o + V^T's product j times the weights; v(e, d): dword d of piece e
+    template <class V>
+    __device__ __forceinline__ f32x4 times(V v, int j, f32x4 o) const {
+        if (F32) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                a[i] = __builtin_amdgcn_perm(v[2 * i + 1][j / 2], v[2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-            const bf16x8 x = as_bf16x8(a[0], a[1], a[2], a[3]);
-#pragma unroll
-            for (int k = NP - 1; k >= 0; k--)
-                O[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(w[k][0], w[k][1], w[k][2], w[k][3]), O[j], 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v(2 * i + j / 4, j % 4)), __uint_as_float(w[0][i]), o, 0, 0, 0);
+            return o;
         }
+        uint32_t a[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(v(2 * i + 1, j / 2), v(2 * i, j / 2), j & 1 ? 0x07060302u : 0x05040100u);
+        const bf16x8 x = as_bf16x8(a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int k = NP - 1; k >= 0; k--)
+            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(w[k][0], w[k][1], w[k][2], w[k][3]), o, 0, 0, 0);
+        return o;
     }
-}
+};
 
 constexpr int PAGED_OW = 132;               // floats between the columns of a wave's outputs in LDS
 
 // The query rows of one unit over tiles t0 .. t_end - 1 of its sequence; the waves joined,
 // and the output, or (several ranges) the partial outputs.
 template <bool F32, bool BF, int W>
-__global__ void __launch_bounds__(64 * W, W >= 8 ? 1 : 2)
+__global__ void __launch_bounds__(64 * W, 2)
 k_paged_attn(PagedArgs c, PagedAttnArgs a) {
     constexpr int HD = 128, NG = F32 ? 1 : 2, TR = 16 * NG, NY = 4 * NG;
     constexpr int NQ = BF ? 1 : 3, NP = BF ? 2 : 3;         // parts of q, of the weights
@@ -295,17 +295,18 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
     const int mine = t_end - t0 > w ? (t_end - t0 - w + W - 1) / W : 0;     // this wave's tiles
     PagedWalk<F32> walk(c, seq.table, mine ? last : -1, t0 + w, W);
     PagedTile<NG> x, xn;
-    PagedRegs cur, nxt;
-    x.live = false;
+    u32x4_t ck[8], cv[8], nk[8], nv[8];
+    x.live = xn.live = false;
     if (mine) {
         walk.tile(0, x);
-        paged_load<F32>(seq, x, cur);
+        paged_load_k<F32>(seq, x, ck);
+        paged_load_v<F32>(seq, x, cv);
     }
 
     // the query columns
-    const size_t qi = (size_t)((un.tok + ct) * a.qts + head * a.qhs);
     float qf[F32 ? 32 : 1];
     bf16x8 qb[F32 ? 1 : NQ][4];
+    const size_t qi = (size_t)((un.tok + ct) * a.qts + head * a.qhs);
     if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -319,34 +320,37 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
         for (int st = 0; st < 4; st++) {
             float y[8];
             load8<BF>(a.q, qi + 32 * st + 8 * g, y);
-            uint32_t b[NQ][4];
+            uint32_t z[NQ][4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t p[NQ];
                 parts_bf16<NQ>(y[2 * e], y[2 * e + 1], p);
 #pragma unroll
-                for (int k = 0; k < NQ; k++) b[k][e] = p[k];
+                for (int k = 0; k < NQ; k++) z[k][e] = p[k];
             }
 #pragma unroll
-            for (int k = 0; k < NQ; k++) qb[k][st] = as_bf16x8(b[k][0], b[k][1], b[k][2], b[k][3]);
+            for (int k = 0; k < NQ; k++) qb[k][st] = as_bf16x8(z[k][0], z[k][1], z[k][2], z[k][3]);
         }
     }
 
     f32x4 O[8];
+    float ref = -INFINITY, l = 0.0f;
+    int seen = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) O[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -INFINITY, l = 0.0f;
-    bool seen = false;
 
     for (int i = 0; i < mine; i++) {
-        if (i + 1 < mine) {
+        const bool more = i + 1 < mine;
+        if (more) {
             walk.tile(i + 1, xn);
-            paged_load<F32>(seq, xn, nxt);
+            paged_load_k<F32>(seq, xn, nk);
+            paged_load_v<F32>(seq, xn, nv);
         }
+        const int row0 = (t0 + w + i * W) * TR;
+        float p[8];
+        bool whole = row0 + TR - 1 <= un.pos;
         if (x.live) {
-            const int row0 = (t0 + w + i * W) * TR;
             // ---- scores
-            float y[8];
 #pragma unroll
             for (int h = 0; h < NG; h++) {
                 f32x4 S = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -354,8 +358,8 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
                     f32x4 S2 = S;
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        S = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[k / 4][k % 4]), qf[k], S, 0, 0, 0);
-                        S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cur.k[k / 4][k % 4 + 1]), qf[k + 1], S2, 0, 0, 0);
+                        S = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ck[k / 4][k % 4]), qf[k], S, 0, 0, 0);
+                        S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ck[k / 4][k % 4 + 1]), qf[k + 1], S2, 0, 0, 0);
                     }
                     S += S2;
                 } else {
@@ -363,27 +367,26 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
                     for (int k = NQ - 1; k >= 0; k--)
 #pragma unroll
                         for (int st = 0; st < 4; st++)
-                            S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, cur.k[4 * h + st]), qb[k][st], S, 0, 0, 0);
+                            S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ck[4 * h + st]), qb[k][st], S, 0, 0, 0);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[4 * h + e] = __fmul_rn(S[e], a.scale2);
+                for (int e = 0; e < 4; e++) p[4 * h + e] = __fmul_rn(S[e], a.scale2);
             }
             // rows that the column does not see: past its own, or without a page
-            bool whole = row0 + TR - 1 <= un.pos;
 #pragma unroll
             for (int h = 0; h < NG; h++) {
                 whole &= x.ok[h];
-                seen |= x.ok[h] && row0 + 16 * h <= crow;
+                seen |= (int)x.ok[h] & (int)(row0 + 16 * h <= crow);
             }
             if (!whole) {
 #pragma unroll
                 for (int e = 0; e < NY; e++)
-                    if (!x.ok[e / 4] || row0 + 16 * (e / 4) + 4 * (e % 4) + g > crow) y[e] = -INFINITY;
+                    if (!x.ok[e / 4] || row0 + 16 * (e / 4) + 4 * (e % 4) + g > crow) p[e] = -INFINITY;
             }
             // ---- the reference: raised to the largest score when one passes it by 2^10
-            float ym = y[0];
+            float ym = p[0];
 #pragma unroll
-            for (int e = 1; e < NY; e++) ym = fmaxf(ym, y[e]);
+            for (int e = 1; e < NY; e++) ym = fmaxf(ym, p[e]);
             if (__any(ym > ref + 10.0f)) {
                 ym = fmaxf(ym, swz_xor16_f(ym));
                 ym = fmaxf(ym, __shfl_xor(ym, 32, JM_WAVE));
@@ -394,18 +397,17 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
                 for (int j = 0; j < 8; j++) O[j] *= f;
                 ref = nref;
             }
-            const float r0 = ref == -INFINITY ? 0.0f : ref;     // (a column that has seen nothing yet)
-            float p[8];
+            const float r0 = ref == -INFINITY ? 0.0f : ref;       // (a column that has seen nothing yet)
 #pragma unroll
             for (int e = 0; e < NY; e++) {
-                p[e] = pow2f(__fsub_rn(y[e], r0));
+                p[e] = pow2f(__fsub_rn(p[e], r0));
                 l = __fadd_rn(l, p[e]);
             }
             // ---- P . V.  A weight of 0 does not hide a value that is not finite: where
             // some column does not see such a row, token by token, each with the rows that
             // it sees.
             bool apart = false;
-            auto row_of = [&](int e) __attribute__((always_inline)) {       // of v[e]; a group without a page holds another's
+            auto row_of = [&](int e) __attribute__((always_inline)) {       // of cv[e]; a group without a page holds another's
                 const int h = F32 ? 0 : e / 4;
                 return x.ok[h] ? row0 + 16 * h + 4 * (F32 ? e / 2 : e % 4) + g : INT_MAX;
             };
@@ -413,42 +415,55 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
                 uint32_t bad = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    uint32_t b = 0;
+                    uint32_t y = 0;
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
-                        b |= (cur.v[e][d] & 0x7F800000u) == 0x7F800000u;
-                        if (!F32) b |= (cur.v[e][d] & 0x7F80u) == 0x7F80u;
+                        y |= (cv[e][d] & 0x7F800000u) == 0x7F800000u;
+                        if (!F32) y |= (cv[e][d] & 0x7F80u) == 0x7F80u;
                     }
-                    bad |= row_of(e) > un.pos ? b : 0u;
+                    bad |= row_of(e) > un.pos ? y : 0u;
                 }
                 apart = __any(bad != 0);
             }
             if (!apart) {
-                paged_pv<F32, NP>(cur.v, p, O);
+                if constexpr (F32) {
+                    // (a row at a time, so that a product never waits for the one before it)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            O[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(cv[2 * i + j / 4][j % 4]), p[i], O[j], 0, 0, 0);
+                } else {
+                    const PagedWeights<F32, NP> pw(p);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) O[j] = pw.times([&](int e, int d) { return cv[e][d]; }, j, O[j]);
+                }
             } else {
 #pragma unroll 1
                 for (int t = 0; t < un.n; t++) {
-                    u32x4_t v[8];
                     float pt[8];
-                    f32x4 T[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        v[e] = row_of(e) <= un.pos + t ? cur.v[e] : u32x4_t{0u, 0u, 0u, 0u};
-                        T[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                        if (e < NY) pt[e] = ct == t ? p[e] : 0.0f;
+                    for (int e = 0; e < NY; e++) pt[e] = ct == t ? p[e] : 0.0f;
+                    const PagedWeights<F32, NP> pw(pt);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const f32x4 T = pw.times([&](int e, int d) { return row_of(e) <= un.pos + t ? cv[e][d] : 0u; }, j,
+                                                 f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int i = 0; i < 4; i++) O[j][i] = ct == t ? O[j][i] + T[i] : O[j][i];
                     }
-                    paged_pv<F32, NP>(v, pt, T);
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (ct == t) O[j] += T[j];
                 }
             }
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            ck[e] = nk[e];
+            cv[e] = nv[e];
+        }
         x = xn;
-        cur = nxt;
     }
 
-    // ---- the wave's outputs: dimensions 32 g + 8 i + j of column n
+    // ---- the wave's outputs: dimensions 32 g + 8 i + j of column 16 b + n
     l += swz_xor16_f(l);
     l += __shfl_xor(l, 32, JM_WAVE);
 #pragma unroll
@@ -499,45 +514,47 @@ k_paged_attn(PagedArgs c, PagedAttnArgs a) {
     }
 }
 
-// The ranges of one (unit, KV head, query row) joined into the output: 8 groups of 32
-// lanes take the ranges in turn, 4 dimensions a lane, and are added in order.
-template <bool BF>
+// The ranges of a (unit, KV head, query row) joined into the output, by 32 lanes, 4
+// dimensions a lane (G = 1), or by 8 groups of them that take the ranges in turn and are
+// added in order (G = 8).
+template <bool BF, int G>
 __global__ void __launch_bounds__(256)
 k_paged_merge(PagedArgs c, PagedAttnArgs a) {
     constexpr int HD = 128;
-    __shared__ __align__(16) float4 acc[8][32];
-    __shared__ float ls[8];
+    __shared__ __align__(16) float4 acc[G][32];
+    __shared__ float ls[G];
     const int nc = a.qpk * a.tp;
-    const int kh = blockIdx.x % c.KH, oc = blockIdx.x / c.KH % nc, u = blockIdx.x / c.KH / nc;
+    const int j = threadIdx.x & 31, gr = G == 1 ? 0 : threadIdx.x >> 5;
+    const int row = G == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    const int oc = row % nc, kh = row / nc % c.KH, u = row / nc / c.KH;
     CallUnit un;
-    if (!call_unit(c, u, a.tp, un)) return;
+    if (u >= a.units || !call_unit(c, u, a.tp, un)) return;
     const int to = oc / a.qpk;
-    if (to >= un.n || un.pos + to >= c.maxT) return;        // (block-uniform)
+    if (to >= un.n || un.pos + to >= c.maxT) return;        // (with G = 8 block-uniform)
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
-    const int j = threadIdx.x & 31, gr = threadIdx.x >> 5;
     float M = -INFINITY;
-    bool any = false;
+    uint32_t any = 0;
     for (int s = j; s < a.S; s += 32) {
         const float2 x = *(const float2*)(a.part_ml + 2 * (p0 + (size_t)s * nc));
         M = fmaxf(M, x.x);
-        any |= x.y != -1.0f;
+        any |= (uint32_t)(x.y != -1.0f);
     }
     M = seg_max<32>(M);
-    any = __any(any);
+    any = (uint32_t)(__ballot(any != 0) >> (threadIdx.x & 32));
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float L = 0.0f;
-    for (int s0 = gr; s0 < a.S; s0 += 32) {
+    for (int s0 = gr; s0 < a.S; s0 += 4 * G) {
         float4 x[4];
         float2 ml[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const size_t p = p0 + (size_t)min(s0 + 8 * q, a.S - 1) * nc;
+            const size_t p = p0 + (size_t)min(s0 + G * q, a.S - 1) * nc;
             ml[q] = *(const float2*)(a.part_ml + 2 * p);
             x[q] = *(const float4*)(a.part_o + p * HD + 4 * j);
         }
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            if (s0 + 8 * q >= a.S || ml[q].y == -1.0f) continue;       // (a range without a row has no output)
+            if (s0 + G * q >= a.S || ml[q].y == -1.0f) continue;       // (a range without a row has no output)
             const float f = pow2f(ml[q].x - M);
             v.x = __builtin_fmaf(x[q].x, f, v.x);
             v.y = __builtin_fmaf(x[q].y, f, v.y);
@@ -546,15 +563,17 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
             L = __builtin_fmaf(ml[q].y, f, L);
         }
     }
-    acc[gr][j] = v;
-    if (j == 0) ls[gr] = L;
-    __syncthreads();
-    if (gr) return;
+    if constexpr (G > 1) {
+        acc[gr][j] = v;
+        if (j == 0) ls[gr] = L;
+        __syncthreads();
+        if (gr) return;
 #pragma unroll
-    for (int i = 1; i < 8; i++) {
-        const float4 y = acc[i][j];
-        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
-        L += ls[i];
+        for (int i = 1; i < G; i++) {
+            const float4 y = acc[i][j];
+            v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+            L += ls[i];
+        }
     }
     const float inv = any ? __fdiv_rn(1.0f, L) : 0.0f;                  // (as in k_paged_attn)
     store_out<BF>(a.out, ((size_t)(un.tok + to) * a.H + kh * a.qpk + oc % a.qpk) * HD + 4 * j,
@@ -590,9 +609,6 @@ __device__ __forceinline__ s16x4 paged_tr16(const uint16_t* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(void*)p);
 }
 
-#ifndef PAGED_AHEAD
-#define PAGED_AHEAD 2
-#endif
 // The phases of k_paged_tile: what must have completed is waited for explicitly, and
 // nothing moves from one to the next.
 __device__ __forceinline__ void paged_meet() {
@@ -607,7 +623,7 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     constexpr int HD = 128, QB = BF ? 2 : 1, NQ = BF ? 1 : 3, PS = 8 / RG, STEP = 32 * PS, TILE = 32 * HD;
     constexpr int RW = 8 * (PS / 2);            // rows of a step that a wave stages, of K and of V
     constexpr int LPS = RW / 2;                 // its loads, 4 rows each
-    constexpr int NROW = 32 * QB * RG, AHEAD = PAGED_AHEAD;
+    constexpr int NROW = 32 * QB * RG, AHEAD = 2;
     constexpr int NS = PS == 2 ? 3 : 2;         // steps in LDS
     // PS tiles of K and of V of NS steps; at the end the outputs being joined
     __shared__ __align__(16) uint16_t kv[2][NS][PS * TILE];
@@ -1093,36 +1109,314 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     }
 }
 
+// The same over float32 pages, in float32 products (v_mfma_f32_16x16x4): block (KV head, unit
+// of 32 query rows, range of the unit's rows), 8 waves = RG = 2 row groups of 16 x PS = 4
+// position strides; a step is 64 rows, of which a wave takes 16.  The products are those of
+// k_paged_attn, but for the dimensions of a lane's V: pieces m and m + 16 of a row.  Chunk x
+// (16 bytes) of row r sits at x ^ (r % 16) in LDS.
+//
+// Bound by the float32 products (32 cycles each, 64 for a wave's 16 rows).  More position
+// strides and fewer row groups win because a step's fixed part (barrier, staging, softmax) is
+// shared by more rows, although each row read from memory serves fewer query rows: two prompts
+// of 1021 tokens behind 260 rows, 16 heads: RG = 2 95 us, RG = 4 120, row groups only (2, 4,
+// 8 waves) 146, 135, 135; k_paged_attn 126.
+template <bool BF>
+__global__ void __launch_bounds__(512, 2)
+k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
+    constexpr int HD = 128, RG = 2, PS = 8 / RG, STEP = 16 * PS, RW = STEP / 8;
+    __shared__ __align__(16) float kv[2][2][STEP * HD];     // [step % 2][K, V][row][dimension]
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = w % RG, ps = w / RG, g = lane >> 4, n = lane & 15;
+    const int kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH;
+    const int u = a.units - 1 - rs % a.units, sr = rs / a.units;        // the longest prefixes first
+    CallUnit un;
+    if (!call_unit(c, u, a.tp, un)) return;
+    const PagedSeq seq(c, un.seq, kh);
+    const int pmax = min(un.pos + un.n - 1, c.maxT - 1);
+    const int steps = pmax < 0 ? 0 : pmax / STEP + 1;
+    const int step0 = (int)((long long)steps * sr / a.S), nstep = (int)((long long)steps * (sr + 1) / a.S) - step0;
+    // this lane's query row, and the last cache row that it sees; of the wave's, the first
+    // token and how many there are
+    const int r = 16 * rg + n, ct = min(r / a.qpk, un.n - 1), head = kh * a.qpk + r % a.qpk;
+    const int crow = min(un.pos + ct, c.maxT - 1);
+    const bool live = r / a.qpk < un.n && un.pos + ct < c.maxT;
+    const int wt0 = min(16 * rg / a.qpk, un.n - 1), wt1 = min((16 * rg + 15) / a.qpk, un.n - 1), wmin = min(un.pos + wt0, c.maxT - 1);
+
+    // ---- staging: wave w has rows RW w .. of each step, 2 rows a load.  Lane PS i + g of `page`
+    // has the page of 16-row group g in the i-th of 64 / PS steps.
+    auto fetch = [&](int batch) __attribute__((always_inline)) {
+        const long long row = (long long)(step0 + 64 / PS * batch) * STEP + 16 * lane;
+        const int p = row <= pmax ? seq.table[row >> c.lp] : -1;
+        return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+    };
+    int page = fetch(0), next = fetch(1);
+    bool has = false, had = false;              // whether this wave's group of the step staged last, and before, has a page
+    auto stage = [&](int t, int slot) __attribute__((always_inline)) {
+        const int i0 = t % (64 / PS) * PS;
+        if (t && i0 == 0) {
+            page = next;
+            next = fetch(t / (64 / PS) + 1);
+        }
+        had = has;
+        has = __builtin_amdgcn_readlane(page, i0 + ps) >= 0;
+        const int p = __builtin_amdgcn_readlane(page, i0 + RW * w / 16), row = (step0 + t) * STEP + RW * w, lim = pmax - row;
+        const size_t at = (size_t)max(p, 0) * c.page_stride + (uint32_t)((row & ((1 << c.lp) - 1)) * 512);
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            float* const to = kv[slot][v] + RW * w * HD;
+            if (p >= 0 && lim >= 0) {
+                uint32_t num = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
+                __asm__ volatile("" : "+s"(num));           // (as in k_paged_tile)
+                const auto dst = (__attribute__((address_space(3))) float*)(uintptr_t)num;
+                const auto base = __builtin_amdgcn_make_buffer_rsrc((void*)((v ? seq.v : seq.k) + at), 0, RW * 512, 0x00020000);
+#pragma unroll
+                for (int j = 0; j < RW / 2; j++) {
+                    const int i = 2 * j + (lane >> 5);      // (rows past the prefixes repeat the last one)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)(dst + 2 * j * HD), 16,
+                                                             min(i, lim) * 512 + 16 * ((lane & 31) ^ ((RW * w + i) & 15)), 0, 0, 0);
+                }
+            } else if (v) {
+#pragma unroll
+                for (int j = 0; j < RW / 2; j++) *(float4*)(to + 2 * j * HD + 4 * lane) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+    };
+
+    float qf[32];
+    const size_t qi = (size_t)((un.tok + ct) * a.qts + head * a.qhs);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float y[4];
+        load4<BF>(a.q, qi + 16 * i + 4 * g, y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) qf[4 * i + e] = y[e];
+    }
+    if (nstep > 0) stage(0, 0);
+
+    f32x4 O[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) O[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = -INFINITY, l = 0.0f;
+    int seen = 0;
+#pragma unroll 1
+    for (int t = 0; t < nstep; t++) {
+        // this wave's rows of the step have arrived and its reads of the step before are done,
+        // then everyone's
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        wave_meet();
+        if (t + 1 < nstep) stage(t + 1, (t + 1) & 1);
+        const int row0 = (step0 + t) * STEP + 16 * ps;
+        if ((t + 1 < nstep ? had : has) && row0 <= min(un.pos + wt1, c.maxT - 1)) {            // (wave-uniform)
+            const float* const kt = kv[t & 1][0] + 16 * ps * HD;
+            const float* const vt = kv[t & 1][1] + 16 * ps * HD;
+            // ---- scores (lane (g, n): query row n at rows 4 i + g)
+            f32x4 S = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, S2 = S;
+            int kr = 4 * (n & 3) + (n >> 2), gg = g;
+            __asm__ volatile("" : "+v"(kr), "+v"(gg));      // (the addresses anew each time: kept, others spill)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float4 x = *(const float4*)(kt + kr * HD + 4 * ((4 * i + gg) ^ kr));
+                S = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, qf[4 * i], S, 0, 0, 0);
+                S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, qf[4 * i + 1], S2, 0, 0, 0);
+                S = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, qf[4 * i + 2], S, 0, 0, 0);
+                S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, qf[4 * i + 3], S2, 0, 0, 0);
+            }
+            float p[4];
+            const bool whole = row0 + 15 <= wmin;
+            seen |= (int)(row0 <= crow);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[e] = __fmul_rn(S[e] + S2[e], a.scale2);
+                if (!whole && row0 + 4 * e + g > crow) p[e] = -INFINITY;
+            }
+            // ---- the reference and the weights, as in k_paged_attn
+            float m = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+            if (__any(m > ref + 10.0f)) {
+                m = fmaxf(m, swz_xor16_f(m));
+                m = fmaxf(m, __shfl_xor(m, 32, JM_WAVE));
+                const float nref = fmaxf(ref, m);
+                const float f = nref == -INFINITY ? 1.0f : pow2f(ref - nref);
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) O[j] *= f;
+                ref = nref;
+            }
+            const float r0 = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[e] = pow2f(__fsub_rn(p[e], r0));
+                l = __fadd_rn(l, p[e]);
+            }
+            // ---- P . V; token by token where some query row of the wave does not see a row
+            // whose V is not finite
+            uint32_t bad = 0;
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int vr = 4 * i + g;
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        const uint4 x = *(const uint4*)(vt + vr * HD + 4 * ((n + 16 * d) ^ vr));
+                        const uint32_t y = (uint32_t)((x.x & 0x7F800000u) == 0x7F800000u) | (uint32_t)((x.y & 0x7F800000u) == 0x7F800000u) |
+                                           (uint32_t)((x.z & 0x7F800000u) == 0x7F800000u) | (uint32_t)((x.w & 0x7F800000u) == 0x7F800000u);
+                        bad |= row0 + vr > wmin ? y : 0u;
+                    }
+                }
+            }
+            if (!__any(bad != 0)) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int vr = 4 * i + g;
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        const float4 x = *(const float4*)(vt + vr * HD + 4 * ((n + 16 * d) ^ vr));
+                        O[4 * d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, p[i], O[4 * d], 0, 0, 0);
+                        O[4 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, p[i], O[4 * d + 1], 0, 0, 0);
+                        O[4 * d + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, p[i], O[4 * d + 2], 0, 0, 0);
+                        O[4 * d + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, p[i], O[4 * d + 3], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int tt = wt0; tt <= wt1; tt++) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        f32x4 T = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int vr = 4 * i + g;
+                            const float x = row0 + vr <= un.pos + tt ? vt[vr * HD + 4 * ((n + 16 * (j / 4)) ^ vr) + j % 4] : 0.0f;
+                            T = __builtin_amdgcn_mfma_f32_16x16x4f32(x, ct == tt ? p[i] : 0.0f, T, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) O[j][i] = ct == tt ? O[j][i] + T[i] : O[j][i];
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- the PS waves of each row group joined by the first of them
+    l += swz_xor16_f(l);
+    l += __shfl_xor(l, 32, JM_WAVE);
+    __shared__ float mls[8][16][2];
+    float4* const ow = (float4*)&kv[0][0][0] + lane;        // [wave, those of ps = 0 left out][8][64 lanes]
+    static_assert((8 - RG) * 8 * 64 * 16 <= sizeof(kv), "the outputs of the others fit");
+    __syncthreads();
+    if (g == 0) {
+        mls[w][n][0] = ref;
+        mls[w][n][1] = seen ? l : -1.0f;
+    }
+    if (ps) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) ow[((w - RG) * 8 + j) * 64] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
+    }
+    __syncthreads();
+    if (ps || !live) return;
+    float M = -INFINITY, L = 0.0f;
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < PS; q++) M = fmaxf(M, mls[q * RG + rg][n][0]);
+    const float f0 = seen ? pow2f(ref - M) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) O[j] *= f0;
+#pragma unroll
+    for (int q = 0; q < PS; q++) {
+        const float lq = mls[q * RG + rg][n][1];
+        if (lq == -1.0f) continue;
+        any = true;
+        const float f = pow2f(mls[q * RG + rg][n][0] - M);
+        L = __builtin_fmaf(lq, f, L);
+        if (q == 0) continue;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float4 x = ow[((q * RG + rg - RG) * 8 + j) * 64];
+            O[j] += f32x4{x.x, x.y, x.z, x.w} * f;
+        }
+    }
+    // dimensions 64 d + 16 g + 4 i + e (register i of product 4 d + e) of the lane's query row
+    const float inv = a.S > 1 ? 1.0f : any ? __fdiv_rn(1.0f, L) : 0.0f;         // (as in k_paged_attn)
+    const size_t row = ((size_t)(u * c.KH + kh) * a.S + sr) * (a.qpk * a.tp) + r;
+    if (a.S > 1 && g == 0) *(float2*)(a.part_ml + 2 * row) = make_float2(M, any ? L : -1.0f);
+    const size_t oi = ((size_t)(un.tok + ct) * a.H + head) * HD;
+#pragma unroll
+    for (int d = 0; d < 2; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 v = make_float4(O[4 * d][i] * inv, O[4 * d + 1][i] * inv, O[4 * d + 2][i] * inv, O[4 * d + 3][i] * inv);
+            const int dim = 64 * d + 16 * g + 4 * i;
+            if (a.S > 1) *(float4*)(a.part_o + row * HD + dim) = v;
+            else store_out<BF>(a.out, oi + dim, v);
+        }
+}
+
+// How a call is cut, by sizes and types alone.  Times are of 32 query heads on 8 KV heads,
+// "T tokens behind R rows, B sequences" (us).
+//
+// Which kernel: a block of k_paged_attn has 16 query rows, so that the cache is multiplied
+// once for each 16, but is done in 8 us; k_paged_tile takes 15 us to begin and end.  The
+// blocks times their rows (512 at least) decide.  bf16 pages, k_paged_attn / k_paged_tile:
+// 64 tokens behind 2000 rows (264 k) 28 / 28, 400 behind none (410 k) 20 / 23, 32 behind
+// 2000, 4 sequences (520 k) 41 / 31, 600 behind none (614 k) 28 / 26, 16 behind 2000, 16
+// sequences (1 M) 77 / 48.  float32 pages, k_paged_attn / k_paged_tile_f32: 16 behind 2000
+// (64 k) 20 / 23, 32 behind 2000 (130 k) 28 / 24, 8 behind 2000, 4 sequences (128 k) 49 /
+// 27, 16 sequences of 16 (1 M) 181 / 120.
+//
+// Units of k_paged_tile: RG 4 (twice the query rows a block, 64 cache rows a step) against
+// RG 2 (128 cache rows a step), by what each takes: a step 1.7 us, a block's beginning and
+// end 6 steps, joined ranges 6 more, 256 blocks at once, the longest prefix bounding all.  RG
+// 2 reads the cache twice as often: it has to be a tenth below.  RG 4 / RG 2: 777 tokens behind
+// none 45 / 31, 800 behind 2000 70 / 56, 2047 behind none 72 / 65, 2047 behind 4099 194 /
+// 197, 4 sequences of 300 behind 500 40 / 54, of 700 84 / 91, 5 of 1201 (28 heads on 4) 80 / 92.
+//
+// Ranges: joining costs a launch and the partial outputs.  k_paged_attn, one token: 500
+// rows 8.9 (one range) / 11.5 (four), 1000 rows 13.2 / 11.4, 1000 rows of 32 sequences
+// 23 / 27; of float32 pages 300 rows 16.6 / 12.3.  The tiles, 512 rows a range against 256:
+// 200 tokens behind 1000 rows 34 / 35; of float32 pages 32 behind 2000 35 / 26.
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     PagedPlan p{};
     const int qpk = H / c.KH;
     rows = std::min(rows, c.maxT);
-    long long blocks;
+    const long long qrows = (long long)c.N * qpk, each = c.cu && c.n_seq ? ((long long)c.N + c.n_seq - 1) / c.n_seq : 1;
+    long long likely = 0;
+    // units of tp tokens: every sequence's tokens are rounded up to whole ones; `likely`
+    // blocks where the sequences have about as many each
     auto cut = [&](int tp) {
         p.tp = tp;
-        // (every sequence's tokens are rounded up to whole units)
         p.units = c.cu ? (int)std::min<long long>(c.N, ((long long)c.N + (long long)c.n_seq * (tp - 1)) / tp) : c.N;
-        blocks = (long long)p.units * c.KH;
+        likely = std::min<long long>(p.units, c.n_seq * ((each + tp - 1) / tp)) * c.KH;
     };
-    // up to `want` blocks while each has `least` rows
+    // ranges for up to `want` blocks while each has `least` rows
     auto ranges = [&](long long want, int least) {
-        return std::min((want + blocks - 1) / blocks, ((long long)rows + least - 1) / least);
+        return (int)std::max(std::min((want + likely - 1) / likely, ((long long)rows + least - 1) / least), 1ll);
     };
-    const long long qrows = (long long)c.N * qpk;
-    if (!c.f32 && c.cu && qrows >= 64ll * c.n_seq) {
-        const int unit = bf ? 256 : 128;
-        p.rg = 4;
-        cut(unit / qpk);
-        if (qrows < (long long)unit * c.n_seq || (blocks < 256 && blocks * rows < 160000)) {
-            p.rg = 2;
-            cut(unit / 2 / qpk);
+    // the same for one round of 256 blocks (a tile's block fills a CU)
+    auto parts = [&](int least) {
+        return (int)std::max(std::min(256 / likely, ((long long)rows + least - 1) / least), 1ll);
+    };
+    cut(c.cu ? 16 / qpk : 1);
+    if (likely == 0) return p;
+    if (c.cu && qrows >= 32ll * c.n_seq && likely * std::max(rows, 512) >= (c.f32 ? 100000 : 450000)) {
+        if (c.f32) {
+            p.rg = 1;
+            cut(32 / qpk);
+        } else {
+            auto steps = [&](int rg) {
+                cut((bf ? 64 : 32) * rg / qpk);
+                const int step = 256 / rg;
+                const long long S = parts(512), most = rows / step / S + 6, mean = std::max(rows - each / 2, 0ll) / step / S + 6;
+                return std::max(most, (likely * S + 255) / 256 * mean) + (S > 1 ? 6 : 0);
+            };
+            p.rg = 10 * steps(2) < 9 * steps(4) ? 2 : 4;
+            cut((bf ? 64 : 32) * p.rg / qpk);
         }
-        p.S = (int)std::max(std::min(256 / blocks, ((long long)rows + 255) / 256), 1ll);
+        p.S = parts(c.f32 ? 256 : 512);
+    } else if (rows <= (c.f32 ? 256 : 512)) {
+        p.S = 1;
     } else {
-        cut(c.cu ? 16 / qpk : 1);
-        p.S = rows <= 1024 ? 1 : (int)std::max(std::max(ranges(256, 128), ranges(1024, 512)), 1ll);
+        p.S = std::max(ranges(256, 128), rows <= 1024 ? 1 : ranges(1024, 512));
     }
-    const size_t cols = (size_t)blocks * p.S * qpk * p.tp;
+    const size_t cols = (size_t)p.units * c.KH * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;
     p.ml_floats = p.S > 1 ? cols * 2 : 0;
     return p;
@@ -1136,7 +1430,10 @@ hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void*
     a.scale2 = scale * 1.4426950408889634f;
     a.out = out; a.units = p.units; a.S = p.S; a.part_o = part_o; a.part_ml = part_ml;
     const dim3 grid((unsigned)c.KH * p.units * p.S);
-    if (p.rg) {
+    if (p.rg == 1) {
+        if (bf) hipLaunchKernelGGL(k_paged_tile_f32<true>, grid, dim3(512), 0, st, c, a);
+        else hipLaunchKernelGGL(k_paged_tile_f32<false>, grid, dim3(512), 0, st, c, a);
+    } else if (p.rg) {
 #define JM_PAGED_TILE(BFV, RGV) \
         if (bf == BFV && p.rg == RGV) hipLaunchKernelGGL((k_paged_tile<BFV, RGV>), grid, dim3(512), 0, st, c, a)
         JM_PAGED_TILE(false, 2); else JM_PAGED_TILE(false, 4); else JM_PAGED_TILE(true, 2); else JM_PAGED_TILE(true, 4);
@@ -1149,9 +1446,15 @@ hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void*
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.S == 1) return e;
-    const dim3 mg((unsigned)c.KH * p.units * (unsigned)(a.qpk * a.tp));
-    if (bf) hipLaunchKernelGGL(k_paged_merge<true>, mg, dim3(256), 0, st, c, a);
-    else hipLaunchKernelGGL(k_paged_merge<false>, mg, dim3(256), 0, st, c, a);
+    const unsigned outs = (unsigned)c.KH * p.units * (unsigned)(a.qpk * a.tp);
+    // (few ranges: more groups a row only leave lanes without work; 32 tokens behind 2000 rows,
+    // 16 sequences in 2 ranges 53 us against 78.  Many: 64 ranges of one token 12.8 against 17.)
+    const bool apart = p.S < 16;
+    const dim3 mg(apart ? (outs + 7) / 8 : outs);
+#define JM_PAGED_MERGE(BFV, GV) hipLaunchKernelGGL((k_paged_merge<BFV, GV>), mg, dim3(256), 0, st, c, a)
+    if (bf) { if (apart) JM_PAGED_MERGE(true, 1); else JM_PAGED_MERGE(true, 8); }
+    else { if (apart) JM_PAGED_MERGE(false, 1); else JM_PAGED_MERGE(false, 8); }
+#undef JM_PAGED_MERGE
     return hipGetLastError();
 }
 

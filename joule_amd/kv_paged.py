@@ -167,11 +167,12 @@ class PagedKVCacheSet:
             raise ValueError(f"{name} must be contiguous")
         return t
 
-    def _vector(self, t, name: str, dtype, shape: tuple) -> None:
-        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self._device
-                              or t.dim() != len(shape) or any(a < b for a, b in zip(t.shape, shape)) or t.shape[-1] != HD
-                              or not t.is_contiguous() or t.data_ptr() % 16):
-            raise ValueError(f"{name} must be a contiguous 16-byte aligned {dtype} tensor {list(shape)} on {self._device}")
+    def _vector(self, t, name: str, dtype, rows: int) -> None:
+        """t is [rows or more, 128], or [128] where rows is 0."""
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self._device or t.dim() != (2 if rows else 1) \
+                or t.shape[-1] != HD or (rows and t.shape[0] < rows) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be a contiguous 16-byte aligned {dtype} tensor "
+                             f"{[rows, HD] if rows else [HD]} on {self._device}")
 
     # ------------------------------------------------------------ operators
 
@@ -206,10 +207,13 @@ class PagedKVCacheSet:
             raise ValueError("q_out and q_norm need q")
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin come together")
-        self._vector(cos, "cos", torch.float32, (self.shape.maxT, HD))
-        self._vector(sin, "sin", torch.float32, (self.shape.maxT, HD))
-        self._vector(q_norm, "q_norm", torch.bfloat16, (HD,))
-        self._vector(k_norm, "k_norm", torch.bfloat16, (HD,))
+        if cos is not None:
+            self._vector(cos, "cos", torch.float32, self.shape.maxT)
+            self._vector(sin, "sin", torch.float32, self.shape.maxT)
+        if q_norm is not None:
+            self._vector(q_norm, "q_norm", torch.bfloat16, 0)
+        if k_norm is not None:
+            self._vector(k_norm, "k_norm", torch.bfloat16, 0)
         with _lib.on(self._device, stream):
             if q is not None:
                 q_out = self._out(q_out, "q_out", (n, H, HD), q.dtype)
@@ -218,7 +222,8 @@ class PagedKVCacheSet:
                                None if q is None else q_out.data_ptr(), None if cos is None else cos.data_ptr(),
                                None if sin is None else sin.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
                                None if k_norm is None else k_norm.data_ptr(), float(eps))
-            _lib.check(_lib.lib().jm_kv_paged_append(self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, ctypes.byref(rows),
+            _lib.check(_lib.lib().jm_kv_paged_append(self._layer(l), start.data_ptr(), None if cu is None else cu.data_ptr(), n,
+                                                     ctypes.byref(rows),
                                                      _lib.stream_handle()), "jm_kv_paged_append")
         return q_out
 
@@ -244,7 +249,7 @@ class PagedKVCacheSet:
         with _lib.on(self._device, stream):
             out = self._out(out, "out", (n, H, HD), q.dtype)
             _lib.check(_lib.lib().jm_kv_paged_attn(
-                self._layer(l), _lib.ptr(start), _lib.ptr(cu), n, _lib.ptr(q), *q.stride()[:2], H,
-                HD ** -0.5 if scale is None else float(scale), min(max_rows, self.shape.maxT), _DTYPES[q.dtype], _lib.ptr(out),
+                self._layer(l), start.data_ptr(), None if cu is None else cu.data_ptr(), n, q.data_ptr(), *q.stride()[:2], H,
+                HD ** -0.5 if scale is None else float(scale), min(max_rows, self.shape.maxT), _DTYPES[q.dtype], out.data_ptr(),
                 _lib.stream_handle()), "jm_kv_paged_attn")
         return out

@@ -21,14 +21,18 @@ def ints(v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 
 
-def cache(B, maxT, KH, page=16, dtype="bf16", layers=1, extra=3, seed=0):
-    """Caches of NaN, every sequence's pages anywhere in the pool."""
+DEEP = 2 ** 19          # a maxT whose calls are cut as if the prefixes were as long
+
+
+def cache(B, maxT, KH, page=16, dtype="bf16", layers=1, extra=3, seed=0, rows=None):
+    """Caches of NaN, every sequence's pages (for maxT rows, or for `rows`) anywhere in
+    the pool."""
     shape = DecoderShape(n_layers=layers, moe=dense_ffn_shape(1024, 512), n_heads=KH, n_kv=KH, maxT=maxT)
-    width = -(-maxT // page)
+    width = -(-(rows or maxT) // page)
     c = PagedKVCacheSet(shape, B, B * width + extra, page=page, dtype=DT[dtype])
     c.data.fill_(float("nan"))
     order = np.random.default_rng(seed).permutation(B * width + extra)[:B * width]
-    c.table.copy_(ints(order.reshape(B, width).tolist()))
+    c.table[:, :width] = ints(order.reshape(B, width).tolist())
     return c
 
 
@@ -70,10 +74,13 @@ def queries(seed, k, start, n, H):
     return q
 
 
-def form_of(c, dt, n, H, KH, n_seq):
-    """As the entry point decides: prompts over bf16 pages from 64 query rows a KV head
-    and sequence."""
-    return "f32" if dt == "f32" else "bf16 prompt" if c.data.dtype == torch.bfloat16 and n * (H // KH) >= 64 * n_seq else "bf16"
+def form_of(c, dt, n, H, KH, n_seq, max_rows=0):
+    """As the entry point decides for a call with cu: a prompt where a sequence has 32 query
+    rows a KV head, and the rows (512 at least) that the units of 16 query rows pass over
+    are 450000."""
+    units = min(n_seq * -(-(-(-n // n_seq)) // (16 * KH // H)), n)
+    prompt = n * (H // KH) >= 32 * n_seq and units * KH * max(min(max_rows or c.shape.maxT, c.shape.maxT), 512) >= 450000
+    return "f32" if dt == "f32" else "bf16 prompt" if c.data.dtype == torch.bfloat16 and prompt else "bf16"
 
 
 def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=None, one=False):
@@ -87,6 +94,7 @@ def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=
     torch.cuda.synchronize()
     g64, q64 = got.double().cpu().numpy(), qd.float().cpu().numpy()
     table = c.table.cpu().numpy()
+    form = "bf16" if one and dt == "bf16" else form_of(c, dt, len(q), H, KH, len(counts), max_rows)
     for b, (s, n) in enumerate(zip(start, counts)):
         T = s + n
         if n == 0 or T <= 0:
@@ -102,7 +110,7 @@ def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=
         pick = pick[s + pick < c.shape.maxT]
         see = paged & (t <= s + pick[:, None])
         for h in range(H):
-            want, tol = attend(q64[cu[b] + pick, h], k[:, h * KH // H], v[:, h * KH // H], see, scale, form_of(c, dt, len(q), H, KH, len(counts)))
+            want, tol = attend(q64[cu[b] + pick, h], k[:, h * KH // H], v[:, h * KH // H], see, scale, form)
             off = np.abs(g64[cu[b] + pick, h] - want)
             worst = np.nanmax(off / np.maximum(tol, 1e-300))
             assert (off <= tol).all(), f"sequence {b} head {h}: {worst:.3g} bounds off, by {np.nanmax(off):.3g}"
@@ -110,7 +118,8 @@ def check(c, q, start, counts, dt, scale=HD ** -0.5, out=None, max_rows=0, only=
 
 
 def run(H, KH, counts, start, dt, cached, page=16, maxT=None, **kw):
-    c = cache(len(counts), maxT or max(s + n for s, n in zip(start, counts)), KH, page, cached)
+    T = max(s + n for s, n in zip(start, counts))
+    c = cache(len(counts), maxT or T, KH, page, cached, rows=max(T, 1) if maxT == DEEP else None)
     q = []
     for b, (s, n) in enumerate(zip(start, counts)):
         k, v = rows(7 * b + 1, max(s + n, 1), KH)
@@ -219,6 +228,16 @@ def test_few_tokens(H, KH, counts, start, dt, cached):
 def test_prompts(H, KH, counts, start, page, dt, cached):
     run(H, KH, counts, start, dt, cached, page, maxT=4000)
     run(H, KH, counts, start, dt, cached, page)
+    run(H, KH, counts, start, dt, cached, page, maxT=DEEP)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start,page", [(64, 64, [260], [100], 32), (128, 128, [260], [77], 16), (128, 32, [130], [400], 16),
+                                                    (112, 16, [70, 140], [0, 250], 64), (40, 40, [90, 33, 99, 1], [200, 31, 0, 409], 16)])
+def test_prompts_of_many_heads(H, KH, counts, start, page, dt, cached):
+    """In one range of rows, without a kernel that joins them."""
+    run(H, KH, counts, start, dt, cached, page, maxT=600)
+    run(H, KH, counts, start, dt, cached, page)
 
 
 @pytest.mark.parametrize("dt,cached", TYPES)
@@ -236,7 +255,7 @@ CALLS = [(4, 2, [1], [40]), (8, 1, [2], [500]), (4, 2, [5, 0, 3], [40, 9, 700]),
 
 
 def prepared(H, KH, counts, start, cached, maxT, page=16, seed=0):
-    c = cache(len(counts), maxT, KH, page, cached, seed=seed)
+    c = cache(len(counts), maxT, KH, page, cached, seed=seed, rows=1500 if maxT == DEEP else None)
     q = []
     for b, (s, n) in enumerate(zip(start, counts)):
         k, v = rows(7 * b + 1, max(s + n, 1), KH)
@@ -248,7 +267,7 @@ def prepared(H, KH, counts, start, cached, maxT, page=16, seed=0):
 
 @pytest.mark.parametrize("dt,cached", TYPES)
 @pytest.mark.parametrize("H,KH,counts,start", CALLS)
-@pytest.mark.parametrize("maxT", [0, 1500])
+@pytest.mark.parametrize("maxT", [0, 1500, DEEP])
 def test_rows_of_later_tokens_may_hold_anything(H, KH, counts, start, maxT, dt, cached):
     """NaN and infinities in K and V of a token's row do not reach the tokens before
     it; the tokens from it on get what the formula gives."""
@@ -282,11 +301,12 @@ def test_rows_of_later_tokens_may_hold_anything(H, KH, counts, start, maxT, dt, 
 
 @pytest.mark.parametrize("dt,cached", TYPES)
 @pytest.mark.parametrize("H,KH,counts,start", CALLS)
-def test_pages_that_are_not_there(H, KH, counts, start, dt, cached):
+@pytest.mark.parametrize("maxT", [1500, DEEP])
+def test_pages_that_are_not_there(H, KH, counts, start, maxT, dt, cached):
     """Rows of pages given back, of numbers outside the pool and of pages still to
     come are not seen; a token that sees none gets 0."""
     for gone in ([0], [1, 2], [3], [0, 1, 2, 3, 4, 5], list(range(400))):
-        c, q = prepared(H, KH, counts, start, cached, 1500)
+        c, q = prepared(H, KH, counts, start, cached, maxT)
         for b in range(c.B):
             for i, p in enumerate(gone):
                 if p < c.table.shape[1]:
@@ -298,7 +318,8 @@ def test_pages_that_are_not_there(H, KH, counts, start, dt, cached):
 
 
 @pytest.mark.parametrize("dt,cached", TYPES)
-@pytest.mark.parametrize("H,KH,counts,start", [(4, 2, [1, 1], [-1, 20]), (4, 2, [3, 5], [-2, -9]), (4, 2, [100, 130], [-40, 900]), (4, 2, [70, 70], [-200, 960])])
+@pytest.mark.parametrize("H,KH,counts,start", [(4, 2, [1, 1], [-1, 20]), (4, 2, [3, 5], [-2, -9]), (4, 2, [100, 130], [-40, 900]), (4, 2, [70, 70], [-200, 960]),
+                                               (64, 64, [300, 70], [-200, 960])])
 def test_tokens_without_rows_and_rows_outside(H, KH, counts, start, dt, cached):
     """A row below 0: 0.  A row past the cache, and tokens behind the last sequence:
     left as they were."""
@@ -326,12 +347,14 @@ def test_tokens_without_rows_and_rows_outside(H, KH, counts, start, dt, cached):
 def test_scales_of_any_sign_and_zero(dt, cached, scale):
     for H, KH, counts, start in CALLS:
         run(H, KH, counts, start, dt, cached, scale=scale)
+        run(H, KH, counts, start, dt, cached, scale=scale, maxT=DEEP)
 
 
 @pytest.mark.parametrize("dt,cached", TYPES)
 @pytest.mark.parametrize("H,KH,counts,start", CALLS)
-def test_an_infinite_query_gives_nan(H, KH, counts, start, dt, cached):
-    c, q = prepared(H, KH, counts, start, cached, 1500)
+@pytest.mark.parametrize("maxT", [1500, DEEP])
+def test_an_infinite_query_gives_nan(H, KH, counts, start, maxT, dt, cached):
+    c, q = prepared(H, KH, counts, start, cached, maxT)
     q[:, 1, 77] = np.inf
     q[0, 0, 5] = -np.inf
     cu = np.concatenate([[0], np.cumsum(counts)])
@@ -344,8 +367,9 @@ def test_an_infinite_query_gives_nan(H, KH, counts, start, dt, cached):
 
 @pytest.mark.parametrize("dt,cached", TYPES)
 @pytest.mark.parametrize("H,KH,counts,start", CALLS)
-def test_weights_far_apart(H, KH, counts, start, dt, cached):
+@pytest.mark.parametrize("maxT", [1500, DEEP])
+def test_weights_far_apart(H, KH, counts, start, maxT, dt, cached):
     """Scores of hundreds: one row has all the weight, the reference rises often."""
-    c, q = prepared(H, KH, counts, start, cached, 1500)
+    c, q = prepared(H, KH, counts, start, cached, maxT)
     check(c, q * 30.0, start, counts, dt)
     check(c, q * 1e-4, start, counts, dt)
