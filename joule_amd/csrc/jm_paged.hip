@@ -15,64 +15,87 @@ namespace jm {
 // ---------------------------------------------------------------- new rows
 
 // 16 lanes a head, 8 dimensions a lane (dimension d and its partner d + 64 lie 8 lanes
-// apart), 16 heads of one token a block: q heads, then k heads, then v heads.
-template <bool BF>
+// apart); a block takes 16 NH heads of one token, NH a group of lanes: q heads, then k heads,
+// then v heads.
+//
+// Bound by what it reads and writes, if the rotation's factors (1 KB of float32 a token, of
+// which a head wants all) are not loaded anew for each head of 256 bytes, and if the heads are
+// on their way before the token's place is known: 13374 bf16 tokens of 48 heads 65 us, 5 TB/s
+// (NH = 3); NH = 1 76 (and 93 with the place first), NH = 2 78, NH = 4 66.  Few tokens wait
+// for each load in turn: 8 of 40 heads 2.9 us (NH = 1) / 3.9 (NH = 3), 1805 of 48 8.1 / 7.8.
+template <bool BF, int NH>
 __global__ void __launch_bounds__(256)
 k_paged_append(PagedArgs c, PagedRows r, int chunks) {
     constexpr int HD = 128;
-    const int t = blockIdx.x / chunks, hr = blockIdx.x % chunks * 16 + (threadIdx.x >> 4);
+    const int t = blockIdx.x / chunks, h0 = blockIdx.x % chunks * 16 * NH + (threadIdx.x >> 4), heads = r.H + 2 * c.KH;
     const int j = threadIdx.x & 15;
+    float x[NH][8];
+    int what[NH], head[NH];
+#pragma unroll
+    for (int i = 0; i < NH; i++) {
+        const int hr = h0 + 16 * i;
+        what[i] = hr < r.H ? 0 : hr < r.H + c.KH ? 1 : hr < heads ? 2 : 3;
+        head[i] = what[i] == 0 ? hr : what[i] == 1 ? hr - r.H : hr - r.H - c.KH;
+        const int w = what[i];
+        if (w < 3) load8<BF>(w == 0 ? r.x[0] : w == 1 ? r.x[1] : r.x[2],
+                             (size_t)(t * (w == 0 ? r.ts[0] : w == 1 ? r.ts[1] : r.ts[2]) + head[i] * (w == 0 ? r.hs[0] : w == 1 ? r.hs[1] : r.hs[2])) + 8 * j, x[i]);
+    }
     int seq, pos;
     if (!call_place(c, t, seq, pos)) return;                // (block-uniform)
-    if (hr >= r.H + 2 * c.KH) return;                       // (whole rows of 16 lanes)
-    const int what = hr < r.H ? 0 : hr < r.H + c.KH ? 1 : 2;
-    const int head = what == 0 ? hr : what == 1 ? hr - r.H : hr - r.H - c.KH;
-    float x[8];
-    load8<BF>(r.x[what], (size_t)(t * r.ts[what] + head * r.hs[what]) + 8 * j, x);
-    const uint16_t* w = what < 2 ? r.w[what] : nullptr;
-    if (w) {
-        const uint4 u = *(const uint4*)(w + 8 * j);
-        const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
-        ss = seg_sum<16>(ss);
-        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(ss * (1.0f / HD), r.eps)));
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[2 * e] = x[2 * e] * inv * __uint_as_float(ww[e] << 16);
-            x[2 * e + 1] = x[2 * e + 1] * inv * __uint_as_float(ww[e] & 0xFFFF0000u);
-        }
-    }
-    if (r.cos && what < 2) {
+    const int page = c.table[seq * c.table_stride + (pos >> c.lp)];
+    float cs[8], sn[8];
+    if (r.cos && h0 < r.H + c.KH) {                         // (the group's first head is one to rotate)
         const size_t at = (size_t)pos * HD + 8 * j;
-        float cs[8], sn[8];
         load8<false>(r.cos, at, cs);
         load8<false>(r.sin, at, sn);
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = dpp_f<DPP_ROR8>(x[e]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(j < 8 ? -y[e] : y[e], sn[e], x[e] * cs[e]);
     }
-    if (what == 0) {
-        store8<BF>(r.q_out, ((size_t)t * r.H + head) * HD + 8 * j, x);
-        return;
+#pragma unroll
+    for (int i = 0; i < NH; i++) {
+        if (what[i] == 3) return;                           // (whole rows of 16 lanes)
+        const uint16_t* w = what[i] == 0 ? r.w[0] : what[i] == 1 ? r.w[1] : nullptr;
+        if (w) {
+            const uint4 u = *(const uint4*)(w + 8 * j);
+            const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[i][e], x[i][e], ss);
+            ss = seg_sum<16>(ss);
+            const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(ss * (1.0f / HD), r.eps)));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[i][2 * e] = x[i][2 * e] * inv * __uint_as_float(ww[e] << 16);
+                x[i][2 * e + 1] = x[i][2 * e + 1] * inv * __uint_as_float(ww[e] & 0xFFFF0000u);
+            }
+        }
+        if (r.cos && what[i] < 2) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = dpp_f<DPP_ROR8>(x[i][e]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = __builtin_fmaf(j < 8 ? -y[e] : y[e], sn[e], x[i][e] * cs[e]);
+        }
+        if (what[i] == 0) {
+            store8<BF>(r.q_out, ((size_t)t * r.H + head[i]) * HD + 8 * j, x[i]);
+            continue;
+        }
+        if ((unsigned)page >= (unsigned)c.n_pages) continue;
+        char* const base = (char*)(what[i] == 1 ? c.k : c.v) + (size_t)page * c.page_stride;
+        const size_t at = (((size_t)head[i] << c.lp) + (pos & ((1 << c.lp) - 1))) * HD + 8 * j;
+        if (c.f32) store8<false>(base, at, x[i]);
+        else store8<true>(base, at, x[i]);
     }
-    const int page = c.table[seq * c.table_stride + (pos >> c.lp)];
-    if ((unsigned)page >= (unsigned)c.n_pages) return;
-    char* const base = (char*)(what == 1 ? c.k : c.v) + (size_t)page * c.page_stride;
-    const size_t at = (((size_t)head << c.lp) + (pos & ((1 << c.lp) - 1))) * HD + 8 * j;
-    if (c.f32) store8<false>(base, at, x);
-    else store8<true>(base, at, x);
 }
 
 hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream_t st) {
     if (c.N == 0) return hipSuccess;
-    const int chunks = (r.H + 2 * c.KH + 15) / 16;
+    const int heads = r.H + 2 * c.KH, one = (heads + 15) / 16;
+    const bool few = (long long)c.N * one <= 2048;          // (8 blocks a CU: all heads at once)
+    const int chunks = few ? one : (heads + 47) / 48;
     const dim3 grid((unsigned)((long long)c.N * chunks));
-    if (r.bf) hipLaunchKernelGGL(k_paged_append<true>, grid, dim3(256), 0, st, c, r, chunks);
-    else hipLaunchKernelGGL(k_paged_append<false>, grid, dim3(256), 0, st, c, r, chunks);
+#define JM_PAGED_APPEND(BFV, NHV) hipLaunchKernelGGL((k_paged_append<BFV, NHV>), grid, dim3(256), 0, st, c, r, chunks)
+    if (r.bf) { if (few) JM_PAGED_APPEND(true, 1); else JM_PAGED_APPEND(true, 3); }
+    else { if (few) JM_PAGED_APPEND(false, 1); else JM_PAGED_APPEND(false, 3); }
+#undef JM_PAGED_APPEND
     return hipGetLastError();
 }
 
@@ -1369,10 +1392,14 @@ k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
 // none 45 / 31, 800 behind 2000 70 / 56, 2047 behind none 72 / 65, 2047 behind 4099 194 /
 // 197, 4 sequences of 300 behind 500 40 / 54, of 700 84 / 91, 5 of 1201 (28 heads on 4) 80 / 92.
 //
-// Ranges: joining costs a launch and the partial outputs.  k_paged_attn, one token: 500
-// rows 8.9 (one range) / 11.5 (four), 1000 rows 13.2 / 11.4, 1000 rows of 32 sequences
-// 23 / 27; of float32 pages 300 rows 16.6 / 12.3.  The tiles, 512 rows a range against 256:
-// 200 tokens behind 1000 rows 34 / 35; of float32 pages 32 behind 2000 35 / 26.
+// Ranges of k_paged_attn: a block of each CU in turn, each as long as its rows and 160 more; a
+// quarter of a block behind the last, as the prefixes differ; joining them 750 rows (of
+// float32, which take twice as long, 200).  One token: 500 rows 8.9 (one range) / 11.5 (four),
+// 1000 rows 13.2 / 11.4, of float32 300 rows 16.6 / 12.3; 1000 rows of 32 sequences 23 / 27
+// (two), 1500 of 40 53 / 46 (three); 3000 of 12 31 (five: 480 blocks), 35 (six), 33 (ten); up
+// to 2048 float32 rows of 8 sequences on 4 heads 24 (eight: 256 blocks) / 31 (nine).  Of the
+// tiles, 512 rows at least against 256: 200 tokens behind 1000 rows 34 / 35; of float32 pages
+// 32 behind 2000 35 / 26.
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     PagedPlan p{};
     const int qpk = H / c.KH;
@@ -1386,13 +1413,9 @@ PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
         p.units = c.cu ? (int)std::min<long long>(c.N, ((long long)c.N + (long long)c.n_seq * (tp - 1)) / tp) : c.N;
         likely = std::min<long long>(p.units, c.n_seq * ((each + tp - 1) / tp)) * c.KH;
     };
-    // ranges for up to `want` blocks while each has `least` rows
-    auto ranges = [&](long long want, int least) {
-        return (int)std::max(std::min((want + likely - 1) / likely, ((long long)rows + least - 1) / least), 1ll);
-    };
-    // the same for one round of 256 blocks (a tile's block fills a CU)
-    auto parts = [&](int least) {
-        return (int)std::max(std::min(256 / likely, ((long long)rows + least - 1) / least), 1ll);
+    // ranges of at least `least` rows for up to `want` blocks
+    auto ranges = [&](int want, int least) {
+        return (int)std::max(std::min(want / likely, ((long long)rows + least - 1) / least), 1ll);
     };
     cut(c.cu ? 16 / qpk : 1);
     if (likely == 0) return p;
@@ -1404,17 +1427,23 @@ PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
             auto steps = [&](int rg) {
                 cut((bf ? 64 : 32) * rg / qpk);
                 const int step = 256 / rg;
-                const long long S = parts(512), most = rows / step / S + 6, mean = std::max(rows - each / 2, 0ll) / step / S + 6;
+                const long long S = ranges(256, 512), most = rows / step / S + 6, mean = std::max(rows - each / 2, 0ll) / step / S + 6;
                 return std::max(most, (likely * S + 255) / 256 * mean) + (S > 1 ? 6 : 0);
             };
             p.rg = 10 * steps(2) < 9 * steps(4) ? 2 : 4;
             cut((bf ? 64 : 32) * p.rg / qpk);
         }
-        p.S = parts(c.f32 ? 256 : 512);
-    } else if (rows <= (c.f32 ? 256 : 512)) {
-        p.S = 1;
+        p.S = ranges(256, c.f32 ? 256 : 512);             // (a tile's block fills a CU)
     } else {
-        p.S = std::max(ranges(256, 128), rows <= 1024 ? 1 : ranges(1024, 512));
+        // what S ranges take, in rows that a block passes over, times 4
+        auto cost = [&](long long S) {
+            return (4 * ((likely * S + 255) / 256) + 1) * ((rows + S - 1) / S + 160) + (S == 1 ? 0 : c.f32 ? 800 : 3000);
+        };
+        p.S = 1;
+        for (int k = 1; k <= 8; k++) {                      // (as many ranges as fit k rounds)
+            const int S = ranges(256 * k, 128);
+            if (cost(S) < cost(p.S)) p.S = S;
+        }
     }
     const size_t cols = (size_t)p.units * c.KH * p.S * qpk * p.tp;
     p.o_floats = p.S > 1 ? cols * 128 : 0;

@@ -50,7 +50,7 @@ class PagedKVCacheSet:
                 or data.data_ptr() % 16:
             raise ValueError(f"cache must be a contiguous 16-byte aligned bfloat16 or float32 CUDA tensor {full}")
         self.shape, self.B, self.n_pages, self.page, self.data = shape, B, n_pages, page, data
-        self._device = data.device
+        self._device, self._index = data.device, data.get_device()
         width = -(-shape.maxT // page)
         self.table = torch.full((B, width), -1, dtype=torch.int32, device=self._device)
         self._free = list(range(n_pages - 1, -1, -1))
@@ -141,7 +141,7 @@ class PagedKVCacheSet:
         for t, name, size in ((start, "start", self.B), (cu, "cu", self.B + 1)):
             if t is None and name == "cu":
                 continue
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self._device \
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.get_device() != self._index \
                     or t.shape != (size,) or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 tensor [{size}] on {self._device}")
         if cu is None and n != self.B:
@@ -149,7 +149,7 @@ class PagedKVCacheSet:
 
     def _heads(self, t, name: str, n: int, heads: int, dtype=None) -> None:
         """t is [n, heads, 128] in float32 or bfloat16, its rows contiguous."""
-        if not isinstance(t, torch.Tensor) or t.device != self._device or t.dtype not in _DTYPES \
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._index or t.dtype not in _DTYPES \
                 or (dtype is not None and t.dtype != dtype):
             raise ValueError(f"{name} must be a {'float32 or bfloat16' if dtype is None else dtype} tensor "
                              f"on {self._device}")
@@ -169,7 +169,7 @@ class PagedKVCacheSet:
 
     def _vector(self, t, name: str, dtype, rows: int) -> None:
         """t is [rows or more, 128], or [128] where rows is 0."""
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self._device or t.dim() != (2 if rows else 1) \
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != self._index or t.dim() != (2 if rows else 1) \
                 or t.shape[-1] != HD or (rows and t.shape[0] < rows) or not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f"{name} must be a contiguous 16-byte aligned {dtype} tensor "
                              f"{[rows, HD] if rows else [HD]} on {self._device}")
