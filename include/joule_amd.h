@@ -590,8 +590,9 @@ typedef struct jm_kv_rows {
  *   cos, sin        then each q and k head is rotated by halves to its row r: dimension
  *                   d < 64 becomes x[d] cos[r][d] - x[d + 64] sin[r][d], d + 64 becomes
  *                   x[d + 64] cos[r][d + 64] + x[d] sin[r][d + 64]
- * in float32, rounded once (to nearest even) to the caches' type, and to q's in q_out.  Of
- * two tokens of a call with one row in one page either may stay. */
+ * in float32, rounded once (to nearest even) to the caches' type, and to q's in q_out.  Two
+ * tokens of a call with one row in one page (of sequences that share it) leave either's
+ * values there, each for itself. */
 int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const jm_kv_rows* rows,
                        void* stream);
 
@@ -603,11 +604,13 @@ int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t
  * (products are taken in parts, of which some are 0); rows that it does not see may hold
  * anything.
  *   max_rows  at least as many rows as the longest sequence has after this call, where
- *             the caller knows (0: maxT): the call is cut by it.  A smaller number is
- *             slower, not wrong.
- * float32 q: scores, weights and sums hold float32's 24 bits.  bf16 q: q and the weights
- * are exact to 2^-16 of the weight; sums are float32.  out may be q where q is
- * contiguous.  The magnitudes of V stay below 2^100.  Workspace: as jm_q4_gemm_f32's. */
+ *             the caller knows (0: maxT): the call is cut by it, which only rounding
+ *             shows.  A smaller number is slower, not wrong.
+ * float32 q: scores, weights and sums hold float32's 24 bits.  bf16 q: q is exact, and a
+ * weight is so to 2^-16 of it; over bf16 pages the weights of long prompts (by the call's
+ * sizes) are rounded to bf16, 2^-8, and their sum is that of the rounded ones, so that
+ * outputs stay means of V's rows.  Sums are float32.  out may be q where q is contiguous.
+ * The magnitudes of V stay below 2^100.  Workspace: as jm_q4_gemm_f32's. */
 int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
                      int64_t q_head, int n_heads, float scale, int max_rows, int dtype, void* out, void* stream);
 

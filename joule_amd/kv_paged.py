@@ -237,8 +237,9 @@ class PagedKVCacheSet:
         below 0, or none with a page) gets 0, other skipped tokens keep what out
         held.  max_rows: at least as many rows as the longest sequence has after the
         call (0: the pages that ``reserve`` and ``share`` gave it, maxT where the host
-        writes the table); it decides how the call is cut, not what it gives.  out
-        may be q."""
+        writes the table); the call is cut by it, which only rounding shows.  out may be
+        q.  With bfloat16 q a weight holds 16 bits, in long prompts over bfloat16 pages
+        8; with float32 q 24."""
         n, H = (q.shape[0], q.shape[1]) if isinstance(q, torch.Tensor) and q.dim() == 3 else (-1, self.shape.n_heads)
         self._heads(q, "q", n, H)
         self._tokens(start, cu, n)
