@@ -10,6 +10,7 @@ Modules
   q4_store  the Q4 format (quantise / dequantise, store writer, index)
   decoder   the decode step around the block, KV caches
   kv_q4     4-bit KV caches: write, read, attention
+  kv_paged  paged KV caches: pages shared and given out, append, attention
   sampling  the next token under temperature, top-k, top-p and min-p
   moe       HbmExpertStore: the store in HBM and layer_ffn_batch
   backend   KernelBackend plugin API with HipBackend (q4_gemv / q4_gemm)

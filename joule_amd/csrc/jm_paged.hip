@@ -123,6 +123,13 @@ hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream
 // bf16 pages: float32 q and weights are three bf16 parts (24 bits, one product each),
 // bf16 q is exact in one, its weights two parts; all their products with K and V are
 // exact, sums float32.  float32 pages: float32 products.
+//
+// Bound by HBM where prefixes are long: one token behind 131001 rows (537 MB) 84 us and 6 to
+// join, 6.0 TB/s; 32 behind up to 16 k rows 260, 5.9 TB/s.  (A large copy here: 4.95 TB/s,
+// reads and writes.)  Short ones wait: 7 us for a block with 6 tiles a wave, most of it the
+// launch and the loads that need one another (cu, start, table, rows), and 4 for the second
+// launch.  Registers, not LDS, hold the tile that is on its way: 235 to 256 of them, two
+// waves a SIMD.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -609,7 +616,7 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
 // unit's rows), 8 waves = RG row groups x PS position strides; in a step wave (rg, ps)
 // takes the 32 cache rows ps of the step's 32 PS for its 32 QB query rows, with an online
 // softmax, and the PS waves of a row group are joined at the end.  A step's rows go
-// straight to LDS (global_load_lds), the steps after it on their way.
+// straight to LDS, those of the NS - 1 steps after it on their way.
 //
 //   scores   v_mfma_f32_32x32x16_bf16, cache rows as A (lane l: row l % 32, dimensions 16
 //            kk + 8 (l / 32) ..), query rows as B: lane l holds query row l % 32 at cache
@@ -622,6 +629,15 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
 // two products; q is exact, a weight is rounded to bf16 once, and the sum is of the
 // rounded weights, so that the output stays a mean of values of V.  float32 queries: q and
 // the weights as three bf16 parts each, as in k_paged_attn.
+//
+// Bound by the issue of instructions: a step takes 4100 cycles for 2112 of products, as the two
+// waves of a SIMD have 380 instructions each, of which a wave issues one in 5 to 7 cycles.  2047 tokens behind 4099 rows
+// (32 heads on 8) 192 us, 893 TFLOP/s; without the weights' work it would be 167, without the
+// reads of LDS 187, without the loads 179, products and barriers alone 138, and 28% of it is
+// the longest prefix's block against the mean one.  What brought it there: the two waves of a
+// SIMD a phase apart instead of in step (206 to 232), a reference that is raised only where
+// the weights' sum tells of a score far above it, loads to LDS as buffers (as flat ones every
+// read of LDS waits for all before it), outputs through LDS in whole lines (200).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -971,7 +987,6 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             }
         }
     };
-    // ---- the vector work of a phase: the weights of step t
     // ---- The two waves of a SIMD (w and w + 4) are one phase apart: while one multiplies,
     // the other weighs.  In the phase in which a wave weighs step t it requests K of step t +
     // NS and V of step t + NS - 1, into the rows that its half multiplied in the phase
