@@ -217,7 +217,8 @@ int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* 
     if (int rc = rows_tensor("out", out, dtype, 0, 0)) return rc;
     hipStream_t st = (hipStream_t)stream;
     const jm::PagedPlan p = jm::paged_plan(a, n_heads, dtype == JM_DTYPE_BF16, max_rows ? max_rows : c->maxT);
-    if ((long long)c->n_kv * p.units * p.S * 512 > MAX_THREADS || (long long)p.units * p.tp * n_heads * 256 > MAX_THREADS)
+    // (the kernel that joins ranges: up to 256 threads a query row)
+    if ((long long)c->n_kv * p.units * p.S * 512 > MAX_THREADS || (p.S > 1 && (long long)p.units * p.tp * n_heads * 256 > MAX_THREADS))
         return fail(JM_ERR_SHAPE, "attention of N=%d tokens and %d heads is more than one launch takes", N, n_heads);
     return with_workspace(st, (p.o_floats + p.ml_floats) * 4, "paged attention launch", [&](float* part) {
         return jm::launch_paged_attn(a, p, q, dtype == JM_DTYPE_BF16, q_token, q_head, n_heads, scale, out, part, part + p.o_floats, st);

@@ -29,8 +29,8 @@ class PagedKVCacheSet:
 
     An entry of the table outside [0, n_pages) is no page: rows there are not
     written, and attention does not see them.  ``reserve``, ``share`` and
-    ``release`` keep the table; a host with an allocator of its own writes it
-    instead (on the stream of the calls)."""
+    ``release`` keep the table, on the current stream, which is that of the calls; a
+    host with an allocator of its own writes it instead."""
 
     def __init__(self, shape: DecoderShape, B: int, n_pages: int, page: int = 16, dtype: torch.dtype = torch.bfloat16,
                  device="cuda", data: torch.Tensor | None = None):

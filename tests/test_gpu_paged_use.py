@@ -280,6 +280,74 @@ def test_append_without_pages_and_behind_the_last_sequence(many, dt, cached):
     assert torch.equal(before.view(torch.uint8), c.data.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dt,cached", TYPES)
+def test_more_sequences_than_a_wave_has_lanes(dt, cached):
+    """130 sequences, some of them empty: a token each, drafts, ragged prompts."""
+    B = 130
+    rng = np.random.default_rng(8)
+    start = rng.integers(0, 60, B).tolist()
+    for counts in ([1] * B, rng.integers(0, 5, B).tolist(), rng.integers(0, 90, B).tolist()):
+        counts[0], counts[64], counts[65], counts[-1] = 1, 1, 1, max(counts[-1], 1)
+        for maxT in (300, 2 ** 19):
+            run(8, 2, counts, start, dt, cached, maxT=maxT, one=max(counts) == 1)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("maxT", [1500, 2 ** 19])
+def test_tokens_in_front_of_the_first_sequence(maxT, dt, cached):
+    """cu[0] above 0: tokens of nobody, left as they were; and a call of fewer sequences'
+    tokens than there are rows for."""
+    H, KH, counts, start = 8, 2, [40, 0, 200], [30, 9, 700]
+    c, q = prepared(H, KH, counts, start, cached, maxT)
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    qd = torch.from_numpy(q).cuda().to(DT[dt])
+    pad = torch.full((7, H, HD), float("nan"), dtype=DT[dt], device="cuda")
+    # (a call of as many tokens, which is cut alike)
+    want = c.attention(0, torch.cat([qd, pad, pad]), ints(start), ints(cu.tolist()))[:-14]
+    out = torch.full((len(q) + 14, H, HD), 7.0, dtype=DT[dt], device="cuda")
+    got = c.attention(0, torch.cat([pad, qd, pad]), ints(start), ints((cu + 7).tolist()), out=out)
+    assert bool((got[:7] == 7.0).all()) and bool((got[-7:] == 7.0).all()) and torch.equal(got[7:-7], want)
+    k = torch.full((len(q) + 14, KH, HD), 3.0, dtype=DT[dt], device="cuda")
+    before = c.data.clone()
+    out.fill_(7.0)
+    c.append(0, k, k, ints(start), ints((cu + 7).tolist()), q=torch.ones_like(out), q_out=out)
+    assert bool((out[:7] == 7.0).all()) and bool((out[-7:] == 7.0).all()) and bool((out[7:-7] == 1.0).all())
+    for b, (s, n) in enumerate(zip(start, counts)):
+        gk, gv = held(c, b, s + n)
+        assert (gk[s:] == 3.0).all() and (gv[s:] == 3.0).all()
+    bits = torch.int32 if cached == "f32" else torch.int16              # (the pages hold NaN elsewhere)
+    assert int((c.data.view(bits) != before.view(bits)).sum()) <= 2 * 240 * KH * HD
+
+
+def test_tensors_past_32_bits():
+    """q, k, v and the outputs of more than 2^32 bytes and 2^31 values, in sequences of 150
+    tokens that share one page table's pages: the last of them against float64."""
+    H, KH, n, B = 32, 2, 150, 3600
+    T, page = 200, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    c = PagedKVCacheSet(shape_of(KH, H, T), B, 4 * B, page=page)
+    c.table.copy_(torch.arange(4 * B, device="cuda").int().view(B, 4))
+    N = n * B
+    assert N * H * HD > 2 ** 31
+    q = torch.randn(N, H, HD, generator=g, device="cuda", dtype=torch.bfloat16)
+    kv = torch.randn(2, N, KH, HD, generator=g, device="cuda", dtype=torch.bfloat16)
+    start, cu = ints([b % 50 for b in range(B)]), ints([n * b for b in range(B + 1)])
+    c.data.fill_(0.5)
+    got = c.append(0, kv[0], kv[1], start, cu, q=q)
+    assert torch.equal(got[-1000:], q[-1000:]) and torch.equal(got[:1000], q[:1000])
+    out = c.attention(0, q, start, cu, out=got)
+    for b in (0, B // 2, B - 1):
+        s = b % 50
+        gk, gv = held(c, b, s + n)
+        assert np.array_equal(gv[s:], kv[1, n * b:n * (b + 1)].float().cpu().numpy())
+        t = np.arange(s + n)
+        pick = np.array([0, 1, 77, n - 1])
+        for h in (0, 13, H - 1):
+            i = h * KH // H
+            want, tol = attend(q[n * b + pick, h].float().cpu().numpy(), gk[:, i], gv[:, i], t <= s + pick[:, None], HD ** -0.5, "bf16 prompt")
+            assert (np.abs(out[n * b + pick, h].double().cpu().numpy() - want) <= tol).all()
+
+
 # -------------------------------------------------- streams, graphs, threads, devices
 
 
