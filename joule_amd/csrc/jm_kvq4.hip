@@ -468,7 +468,7 @@ k_q4_attn(Q4KvArgs c, Q4AttnArgs a) {
     __shared__ float mls[4][8][2];
     const int kh = blockIdx.x % c.KH, u = blockIdx.x / c.KH % a.units, s = blockIdx.x / c.KH / a.units;
     CallUnit un;
-    if (!call_unit(c, u, a.tp, un)) return;                   // (block-uniform)
+    if (!call_unit(c, u, a.tp, un)) return;                 // (block-uniform)
     const int last = min(un.pos + un.n - 1, c.maxT - 1);    // the last row any token sees
     const int NT = (last + 32) / 32;                        // (0 where last < 0)
     q4_attn_unit<NG, BF, 4>(c, a, un, kh, (int)((long long)NT * s / a.S), (int)((long long)NT * (s + 1) / a.S), u, s, 0, ow, mls);
