@@ -555,12 +555,13 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
     __shared__ float ls[G];
     const int nc = a.qpk * a.tp;
     const int j = threadIdx.x & 31, gr = G == 1 ? 0 : threadIdx.x >> 5;
-    const int row = G == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    const int oc = row % nc, kh = row / nc % c.KH, u = row / nc / c.KH;
+    // (a block's rows are of one unit: call_unit wants the same in every lane)
+    const int nb = G == 1 ? (nc + 7) / 8 : nc, kh = blockIdx.x % c.KH, rs = blockIdx.x / c.KH, u = rs / nb;
+    const int oc = G == 1 ? 8 * (rs % nb) + (threadIdx.x >> 5) : rs % nb;
     CallUnit un;
-    if (u >= a.units || !call_unit(c, u, a.tp, un)) return;
+    if (!call_unit(c, u, a.tp, un)) return;
     const int to = oc / a.qpk;
-    if (to >= un.n || un.pos + to >= c.maxT) return;        // (with G = 8 block-uniform)
+    if (oc >= nc || to >= un.n || un.pos + to >= c.maxT) return;        // (with G = 8 block-uniform)
     const size_t p0 = ((size_t)u * c.KH + kh) * a.S * nc + oc;
     float M = -INFINITY;
     uint32_t any = 0;
@@ -1400,21 +1401,25 @@ k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
 // (64 k) 20 / 23, 32 behind 2000 (130 k) 28 / 24, 8 behind 2000, 4 sequences (128 k) 49 /
 // 27, 16 sequences of 16 (1 M) 181 / 120.
 //
-// Units of k_paged_tile: RG 4 (twice the query rows a block, 64 cache rows a step) against
-// RG 2 (128 cache rows a step), by what each takes: a step 1.7 us, a block's beginning and
-// end 6 steps, joined ranges 6 more, 256 blocks at once, the longest prefix bounding all.  RG
-// 2 reads the cache twice as often: it has to be a tenth below.  RG 4 / RG 2: 777 tokens behind
-// none 45 / 31, 800 behind 2000 70 / 56, 2047 behind none 72 / 65, 2047 behind 4099 194 /
-// 197, 4 sequences of 300 behind 500 40 / 54, of 700 84 / 91, 5 of 1201 (28 heads on 4) 80 / 92.
+// (A sequence with 17 query rows over float32 pages, the second unit of k_paged_attn, goes to
+// the tiles: 5 tokens behind 4000 rows, 8 sequences 95 / 75.)
+//
+// Units and ranges of the tiles, by what they take: a step (2 us at most), a block's beginning
+// and end 6 steps, 256 blocks at once, the longest prefix bounding all; joined ranges 2 steps
+// and what their partial outputs are to move.  661 tokens behind 3761 float32 rows, 2
+// sequences of 4 heads on one 142 us (468 blocks of a third of the rows), 209 (156 blocks).
+// RG 2 reads the cache twice as often as RG 4: it has to be a tenth below.  RG 4 / RG 2: 777
+// tokens behind none 45 / 31, 800 behind 2000 70 / 56, 2047 behind none 72 / 65, 2047 behind
+// 4099 194 / 197, 4 sequences of 300 behind 500 40 / 54, of 700 84 / 91, 5 of 1201 (28 heads on
+// 4) 80 / 92.  512 rows a range at least against 256: 200 tokens behind 1000 rows 34 / 35; of
+// float32 pages 32 behind 2000 35 / 26.
 //
 // Ranges of k_paged_attn: a block of each CU in turn, each as long as its rows and 160 more; a
 // quarter of a block behind the last, as the prefixes differ; joining them 750 rows (of
 // float32, which take twice as long, 200).  One token: 500 rows 8.9 (one range) / 11.5 (four),
 // 1000 rows 13.2 / 11.4, of float32 300 rows 16.6 / 12.3; 1000 rows of 32 sequences 23 / 27
 // (two), 1500 of 40 53 / 46 (three); 3000 of 12 31 (five: 480 blocks), 35 (six), 33 (ten); up
-// to 2048 float32 rows of 8 sequences on 4 heads 24 (eight: 256 blocks) / 31 (nine).  Of the
-// tiles, 512 rows at least against 256: 200 tokens behind 1000 rows 34 / 35; of float32 pages
-// 32 behind 2000 35 / 26.
+// to 2048 float32 rows of 8 sequences on 4 heads 24 (eight: 256 blocks) / 31 (nine).
 PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     PagedPlan p{};
     const int qpk = H / c.KH;
@@ -1434,21 +1439,34 @@ PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     };
     cut(c.cu ? 16 / qpk : 1);
     if (likely == 0) return p;
-    if (c.cu && qrows >= 32ll * c.n_seq && likely * std::max(rows, 512) >= (c.f32 ? 100000 : 450000)) {
+    if (c.cu && qrows >= (c.f32 ? 17ll : 32ll) * c.n_seq && likely * std::max(rows, 512) >= (c.f32 ? 100000 : 450000)) {
+        // the cut into units of tp tokens and steps of `step` rows: what it takes, in steps
+        auto tiles = [&](int tp, int step, int least) {
+            long long best = LLONG_MAX;
+            cut(tp);
+            for (int k = 0; k <= 4; k++) {                  // (as many ranges as fit k rounds; one)
+                const long long S = k ? ranges(256 * k, least) : 1;
+                const long long most = rows / step / S + 6, mean = std::max(rows - each / 2, 0ll) / step / S + 6;
+                const long long all = std::max(most, (likely * S + 255) / 256 * mean) + (S > 1 ? 2 + c.N * S * H / 8192 : 0);
+                if (all < best) {
+                    best = all;
+                    p.S = (int)S;
+                }
+            }
+            return best;
+        };
         if (c.f32) {
             p.rg = 1;
-            cut(32 / qpk);
+            tiles(32 / qpk, 64, 256);
         } else {
-            auto steps = [&](int rg) {
-                cut((bf ? 64 : 32) * rg / qpk);
-                const int step = 256 / rg;
-                const long long S = ranges(256, 512), most = rows / step / S + 6, mean = std::max(rows - each / 2, 0ll) / step / S + 6;
-                return std::max(most, (likely * S + 255) / 256 * mean) + (S > 1 ? 6 : 0);
-            };
-            p.rg = 10 * steps(2) < 9 * steps(4) ? 2 : 4;
-            cut((bf ? 64 : 32) * p.rg / qpk);
+            const int tp = (bf ? 64 : 32) * 2 / qpk;
+            const long long two = tiles(tp, 128, 512), four = tiles(2 * tp, 64, 512);
+            p.rg = 4;
+            if (10 * two < 9 * four) {
+                p.rg = 2;
+                tiles(tp, 128, 512);
+            }
         }
-        p.S = ranges(256, c.f32 ? 256 : 512);             // (a tile's block fills a CU)
     } else {
         // what S ranges take, in rows that a block passes over, times 4
         auto cost = [&](long long S) {
@@ -1490,11 +1508,11 @@ hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void*
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.S == 1) return e;
-    const unsigned outs = (unsigned)c.KH * p.units * (unsigned)(a.qpk * a.tp);
     // (few ranges: more groups a row only leave lanes without work; 32 tokens behind 2000 rows,
     // 16 sequences in 2 ranges 53 us against 78.  Many: 64 ranges of one token 12.8 against 17.)
     const bool apart = p.S < 16;
-    const dim3 mg(apart ? (outs + 7) / 8 : outs);
+    const int nc = a.qpk * a.tp;
+    const dim3 mg((unsigned)c.KH * p.units * (unsigned)(apart ? (nc + 7) / 8 : nc));
 #define JM_PAGED_MERGE(BFV, GV) hipLaunchKernelGGL((k_paged_merge<BFV, GV>), mg, dim3(256), 0, st, c, a)
     if (bf) { if (apart) JM_PAGED_MERGE(true, 1); else JM_PAGED_MERGE(true, 8); }
     else { if (apart) JM_PAGED_MERGE(false, 1); else JM_PAGED_MERGE(false, 8); }

@@ -223,6 +223,15 @@ def test_few_tokens(H, KH, counts, start, dt, cached):
 
 
 @pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH", [(3, 1), (5, 1), (9, 1), (11, 1), (13, 1), (15, 1), (10, 2), (28, 4)])
+@pytest.mark.parametrize("counts,start", [([1, 1], [1039, 746]), ([1, 0, 2, 7, 1], [2100, 5, 1500, 900, 1039]), ([40, 133], [700, 1515])])
+def test_ranges_of_heads_that_do_not_fill_a_unit(H, KH, counts, start, dt, cached):
+    """Units of 9 to 15 query rows (of 117 to 126 in a long cache) whose outputs are joined."""
+    run(H, KH, counts, start, dt, cached, 64)
+    run(H, KH, counts, start, dt, cached, 64, maxT=DEEP)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
 @pytest.mark.parametrize("H,KH,counts,start,page", [(8, 1, [64], [1500], 16), (2, 2, [129], [2000], 64), (6, 2, [300], [97], 32),
                                                     (8, 8, [130], [700], 16), (4, 2, [130, 0, 90], [900, 5, 1800], 128), (7, 1, [201], [0], 16)])
 def test_prompts(H, KH, counts, start, page, dt, cached):
