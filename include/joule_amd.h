@@ -607,9 +607,8 @@ int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t
  *             the caller knows (0: maxT): the call is cut by it, which only rounding
  *             shows.  A smaller number is slower, not wrong.
  * float32 q: scores, weights and sums hold float32's 24 bits.  bf16 q: q is exact, and a
- * weight is so to 2^-16 of it; over bf16 pages the weights of long prompts (by the call's
- * sizes) are rounded to bf16, 2^-8, and their sum is that of the rounded ones, so that
- * outputs stay means of V's rows.  Sums are float32.  out may be q where q is contiguous.
+ * weight is so to 2^-16 of it, whatever the call's sizes.  Sums are float32.  out may be q
+ * where q is contiguous.
  * The magnitudes of V stay below 2^100, those of q below 2^127.  Workspace: as
  * jm_q4_gemm_f32's. */
 int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,

@@ -627,18 +627,20 @@ k_paged_merge(PagedArgs c, PagedAttnArgs a) {
 //            contraction index j of half h in step s is row 16 s + 8 (j / 4) + 4 h + j % 4
 //
 // bf16 queries (BF): 64 query rows a wave (QB = 2), so that an operand read from LDS serves
-// two products; q is exact, a weight is rounded to bf16 once, and the sum is of the
-// rounded weights, so that the output stays a mean of values of V.  float32 queries: q and
-// the weights as three bf16 parts each, as in k_paged_attn.
+// two products; q is exact, the weights are two bf16 parts.  float32 queries: q and the
+// weights as three bf16 parts each.  Both as in k_paged_attn, so that a token gets the same
+// precision whichever kernel its call takes.  (The weights of bf16 queries in one part: 2047
+// tokens behind 4099 rows 190 us instead of 236, but two outputs in five come out another bf16
+// number, and the error against float64 is 1.4 times that of the output's own rounding.)
 //
-// Bound by the issue of instructions: a step takes 4100 cycles for 2112 of products, as the two
-// waves of a SIMD have 380 instructions each, of which a wave issues one in 5 to 7 cycles.  2047 tokens behind 4099 rows
-// (32 heads on 8) 192 us, 893 TFLOP/s; without the weights' work it would be 167, without the
-// reads of LDS 187, without the loads 179, products and barriers alone 138, and 28% of it is
-// the longest prefix's block against the mean one.  What brought it there: the two waves of a
-// SIMD a phase apart instead of in step (206 to 232), a reference that is raised only where
-// the weights' sum tells of a score far above it, loads to LDS as buffers (as flat ones every
-// read of LDS waits for all before it), outputs through LDS in whole lines (200).
+// Bound by the issue of instructions: a step takes 5100 cycles for 3168 of products, as the two
+// waves of a SIMD have 480 instructions each, of which a wave issues one in 5 to 7 cycles.  2047
+// tokens behind 4099 rows (32 heads on 8) 236 us, 727 TFLOP/s of the formula's products, and
+// 28% of it is the longest prefix's block against the mean one.  What brought it there
+// (measured with weights of one part, 192 us): the two waves of a SIMD a phase apart instead of
+// in step (206 to 232), a reference that is raised only where the weights' sum tells of a score
+// far above it, loads to LDS as buffers (as flat ones every read of LDS waits for all before
+// it), outputs through LDS in whole lines (200).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -660,7 +662,7 @@ __device__ __forceinline__ void paged_meet() {
 template <bool BF, int RG>
 __global__ void __launch_bounds__(512, 2)
 k_paged_tile(PagedArgs c, PagedAttnArgs a) {
-    constexpr int HD = 128, QB = BF ? 2 : 1, NQ = BF ? 1 : 3, PS = 8 / RG, STEP = 32 * PS, TILE = 32 * HD;
+    constexpr int HD = 128, QB = BF ? 2 : 1, NQ = BF ? 1 : 3, NP = BF ? 2 : 3, PS = 8 / RG, STEP = 32 * PS, TILE = 32 * HD;
     constexpr int RW = 8 * (PS / 2);            // rows of a step that a wave stages, of K and of V
     constexpr int LPS = RW / 2;                 // its loads, 4 rows each
     constexpr int NROW = 32 * QB * RG, AHEAD = 2;
@@ -820,7 +822,7 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     int seen[QB];                               // whether the lane's query rows saw a row; all: all of them did
     bool all = false;
     f32x16 S[QB];
-    u32x4_t P[QB][NQ][2];
+    u32x4_t P[QB][NP][2];
 #pragma unroll
     for (int b = 0; b < QB; b++) {
         ref[b] = -INFINITY;
@@ -842,12 +844,11 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             const float r0 = ref[b] == -INFINITY ? 0.0f : ref[b];
             const float x0 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e], cs, -r0));
             const float x1 = pow2f(__builtin_fmaf(S[b][8 * s + 2 * e + 1], cs, -r0));
-            uint32_t p[NQ];
-            parts_bf16<NQ>(x0, x1, p);
+            uint32_t p[NP];
+            parts_bf16<NP>(x0, x1, p);
 #pragma unroll
-            for (int q = 0; q < NQ; q++) P[b][q][s][e] = p[q];
-            if (BF) l[b] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p[0]), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l[b], false);
-            else l[b] += x0 + x1;
+            for (int q = 0; q < NP; q++) P[b][q][s][e] = p[q];
+            l[b] += x0 + x1;
         }
     };
     // The vector work of a phase: of step t, the scores that are not seen, the weights, the
@@ -903,7 +904,7 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
 #pragma unroll
         for (int b = 0; b < QB; b++) {
 #pragma unroll
-            for (int q = 0; q < NQ; q++) __asm__ volatile("" : "+v"(P[b][q][0]), "+v"(P[b][q][1]));
+            for (int q = 0; q < NP; q++) __asm__ volatile("" : "+v"(P[b][q][0]), "+v"(P[b][q][1]));
             __asm__ volatile("" : "+v"(l[b]));
         }
     };
@@ -976,9 +977,9 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
             }
             if (j < 8) {
 #pragma unroll
-                for (int b = 0; b < QB; b++)
+                for (int q = NP - 1; q >= 0; q--)
 #pragma unroll
-                    for (int q = NQ - 1; q >= 0; q--)
+                    for (int b = 0; b < QB; b++)
                         O[b][j % 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[j], __builtin_bit_cast(bf16x8, P[b][q][j / 4]), O[b][j % 4], 0, 0, 0);
                 if (j == 4) locate(t + 1 + NS);
             } else {
@@ -1394,24 +1395,26 @@ k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
 //
 // Which kernel: a block of k_paged_attn has 16 query rows, so that the cache is multiplied
 // once for each 16, but is done in 8 us; k_paged_tile takes 15 us to begin and end.  The
-// blocks times their rows (512 at least) decide.  bf16 pages, k_paged_attn / k_paged_tile:
-// 64 tokens behind 2000 rows (264 k) 28 / 28, 400 behind none (410 k) 20 / 23, 32 behind
-// 2000, 4 sequences (520 k) 41 / 31, 600 behind none (614 k) 28 / 26, 16 behind 2000, 16
-// sequences (1 M) 77 / 48.  float32 pages, k_paged_attn / k_paged_tile_f32: 16 behind 2000
-// (64 k) 20 / 23, 32 behind 2000 (130 k) 28 / 24, 8 behind 2000, 4 sequences (128 k) 49 /
-// 27, 16 sequences of 16 (1 M) 181 / 120.
+// blocks times their rows (512 at least) decide.  bf16 q and pages, k_paged_attn /
+// k_paged_tile: 64 tokens behind 2000 rows (264 k) 21 / 31, 2 such sequences (528 k) 28 / 34,
+// 600 behind none (614 k) 28 / 28, 40 behind 2000, 4 sequences (653 k) 44 / 34, 700 behind
+// none (717 k) 34 / 32, 16 behind 2000, 16 sequences (1 M) 62 / 52.  float32 q over bf16
+// pages: 100 behind 2000 (420 k) 29 / 29, 400 behind none (410 k) 25 / 23, 200 behind 1000 (480
+// k) 33 / 30, 16 behind 2000, 16 sequences (1 M) 76 / 46.  float32 pages, k_paged_attn /
+// k_paged_tile_f32: 16 behind 2000 (64 k) 21 / 23, 32 behind 2000 (130 k) 27 / 24, 8 behind
+// 2000, 4 sequences (128 k) 49 / 27, 16 sequences of 16 (1 M) 162 / 120.
 //
 // (A sequence with 17 query rows over float32 pages, the second unit of k_paged_attn, goes to
-// the tiles: 5 tokens behind 4000 rows, 8 sequences 95 / 75.)
+// the tiles: 5 tokens behind 4000 rows, 8 sequences 94 / 75.)
 //
-// Units and ranges of the tiles, by what they take: a step (2 us at most), a block's beginning
+// Units and ranges of the tiles, by what they take: a step (2.5 us at most), a block's beginning
 // and end 6 steps, 256 blocks at once, the longest prefix bounding all; joined ranges 2 steps
 // and what their partial outputs are to move.  661 tokens behind 3761 float32 rows, 2
 // sequences of 4 heads on one 142 us (468 blocks of a third of the rows), 209 (156 blocks).
 // RG 2 reads the cache twice as often as RG 4: it has to be a tenth below.  RG 4 / RG 2: 777
-// tokens behind none 45 / 31, 800 behind 2000 70 / 56, 2047 behind none 72 / 65, 2047 behind
-// 4099 194 / 197, 4 sequences of 300 behind 500 40 / 54, of 700 84 / 91, 5 of 1201 (28 heads on
-// 4) 80 / 92.  512 rows a range at least against 256: 200 tokens behind 1000 rows 34 / 35; of
+// tokens behind none 41 / 34, 800 behind 2000 75 / 67, 2047 behind none 80 / 75, 2047 behind
+// 4099 236 / 247, 4 sequences of 300 behind 500 43 / 59, of 700 94 / 105, 5 of 1201 (28 heads on
+// 4) 120 / 166.  512 rows a range at least against 256: 200 tokens behind 1000 rows 34 / 35; of
 // float32 pages 32 behind 2000 35 / 26.
 //
 // Ranges of k_paged_attn: a block of each CU in turn, each as long as its rows and 160 more; a
@@ -1439,7 +1442,7 @@ PagedPlan paged_plan(const PagedArgs& c, int H, bool bf, int rows) {
     };
     cut(c.cu ? 16 / qpk : 1);
     if (likely == 0) return p;
-    if (c.cu && qrows >= (c.f32 ? 17ll : 32ll) * c.n_seq && likely * std::max(rows, 512) >= (c.f32 ? 100000 : 450000)) {
+    if (c.cu && qrows >= (c.f32 ? 17ll : 32ll) * c.n_seq && likely * std::max(rows, 512) >= (c.f32 ? 100000 : bf ? 620000 : 450000)) {
         // the cut into units of tp tokens and steps of `step` rows: what it takes, in steps
         auto tiles = [&](int tp, int step, int least) {
             long long best = LLONG_MAX;

@@ -238,8 +238,7 @@ class PagedKVCacheSet:
         held.  max_rows: at least as many rows as the longest sequence has after the
         call (0: the pages that ``reserve`` and ``share`` gave it, maxT where the host
         writes the table); the call is cut by it, which only rounding shows.  out may be
-        q.  With bfloat16 q a weight holds 16 bits, in long prompts over bfloat16 pages
-        8; with float32 q 24."""
+        q.  With bfloat16 q a weight holds 16 bits, with float32 q 24."""
         n, H = (q.shape[0], q.shape[1]) if isinstance(q, torch.Tensor) and q.dim() == 3 else (-1, self.shape.n_heads)
         self._heads(q, "q", n, H)
         self._tokens(start, cu, n)

@@ -13,9 +13,9 @@ library's header states gives, n being the rows that a token sees:
                  of A_t each), the scale and the exponential; f_t = (n + 64) 2^-24: a
                  float32 sum of n products and of n weights
   bf16           weights in two parts, 2^-17; the output, 2^-8 of it
-  bf16 prompt    weights rounded once, 2^-8 (the sum is of the rounded ones: a common
-                 factor drops out, the difference of two values is what counts, which
-                 |v| + |o| covers)
+  bf16 prompt    a looser bound, of weights rounded once, 2^-8 (their sum that of the
+                 rounded ones: a common factor drops out, the difference of two values is
+                 what counts, which |v| + |o| covers)
 """
 
 from __future__ import annotations
