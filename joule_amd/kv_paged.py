@@ -30,7 +30,10 @@ class PagedKVCacheSet:
     An entry of the table outside [0, n_pages) is no page: rows there are not
     written, and attention does not see them.  ``reserve``, ``share`` and
     ``release`` keep the table, on the current stream, which is that of the calls; a
-    host with an allocator of its own writes it instead."""
+    host with an allocator of its own writes it instead.  They are for one host thread at a
+    time, and not for a stream that is being captured; where one raises, it has changed
+    nothing.  ``reserve`` and ``share`` wait for the stream's work where they give out pages
+    (they copy page numbers from the host): in a serving loop, reserve for some rows ahead."""
 
     def __init__(self, shape: DecoderShape, B: int, n_pages: int, page: int = 16, dtype: torch.dtype = torch.bfloat16,
                  device="cuda", data: torch.Tensor | None = None):
@@ -70,6 +73,12 @@ class PagedKVCacheSet:
             raise ValueError(f"sequence {b} outside [0, {self.B})")
         return self._pages[b]
 
+    def _writable(self) -> None:
+        # (a captured write is done at each replay, and not now)
+        with _lib.on(self._device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("pages are given out and taken back outside a captured graph")
+
     def _publish(self, b: int, at: int, pages: list[int]) -> None:
         if pages:
             self.table[b, at:at + len(pages)] = torch.tensor(pages, dtype=torch.int32).to(self._device)
@@ -89,10 +98,12 @@ class PagedKVCacheSet:
             return
         if n > len(self._free):
             raise RuntimeError(f"sequence {b} needs {n} more pages, {len(self._free)} are free")
-        got = [self._free.pop() for _ in range(n)]
+        self._writable()
+        got = self._free[:-n - 1:-1]
+        self._publish(b, len(have), got)
+        del self._free[-n:]
         for p in got:
             self._uses[p] = 1
-        self._publish(b, len(have), got)
         have += got
 
     def share(self, src: int, dst: int, rows: int) -> None:
@@ -108,25 +119,28 @@ class PagedKVCacheSet:
         if rows % self.page and not self._free:
             raise RuntimeError("no page is free for the rows that are copied")
         got = a[:whole]
+        if rows:
+            self._writable()
+        if rows % self.page:
+            got.append(self._free[-1])
+            self.data[:, got[-1]] = self.data[:, a[whole]]
+        self._publish(dst, 0, got)
+        if rows % self.page:
+            self._free.pop()
         for p in got:
             self._uses[p] += 1
-        if rows % self.page:
-            p = self._free.pop()
-            self._uses[p] = 1
-            self.data[:, p] = self.data[:, a[whole]]
-            got.append(p)
-        self._publish(dst, 0, got)
         b += got
 
     def release(self, b: int) -> None:
         """Give sequence b's pages back (those that others hold stay theirs)."""
         held = self._sequence(b)
+        if held:
+            self._writable()
+            self.table[b] = -1
         for p in held:
             self._uses[p] -= 1
             if self._uses[p] == 0:
                 self._free.append(p)
-        if held:
-            self.table[b] = -1
         held.clear()
 
     # ------------------------------------------------------------ arguments
