@@ -786,9 +786,9 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     }
     locate(NS);
 
-    // ---- the query rows, with the score scale's sign (a scale of 0, or a smaller one, as
-    // 2^-100: masked scores stay -inf behind it)
-    const float cs = fmaxf(fabsf(a.scale2), 0x1p-100f);
+    // ---- the query rows, with the score scale's sign (a scale of 0 as 2^-149, of which the
+    // largest score makes 2^-21: masked scores stay -inf behind it)
+    const float cs = fmaxf(fabsf(a.scale2), 0x1p-149f);
     const uint32_t sign = a.scale2 < 0.0f ? 0x80008000u : 0u;
     bf16x8 qr[NQ][8];
 #pragma unroll
