@@ -599,18 +599,21 @@ int jm_kv_paged_append(const jm_kv_paged* c, const int32_t* start, const int32_t
 /* out [N][n_heads][128] = softmax(scale q . K) V over the rows 0 .. the token's own that
  * the table has pages for, which are in the cache already; n_heads / n_kv is a whole
  * number from 1 to 16.  A token that sees no row (its own below 0, or none with a page)
- * gets 0; other skipped tokens keep what out held.  A NaN or an infinity in q, or in K in
- * a row that a token sees, makes its output NaN, one in V that dimension NaN or infinite
- * (products are taken in parts, of which some are 0); rows that it does not see may hold
- * anything.
+ * gets 0; other skipped tokens keep what out held.  A NaN or an infinity in q, or a NaN in
+ * K in a row that a token sees, makes its output NaN.  An infinity in K there makes it NaN
+ * where the score is +infinity (or no number), and gives the row no weight where it is
+ * -infinity; with float32 q over bf16 pages that may be NaN too, and one in V makes that
+ * dimension NaN or infinite, as products are taken in parts.  Rows that a token does not see
+ * may hold anything.
  *   max_rows  at least as many rows as the longest sequence has after this call, where
  *             the caller knows (0: maxT): the call is cut by it, which only rounding
  *             shows.  A smaller number is slower, not wrong.
  * float32 q: scores, weights and sums hold float32's 24 bits.  bf16 q: q is exact, and a
  * weight is so to 2^-16 of it, whatever the call's sizes.  Sums are float32.  out may be q
  * where q is contiguous.
- * The magnitudes of V stay below 2^100, those of q below 2^127.  Workspace: as
- * jm_q4_gemm_f32's. */
+ * The magnitudes of V stay below 2^100 (of n rows below 2^118 / n where that is less: rows of V
+ * are summed in float32 times weights of up to 2^12, and divided by the weights' sum at the
+ * end), those of q below 2^127.  Workspace: as jm_q4_gemm_f32's. */
 int jm_kv_paged_attn(const jm_kv_paged* c, const int32_t* start, const int32_t* cu, int N, const void* q, int64_t q_token,
                      int64_t q_head, int n_heads, float scale, int max_rows, int dtype, void* out, void* stream);
 

@@ -67,3 +67,15 @@ def test_large_scores_under_a_scale_near_0(H, KH, counts, start, maxT, scale, dt
     c, q = prepared(H, KH, counts, start, cached, maxT)
     c.data[:, :, 0] *= 2.0 ** 105
     check(c, q, start, counts, dt, scale=scale)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+@pytest.mark.parametrize("H,KH,counts,start", CALLS)
+@pytest.mark.parametrize("maxT", [1500, DEEP])
+def test_the_largest_values_allowed(H, KH, counts, start, maxT, dt, cached):
+    """V up to 2^100, under weights that pass the reference."""
+    c, q = prepared(H, KH, counts, start, cached, maxT)
+    v = c.data[:, :, 1]
+    v *= 2.0 ** 99 / float(v[v.isfinite()].abs().max())
+    for x in (1.0, 8.0):
+        check(c, q * x, start, counts, dt)
