@@ -386,7 +386,6 @@ struct PagedArgs {
     const int* start;         // as in Q4KvArgs
     const int* cu;
     int N;
-    const int* pos;           // NULL (the decoder's form)
 };
 // q, k and v of the tokens as the projections give them, and what is done to them on
 // the way.

@@ -102,7 +102,7 @@ hipError_t launch_paged_append(const PagedArgs& c, const PagedRows& r, hipStream
 // ------------------------------------------------------- few query tokens
 //
 // Block (KV head, unit of up to 16 query rows: tokens x heads of the KV head, range of
-// the unit's rows), W waves that take the range's tiles in turn, with a softmax each,
+// the unit's rows), 4 waves that take the range's tiles in turn, with a softmax each,
 // joined at the end; the ranges of a unit are joined by a second launch
 // (k_paged_merge).  A tile (8 KB of K and of V: 32 bf16 rows, 16 float32 ones) goes
 // straight to the lanes' registers in the order in which the matrix cores take it, the
@@ -299,13 +299,14 @@ struct PagedWeights {
 };
 
 constexpr int PAGED_OW = 132;               // floats between the columns of a wave's outputs in LDS
+constexpr int PAGED_W = 4;                  // waves of a block
 
 // The query rows of one unit over tiles t0 .. t_end - 1 of its sequence; the waves joined,
 // and the output, or (several ranges) the partial outputs.
-template <bool F32, bool BF, int W>
-__global__ void __launch_bounds__(64 * W, 2)
+template <bool F32, bool BF>
+__global__ void __launch_bounds__(64 * PAGED_W, 2)
 k_paged_attn(PagedArgs c, PagedAttnArgs a) {
-    constexpr int HD = 128, NG = F32 ? 1 : 2, TR = 16 * NG, NY = 4 * NG;
+    constexpr int HD = 128, W = PAGED_W, NG = F32 ? 1 : 2, TR = 16 * NG, NY = 4 * NG;
     constexpr int NQ = BF ? 1 : 3, NP = BF ? 2 : 3;         // parts of q, of the weights
     __shared__ __align__(16) float ow[W][16][PAGED_OW];
     __shared__ float mls[W][16][2];
@@ -674,7 +675,6 @@ k_paged_tile(PagedArgs c, PagedAttnArgs a) {
     // the second block of query rows of each row group (BF)
     __shared__ __align__(16) uint4 q1[BF ? RG : 1][8][64];
     __shared__ float mls[8][32 * QB][2];
-    __shared__ uint8_t okf[NS][2 * PS];          // whether a step's 16-row groups have pages
     // which dimensions met a V value of +inf (bit 0), -inf (bit 1) or NaN (both) that not
     // every query row of a wave sees, 16 dimensions a word
     __shared__ uint32_t taint[NROW][HD / 16];
@@ -1505,7 +1505,7 @@ hipError_t launch_paged_attn(const PagedArgs& c, const PagedPlan& p, const void*
 #undef JM_PAGED_TILE
     } else {
 #define JM_PAGED(F32V, BFV) \
-        if ((c.f32 != 0) == F32V && bf == BFV) hipLaunchKernelGGL((k_paged_attn<F32V, BFV, 4>), grid, dim3(256), 0, st, c, a)
+        if ((c.f32 != 0) == F32V && bf == BFV) hipLaunchKernelGGL((k_paged_attn<F32V, BFV>), grid, dim3(64 * PAGED_W), 0, st, c, a)
         JM_PAGED(false, false); else JM_PAGED(false, true); else JM_PAGED(true, false); else JM_PAGED(true, true);
 #undef JM_PAGED
     }

@@ -47,6 +47,9 @@ __device__ __forceinline__ unsigned long long q4_plane(const Q4KvArgs& c, int se
     return (unsigned long long)(uintptr_t)(which ? c.v : c.k) + (unsigned long long)seq * c.seq_stride;
 }
 
+// (the decoder's form has its tokens' rows)
+__device__ __forceinline__ int call_row(const Q4KvArgs& c, int u) { return c.pos ? c.pos[u] : c.start[u]; }
+
 // A group's scale from the bits of its largest magnitude (a NaN's are the
 // largest of all), and its values' codes + 8.  The quotient is the correctly
 // rounded fp32 one: the scale's reciprocal rounded, then one Newton step on the

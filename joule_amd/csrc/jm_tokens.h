@@ -1,6 +1,6 @@
 // The tokens of a call over caches: their values, and which sequence and cache row each
 // has.  C is the call's arguments (Q4KvArgs, PagedArgs): n_seq, N, maxT, start and cu
-// (NULL: token t is sequence t's only one) and, for the decoder's form, pos.
+// (NULL: token t is sequence t's only one).
 #pragma once
 
 #include "jm_device.h"
@@ -119,6 +119,10 @@ struct CallUnit {
     int seq, tok, n, pos;
 };
 
+// The cache row of token u where tokens have a sequence each (call_unit without cu).
+template <class C>
+__device__ __forceinline__ int call_row(const C& c, int u) { return c.start[u]; }
+
 // Unit u of the call for tp tokens a unit (without cu and in the decoder's form:
 // token u alone); false if there is none.  The same in every lane.
 template <class C>
@@ -126,7 +130,7 @@ __device__ __forceinline__ bool call_unit(const C& c, int u, int tp, CallUnit& q
     if (!c.cu) {
         q.seq = q.tok = u;
         q.n = 1;
-        q.pos = c.pos ? c.pos[u] : c.start[u];
+        q.pos = min(call_row(c, u), c.maxT);                // (so that sums with q.n stay within an int)
         return true;
     }
     const int lane = threadIdx.x & 63;

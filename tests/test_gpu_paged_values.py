@@ -79,3 +79,20 @@ def test_the_largest_values_allowed(H, KH, counts, start, maxT, dt, cached):
     v *= 2.0 ** 99 / float(v[v.isfinite()].abs().max())
     for x in (1.0, 8.0):
         check(c, q * x, start, counts, dt)
+
+
+@pytest.mark.parametrize("dt,cached", TYPES)
+def test_rows_at_the_ends_of_their_type(dt, cached):
+    """A token a sequence, at rows that int32 just holds: past the cache, and below 0."""
+    c, q = prepared(8, 2, [1, 1, 1, 1], [0, 0, 40, 0], cached, 900)
+    start = [2 ** 31 - 1, -2 ** 31, 40, 2 ** 31 - 1]
+    out = torch.full((4, 8, HD), 7.0, dtype=DT[dt], device="cuda")
+    qd, k = torch.from_numpy(q).cuda().to(DT[dt]), torch.ones(4, 2, HD, dtype=DT[dt], device="cuda")
+    got = c.attention(0, qd, ints(start), out=out)
+    want = c.attention(0, qd, ints([0, 0, 40, 0]))
+    assert bool((got[[0, 3]] == 7.0).all()) and not bool(got[1].any()) and torch.equal(got[2], want[2])
+    before = c.data.clone()
+    c.append(0, k, k, ints(start), q=torch.ones_like(out), q_out=out.fill_(7.0))
+    assert bool((out[[0, 1, 3]] == 7.0).all()) and bool((out[2] == 1.0).all())
+    bits = torch.int32 if cached == "f32" else torch.int16              # (the pages hold NaN elsewhere)
+    assert 0 < int((c.data.view(bits) != before.view(bits)).sum()) <= 2 * 2 * HD
