@@ -1390,8 +1390,14 @@ k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
         }
 }
 
-// How a call is cut, by sizes and types alone.  Times are of 32 query heads on 8 KV heads,
-// "T tokens behind R rows, B sequences" (us).
+// How a call is cut, by sizes and types alone: the host does not know cu, and takes the
+// tokens as spread evenly over all sequences, idle ones too.  What that costs where they are
+// not (bf16): 2047 tokens behind 4099 rows take 243 us alone and in a set of up to 128
+// sequences, 979 in one of 256, where k_paged_attn gets them; 512 tokens 81 alone, 99 in a set
+// of 64, 173 from 128 on.  A prompt of 2048 (80) beside 63 single tokens behind 16000 rows
+// (611) 1340, as each of those goes through the tiles.
+//
+// Times are of 32 query heads on 8 KV heads, "T tokens behind R rows, B sequences" (us).
 //
 // Which kernel: a block of k_paged_attn has 16 query rows, so that the cache is multiplied
 // once for each 16, but is done in 8 us; k_paged_tile takes 15 us to begin and end.  The
@@ -1414,8 +1420,8 @@ k_paged_tile_f32(PagedArgs c, PagedAttnArgs a) {
 // RG 2 reads the cache twice as often as RG 4: it has to be a tenth below.  RG 4 / RG 2: 777
 // tokens behind none 41 / 34, 800 behind 2000 75 / 67, 2047 behind none 80 / 75, 2047 behind
 // 4099 236 / 247, 4 sequences of 300 behind 500 43 / 59, of 700 94 / 105, 5 of 1201 (28 heads on
-// 4) 120 / 166.  512 rows a range at least against 256: 200 tokens behind 1000 rows 34 / 35; of
-// float32 pages 32 behind 2000 35 / 26.
+// 4) 120 / 166.  512 rows a range at least against 256: 300 tokens behind 1000 rows 37 / 37, 150
+// behind 2000 34 / 33; of float32 pages 32 behind 2000 35 / 26.
 //
 // Ranges of k_paged_attn: a block of each CU in turn, each as long as its rows and 160 more; a
 // quarter of a block behind the last, as the prefixes differ; joining them 750 rows (of
